@@ -425,6 +425,54 @@ int tvmkv_compact_kv_copy(void* pages, const int32_t* copy_length_indptr,
                           int32_t total_copy_length, int64_t num_pages, int32_t num_kv_heads,
                           int32_t page_size, int32_t head_dim, void* stream);
 
+/* ---- a cache held in 4 bits (no counterpart among the reference's kernels) -----------------------
+ *
+ * Format (block-scaled FP4: element and scale types of the OCP microscaling format MXFP4).  A row is one
+ * token's K or V of one kv head.  32 consecutive elements are a block: 32 FP4 codes (sign, 2 exponent bits,
+ * 1 mantissa bit: 0, .5, 1, 1.5, 2, 3, 4, 6; element 2i in the low half of byte i) and one scale byte s that
+ * stands for 2^(s - 127), 255 for NaN.  The pool is (num_pages, 2, h_kv, page_size, 17 * head_dim / 32) bytes:
+ * 4.25 bits an element.  The bytes of one (page, K or V, kv head) are the codes of its page_size tokens,
+ * head_dim / 2 bytes each, then their scales, head_dim / 32 bytes each.
+ *
+ * Built for head dims 64, 96, 128 and 256 and pages of any multiple of 16 tokens; keys are stored rotated
+ * (the kernels have no RoPE).  Rows, queries and outputs are fp16, log-sum-exps fp32 (base 2); data pointers
+ * are aligned to 16 bytes.  Page tables, length_info and slots (page * page_size + offset) are those of the fp16 kernels. */
+
+/* k_data, v_data (ntoken, h_kv, head_dim) -> slots position_map (ntoken); a negative slot: the token is not
+ * written.  A block's scale is 2^e with the smallest e in [-23, 13] at which its largest magnitude is at most
+ * 7 * 2^e (13 if none is); codes round to nearest, ties to the even code, and saturate at 6.  A block with a
+ * value that is not finite is NaN. */
+int tvmkv_mxfp4_append(void* pages, const void* k_data, const void* v_data, const int32_t* position_map,
+                       int64_t ntoken, int64_t num_pages, int32_t num_kv_heads, int32_t page_size,
+                       int32_t head_dim, void* stream);
+
+/* The rows of slots position_map (ntoken) as fp16, exactly: k_data, v_data (ntoken, h_kv, head_dim).  A
+ * negative slot gives rows of zeros. */
+int tvmkv_mxfp4_read_kv(const void* pages, const int32_t* position_map, void* k_data, void* v_data,
+                        int64_t ntoken, int64_t num_pages, int32_t num_kv_heads, int32_t page_size,
+                        int32_t head_dim, void* stream);
+
+/* Decode: one query token a sequence, q and output (batch, h_q, head_dim), lse (batch, h_q).  length_info
+ * (batch): tokens on the last page, or with sliding_window (3, batch): those, the first stored token behind the
+ * evicted ones, the attention sinks in front of them.  A sequence without keys: output 0, lse -5e4.  Splits
+ * long sequences; scratch memory per (device, stream) as the fp16 decode entry point. */
+int tvmkv_mxfp4_batch_decode_paged_kv(const void* q, const void* pages, const int32_t* page_indptr,
+                                      const int32_t* page_values, const int32_t* length_info, void* output,
+                                      float* lse, double sm_scale, int32_t batch_size, int64_t nnz_pages,
+                                      int64_t num_pages, int32_t h_q, int32_t h_kv, int32_t head_dim,
+                                      int32_t page_size, int32_t sliding_window, void* stream);
+
+/* Prefill: q_indptr (batch + 1) query tokens of each sequence, q and output (total_q, h_q, head_dim), lse
+ * (total_q, h_q).  causal: the last query sees all keys, one before it one fewer, and so on (a sequence's new
+ * tokens are in the cache already); otherwise every query sees all keys (e.g. new rows apart from the cache, joined
+ * with tvmkv_merge_state_inplace).  A query without keys: output 0, lse -5e4. */
+int tvmkv_mxfp4_batch_prefill_paged_kv(const void* q, const int32_t* q_indptr, const void* pages,
+                                       const int32_t* page_indptr, const int32_t* page_values,
+                                       const int32_t* length_info, void* output, float* lse, int64_t causal,
+                                       double sm_scale, int32_t batch_size, int64_t total_q, int64_t nnz_pages,
+                                       int64_t num_pages, int32_t h_q, int32_t h_kv, int32_t head_dim,
+                                       int32_t page_size, int32_t sliding_window, void* stream);
+
 /* Tuning options (no counterpart in the reference).  Each starts from an environment variable read
  * once when the library is loaded (TVMKV_ + the upper-case name) and defaults to 0:
  *   decode_chunk_pages     pages per split-KV chunk of the decode kernel (a multiple of 8); 0 = from shapes

@@ -67,6 +67,11 @@ SIGNATURES = {
     "tvmkv_kv_cache_debug_get_kv": [c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_i32, c_i32, c_i32, c_vp],
     "tvmkv_kv_cache_debug_get_kv_mla": [c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_i32, c_i32, c_vp],
     "tvmkv_compact_kv_copy": [c_vp, c_vp, c_vp, c_i32, c_i32, c_i64, c_i32, c_i32, c_i32, c_vp],
+    "tvmkv_mxfp4_append": [c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_i32, c_i32, c_i32, c_vp],
+    "tvmkv_mxfp4_read_kv": [c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_i32, c_i32, c_i32, c_vp],
+    "tvmkv_mxfp4_batch_decode_paged_kv": [c_vp] * 7 + [c_f64, c_i32, c_i64, c_i64, c_i32, c_i32, c_i32, c_i32, c_i32, c_vp],
+    "tvmkv_mxfp4_batch_prefill_paged_kv": [c_vp] * 8 + [c_i64, c_f64, c_i32, c_i64, c_i64, c_i64, c_i32, c_i32, c_i32, c_i32,
+                                                        c_i32, c_vp],
     "tvmkv_set_option": [ctypes.c_char_p, c_i64],
     "tvmkv_get_option": [ctypes.c_char_p, p_i64],
     "tvmkv_release_scratch": [c_vp],

@@ -283,3 +283,82 @@ def compact_kv_copy(pages, copy_length_indptr, copy_src_dst_pos, batch_size):
     num_pages, _, hkv, ps, d = pages.shape
     check(lib().tvmkv_compact_kv_copy(_p(pages), _p(copy_length_indptr), _p(copy_src_dst_pos), batch_size,
                                       copy_src_dst_pos.shape[1], num_pages, hkv, ps, d, _stream()))
+
+
+# ---- a cache held in 4 bits (include/tvmkv.h has its format) ----------------------------------------------------
+
+
+def mxfp4_pages(num_pages, h_kv, page_size, head_dim, device="cuda"):
+    """A pool of pages for mxfp4_append and the kernels that read them: 17 * head_dim / 32 bytes a row."""
+    return torch.zeros((num_pages, 2, h_kv, page_size, 17 * head_dim // 32), dtype=torch.uint8, device=device)
+
+
+def _mxfp4_pool(pages, head_dim):
+    if pages.dtype != torch.uint8:
+        raise KVError(-1, f"pages of 4-bit rows must be uint8, got {pages.dtype}")
+    if pages.dim() != 5 or pages.shape[1] != 2 or pages.shape[4] * 32 != 17 * head_dim:
+        raise KVError(-1, f"pages has shape {tuple(pages.shape)}, expected (num_pages, 2, h_kv, page_size, 17 * {head_dim} / 32)")
+    num_pages, _, hkv, ps, _ = pages.shape
+    return num_pages, hkv, ps
+
+
+def _shape(t, name, *expected):
+    if tuple(t.shape) != expected:
+        raise KVError(-1, f"{name} has shape {tuple(t.shape)}, expected {expected}")
+
+
+def mxfp4_append(pages, k_data, v_data, position_map):
+    """Quantises the rows k_data, v_data (tokens, h_kv, head_dim) into the slots position_map (negative: none)."""
+    _f16(k_data, v_data)
+    _i32(position_map)
+    d = k_data.shape[-1]
+    num_pages, hkv, ps = _mxfp4_pool(pages, d)
+    n = position_map.shape[0]
+    _shape(k_data, "k_data", n, hkv, d)
+    _shape(v_data, "v_data", n, hkv, d)
+    check(lib().tvmkv_mxfp4_append(_p(pages), _p(k_data), _p(v_data), _p(position_map), n, num_pages, hkv, ps, d, _stream()))
+
+
+def mxfp4_read_kv(pages, position_map, k_data, v_data):
+    """The rows of the slots position_map as fp16, into k_data and v_data (tokens, h_kv, head_dim)."""
+    _f16(k_data, v_data)
+    _i32(position_map)
+    d = k_data.shape[-1]
+    num_pages, hkv, ps = _mxfp4_pool(pages, d)
+    n = position_map.shape[0]
+    _shape(k_data, "k_data", n, hkv, d)
+    _shape(v_data, "v_data", n, hkv, d)
+    check(lib().tvmkv_mxfp4_read_kv(_p(pages), _p(position_map), _p(k_data), _p(v_data), n, num_pages, hkv, ps, d, _stream()))
+
+
+def _mxfp4_attention(q, pages, page_indptr, page_values, length_info, output, lse):
+    _f16(q, output)
+    _i32(page_indptr, page_values, length_info)
+    if lse.dtype != torch.float32:
+        raise KVError(-1, f"lse must be float32, got {lse.dtype}")
+    rows, hq, d = q.shape
+    num_pages, hkv, ps = _mxfp4_pool(pages, d)
+    batch = page_indptr.shape[0] - 1
+    _shape(output, "output", rows, hq, d)
+    _shape(lse, "lse", rows, hq)
+    _shape(length_info, "length_info", *((3, batch) if length_info.dim() == 2 else (batch,)))
+    return rows, hq, d, num_pages, hkv, ps, batch
+
+
+def mxfp4_batch_decode_paged_kv(q, pages, page_indptr, page_values, length_info, output, lse, sm_scale):
+    """batch_decode_paged_kv over 4-bit pages: one query token a sequence, keys stored rotated."""
+    rows, hq, d, num_pages, hkv, ps, batch = _mxfp4_attention(q, pages, page_indptr, page_values, length_info, output, lse)
+    _shape(q, "q", batch, hq, d)
+    check(lib().tvmkv_mxfp4_batch_decode_paged_kv(
+        _p(q), _p(pages), _p(page_indptr), _p(page_values), _p(length_info), _p(output), _p(lse), float(sm_scale), batch,
+        page_values.shape[0], num_pages, hq, hkv, d, ps, int(length_info.dim() == 2), _stream()))
+
+
+def mxfp4_batch_prefill_paged_kv(q, q_indptr, pages, page_indptr, page_values, length_info, output, lse, causal, sm_scale):
+    """batch_prefill_paged_kv over 4-bit pages: q_indptr (batch + 1) query tokens of each sequence, keys stored rotated."""
+    rows, hq, d, num_pages, hkv, ps, batch = _mxfp4_attention(q, pages, page_indptr, page_values, length_info, output, lse)
+    _i32(q_indptr)
+    _shape(q_indptr, "q_indptr", batch + 1)
+    check(lib().tvmkv_mxfp4_batch_prefill_paged_kv(
+        _p(q), _p(q_indptr), _p(pages), _p(page_indptr), _p(page_values), _p(length_info), _p(output), _p(lse), int(causal),
+        float(sm_scale), batch, rows, page_values.shape[0], num_pages, hq, hkv, d, ps, int(length_info.dim() == 2), _stream()))
