@@ -111,17 +111,18 @@ __global__ __launch_bounds__(256) void mxfp4_read_kernel(const uint8_t* __restri
 
 // ------------------------------------------------------------------------------------------
 // Attention.  With s = sm_scale log2(e) q.k the output of a row is sum 2^(s - m) v / sum 2^(s - m) and its
-// log-sum-exp (base 2) m + log2(sum), m the running maximum; sums, statistics and outputs in float32, the weights
-// rounded to fp16 for the second matrix product (11 bits, as the output itself).
+// log-sum-exp (base 2) m + log2(sum), for any m; sums, statistics and outputs in float32, the weights rounded to fp16
+// for the second matrix product (11 bits, as the output itself).
 //
-// A row of a kv head is (query token, query head of its group), token-major.  A workgroup of four waves takes 16
-// rows of a kv head and a range of the sequence's keys, a wave every fourth step of 32 keys (two runs of 16 tokens;
-// page sizes are multiples of 16, so a run lies in one page):
+// A row of a kv head is (query token, query head of its group), token-major.  A workgroup of four waves takes up to
+// 16 RB rows of a kv head and a range of the sequence's keys, a wave every fourth step of 32 keys (two runs of 16
+// tokens; page sizes are multiples of 16, so a run lies in one page):
 //   S^T[token, row] = K Q^T    the lane (token, quarter of the row) loads its codes straight from memory, turns
 //                              them into fp16 in registers and has the matrix instruction's A operand: the order of
 //                              the contraction is free, q is loaded in the same one;
 //   O^T[d, row]     = V^T P^T  V is turned into fp16 the same way and put into the wave's LDS tile, from where the
 //                              transposing read takes it; P stays in registers.
+// The codes of a wave's next step are on their way while it works on one.
 // ------------------------------------------------------------------------------------------
 struct Mxfp4Params {
   const half_t* q;
@@ -134,48 +135,92 @@ struct Mxfp4Params {
   const int32_t* sink_size;      // (B) first tokens that are never evicted, or NULL
   half_t* output;
   float* lse;
-  float* part_o;   // (slots, h_q, D) outputs of the chunks, not normalised
-  float* part_ml;  // (slots, h_q, 2) their maxima and sums
+  // states of work items that have only some of a row's keys: (slot, row block, kv head, row of the block)
+  float* part_o;   // D each, not normalised
+  float* part_ml;  // reference point, sum
+  unsigned* arrivals;  // of the work items of some rows; 0 between launches
   int batch;
   int h_q;
   int h_kv;
   int group;
-  int row_blocks;  // blocks of 16 rows of a sequence with one query token
+  int row_blocks;  // of a sequence with one query token
   int causal;
   int page_size;
   uint32_t runs_per_page;
   uint32_t run_magic;  // 2^32 / runs_per_page, rounded up (0: 1)
-  int chunk_runs;      // keys of a work item of a decode launch, in runs; even
-  float scale_log2;
+  uint32_t chunk_runs;  // decode: keys of a work item, in runs; a multiple of 8
+  int shares;           // prefill: work items that share the keys of a row block
+  float scale_log2;     // > 0: |sm_scale| log2(e), never 0
+  uint32_t q_sign;      // of sm_scale, at the sign bits of two fp16
 };
 
-// The last of n sequences whose begin(i) is at most `slot` (begin increases, begin(0) <= slot): the lanes of the
-// wave probe 64 of them at a time, one round trip to memory per factor of 64.
-template <class Begin>
-__device__ __forceinline__ int sequence_of(int n, int slot, int lane, Begin begin) {
-  int lo = 0;
+// First work item of a sequence whose first page is page_indptr[i] == first.  Decode: with it sequence i has chunks for all
+// tokens that its pages could hold (the launcher makes sure that the runs of all pages are a 31-bit number).  Prefill:
+// q_indptr[i] == first, and it has blocks for all of its rows.
+__device__ __forceinline__ int chunk_begin(const Mxfp4Params& p, int i, int first) {
+  return static_cast<int>(static_cast<uint32_t>(first) * p.runs_per_page / p.chunk_runs) + i;
+}
+template <int R>
+__device__ __forceinline__ int block_begin(const Mxfp4Params& p, int i, int first) {
+  return static_cast<int>(static_cast<int64_t>(first) * p.group / R) + i;
+}
+
+// The sequence of a work item, and what the arrays hold for it.  begin(i) increases with i: the wave looks for the last
+// sequence with begin(i) <= slot, 64 at a time, and the lanes of the last round fetch the other values along with it, so
+// that up to 64 sequences take one round trip to memory.
+struct Sequence {
+  int index, begin;  // begin: its first work item
+  int page_begin, num_pages, last_page_len, sink, window;
+  int q_begin, q_len;
+};
+template <bool PREFILL, class Begin>
+__device__ __forceinline__ Sequence sequence_of(const Mxfp4Params& p, int slot, int lane, Begin begin) {
+  const int32_t* const indptr = PREFILL ? p.q_indptr : p.page_indptr;
+  int lo = 0, n = p.batch;
   while (n > 64) {
     const int stride = (n + 63) >> 6;
     const int at = lo + lane * stride;
-    const bool hit = at < lo + n && begin(at) <= slot;
+    const bool hit = at < lo + n && begin(at, indptr[at]) <= slot;
     const int first = lo + (__popcll(__ballot(hit)) - 1) * stride;
     n = min(stride, lo + n - first);
     lo = first;
   }
-  const bool hit = lane < n && begin(lo + lane) <= slot;
-  return __builtin_amdgcn_readfirstlane(lo + max(static_cast<int>(__popcll(__ballot(hit))), 1) - 1);
+  const int at = lo + min(lane, n - 1);
+  const int page = p.page_indptr[at], next_page = p.page_indptr[at + 1], last = p.last_page_len[at];
+  const int sink = p.sink_size != nullptr ? p.sink_size[at] : 0, window = p.window_offset != nullptr ? p.window_offset[at] : 0;
+  const int q = PREFILL ? p.q_indptr[at] : at, next_q = PREFILL ? p.q_indptr[at + 1] : at + 1;
+  const int mine = begin(at, PREFILL ? q : page);
+  const int who = max(static_cast<int>(__popcll(__ballot(lane < n && mine <= slot))), 1) - 1;
+  const auto of = [&](int x) { return __builtin_amdgcn_readlane(x, who); };
+  Sequence s = {lo + who, of(mine), of(page), of(next_page) - of(page), of(last), of(sink), of(window), of(q), of(next_q) - of(q)};
+  if (s.num_pages == 0) s.sink = s.window = 0;
+  return s;
 }
 
-// First work item of a sequence: with it sequence i has chunks for all tokens that its pages could hold.
-__device__ __forceinline__ int chunk_begin(const Mxfp4Params& p, int i) {
-  return static_cast<int>(static_cast<int64_t>(p.page_indptr[i]) * p.runs_per_page / p.chunk_runs) + i;
+// A global address that is the same in every lane.  (The address space is spelled out: behind the lane reads the compiler
+// no longer knows it, and flat loads are waited for together with LDS reads.)
+typedef __attribute__((address_space(1))) const uint8_t* global_bytes_t;
+typedef uint32_t uint32x2_t __attribute__((ext_vector_type(2)));
+typedef uint32_t uint32x4_t __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ global_bytes_t uniform_bytes(const uint8_t* p) {
+  const uint64_t v = reinterpret_cast<uint64_t>(p);
+  const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v));
+  const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v >> 32));
+  return reinterpret_cast<global_bytes_t>(static_cast<uint64_t>(hi) << 32 | lo);
+}
+// ONCE: the codes are read by one work item only and streamed through the caches (a plain read of a large array reaches
+// 6.2 TB/s here, one with the streaming hint 6.9).  The scales are not, whose 64 bytes share a line with others' codes.
+template <class T, bool ONCE = false>
+__device__ __forceinline__ T load_global(global_bytes_t base, uint32_t offset) {
+  const auto at = reinterpret_cast<__attribute__((address_space(1))) const T*>(base + offset);
+  return ONCE ? __builtin_nontemporal_load(at) : *at;
 }
 
 // What a lane holds of a row: D / 4 elements in chunks of 8, and the scales of their blocks.  The lane group g4
 // (0..3) has consecutive chunks, at head dim 256 four of either half of the row.
 template <int D>
 struct LaneRow {
-  static constexpr int CH = D / 32;             // chunks
+  static constexpr int CH = D / 32;                       // chunks
   static constexpr int NS = D == 96 || D == 256 ? 2 : 1;  // blocks they lie in
   uint32_t w[CH];
   uint32_t s[NS];
@@ -187,25 +232,26 @@ struct LaneRow {
   static __device__ __forceinline__ int scale_index(int g4, int c) {
     return D == 256 ? c >> 2 : D == 96 ? ((3 * g4 + c) >> 2) - ((3 * g4) >> 2) : 0;
   }
-  __device__ __forceinline__ void load(const uint8_t* slab, int page_size, int slot, int g4) {
-    const uint8_t* row = slab + slot * (D / 2);
+  // codes, scales: of the run's first token
+  template <bool ONCE>
+  __device__ __forceinline__ void load(global_bytes_t codes, global_bytes_t scales, uint32_t token, uint32_t g4) {
     if constexpr (D == 64) {
-      const uint2 v = *reinterpret_cast<const uint2*>(row + g4 * 8);
-      w[0] = v.x;
-      w[1] = v.y;
+      const auto x = load_global<uint32x2_t, ONCE>(codes, token * (D / 2) + g4 * 8);
+      w[0] = x[0];
+      w[1] = x[1];
     } else if constexpr (D == 96) {
 #pragma unroll
-      for (int c = 0; c < CH; ++c) w[c] = *reinterpret_cast<const uint32_t*>(row + g4 * 12 + c * 4);
+      for (int c = 0; c < CH; ++c) w[c] = load_global<uint32_t, ONCE>(codes, token * (D / 2) + g4 * 12 + c * 4);
     } else {
 #pragma unroll
       for (int i = 0; i < D / 128; ++i) {
-        const Vec16 v = ld16(row + i * 64 + g4 * 16);
+        const auto x = load_global<uint32x4_t, ONCE>(codes, token * (D / 2) + g4 * 16 + i * 64);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) w[i * 4 + c] = v.w[c];
+        for (int c = 0; c < 4; ++c) w[i * 4 + c] = x[c];
       }
     }
 #pragma unroll
-    for (int i = 0; i < NS; ++i) s[i] = slab[page_size * (D / 2) + slot * (D / 32) + block(g4, i)];
+    for (int i = 0; i < NS; ++i) s[i] = load_global<uint8_t>(scales, token * (D / 32) + block(g4, i));
   }
   __device__ __forceinline__ half8_t values(int g4, int c) const {
     const int i = scale_index(g4, c);
@@ -213,148 +259,225 @@ struct LaneRow {
   }
 };
 
-template <int D, bool PREFILL>
-__global__ __launch_bounds__(256) void mxfp4_attn_kernel(Mxfp4Params p) {
+// Device-scope accesses: the states of a row's work items, which other XCDs may have written (each has its own L2).
+constexpr int kDeviceScope = 16;  // the sc1 bit of a buffer access
+struct SharedStates {
+  __amdgpu_buffer_rsrc_t at;
+  __device__ __forceinline__ SharedStates(float* base) : at(__builtin_amdgcn_make_buffer_rsrc(base, 0, -1, 0x00027000)) {}
+  __device__ __forceinline__ void store4(uint32_t offset, float4_t v) {
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(uint32x4_t, v), at, offset * 4, 0, kDeviceScope);
+  }
+  __device__ __forceinline__ void store2(uint32_t offset, float a, float b) {
+    __builtin_amdgcn_raw_buffer_store_b64(uint32x2_t{__float_as_uint(a), __float_as_uint(b)}, at, offset * 4, 0, kDeviceScope);
+  }
+  __device__ __forceinline__ float4_t load4(uint32_t offset) const {
+    return __builtin_bit_cast(float4_t, __builtin_amdgcn_raw_buffer_load_b128(at, offset * 4, 0, kDeviceScope));
+  }
+  __device__ __forceinline__ float2 load2(uint32_t offset) const {
+    const uint32x2_t v = __builtin_amdgcn_raw_buffer_load_b64(at, offset * 4, 0, kDeviceScope);
+    return make_float2(__uint_as_float(v[0]), __uint_as_float(v[1]));
+  }
+};
+
+// Halfs of a row of a wave's V tile in LDS.  Sixteen lanes write the same 16 bytes of the 16 rows of a run, sixteen lanes
+// of the transposing read take 32 bytes of four consecutive rows: at 12, 36 or 52 banks (of 64) from row to row neither
+// meets a bank twice.  (At 8 banks the writes did, and a third of the tile's LDS cycles were conflicts.)
+constexpr int v_row(int d) { return d == 64 || d == 96 ? d + 8 : d + 24; }
+
+// Workgroups of a compute unit, by the registers of a work item of rb blocks of 16 rows.
+constexpr int mxfp4_waves(int d, int rb) { return d == 256 ? (rb == 1 ? 2 : 1) : rb == 1 ? 4 : d == 64 && rb == 2 ? 3 : 2; }
+
+template <int D, int RB, bool PREFILL, bool ONCE>
+__global__ __launch_bounds__(256, mxfp4_waves(D, RB)) void mxfp4_attn_kernel(Mxfp4Params p) {
   constexpr int CH = LaneRow<D>::CH;
   constexpr int DB = D / 16;
-  constexpr int VS = D + 16;  // halfs of a row of the V tile: 32 bytes on, so that rows meet other banks
-  constexpr int OS = D + 4;   // floats of a row of the merge buffer
-  static_assert(32 * VS * sizeof(half_t) >= 16 * OS * sizeof(float), "the merge buffer takes the V tile's place");
-  __shared__ __attribute__((aligned(16))) half_t v_tiles[4][32 * VS];
+  constexpr int R = 16 * RB;
+  constexpr int VS = v_row(D);
+  static_assert(32 * VS * sizeof(half_t) >= 16 * D * sizeof(float), "the merge buffer takes the V tile's place");
+  constexpr int kJoinBytes = (R * 64 + 4 * R) * sizeof(float) + 256 * sizeof(float4_t);  // the join of states, below
+  constexpr int kTileHalfs = std::max<int>(32 * VS, kJoinBytes / 8);
+  __shared__ __attribute__((aligned(16))) half_t v_tiles[4][kTileHalfs];
   __shared__ float sm_m[4][16], sm_l[4][16];
+  __shared__ int sm_last;
 
-  const int wave = threadIdx.x >> 6;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
   const int c16 = lane & 15;
   const int g4 = lane >> 4;
 
   // ---- which rows, which keys ----------------------------------------------------------------
   const int kvh = blockIdx.x % p.h_kv;
-  int slot, rb;
-  if (PREFILL) {
-    slot = blockIdx.x / p.h_kv;
-    rb = 0;
-  } else {
-    slot = blockIdx.x / (p.h_kv * p.row_blocks);
-    rb = blockIdx.x / p.h_kv % p.row_blocks;
-  }
-  const auto row_begin = [&](int i) { return static_cast<int>(static_cast<int64_t>(p.q_indptr[i]) * p.group / 16) + i; };
-  const int b = PREFILL ? sequence_of(p.batch, slot, lane, row_begin)
-                        : sequence_of(p.batch, slot, lane, [&](int i) { return chunk_begin(p, i); });
-  const int page_begin = p.page_indptr[b];
-  const int num_pages = p.page_indptr[b + 1] - page_begin;
-  const int stored = num_pages > 0 ? (num_pages - 1) * p.page_size + p.last_page_len[b] : 0;
-  const int sink = num_pages > 0 && p.sink_size != nullptr ? p.sink_size[b] : 0;
-  const int window = num_pages > 0 && p.window_offset != nullptr ? p.window_offset[b] : 0;
+  const int blocks = PREFILL ? 1 : p.row_blocks;
+  const int slot = blockIdx.x / (p.h_kv * blocks);
+  const Sequence seq = sequence_of<PREFILL>(p, slot, lane, [&](int i, int first) {
+    if constexpr (PREFILL) return block_begin<R>(p, i, first);
+    return chunk_begin(p, i, first);
+  });
+  const int b = seq.index, page_begin = seq.page_begin, sink = seq.sink, window = seq.window;
+  const int stored = seq.num_pages > 0 ? (seq.num_pages - 1) * p.page_size + seq.last_page_len : 0;
   const int keys = stored - window + sink;
-  const int q_begin = PREFILL ? p.q_indptr[b] : b;
-  const int q_len = PREFILL ? p.q_indptr[b + 1] - q_begin : 1;
+  const int q_begin = seq.q_begin, q_len = seq.q_len;
   const int rows = q_len * p.group;
-  if (PREFILL) rb = slot - row_begin(b);
-  const int row0 = rb * 16;
+  const int block = PREFILL ? slot - seq.begin : blockIdx.x / p.h_kv % blocks;
+  const int row0 = block * R;
   if (row0 >= rows) return;  // a spare slot
-  const int rows_here = min(16, rows - row0);
+  const int rows_here = min(R, rows - row0);
   // stored tokens [0, end) hold the first n keys; token t of them is one iff t < sink or t >= window
   const auto end_of = [&](int n) { return n <= sink ? n : n - sink + window; };
   const auto end_of_row = [&](int r) { return end_of(p.causal ? min(max(keys - q_len + 1 + r / p.group, 0), keys) : keys); };
-  const int my_row = row0 + c16;
-  const int my_end = c16 < rows_here ? end_of_row(my_row) : 0;
-  const int first_end = end_of_row(row0);                  // every row sees the keys in front of it
-  const int last_end = end_of_row(row0 + rows_here - 1);   // no row sees a key behind it
-  int run_lo = 0, run_hi = (last_end + kRun - 1) / kRun;
-  int chunks = 1;
-  if (!PREFILL) {
-    const int chunk = slot - chunk_begin(p, b);
-    chunks = max(1, (run_hi + p.chunk_runs - 1) / p.chunk_runs);
-    if (chunk >= chunks) return;
-    run_lo = chunk * p.chunk_runs;
-    run_hi = min(run_hi, run_lo + p.chunk_runs);
-  }
+  const int first_end = end_of_row(row0);                 // every row sees the keys in front of it
+  const int last_end = end_of_row(row0 + rows_here - 1);  // no row sees a key behind it
+  const int all_runs = (last_end + kRun - 1) / kRun;
+  const int chunk = PREFILL ? static_cast<int>(blockIdx.z) : slot - seq.begin;
+  const int per_chunk = PREFILL ? ((all_runs + p.shares - 1) / p.shares + 7) & ~7 : static_cast<int>(p.chunk_runs);
+  const int chunks = all_runs > per_chunk ? (all_runs + per_chunk - 1) / per_chunk : 1;
+  if (chunk >= chunks) return;
+  const int run_lo = chunk * per_chunk;
+  const int run_hi = min(all_runs, run_lo + per_chunk);
 
-  half8_t qf[CH];
-  {
-    const int token = q_begin + my_row / p.group;
-    const half_t* q = p.q + (static_cast<int64_t>(token) * p.h_q + kvh * p.group + my_row % p.group) * D;
+  // Where the codes and the scales of the wave's next 64 steps are, a step a lane: of its two runs' K, in units of 16 bytes
+  // (slabs are a multiple of that, and so are a run's codes and scales).
+  const uint32_t slab16 = static_cast<uint32_t>(p.page_size) / kRun * (17 * D / 32);
+  uint32_t codes16[2], scales16[2];
+  const auto load_ids = [&](int run) {
 #pragma unroll
-    for (int c = 0; c < CH; ++c) qf[c] = c16 < rows_here ? ld16(q + LaneRow<D>::chunk(g4, c) * 8).h8 : zero16().h8;
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t at = min(run + 8 * lane + h, run_hi - 1);
+      const uint32_t nth = p.run_magic != 0 ? __umulhi(at, p.run_magic) : at;
+      const uint32_t in_page = at - nth * p.runs_per_page;
+      const uint32_t slab = (p.page_values[page_begin + nth] * 2u * p.h_kv + kvh) * slab16;
+      codes16[h] = slab + in_page * (D / 2);
+      scales16[h] = slab + p.runs_per_page * (D / 2) + in_page * (D / 32);
+    }
+  };
+  int run = run_lo + 2 * wave;
+  if (run < run_hi) load_ids(run);
+
+  int my_end[RB];
+  half8_t qf[RB][CH];
+#pragma unroll
+  for (int r = 0; r < RB; ++r) {
+    const int my_row = row0 + r * 16 + c16;
+    const bool there = r * 16 + c16 < rows_here;
+    my_end[r] = there ? (PREFILL ? end_of_row(my_row) : last_end) : 0;
+    const half_t* q = p.q + (static_cast<int64_t>(q_begin + my_row / p.group) * p.h_q + kvh * p.group + my_row % p.group) * D;
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      Vec16 x = there ? ld16(q + LaneRow<D>::chunk(g4, c) * 8) : zero16();
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x.w[i] ^= p.q_sign;
+      qf[r][c] = x.h8;
+    }
   }
-  float4_t o[DB];
+  float4_t o[RB][DB];
+  float m[RB], l[RB];
 #pragma unroll
-  for (int i = 0; i < DB; ++i) o[i] = float4_t{0.f, 0.f, 0.f, 0.f};
-  float m = kNoKey, l = 0.f;
-  uint32_t poisoned = 0;  // 32-element parts of the output that are NaN, see below
+  for (int r = 0; r < RB; ++r) {
+#pragma unroll
+    for (int i = 0; i < DB; ++i) o[r][i] = float4_t{0.f, 0.f, 0.f, 0.f};
+    m[r] = kNoKey;
+    l[r] = 0.f;
+  }
+  uint32_t poisoned[RB] = {};  // 32-element parts of the output that are NaN, see below
 
   half_t* const vt = v_tiles[wave];
-  const int64_t slab_bytes = static_cast<int64_t>(p.page_size) * (17 * D / 32);
-  for (int run = run_lo + 2 * wave; run < run_hi; run += 8) {
+  struct Step {
     LaneRow<D> k[2], v[2];
+  };
+  const global_bytes_t pool = uniform_bytes(p.pages);
+  const uint32_t v_slab = slab16 * p.h_kv * 16;  // from K to V of a page
+  const auto load = [&](int nth, Step& x) {  // the nth step of the 64 whose pages are here
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const uint32_t at = min(run + h, run_hi - 1);
-      const uint32_t nth = p.run_magic != 0 ? __umulhi(at, p.run_magic) : at;
-      const int page = __builtin_amdgcn_readfirstlane(p.page_values[page_begin + nth]);
-      const int in_page = static_cast<int>(at - nth * p.runs_per_page) * kRun + c16;
-      const uint8_t* slab = p.pages + (static_cast<int64_t>(page) * 2 * p.h_kv + kvh) * slab_bytes;
-      k[h].load(slab, p.page_size, in_page, g4);
-      v[h].load(slab + p.h_kv * slab_bytes, p.page_size, in_page, g4);
+      global_bytes_t k = pool + static_cast<uint64_t>(__builtin_amdgcn_readlane(codes16[h], nth)) * 16;
+      global_bytes_t k_scales = pool + static_cast<uint64_t>(__builtin_amdgcn_readlane(scales16[h], nth)) * 16;
+      global_bytes_t v = k + v_slab, v_scales = k_scales + v_slab;
+      // kept in scalar registers: added up with the lanes' offsets first, they cost a 64-bit vector addition a load
+      asm volatile("" : "+s"(k), "+s"(v), "+s"(k_scales), "+s"(v_scales));
+      x.k[h].template load<ONCE>(k, k_scales, c16, g4);
+      x.v[h].template load<ONCE>(v, v_scales, c16, g4);
     }
-    const int t0 = run * kRun;
+  };
+  const auto work = [&](int t0, Step& x) {
     const bool whole = t0 + 2 * kRun <= first_end && (t0 >= window || t0 + 2 * kRun <= sink);  // no key of the step is masked
-    float s[2][4];
+    float4_t s[RB][2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      float4_t acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int c = 0; c < CH; ++c) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[h].values(g4, c), qf[c], acc, 0, 0, 0);
+      for (int r = 0; r < RB; ++r) s[r][h] = float4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int t = t0 + h * kRun + 4 * g4 + i;
-        s[h][i] = acc[i] * p.scale_log2;
-        if (!whole) s[h][i] = t < my_end && (t < sink || t >= window) ? s[h][i] : -INFINITY;
+      for (int c = 0; c < CH; ++c) {
+        const half8_t a = x.k[h].values(g4, c);
+#pragma unroll
+        for (int r = 0; r < RB; ++r) s[r][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qf[r][c], s[r][h], 0, 0, 0);
       }
     }
     if (!whole) {
+#pragma unroll
+      for (int r = 0; r < RB; ++r) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int t = t0 + h * kRun + 4 * g4 + i;
+            const bool sees = (t < my_end[r]) & ((t < sink) | (t >= window));
+            s[r][h][i] = sees ? s[r][h][i] : -INFINITY;
+          }
+        }
+      }
       // A weight of 0 times NaN is NaN: what no row of the item sees is read as 0, and blocks that are NaN reach
       // the rows that see them by a mark of their own.
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int t = t0 + h * kRun + c16;
-        const bool seen = t < last_end && (t < sink || t >= window);
+        const bool seen = (t < last_end) & ((t < sink) | (t >= window));
 #pragma unroll
         for (int i = 0; i < LaneRow<D>::NS; ++i) {
-          const bool nan = seen && v[h].s[i] == 255;
+          const bool nan = seen && x.v[h].s[i] == 255;
           for (uint64_t left = __ballot(nan); left != 0; left &= left - 1) {
             const int who = __ffsll(static_cast<long long>(left)) - 1;
             const int at = t0 + h * kRun + (who & 15);
-            if (at < my_end) poisoned |= 1u << LaneRow<D>::block(who >> 4, i);
+#pragma unroll
+            for (int r = 0; r < RB; ++r) {
+              if (at < my_end[r]) poisoned[r] |= 1u << LaneRow<D>::block(who >> 4, i);
+            }
           }
-          if (nan || !seen) v[h].s[i] = 0;
+          if (nan || !seen) x.v[h].s[i] = 0;
         }
-      }
-    }
-    // softmax statistics: the lane has 8 of the step's 32 keys of row c16
-    float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
-    top = fmaxf(m, max_xor32(max_xor16(top)));
-    const float alpha = fast_exp2(m - top);
-    m = top;
-    l *= alpha;
-#pragma unroll
-    for (int i = 0; i < DB; ++i) o[i] *= alpha;
-    half8_t pf;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float w = fast_exp2(s[h][i] - m);
-        l += w;
-        pf[h * 4 + i] = static_cast<half_t>(w);
       }
     }
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
 #pragma unroll
       for (int c = 0; c < CH; ++c)
-        *reinterpret_cast<half8_t*>(vt + (h * kRun + c16) * VS + LaneRow<D>::chunk(g4, c) * 8) = v[h].values(g4, c);
+        *reinterpret_cast<half8_t*>(vt + (h * kRun + c16) * VS + LaneRow<D>::chunk(g4, c) * 8) = x.v[h].values(g4, c);
+    }
+    // Weights: the lane has 8 of the step's 32 keys of its row.  The reference point only has to keep them in fp16's
+    // range: it moves when the row's maximum is 2^14 above it, to 2^-6 of that, and mostly stays after the first
+    // steps, so that O is seldom rescaled; weights far below the maximum stay out of fp16's subnormal range.
+    half8_t pf[RB];
+#pragma unroll
+    for (int r = 0; r < RB; ++r) {
+      float top = fmaxf(fmaxf(fmaxf(s[r][0][0], s[r][0][1]), fmaxf(s[r][0][2], s[r][0][3])),
+                        fmaxf(fmaxf(s[r][1][0], s[r][1][1]), fmaxf(s[r][1][2], s[r][1][3])));
+      top = max_xor32(max_xor16(top)) * p.scale_log2;
+      if (__ballot(top > m[r] + 14.f) != 0) {
+        const float to = top > m[r] + 14.f ? top - 6.f : m[r];
+        const float alpha = fast_exp2(m[r] - to);
+        m[r] = to;
+        l[r] *= alpha;
+#pragma unroll
+        for (int i = 0; i < DB; ++i) o[r][i] *= alpha;
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float w = fast_exp2(fmaf(s[r][h][i], p.scale_log2, -m[r]));
+          l[r] += w;
+          pf[r][h * 4 + i] = static_cast<half_t>(w);
+        }
+      }
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
@@ -363,92 +486,192 @@ __global__ __launch_bounds__(256) void mxfp4_attn_kernel(Mxfp4Params p) {
       const half_t* src = vt + (4 * g4 + (c16 >> 2)) * VS + i * 16 + (c16 & 3) * 4;
       const half4_t lo = lds_read_tr16(src), hi = lds_read_tr16(src + kRun * VS);
       const half8_t a = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-      o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, pf, o[i], 0, 0, 0);
+#pragma unroll
+      for (int r = 0; r < RB; ++r) o[r][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, pf[r], o[r][i], 0, 0, 0);
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
+  };
+  if (run < run_hi) {
+    // Two steps in flight, and every load is issued whether or not its step exists (past the end the last run is loaded
+    // again): with a branch around them the compiler waits for the next step's loads in front of this one's work.
+    Step x, y;
+    load(0, x);
+    int nth = 1;
+    const auto next = [&](Step& z) {
+      if (nth == 64) {
+        nth = 0;
+        load_ids(run + 8);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) asm volatile("" : "+v"(codes16[h]), "+v"(scales16[h]));  // waited for in here
+      }
+      load(nth++, z);
+    };
+    while (true) {
+      next(y);
+      work(run * kRun, x);
+      if ((run += 8) >= run_hi) break;
+      next(x);
+      work(run * kRun, y);
+      if ((run += 8) >= run_hi) break;
+    }
   }
 
   // ---- the four waves' states become one ------------------------------------------------------
-  l = sum_xor32(sum_xor16(l));
-  if (__ballot(poisoned != 0) != 0) {
-    poisoned |= __shfl_xor(poisoned, 16);
-    poisoned |= __shfl_xor(poisoned, 32);
+  const uint32_t state = ((static_cast<uint32_t>(PREFILL ? slot * p.shares + chunk : slot) * blocks + (PREFILL ? 0 : block)) * p.h_kv + kvh) * R;
+  SharedStates part_o(p.part_o), part_ml(p.part_ml);
+  const auto finish = [&](int r, int f, float most, float sum, float4_t acc) {  // elements f.. f + 3 of row r
+    const int row = row0 + r;
+    const int64_t out = static_cast<int64_t>(q_begin + row / p.group) * p.h_q + kvh * p.group + row % p.group;
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    half4_t h;
 #pragma unroll
-    for (int i = 0; i < DB; ++i) {
-      if (poisoned >> (i / 2) & 1) o[i] = float4_t{NAN, NAN, NAN, NAN};
+    for (int i = 0; i < 4; ++i) h[i] = static_cast<half_t>(acc[i] * inv);
+    *reinterpret_cast<half4_t*>(p.output + out * D + f) = h;
+    if (f == 0) p.lse[out] = sum == 0.f ? kEmptyLse : most + fast_log2(sum);
+  };
+#pragma unroll
+  for (int r = 0; r < RB; ++r) {
+    if (r * 16 >= rows_here) break;
+    if (r > 0) __syncthreads();
+    l[r] = sum_xor32(sum_xor16(l[r]));
+    if (__ballot(poisoned[r] != 0) != 0) {
+      poisoned[r] |= __shfl_xor(poisoned[r], 16);
+      poisoned[r] |= __shfl_xor(poisoned[r], 32);
+#pragma unroll
+      for (int i = 0; i < DB; ++i) {
+        if (poisoned[r] >> (i / 2) & 1) o[r][i] = float4_t{NAN, NAN, NAN, NAN};
+      }
     }
-  }
-  if (g4 == 0) {
-    sm_m[wave][c16] = m;
-    sm_l[wave][c16] = l;
-  }
-  float* const mine = reinterpret_cast<float*>(vt);
-#pragma unroll
-  for (int i = 0; i < DB; ++i) *reinterpret_cast<float4_t*>(mine + c16 * OS + i * 16 + 4 * g4) = o[i];
-  __syncthreads();
-  for (int at = threadIdx.x; at < rows_here * (D / 4); at += 256) {
-    const int r = at / (D / 4), f = at % (D / 4) * 4;
-    const float most = fmaxf(fmaxf(sm_m[0][r], sm_m[1][r]), fmaxf(sm_m[2][r], sm_m[3][r]));
-    float sum = 0.f;
-    float4_t acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const float part = fast_exp2(sm_m[w][r] - most);
-      sum += sm_l[w][r] * part;
-      acc += *reinterpret_cast<const float4_t*>(reinterpret_cast<const float*>(v_tiles[w]) + r * OS + f) * part;
+    if (g4 == 0) {
+      sm_m[wave][c16] = m[r];
+      sm_l[wave][c16] = l[r];
     }
-    const int hq = kvh * p.group + (row0 + r) % p.group;
-    if (chunks == 1) {
-      const int64_t out = static_cast<int64_t>(q_begin + (row0 + r) / p.group) * p.h_q + hq;
-      const float inv = sum == 0.f ? 0.f : 1.f / sum;
-      half4_t h;
+    float* const mine = reinterpret_cast<float*>(vt);
+    if (r * 16 + c16 < rows_here) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) h[i] = static_cast<half_t>(acc[i] * inv);
-      *reinterpret_cast<half4_t*>(p.output + out * D + f) = h;
-      if (f == 0) p.lse[out] = sum == 0.f ? kEmptyLse : most + fast_log2(sum);
-    } else {
-      const int64_t out = static_cast<int64_t>(slot) * p.h_q + hq;
-      *reinterpret_cast<float4_t*>(p.part_o + out * D + f) = acc;
-      if (f == 0) {
-        p.part_ml[out * 2] = most;
-        p.part_ml[out * 2 + 1] = sum;
+      for (int i = 0; i < DB; ++i) *reinterpret_cast<float4_t*>(mine + c16 * D + ((i * 4 + g4) ^ (c16 & 7)) * 4) = o[r][i];
+    }
+    __syncthreads();
+    for (int at = threadIdx.x; at < min(16, rows_here - r * 16) * (D / 4); at += 256) {
+      const int row = at / (D / 4), f = at % (D / 4) * 4;
+      const float most = fmaxf(fmaxf(sm_m[0][row], sm_m[1][row]), fmaxf(sm_m[2][row], sm_m[3][row]));
+      float sum = 0.f;
+      float4_t acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float part = fast_exp2(sm_m[w][row] - most);
+        sum += sm_l[w][row] * part;
+        acc += *reinterpret_cast<const float4_t*>(reinterpret_cast<const float*>(v_tiles[w]) + row * D + (f / 4 ^ (row & 7)) * 4) * part;
+      }
+      if (chunks == 1) {
+        finish(r * 16 + row, f, most, sum, acc);
+      } else {
+        const uint32_t out = state + r * 16 + row;
+        part_o.store4(out * D + f, acc);
+        if (f == 0) part_ml.store2(out * 2, most, sum);
       }
     }
   }
-}
+  if (chunks == 1) return;
 
-// Joins the chunks of a sequence's row: one wave per (sequence, query head).
-template <int D>
-__global__ __launch_bounds__(256) void mxfp4_merge_kernel(Mxfp4Params p) {
-  const int lane = threadIdx.x & 63;
-  const int row = blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (row >= p.batch * p.h_q) return;
-  const int b = row / p.h_q;
-  const int hq = row % p.h_q;
-  const int num_pages = p.page_indptr[b + 1] - p.page_indptr[b];
-  const int stored = num_pages > 0 ? (num_pages - 1) * p.page_size + p.last_page_len[b] : 0;
-  const int chunks = ((stored + kRun - 1) / kRun + p.chunk_runs - 1) / p.chunk_runs;
-  if (chunks <= 1) return;  // the attention kernel wrote the row
-  const int64_t first = static_cast<int64_t>(chunk_begin(p, b)) * p.h_q + hq;
-  float most = kNoKey;
-  for (int c = 0; c < chunks; ++c) most = fmaxf(most, p.part_ml[(first + static_cast<int64_t>(c) * p.h_q) * 2]);
-  float sum = 0.f, acc[(D + 63) / 64] = {};
-  for (int c = 0; c < chunks; ++c) {
-    const int64_t at = first + static_cast<int64_t>(c) * p.h_q;
-    const float part = fast_exp2(p.part_ml[at * 2] - most);
-    sum += p.part_ml[at * 2 + 1] * part;
+  // ---- the work item that comes last joins the states of its rows' items ------------------------
+  // Without device-scope fences, which write back and invalidate a whole L2: the states are stored at device scope,
+  // every wave waits for its own stores, one thread counts the workgroup in.
+  wait_vmcnt<0>();
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    // the counter goes back to 0 by itself when the last one arrives
+    unsigned* counter = p.arrivals + (PREFILL ? slot : b * blocks + block) * p.h_kv + kvh;
+    sm_last = __builtin_amdgcn_atomic_inc32(counter, chunks - 1, __ATOMIC_RELAXED, "agent") == static_cast<unsigned>(chunks - 1);
+  }
+  __syncthreads();
+  if (!sm_last) return;
+  // 64 states at a time: a wave has a row's reference points and sums, a state a lane, and leaves their weights in LDS;
+  // then every thread adds up four elements of a row, of all states or, where the rows leave threads over, of some.  What
+  // this costs is round trips to memory (device-scope loads miss this XCD's L2), so that many loads are on their way
+  // together, those of the outputs beside those of the statistics.
+  constexpr int ITEMS = (R * (D / 4) + 255) / 256;
+  constexpr int BATCH = 8;
+  float* const weight = reinterpret_cast<float*>(v_tiles[0]);  // (R, 64)
+  float* const row_most = weight + R * 64;                     // then the factor of what has been added up, then the sum
+  float4_t* const partial = reinterpret_cast<float4_t*>(row_most + 4 * R);  // (256)
+  static_assert(sizeof(v_tiles) >= kJoinBytes, "they take the V tiles' place");
+  const uint32_t stride = static_cast<uint32_t>(blocks) * p.h_kv * R;  // states between neighbouring chunks
+  const uint32_t first = state - chunk * stride;
+  const int items = rows_here * (D / 4);
+  const int span = items <= 32 ? 32 : items <= 64 ? 64 : items <= 128 ? 128 : 256;  // threads that share a state
+  const int parts = 256 / span, part = threadIdx.x / span, item0 = threadIdx.x % span;
+  float4_t acc[ITEMS];
 #pragma unroll
-    for (int i = 0; i < (D + 63) / 64; ++i) {
-      if (i * 64 + lane < D) acc[i] += p.part_o[at * D + i * 64 + lane] * part;
+  for (int i = 0; i < ITEMS; ++i) acc[i] = float4_t{0.f, 0.f, 0.f, 0.f};
+  for (int c0 = 0; c0 < chunks; c0 += 64) {
+    const int here = min(64, chunks - c0);
+    const int per_part = (here + parts - 1) / parts;
+    const int c_lo = part * per_part, c_hi = min(here, c_lo + per_part);
+    float4_t v[BATCH];
+    const auto load_batch = [&](int item, int c) {
+      const int row = item / (D / 4), f = item % (D / 4) * 4;
+      const uint32_t src = (first + c0 * stride + row) * D + f;
+#pragma unroll
+      for (int j = 0; j < BATCH; ++j) {
+        if (j % 4 == 0 && c + j >= c_hi) break;
+        v[j] = part_o.load4(src + min(c + j, here - 1) * stride * D);
+      }
+    };
+    if (item0 < items && c_lo < c_hi) load_batch(item0, c_lo);
+    float2 ml[R / 4];
+#pragma unroll
+    for (int i = 0; i < R / 4; ++i) {
+      const int row = wave + 4 * i;
+      ml[i] = make_float2(kNoKey, 0.f);
+      if (row < rows_here && lane < here) ml[i] = part_ml.load2((first + (c0 + lane) * stride + row) * 2);
     }
-  }
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
-  for (int i = 0; i < (D + 63) / 64; ++i) {
-    if (i * 64 + lane < D) p.output[static_cast<int64_t>(row) * D + i * 64 + lane] = static_cast<half_t>(acc[i] * inv);
+    for (int i = 0; i < R / 4; ++i) {
+      const int row = wave + 4 * i;
+      if (row >= rows_here) break;
+      const float old = c0 == 0 ? kNoKey : row_most[row];
+      const float most = fmaxf(wave_max(ml[i].x), old);
+      const float w = fast_exp2(ml[i].x - most), rescale = fast_exp2(old - most);
+      weight[row * 64 + lane] = w;
+      const float sum = sum_xor32(sum_xor16(group_sum<16>(ml[i].y * w))) + (c0 == 0 ? 0.f : row_most[2 * R + row] * rescale);
+      if (lane == 0) {
+        row_most[row] = most;
+        row_most[R + row] = rescale;
+        row_most[2 * R + row] = sum;
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      const int item = item0 + i * 256;
+      if (item >= items) break;
+      const int row = item / (D / 4);
+      acc[i] *= row_most[R + row];
+      for (int c = c_lo; c < c_hi; c += BATCH) {
+        if (i > 0 || c > c_lo) load_batch(item, c);
+#pragma unroll
+        for (int j = 0; j < BATCH; ++j) {
+          if (c + j < c_hi) acc[i] += v[j] * weight[row * 64 + c + j];
+        }
+      }
+    }
+    __syncthreads();
   }
-  if (lane == 0) p.lse[row] = sum == 0.f ? kEmptyLse : most + fast_log2(sum);
+  if (parts > 1) {
+    partial[threadIdx.x] = acc[0];
+    __syncthreads();
+    if (part > 0) return;
+    for (int i = 1; i < parts; ++i) acc[0] += partial[threadIdx.x + i * span];
+  }
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) {
+    const int item = item0 + i * 256;
+    if (item >= items) break;
+    const int row = item / (D / 4);
+    finish(row, item % (D / 4) * 4, row_most[row], row_most[2 * R + row], acc[i]);
+  }
 }
 
 static void check_mxfp4(const char* what, int32_t h_kv, int32_t page_size, int32_t d) {
@@ -467,22 +690,143 @@ static dim3 blocks_for(const char* what, int64_t threads) {
   return dim3(static_cast<unsigned>(blocks));
 }
 
-template <class Launch>
-static void for_head_dim(int d, Launch&& launch) {
-  switch (d) {
-    case 64: launch(std::integral_constant<int, 64>{}); break;
-    case 96: launch(std::integral_constant<int, 96>{}); break;
-    case 128: launch(std::integral_constant<int, 128>{}); break;
-    default: launch(std::integral_constant<int, 256>{}); break;
+// Work items that the chip holds at once.
+static int64_t resident_items(int cus, int d, int row_blocks) { return static_cast<int64_t>(mxfp4_waves(d, row_blocks)) * cus; }
+
+template <bool PREFILL, int D>
+static void launch_rows(const Mxfp4Params& p, int row_blocks, dim3 grid, hipStream_t s) {
+  // (prefill: a sequence with more rows than an item has several of them for a key)
+  const bool once = !PREFILL && p.row_blocks == 1;
+  const auto launch = [&](auto blocks) {
+    constexpr int RB = decltype(blocks)::value;
+    if constexpr (!PREFILL) {
+      if (once) {
+        hipLaunchKernelGGL((mxfp4_attn_kernel<D, RB, PREFILL, true>), grid, dim3(256), 0, s, p);
+        return;
+      }
+    }
+    hipLaunchKernelGGL((mxfp4_attn_kernel<D, RB, PREFILL, false>), grid, dim3(256), 0, s, p);
+  };
+  if (row_blocks == 1) launch(std::integral_constant<int, 1>{});
+  if (row_blocks == 2) launch(std::integral_constant<int, 2>{});
+  if constexpr (D <= 128) {
+    if (row_blocks == 3) launch(std::integral_constant<int, 3>{});
   }
+  KV_LAUNCH_CHECK();
+}
+
+template <bool PREFILL>
+static void launch_attention(const Mxfp4Params& p, int d, int row_blocks, dim3 grid, hipStream_t s) {
+  switch (d) {
+    case 64: return launch_rows<PREFILL, 64>(p, row_blocks, grid, s);
+    case 96: return launch_rows<PREFILL, 96>(p, row_blocks, grid, s);
+    case 128: return launch_rows<PREFILL, 128>(p, row_blocks, grid, s);
+    default: return launch_rows<PREFILL, 256>(p, row_blocks, grid, s);
+  }
+}
+
+// Scratch memory of a launch: arrival counters (0 when it is allocated and after every launch), then the states.
+constexpr int64_t kMaxCounters = 1 << 18;
+static bool states_fit(int64_t states, int d) { return states * d < int64_t{1} << 30; }  // 32-bit addresses of bytes
+static ScratchLease lease_states(const char* what, Mxfp4Params& p, hipStream_t s, int64_t states, int d) {
+  if (states == 0) return {};  // no row's keys are shared
+  KV_CHECK(states_fit(states, d)) << what << ": too many work items";
+  constexpr size_t counter_bytes = kMaxCounters * sizeof(unsigned);
+  const size_t o_bytes = static_cast<size_t>(states) * d * sizeof(float);
+  ScratchLease ws = lease_scratch(kScratchMxfp4, s, counter_bytes + o_bytes + static_cast<size_t>(states) * 2 * sizeof(float), counter_bytes);
+  p.arrivals = reinterpret_cast<unsigned*>(ws.ptr);
+  p.part_o = reinterpret_cast<float*>(ws.ptr + counter_bytes);
+  p.part_ml = reinterpret_cast<float*>(ws.ptr + counter_bytes + o_bytes);
+  return ws;
+}
+
+// Blocks of 16 rows that a work item of a decode launch takes (three are what fits the registers at two waves a SIMD; head
+// dim 256: two at one): for few keys one, which starts and ends sooner; where they fill the chip the fewest items for the
+// group, of equal size.  32 sequences of U[1000,3000] tokens, 32 heads on one: 14.2 us with one block, 17.4 with two; 64 of
+// U[20000,40000]: 102 and 74.
+static int decode_row_blocks(int cus, int64_t group, int64_t runs, int64_t h_kv, int d) {
+  const int64_t blocks = (group + 15) / 16, most = d == 256 ? 2 : 3;
+  const int64_t items = (blocks + most - 1) / most;
+  const int64_t fewest = (blocks + items - 1) / items;
+  return runs * h_kv > 24 * resident_items(cus, d, static_cast<int>(fewest)) ? static_cast<int>(fewest) : 1;
+}
+
+// Keys of a work item in runs, a multiple of 8 (a step of its four waves), from shapes alone: `avg` runs a sequence, per_slot
+// items for the same keys, `resident` items that the chip holds at once.
+//  * Never under sqrt(2 avg): a step takes a work item 0.47 us on an idle chip, a further state its row 0.12 us.
+//  * Small launches, whose items can all start at once with half of the chip's room to themselves: that many.
+//  * Long sequences: all of that room, once.
+//  * Between them sequences of unlike lengths leave workgroups over at the end: about three items a sequence.
+// Measured in us, 32 / 8 heads of dim 128 unless said, runs an item -> time, * = this rule:
+//   1 x 2000 tokens       8: 8.7   16*: 8.4   32: 9.3   64: 11.9       1 x 32768    32: 19.1  64*: 16.1  128: 18.9
+//   1 x 131072           64: 39.8  128*: 33.8  256: 33.3               8 x U[2000,6000]      16: 15.9  40*: 13.6  96: 15.3
+//   16 x U[100,4000]     16: 16.0  48*: 14.7  96: 17.7  256: 25.6      64 x U[64,512]  16: 13.5  96*: 10.9  256: 11.0
+//   64 x U[1024,8192]    32: 69.8  64: 63.6  96*: 58.9  256: 72.8      8 x U[32768,131072], 64 / 8   96: 140  328*: 124
+//   32 x U[1000,3000], 32 / 1   8: 30.5  24*: 17.2  64: 19.8           20 x U[1500,2500], 16 / 2 of dim 256   8: 25.8  24*: 15.2
+static int64_t pick_chunk_runs(int64_t runs, int64_t batch, int64_t per_slot, int64_t resident) {
+  const int64_t forced = option(kOptDecodeChunkPages);
+  if (forced >= 8 && forced % 8 == 0) return forced;
+  const auto steps = [](int64_t n) { return std::max<int64_t>((n + 7) / 8 * 8, 8); };
+  const auto for_items = [&](int64_t items) {  // the shortest that leaves at most so many items
+    const int64_t slots = items / per_slot - batch;
+    return slots > 0 ? steps((runs + slots - 1) / slots) : runs + 8;
+  };
+  const int64_t avg = runs / batch;
+  const int64_t least = steps(static_cast<int64_t>(std::sqrt(2.0 * static_cast<double>(avg))));
+  const int64_t small = for_items(resident / 2), full = for_items(resident);
+  int64_t chunk = std::max<int64_t>(96, steps(avg / 3));
+  if (small <= 48) chunk = std::max(small, least);
+  else if (avg >= 4 * full) chunk = std::max(full, least);
+  return std::min<int64_t>(chunk, 1 << 20);
+}
+
+// How a prefill launch is cut, from shapes alone: blocks of 16 rows that a work item takes, and work items that share the keys
+// of a row block.  An item turns a key's codes into fp16 once for all of its rows, so that more blocks are faster where the
+// chip is full (8 chunks of 2048 tokens on 4096 + 2048 keys, 32 / 8 heads of dim 128, TFLOP/s at 1 / 2 / 3 blocks: 660 / 838 /
+// 949; of dim 64: 512 / 682 / 730; 8 / 4 heads of dim 256: 471 / 540), and slower where it is not (40 tokens on 4000:
+// 20.3 / 22.2 / 25.9 us).  What the rows of a sequence, the rounds that the items take and the steps of an item come to is
+// estimated in us: an item's start and end 4 + 2 a block, a step t_idle to t_full with the room that is taken (measured), the
+// join of the shares.
+struct Cut {
+  int row_blocks;
+  int shares;
+};
+static Cut cut_prefill(int cus, int64_t rows, int64_t batch, int64_t h_kv, int64_t runs, int d) {
+  const double t_full[4][3] = {{1.05, 1.18, 1.10}, {1.35, 1.23, 1.40}, {1.63, 1.28, 1.70}, {2.28, 2.00, 0}};
+  const int64_t forced = option(kOptPrefillKvSplits);
+  const int64_t sequence = (rows + batch - 1) / batch;  // rows of one
+  Cut best = {1, 1};
+  double least = 1e30;
+  for (int blocks = 1; blocks <= (d == 256 ? 2 : 3); ++blocks) {
+    const int64_t items = (sequence + 16 * blocks - 1) / (16 * blocks) * batch * h_kv;
+    const int64_t resident = resident_items(cus, d, blocks);
+    const double idle = (0.35 + 0.15 * blocks) * (d == 256 ? 1.6 : 1.0);
+    const double full = t_full[d == 64 ? 0 : d == 96 ? 1 : d == 128 ? 2 : 3][blocks - 1];
+    const int64_t most = forced > 0 ? forced : items >= 2 * resident ? 1 : std::min<int64_t>(std::max<int64_t>(runs / 8, 1), 64);
+    for (int64_t n = forced > 0 ? forced : 1; n <= most; ++n) {
+      const double rounds = static_cast<double>((items * n + resident - 1) / resident);
+      const double room = std::min(1.0, static_cast<double>(items * n) / static_cast<double>(resident));
+      const double step = idle + (full - idle) * room;
+      const double steps = static_cast<double>((runs + 8 * n - 1) / (8 * n));
+      const double us = rounds * (4.0 + 2.0 * blocks + step * steps) + (n > 1 ? 1.5 + 0.12 * blocks * static_cast<double>(n) : 0.0);
+      if (us < least) {
+        least = us;
+        best = {blocks, static_cast<int>(n)};
+      }
+    }
+  }
+  return best;
 }
 
 static Mxfp4Params attn_params(const char* what, const void* q, const void* pages, const int32_t* page_indptr,
                                const int32_t* page_values, const int32_t* length_info, void* output, float* lse, double sm_scale,
-                               int32_t batch, int64_t nnz_pages, int32_t h_q, int32_t h_kv, int32_t d, int32_t page_size,
-                               int32_t sliding_window) {
+                               int32_t batch, int64_t nnz_pages, int64_t num_pages, int32_t h_q, int32_t h_kv, int32_t d,
+                               int32_t page_size, int32_t sliding_window) {
   KV_CHECK(batch >= 0 && nnz_pages >= 0 && h_q > 0 && h_kv > 0 && h_q % h_kv == 0) << what << ": bad shape";
   check_mxfp4(what, h_kv, page_size, d);
+  // 36-bit addresses within the pool; K of a page is less than 4 GiB in front of its V
+  const double page_bytes = 2.0 * h_kv * page_size * (17 * d / 32);
+  KV_UNSUPPORTED(num_pages * page_bytes >= 68719476736.0 || page_bytes >= 8589934592.0) << what << ": a pool of 64 GiB or more is not built";
   Mxfp4Params p = {};
   p.q = static_cast<const half_t*>(q);
   p.pages = static_cast<const uint8_t*>(pages);
@@ -497,11 +841,13 @@ static Mxfp4Params attn_params(const char* what, const void* q, const void* page
   p.h_q = h_q;
   p.h_kv = h_kv;
   p.group = h_q / h_kv;
-  p.row_blocks = (p.group + 15) / 16;
   p.page_size = page_size;
   p.runs_per_page = page_size / kRun;
   p.run_magic = p.runs_per_page == 1 ? 0 : static_cast<uint32_t>(((uint64_t{1} << 32) + p.runs_per_page - 1) / p.runs_per_page);
-  p.scale_log2 = static_cast<float>(sm_scale) * kLog2e;
+  // The kernel takes maxima of scores that are not scaled yet and masks with -inf: a scale below 0 goes to q, and one of
+  // 0 (all weights equal) becomes one that is as good as 0.
+  p.scale_log2 = std::max(std::fabs(static_cast<float>(sm_scale)) * kLog2e, 1e-30f);
+  p.q_sign = sm_scale < 0 ? 0x80008000u : 0;
   return p;
 }
 
@@ -550,30 +896,24 @@ int tvmkv_mxfp4_batch_decode_paged_kv(const void* q, const void* pages, const in
   KV_API_BEGIN();
   const char* const what = "mxfp4_batch_decode_paged_kv";
   Mxfp4Params p = attn_params(what, q, pages, page_indptr, page_values, length_info, output, lse, sm_scale, batch_size, nnz_pages,
-                              h_q, h_kv, head_dim, page_size, sliding_window);
+                              num_pages, h_q, h_kv, head_dim, page_size, sliding_window);
   if (batch_size == 0) return TVMKV_OK;
   KV_CHECK(q && pages && page_indptr && length_info && output && lse) << what << ": NULL tensor";
   KV_CHECK(nnz_pages == 0 || page_values) << what << ": NULL page table";
   check_aligned(what, {q, pages, output});
-  // chunks: about six work items for every compute unit, at least one step of the four waves
+  const int cus = compute_units();
   const int64_t runs = nnz_pages * p.runs_per_page;
-  const int64_t wanted = std::max<int64_t>(1, 6 * compute_units() / (static_cast<int64_t>(h_kv) * p.row_blocks));
-  p.chunk_runs = static_cast<int>(std::min<int64_t>(std::max<int64_t>((runs + wanted - 1) / wanted, 8) + 7, 1 << 20) / 8 * 8);
+  const int row_blocks = decode_row_blocks(cus, p.group, runs, h_kv, head_dim), rows = 16 * row_blocks;
+  p.row_blocks = (p.group + rows - 1) / rows;
+  const int64_t per_slot = static_cast<int64_t>(h_kv) * p.row_blocks;
+  KV_CHECK(runs < (int64_t{1} << 31)) << what << ": too many pages";
+  p.chunk_runs = batch_size * per_slot > kMaxCounters ? 1 << 30
+                                                      : static_cast<uint32_t>(pick_chunk_runs(runs, batch_size, per_slot, resident_items(cus, head_dim, row_blocks)));
   const int64_t slots = runs / p.chunk_runs + batch_size;
-  const int64_t items = slots * h_kv * p.row_blocks;
-  KV_CHECK(items < (int64_t{1} << 31)) << what << ": too many work items";
+  KV_CHECK(slots * per_slot < (int64_t{1} << 31)) << what << ": too many work items";
   const hipStream_t s = as_stream(stream);
-  const size_t o_bytes = static_cast<size_t>(slots) * h_q * head_dim * sizeof(float);
-  const ScratchLease ws = lease_scratch(kScratchMxfp4, s, o_bytes + static_cast<size_t>(slots) * h_q * 2 * sizeof(float), 0);
-  p.part_o = reinterpret_cast<float*>(ws.ptr);
-  p.part_ml = reinterpret_cast<float*>(ws.ptr + o_bytes);
-  for_head_dim(head_dim, [&](auto dim) {
-    constexpr int D = decltype(dim)::value;
-    hipLaunchKernelGGL((mxfp4_attn_kernel<D, false>), dim3(static_cast<unsigned>(items)), dim3(256), 0, s, p);
-    KV_LAUNCH_CHECK();
-    hipLaunchKernelGGL(mxfp4_merge_kernel<D>, dim3((batch_size * h_q + 3) / 4), dim3(256), 0, s, p);
-    KV_LAUNCH_CHECK();
-  });
+  const ScratchLease ws = lease_states(what, p, s, runs > p.chunk_runs ? slots * per_slot * rows : 0, head_dim);
+  launch_attention<false>(p, head_dim, row_blocks, dim3(static_cast<unsigned>(slots * per_slot)), s);
   KV_API_END();
 }
 
@@ -585,7 +925,7 @@ int tvmkv_mxfp4_batch_prefill_paged_kv(const void* q, const int32_t* q_indptr, c
   KV_API_BEGIN();
   const char* const what = "mxfp4_batch_prefill_paged_kv";
   Mxfp4Params p = attn_params(what, q, pages, page_indptr, page_values, length_info, output, lse, sm_scale, batch_size, nnz_pages,
-                              h_q, h_kv, head_dim, page_size, sliding_window);
+                              num_pages, h_q, h_kv, head_dim, page_size, sliding_window);
   KV_CHECK(total_q >= 0) << what << ": bad shape";
   if (batch_size == 0 || total_q == 0) return TVMKV_OK;
   KV_CHECK(q && q_indptr && pages && page_indptr && length_info && output && lse) << what << ": NULL tensor";
@@ -593,14 +933,15 @@ int tvmkv_mxfp4_batch_prefill_paged_kv(const void* q, const int32_t* q_indptr, c
   check_aligned(what, {q, pages, output});
   p.q_indptr = q_indptr;
   p.causal = causal != 0;
-  const int64_t items = (total_q * p.group / 16 + batch_size) * h_kv;
-  KV_CHECK(items < (int64_t{1} << 31)) << what << ": too many work items";
   const hipStream_t s = as_stream(stream);
-  for_head_dim(head_dim, [&](auto dim) {
-    constexpr int D = decltype(dim)::value;
-    hipLaunchKernelGGL((mxfp4_attn_kernel<D, true>), dim3(static_cast<unsigned>(items)), dim3(256), 0, s, p);
-    KV_LAUNCH_CHECK();
-  });
+  const Cut cut = cut_prefill(compute_units(), total_q * p.group, batch_size, h_kv, nnz_pages * p.runs_per_page / batch_size, head_dim);
+  const int row_blocks = cut.row_blocks, rows = 16 * row_blocks;
+  const int64_t slots = total_q * p.group / rows + batch_size;
+  KV_CHECK(slots * h_kv < (int64_t{1} << 31)) << what << ": too many work items";
+  p.shares = cut.shares;
+  if (slots * h_kv > kMaxCounters || !states_fit(slots * p.shares * h_kv * rows, head_dim)) p.shares = 1;
+  const ScratchLease ws = lease_states(what, p, s, p.shares > 1 ? slots * p.shares * h_kv * rows : 0, head_dim);
+  launch_attention<true>(p, head_dim, row_blocks, dim3(static_cast<unsigned>(slots * h_kv), 1, p.shares), s);
   KV_API_END();
 }
 

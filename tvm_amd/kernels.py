@@ -293,42 +293,54 @@ def mxfp4_pages(num_pages, h_kv, page_size, head_dim, device="cuda"):
     return torch.zeros((num_pages, 2, h_kv, page_size, 17 * head_dim // 32), dtype=torch.uint8, device=device)
 
 
+# These calls take a few microseconds on the device, so that their checks are written to be cheap: one pass over the tensors
+# of a kind, shapes compared as they are, addresses as integers.
+
+
+# (torch.cuda.current_stream builds an object first, 2.8 us; the handle alone takes 0.1)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", lambda device: torch.cuda.current_stream(device).cuda_stream)
+
+
+def _mxfp4_call(entry, tensors, *rest):
+    for t in tensors:
+        if not t.is_cuda or not t.is_contiguous():
+            _p(t)  # refuses it
+    check(entry(*[t.data_ptr() for t in tensors], *rest, _raw_stream(tensors[0].get_device())))
+
+
 def _mxfp4_pool(pages, head_dim):
+    shape = pages.shape
     if pages.dtype != torch.uint8:
         raise KVError(-1, f"pages of 4-bit rows must be uint8, got {pages.dtype}")
-    if pages.dim() != 5 or pages.shape[1] != 2 or pages.shape[4] * 32 != 17 * head_dim:
-        raise KVError(-1, f"pages has shape {tuple(pages.shape)}, expected (num_pages, 2, h_kv, page_size, 17 * {head_dim} / 32)")
-    num_pages, _, hkv, ps, _ = pages.shape
-    return num_pages, hkv, ps
+    if len(shape) != 5 or shape[1] != 2 or shape[4] * 32 != 17 * head_dim:
+        raise KVError(-1, f"pages has shape {tuple(shape)}, expected (num_pages, 2, h_kv, page_size, 17 * {head_dim} / 32)")
+    return shape
 
 
-def _shape(t, name, *expected):
-    if tuple(t.shape) != expected:
+def _shape(t, name, expected):
+    if t.shape != expected:
         raise KVError(-1, f"{name} has shape {tuple(t.shape)}, expected {expected}")
+
+
+def _mxfp4_rows(entry, pages, k_data, v_data, position_map, tensors):
+    _f16(k_data, v_data)
+    _i32(position_map)
+    d = k_data.shape[-1]
+    num_pages, _, hkv, ps, _ = _mxfp4_pool(pages, d)
+    n = position_map.shape[0]
+    _shape(k_data, "k_data", (n, hkv, d))
+    _shape(v_data, "v_data", (n, hkv, d))
+    _mxfp4_call(entry, tensors, n, num_pages, hkv, ps, d)
 
 
 def mxfp4_append(pages, k_data, v_data, position_map):
     """Quantises the rows k_data, v_data (tokens, h_kv, head_dim) into the slots position_map (negative: none)."""
-    _f16(k_data, v_data)
-    _i32(position_map)
-    d = k_data.shape[-1]
-    num_pages, hkv, ps = _mxfp4_pool(pages, d)
-    n = position_map.shape[0]
-    _shape(k_data, "k_data", n, hkv, d)
-    _shape(v_data, "v_data", n, hkv, d)
-    check(lib().tvmkv_mxfp4_append(_p(pages), _p(k_data), _p(v_data), _p(position_map), n, num_pages, hkv, ps, d, _stream()))
+    _mxfp4_rows(lib().tvmkv_mxfp4_append, pages, k_data, v_data, position_map, (pages, k_data, v_data, position_map))
 
 
 def mxfp4_read_kv(pages, position_map, k_data, v_data):
     """The rows of the slots position_map as fp16, into k_data and v_data (tokens, h_kv, head_dim)."""
-    _f16(k_data, v_data)
-    _i32(position_map)
-    d = k_data.shape[-1]
-    num_pages, hkv, ps = _mxfp4_pool(pages, d)
-    n = position_map.shape[0]
-    _shape(k_data, "k_data", n, hkv, d)
-    _shape(v_data, "v_data", n, hkv, d)
-    check(lib().tvmkv_mxfp4_read_kv(_p(pages), _p(position_map), _p(k_data), _p(v_data), n, num_pages, hkv, ps, d, _stream()))
+    _mxfp4_rows(lib().tvmkv_mxfp4_read_kv, pages, k_data, v_data, position_map, (pages, position_map, k_data, v_data))
 
 
 def _mxfp4_attention(q, pages, page_indptr, page_values, length_info, output, lse):
@@ -337,28 +349,28 @@ def _mxfp4_attention(q, pages, page_indptr, page_values, length_info, output, ls
     if lse.dtype != torch.float32:
         raise KVError(-1, f"lse must be float32, got {lse.dtype}")
     rows, hq, d = q.shape
-    num_pages, hkv, ps = _mxfp4_pool(pages, d)
+    num_pages, _, hkv, ps, _ = _mxfp4_pool(pages, d)
     batch = page_indptr.shape[0] - 1
-    _shape(output, "output", rows, hq, d)
-    _shape(lse, "lse", rows, hq)
-    _shape(length_info, "length_info", *((3, batch) if length_info.dim() == 2 else (batch,)))
-    return rows, hq, d, num_pages, hkv, ps, batch
+    _shape(output, "output", (rows, hq, d))
+    _shape(lse, "lse", (rows, hq))
+    sliding = length_info.dim() == 2
+    _shape(length_info, "length_info", (3, batch) if sliding else (batch,))
+    return rows, batch, (page_values.shape[0], num_pages, hq, hkv, d, ps, int(sliding))
 
 
 def mxfp4_batch_decode_paged_kv(q, pages, page_indptr, page_values, length_info, output, lse, sm_scale):
     """batch_decode_paged_kv over 4-bit pages: one query token a sequence, keys stored rotated."""
-    rows, hq, d, num_pages, hkv, ps, batch = _mxfp4_attention(q, pages, page_indptr, page_values, length_info, output, lse)
-    _shape(q, "q", batch, hq, d)
-    check(lib().tvmkv_mxfp4_batch_decode_paged_kv(
-        _p(q), _p(pages), _p(page_indptr), _p(page_values), _p(length_info), _p(output), _p(lse), float(sm_scale), batch,
-        page_values.shape[0], num_pages, hq, hkv, d, ps, int(length_info.dim() == 2), _stream()))
+    rows, batch, sizes = _mxfp4_attention(q, pages, page_indptr, page_values, length_info, output, lse)
+    if rows != batch:
+        raise KVError(-1, f"q has shape {tuple(q.shape)}, expected {(batch,) + tuple(q.shape[1:])}")
+    _mxfp4_call(lib().tvmkv_mxfp4_batch_decode_paged_kv, (q, pages, page_indptr, page_values, length_info, output, lse), sm_scale,
+                batch, *sizes)
 
 
 def mxfp4_batch_prefill_paged_kv(q, q_indptr, pages, page_indptr, page_values, length_info, output, lse, causal, sm_scale):
     """batch_prefill_paged_kv over 4-bit pages: q_indptr (batch + 1) query tokens of each sequence, keys stored rotated."""
-    rows, hq, d, num_pages, hkv, ps, batch = _mxfp4_attention(q, pages, page_indptr, page_values, length_info, output, lse)
+    rows, batch, sizes = _mxfp4_attention(q, pages, page_indptr, page_values, length_info, output, lse)
     _i32(q_indptr)
-    _shape(q_indptr, "q_indptr", batch + 1)
-    check(lib().tvmkv_mxfp4_batch_prefill_paged_kv(
-        _p(q), _p(q_indptr), _p(pages), _p(page_indptr), _p(page_values), _p(length_info), _p(output), _p(lse), int(causal),
-        float(sm_scale), batch, rows, page_values.shape[0], num_pages, hq, hkv, d, ps, int(length_info.dim() == 2), _stream()))
+    _shape(q_indptr, "q_indptr", (batch + 1,))
+    _mxfp4_call(lib().tvmkv_mxfp4_batch_prefill_paged_kv, (q, q_indptr, pages, page_indptr, page_values, length_info, output, lse),
+                causal, sm_scale, batch, rows, *sizes)
