@@ -148,51 +148,93 @@ struct Mxfp4Params {
   int page_size;
   uint32_t runs_per_page;
   uint32_t run_magic;  // 2^32 / runs_per_page, rounded up (0: 1)
-  uint32_t chunk_runs;  // decode: keys of a work item, in runs; a multiple of 8
+  uint32_t chunk_runs;  // decode: most keys of a work item, in runs; a multiple of 8
   int shares;           // prefill: work items that share the keys of a row block
   float scale_log2;     // > 0: |sm_scale| log2(e), never 0
   uint32_t q_sign;      // of sm_scale, at the sign bits of two fp16
 };
 
-// First work item of a sequence whose first page is page_indptr[i] == first.  Decode: with it sequence i has chunks for all
-// tokens that its pages could hold (the launcher makes sure that the runs of all pages are a 31-bit number).  Prefill:
-// q_indptr[i] == first, and it has blocks for all of its rows.
-__device__ __forceinline__ int chunk_begin(const Mxfp4Params& p, int i, int first) {
-  return static_cast<int>(static_cast<uint32_t>(first) * p.runs_per_page / p.chunk_runs) + i;
-}
-template <int R>
-__device__ __forceinline__ int block_begin(const Mxfp4Params& p, int i, int first) {
-  return static_cast<int>(static_cast<int64_t>(first) * p.group / R) + i;
+// Sum of x over the lanes up to this one.
+__device__ __forceinline__ int prefix_sum(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // from 1, 2, 4 and 8 lanes below in the row of 16
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // the row below's last to rows 1 and 3
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // lane 31's to rows 2 and 3
+  return x;
 }
 
-// The sequence of a work item, and what the arrays hold for it.  begin(i) increases with i: the wave looks for the last
-// sequence with begin(i) <= slot, 64 at a time, and the lanes of the last round fetch the other values along with it, so
-// that up to 64 sequences take one round trip to memory.
+// The sequence of a work item, and what the arrays hold for it.  Sequence i has items_of(entries of indptr i, i + 1) work
+// items, one behind the other without gaps: the launch has more workgroups than items, since only the device knows the
+// lengths, and spare ones between the others put the real ones on some of the compute units (64 sequences of 4096 tokens, 512
+// items: 79 us with a spare one beside every real one, 50 without).  The wave adds the items up, a sequence a lane, or up
+// to 8 neighbours a lane; with more sequences each has a fixed range of items instead, spare_begin(i, indptr[i]) onwards, and
+// the wave looks for the last that begins at or before the slot.
 struct Sequence {
   int index, begin;  // begin: its first work item
   int page_begin, num_pages, last_page_len, sink, window;
   int q_begin, q_len;
 };
-template <bool PREFILL, class Begin>
-__device__ __forceinline__ Sequence sequence_of(const Mxfp4Params& p, int slot, int lane, Begin begin) {
+template <bool PREFILL, class Items, class Begin>
+__device__ __forceinline__ Sequence sequence_of(const Mxfp4Params& p, int slot, int lane, Items items_of, Begin spare_begin) {
   const int32_t* const indptr = PREFILL ? p.q_indptr : p.page_indptr;
-  int lo = 0, n = p.batch;
-  while (n > 64) {
-    const int stride = (n + 63) >> 6;
-    const int at = lo + lane * stride;
-    const bool hit = at < lo + n && begin(at, indptr[at]) <= slot;
-    const int first = lo + (__popcll(__ballot(hit)) - 1) * stride;
-    n = min(stride, lo + n - first);
-    lo = first;
+  int at, begin, who;  // who: the lane that has the sequence's values
+  bool found = true;
+  if (p.batch > 64) {
+    if (p.batch <= 512) {
+      const int each = (p.batch + 63) >> 6;
+      int x[9], count = 0;
+#pragma unroll
+      for (int j = 0; j <= 8; ++j) x[j] = indptr[min(lane * each + min(j, each), p.batch)];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) count += j < each && lane * each + j < p.batch ? items_of(x[j], x[j + 1]) : 0;
+      const int upto = prefix_sum(count);
+      const int lanes = __popcll(__ballot(upto <= slot));
+      found = lanes < 64;
+      const int owner = min(lanes, 63);
+      begin = __builtin_amdgcn_readlane(upto - count, owner);
+      int n = owner * each;
+      bool here = false;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int count_j = items_of(__builtin_amdgcn_readlane(x[j], owner), __builtin_amdgcn_readlane(x[j + 1], owner));
+        here |= begin + count_j > slot || j + 1 >= each || n + 1 >= p.batch;
+        begin += here ? 0 : count_j;
+        n += here ? 0 : 1;
+      }
+      at = min(n, p.batch - 1);
+    } else {
+      int lo = 0, n = p.batch;
+      while (n > 1) {
+        const int stride = (n + 63) >> 6;
+        const int i = lo + lane * stride;
+        const bool hit = i < lo + n && spare_begin(i, indptr[i]) <= slot;
+        const int first = lo + (max(static_cast<int>(__popcll(__ballot(hit))), 1) - 1) * stride;
+        n = min(stride, lo + n - first);
+        lo = first;
+      }
+      at = lo;
+      begin = spare_begin(at, indptr[at]);
+    }
+    who = 0;
+  } else {
+    at = min(lane, p.batch - 1);
   }
-  const int at = lo + min(lane, n - 1);
   const int page = p.page_indptr[at], next_page = p.page_indptr[at + 1], last = p.last_page_len[at];
   const int sink = p.sink_size != nullptr ? p.sink_size[at] : 0, window = p.window_offset != nullptr ? p.window_offset[at] : 0;
   const int q = PREFILL ? p.q_indptr[at] : at, next_q = PREFILL ? p.q_indptr[at + 1] : at + 1;
-  const int mine = begin(at, PREFILL ? q : page);
-  const int who = max(static_cast<int>(__popcll(__ballot(lane < n && mine <= slot))), 1) - 1;
+  if (p.batch <= 64) {
+    const int count = lane < p.batch ? (PREFILL ? items_of(q, next_q) : items_of(page, next_page)) : 0;
+    const int upto = prefix_sum(count);
+    const int lanes = __popcll(__ballot(upto <= slot));
+    found = lanes < p.batch;
+    who = min(lanes, p.batch - 1);
+    begin = __builtin_amdgcn_readlane(upto - count, who);
+  }
   const auto of = [&](int x) { return __builtin_amdgcn_readlane(x, who); };
-  Sequence s = {lo + who, of(mine), of(page), of(next_page) - of(page), of(last), of(sink), of(window), of(q), of(next_q) - of(q)};
+  const int index = p.batch <= 64 ? who : __builtin_amdgcn_readfirstlane(at);
+  Sequence s = {found ? index : -1, __builtin_amdgcn_readfirstlane(begin), of(page), of(next_page) - of(page), of(last), of(sink), of(window), of(q), of(next_q) - of(q)};
   if (s.num_pages == 0) s.sink = s.window = 0;
   return s;
 }
@@ -309,10 +351,22 @@ __global__ __launch_bounds__(256, mxfp4_waves(D, RB)) void mxfp4_attn_kernel(Mxf
   const int kvh = blockIdx.x % p.h_kv;
   const int blocks = PREFILL ? 1 : p.row_blocks;
   const int slot = blockIdx.x / (p.h_kv * blocks);
-  const Sequence seq = sequence_of<PREFILL>(p, slot, lane, [&](int i, int first) {
-    if constexpr (PREFILL) return block_begin<R>(p, i, first);
-    return chunk_begin(p, i, first);
-  });
+  // Decode: items for a sequence's chunks, by what its pages could hold, and one for a sequence without pages (the launcher
+  // makes sure that the runs of all pages are a 31-bit number).  Prefill: items for the blocks of its rows.
+  const auto chunks_of = [&](int pages) {
+    return max(static_cast<int>((static_cast<uint32_t>(pages) * p.runs_per_page + p.chunk_runs - 1) / p.chunk_runs), 1);
+  };
+  const Sequence seq = sequence_of<PREFILL>(
+      p, slot, lane,
+      [&](int first, int end) {
+        if constexpr (PREFILL) return static_cast<int>((static_cast<int64_t>(end - first) * p.group + R - 1) / R);
+        return chunks_of(end - first);
+      },
+      [&](int i, int first) {
+        if constexpr (PREFILL) return static_cast<int>(static_cast<int64_t>(first) * p.group / R) + i;
+        return static_cast<int>(static_cast<uint32_t>(first) * p.runs_per_page / p.chunk_runs) + i;
+      });
+  if (seq.index < 0) return;  // a spare slot
   const int b = seq.index, page_begin = seq.page_begin, sink = seq.sink, window = seq.window;
   const int stored = seq.num_pages > 0 ? (seq.num_pages - 1) * p.page_size + seq.last_page_len : 0;
   const int keys = stored - window + sink;
@@ -329,7 +383,9 @@ __global__ __launch_bounds__(256, mxfp4_waves(D, RB)) void mxfp4_attn_kernel(Mxf
   const int last_end = end_of_row(row0 + rows_here - 1);  // no row sees a key behind it
   const int all_runs = (last_end + kRun - 1) / kRun;
   const int chunk = PREFILL ? static_cast<int>(blockIdx.z) : slot - seq.begin;
-  const int per_chunk = PREFILL ? ((all_runs + p.shares - 1) / p.shares + 7) & ~7 : static_cast<int>(p.chunk_runs);
+  // chunks of one length: whole ones and a rest end at different times (64 sequences of 1024-8192 tokens: 62 us, 57 so)
+  const int most_chunks = PREFILL ? p.shares : chunks_of(seq.num_pages);
+  const int per_chunk = ((all_runs + most_chunks - 1) / most_chunks + 7) & ~7;
   const int chunks = all_runs > per_chunk ? (all_runs + per_chunk - 1) / per_chunk : 1;
   if (chunk >= chunks) return;
   const int run_lo = chunk * per_chunk;
@@ -756,13 +812,13 @@ static int decode_row_blocks(int cus, int64_t group, int64_t runs, int64_t h_kv,
 //  * Never under sqrt(2 avg): a step takes a work item 0.47 us on an idle chip, a further state its row 0.12 us.
 //  * Small launches, whose items can all start at once with half of the chip's room to themselves: that many.
 //  * Long sequences: all of that room, once.
-//  * Between them sequences of unlike lengths leave workgroups over at the end: about three items a sequence.
+//  * Between them sequences of unlike lengths leave workgroups over at the end: about two items a sequence.
 // Measured in us, 32 / 8 heads of dim 128 unless said, runs an item -> time, * = this rule:
-//   1 x 2000 tokens       8: 8.7   16*: 8.4   32: 9.3   64: 11.9       1 x 32768    32: 19.1  64*: 16.1  128: 18.9
-//   1 x 131072           64: 39.8  128*: 33.8  256: 33.3               8 x U[2000,6000]      16: 15.9  40*: 13.6  96: 15.3
-//   16 x U[100,4000]     16: 16.0  48*: 14.7  96: 17.7  256: 25.6      64 x U[64,512]  16: 13.5  96*: 10.9  256: 11.0
-//   64 x U[1024,8192]    32: 69.8  64: 63.6  96*: 58.9  256: 72.8      8 x U[32768,131072], 64 / 8   96: 140  328*: 124
-//   32 x U[1000,3000], 32 / 1   8: 30.5  24*: 17.2  64: 19.8           20 x U[1500,2500], 16 / 2 of dim 256   8: 25.8  24*: 15.2
+//   1 x 2000 tokens       8: 8.7   16*: 8.4   32: 9.3   64: 12.0       1 x 32768    32: 19.1  64*: 16.2  128: 19.0
+//   1 x 131072           64: 39.8  128*: 33.9  256: 33.4               8 x U[2000,6000]      24: 14.4  40*: 14.2  96: 15.5
+//   16 x U[100,4000]     24: 14.6  48*: 15.1  96: 15.8  256: 25.5      64 x U[64,512]  16: 13.5  96*: 9.6  256: 9.7
+//   64 x U[1024,8192]    64: 64.1  96: 61.2  160*: 57.3  256: 62.8     8 x U[32768,131072], 64 / 8   96: 141  328*: 123
+//   32 x U[1000,3000], 32 / 1   8: 23.7  24*: 13.9  64: 14.6           20 x U[1500,2500], 16 / 2 of dim 256   8: 25.4  24*: 15.0
 static int64_t pick_chunk_runs(int64_t runs, int64_t batch, int64_t per_slot, int64_t resident) {
   const int64_t forced = option(kOptDecodeChunkPages);
   if (forced >= 8 && forced % 8 == 0) return forced;
@@ -774,7 +830,7 @@ static int64_t pick_chunk_runs(int64_t runs, int64_t batch, int64_t per_slot, in
   const int64_t avg = runs / batch;
   const int64_t least = steps(static_cast<int64_t>(std::sqrt(2.0 * static_cast<double>(avg))));
   const int64_t small = for_items(resident / 2), full = for_items(resident);
-  int64_t chunk = std::max<int64_t>(96, steps(avg / 3));
+  int64_t chunk = std::max<int64_t>(96, steps(avg * 5 / 8));
   if (small <= 48) chunk = std::max(small, least);
   else if (avg >= 4 * full) chunk = std::max(full, least);
   return std::min<int64_t>(chunk, 1 << 20);
