@@ -121,7 +121,10 @@ __global__ __launch_bounds__(256) void mxfp4_read_kernel(const uint8_t* __restri
 //                              them into fp16 in registers and has the matrix instruction's A operand: the order of
 //                              the contraction is free, q is loaded in the same one;
 //   O^T[d, row]     = V^T P^T  V is turned into fp16 the same way and put into the wave's LDS tile, from where the
-//                              transposing read takes it; P stays in registers.
+//                              transposing read takes it; P stays in registers.  Decode loads it in the order of memory
+//                              (sixteen lanes touch 256 bytes instead of 16 rows: 10 % of a launch at head dim 64);
+//                              prefill, which waits for LDS rather than for memory, as K (at head dim 64 the other order
+//                              writes with conflicts, 640 instead of 733 TFLOP/s).
 // The codes of a wave's next step are on their way while it works on one.
 // ------------------------------------------------------------------------------------------
 struct Mxfp4Params {
@@ -243,6 +246,7 @@ __device__ __forceinline__ Sequence sequence_of(const Mxfp4Params& p, int slot, 
 // no longer knows it, and flat loads are waited for together with LDS reads.)
 typedef __attribute__((address_space(1))) const uint8_t* global_bytes_t;
 typedef uint32_t uint32x2_t __attribute__((ext_vector_type(2)));
+typedef uint32_t uint32x3_t __attribute__((ext_vector_type(3), aligned(4)));
 typedef uint32_t uint32x4_t __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ global_bytes_t uniform_bytes(const uint8_t* p) {
   const uint64_t v = reinterpret_cast<uint64_t>(p);
@@ -282,8 +286,9 @@ struct LaneRow {
       w[0] = x[0];
       w[1] = x[1];
     } else if constexpr (D == 96) {
+      const auto x = load_global<uint32x3_t, ONCE>(codes, token * (D / 2) + g4 * 12);
 #pragma unroll
-      for (int c = 0; c < CH; ++c) w[c] = load_global<uint32_t, ONCE>(codes, token * (D / 2) + g4 * 12 + c * 4);
+      for (int c = 0; c < CH; ++c) w[c] = x[c];
     } else {
 #pragma unroll
       for (int i = 0; i < D / 128; ++i) {
@@ -346,6 +351,7 @@ __global__ __launch_bounds__(256, mxfp4_waves(D, RB)) void mxfp4_attn_kernel(Mxf
   const int lane = threadIdx.x & 63;
   const int c16 = lane & 15;
   const int g4 = lane >> 4;
+  const int v_token = PREFILL ? c16 : lane >> 2, v_quarter = PREFILL ? g4 : lane & 3;  // what the lane loads of V
 
   // ---- which rows, which keys ----------------------------------------------------------------
   const int kvh = blockIdx.x % p.h_kv;
@@ -451,7 +457,7 @@ __global__ __launch_bounds__(256, mxfp4_waves(D, RB)) void mxfp4_attn_kernel(Mxf
       // kept in scalar registers: added up with the lanes' offsets first, they cost a 64-bit vector addition a load
       asm volatile("" : "+s"(k), "+s"(v), "+s"(k_scales), "+s"(v_scales));
       x.k[h].template load<ONCE>(k, k_scales, c16, g4);
-      x.v[h].template load<ONCE>(v, v_scales, c16, g4);
+      x.v[h].template load<ONCE>(v, v_scales, v_token, v_quarter);
     }
   };
   const auto work = [&](int t0, Step& x) {
@@ -485,17 +491,17 @@ __global__ __launch_bounds__(256, mxfp4_waves(D, RB)) void mxfp4_attn_kernel(Mxf
       // the rows that see them by a mark of their own.
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int t = t0 + h * kRun + c16;
+        const int t = t0 + h * kRun + v_token;
         const bool seen = (t < last_end) & ((t < sink) | (t >= window));
 #pragma unroll
         for (int i = 0; i < LaneRow<D>::NS; ++i) {
           const bool nan = seen && x.v[h].s[i] == 255;
           for (uint64_t left = __ballot(nan); left != 0; left &= left - 1) {
             const int who = __ffsll(static_cast<long long>(left)) - 1;
-            const int at = t0 + h * kRun + (who & 15);
+            const int at = t0 + h * kRun + (PREFILL ? who & 15 : who >> 2);
 #pragma unroll
             for (int r = 0; r < RB; ++r) {
-              if (at < my_end[r]) poisoned[r] |= 1u << LaneRow<D>::block(who >> 4, i);
+              if (at < my_end[r]) poisoned[r] |= 1u << LaneRow<D>::block(PREFILL ? who >> 4 : who & 3, i);
             }
           }
           if (nan || !seen) x.v[h].s[i] = 0;
@@ -506,7 +512,7 @@ __global__ __launch_bounds__(256, mxfp4_waves(D, RB)) void mxfp4_attn_kernel(Mxf
     for (int h = 0; h < 2; ++h) {
 #pragma unroll
       for (int c = 0; c < CH; ++c)
-        *reinterpret_cast<half8_t*>(vt + (h * kRun + c16) * VS + LaneRow<D>::chunk(g4, c) * 8) = x.v[h].values(g4, c);
+        *reinterpret_cast<half8_t*>(vt + (h * kRun + v_token) * VS + LaneRow<D>::chunk(v_quarter, c) * 8) = x.v[h].values(v_quarter, c);
     }
     // Weights: the lane has 8 of the step's 32 keys of its row.  The reference point only has to keep them in fp16's
     // range: it moves when the row's maximum is 2^14 above it, to 2^-6 of that, and mostly stays after the first
