@@ -40,26 +40,44 @@ __device__ __forceinline__ half8_t dequantise8(uint32_t codes, float scale) {
   return half8_t{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
+// Where a work item of the append and the read kernel is: a thread has 8 elements of K and of V of a (token, head), its
+// neighbours the next 8, so that the fp16 rows of a workgroup are one stretch of memory.  All 32 bits: the launchers cut
+// calls of more than 2^31 threads into several.
+struct RowPiece {
+  bool there;
+  uint32_t piece;    // of 8 elements
+  uint32_t row;      // token * h_kv + head
+  int32_t position;  // slot of the token
+  uint8_t* k;        // slab of the page's K and of its V
+  uint8_t* v;
+  uint32_t codes, scale;  // offsets of the piece's codes and of its block's scale
+};
+template <int D>
+__device__ __forceinline__ RowPiece row_piece(uint8_t* pages, const int32_t* position_map, uint32_t rows, uint32_t h_kv, uint32_t page_size) {
+  constexpr uint32_t kPieces = D / 8;
+  const uint32_t gid = blockIdx.x * 256 + threadIdx.x;
+  RowPiece x;
+  x.row = gid / kPieces;
+  x.piece = gid % kPieces;
+  x.there = x.row < rows;
+  x.row = min(x.row, rows - 1);
+  const uint32_t token = x.row / h_kv, head = x.row - token * h_kv;
+  x.position = position_map[token];
+  const uint32_t at = max(x.position, 0), page = at / page_size, slot = at - page * page_size;
+  const uint32_t slab = page_size * (17 * D / 32);
+  x.k = pages + (static_cast<uint64_t>(page) * 2 * h_kv + head) * slab;
+  x.v = x.k + static_cast<uint64_t>(h_kv) * slab;
+  x.codes = slot * (D / 2) + x.piece * 4;
+  x.scale = page_size * (D / 2) + slot * (D / 32) + x.piece / 4;
+  return x;
+}
+
 // ------------------------------------------------------------------------------------------
-// append: k|v[i, h, :] -> slot position_map[i] (negative: none).  A lane quantises 8 elements, the four lanes of a
-// block share its largest magnitude; as 16-bit integers magnitudes order like the values, infinities and NaN above
-// all others.  Bound by its bytes: 2 D read and 17 D / 32 written per row.
+// append: k|v[i, h, :] -> slot position_map[i] (negative: none).  The four lanes of a block share its largest
+// magnitude; as 16-bit integers magnitudes order like the values, infinities and NaN above all others.  Bound by its
+// bytes, 2 D read and 17 D / 32 written per row.
 // ------------------------------------------------------------------------------------------
-__global__ __launch_bounds__(256) void mxfp4_append_kernel(uint8_t* __restrict__ pages, const half_t* __restrict__ k_data,
-                                                           const half_t* __restrict__ v_data,
-                                                           const int32_t* __restrict__ position_map, int64_t rows,
-                                                           int h_kv, int page_size, int d) {
-  const int chunks = d / 8;
-  const int64_t gid = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
-  const int64_t row = gid / chunks;  // (token, K or V, head)
-  if (row >= rows) return;           // whole blocks: chunks is a multiple of 4
-  const int c = gid % chunks;
-  const int h = row % h_kv;
-  const int kv = row / h_kv & 1;
-  const int64_t token = row / (2 * h_kv);
-  const int32_t position = position_map[token];
-  if (position < 0) return;
-  Vec16 x = ld16((kv ? v_data : k_data) + (token * h_kv + h) * d + c * 8);
+__device__ __forceinline__ void quantise8(const Vec16& x, uint32_t piece, uint32_t* codes_at, uint8_t* scale_at) {
   uint32_t most = 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i) most = max(most, max(x.w[i] & 0x7fffu, x.w[i] >> 16 & 0x7fffu));
@@ -75,38 +93,43 @@ __global__ __launch_bounds__(256) void mxfp4_append_kernel(uint8_t* __restrict__
   codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(codes, x.h2[1], scale, 1);
   codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(codes, x.h2[2], scale, 2);
   codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(codes, x.h2[3], scale, 3);
-  const int64_t page = position / page_size;
-  const int slot = position % page_size;
-  uint8_t* slab = pages + ((page * 2 + kv) * h_kv + h) * (static_cast<int64_t>(page_size) * (17 * d / 32));
-  *reinterpret_cast<uint32_t*>(slab + slot * (d / 2) + c * 4) = finite ? codes : 0;
-  if ((c & 3) == 0) slab[page_size * (d / 2) + slot * (d / 32) + c / 4] = finite ? byte : 255;
+  *codes_at = finite ? codes : 0;
+  if ((piece & 3) == 0) *scale_at = finite ? byte : 255;
+}
+
+template <int D>
+__global__ __launch_bounds__(256) void mxfp4_append_kernel(uint8_t* __restrict__ pages, const half_t* __restrict__ k_data,
+                                                           const half_t* __restrict__ v_data,
+                                                           const int32_t* __restrict__ position_map, uint32_t rows, uint32_t h_kv,
+                                                           uint32_t page_size) {
+  const RowPiece x = row_piece<D>(pages, position_map, rows, h_kv, page_size);
+  const uint64_t at = static_cast<uint64_t>(x.row) * D + x.piece * 8;
+  const Vec16 k = ld16_nt(k_data + at), v = ld16_nt(v_data + at);
+  if (!x.there || x.position < 0) return;  // whole blocks: four lanes have the same token
+  quantise8(k, x.piece, reinterpret_cast<uint32_t*>(x.k + x.codes), x.k + x.scale);
+  quantise8(v, x.piece, reinterpret_cast<uint32_t*>(x.v + x.codes), x.v + x.scale);
 }
 
 // ------------------------------------------------------------------------------------------
 // read: slot position_map[i] -> k|v[i, h, :] in fp16, exact; a negative position gives zeros.
 // ------------------------------------------------------------------------------------------
+template <int D>
 __global__ __launch_bounds__(256) void mxfp4_read_kernel(const uint8_t* __restrict__ pages, half_t* __restrict__ k_data,
                                                          half_t* __restrict__ v_data,
-                                                         const int32_t* __restrict__ position_map, int64_t rows, int h_kv,
-                                                         int page_size, int d) {
-  const int chunks = d / 8;
-  const int64_t gid = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
-  const int64_t row = gid / chunks;
-  if (row >= rows) return;
-  const int c = gid % chunks;
-  const int h = row % h_kv;
-  const int kv = row / h_kv & 1;
-  const int64_t token = row / (2 * h_kv);
-  const int32_t position = position_map[token];
-  Vec16 x = zero16();
-  if (position >= 0) {
-    const int64_t page = position / page_size;
-    const int slot = position % page_size;
-    const uint8_t* slab = pages + ((page * 2 + kv) * h_kv + h) * (static_cast<int64_t>(page_size) * (17 * d / 32));
-    const uint32_t codes = *reinterpret_cast<const uint32_t*>(slab + slot * (d / 2) + c * 4);
-    x.h8 = dequantise8(codes, scale_of(slab[page_size * (d / 2) + slot * (d / 32) + c / 4]));
+                                                         const int32_t* __restrict__ position_map, uint32_t rows, uint32_t h_kv,
+                                                         uint32_t page_size) {
+  const RowPiece x = row_piece<D>(const_cast<uint8_t*>(pages), position_map, rows, h_kv, page_size);
+  Vec16 k = zero16(), v = zero16();
+  if (x.position >= 0) {
+    const uint32_t k_codes = *reinterpret_cast<const uint32_t*>(x.k + x.codes), v_codes = *reinterpret_cast<const uint32_t*>(x.v + x.codes);
+    const uint32_t k_scale = x.k[x.scale], v_scale = x.v[x.scale];
+    k.h8 = dequantise8(k_codes, scale_of(k_scale));
+    v.h8 = dequantise8(v_codes, scale_of(v_scale));
   }
-  st16((kv ? v_data : k_data) + (token * h_kv + h) * d + c * 8, x);
+  if (!x.there) return;
+  const uint64_t at = static_cast<uint64_t>(x.row) * D + x.piece * 8;
+  st16(k_data + at, k);
+  st16(v_data + at, v);
 }
 
 // ------------------------------------------------------------------------------------------
@@ -746,10 +769,21 @@ static void check_aligned(const char* what, std::initializer_list<const void*> d
   for (const void* p : data) KV_CHECK(reinterpret_cast<uintptr_t>(p) % 16 == 0) << what << ": data must be aligned to 16 bytes";
 }
 
-static dim3 blocks_for(const char* what, int64_t threads) {
-  const int64_t blocks = (threads + 255) / 256;
-  KV_CHECK(blocks < (int64_t{1} << 31)) << what << ": too many rows";
-  return dim3(static_cast<unsigned>(blocks));
+// Launches over the (token, head) rows of a call: launch(head dim, first token, rows, grid), of at most 2^30 threads each.
+template <class Launch>
+static void for_row_pieces(int d, int64_t ntoken, int64_t h_kv, Launch&& launch) {
+  const int64_t most = std::max<int64_t>((int64_t{1} << 30) / (h_kv * (d / 8)), 1);
+  for (int64_t first = 0; first < ntoken; first += most) {
+    const int64_t rows = std::min(most, ntoken - first) * h_kv;
+    const dim3 grid(static_cast<unsigned>((rows * (d / 8) + 255) / 256));
+    switch (d) {
+      case 64: launch(std::integral_constant<int, 64>{}, first, static_cast<uint32_t>(rows), grid); break;
+      case 96: launch(std::integral_constant<int, 96>{}, first, static_cast<uint32_t>(rows), grid); break;
+      case 128: launch(std::integral_constant<int, 128>{}, first, static_cast<uint32_t>(rows), grid); break;
+      default: launch(std::integral_constant<int, 256>{}, first, static_cast<uint32_t>(rows), grid); break;
+    }
+    KV_LAUNCH_CHECK();
+  }
 }
 
 // Work items that the chip holds at once.
@@ -927,11 +961,13 @@ int tvmkv_mxfp4_append(void* pages, const void* k_data, const void* v_data, cons
   if (ntoken == 0) return TVMKV_OK;
   KV_CHECK(pages && k_data && v_data && position_map) << "mxfp4_append: NULL tensor";
   check_aligned("mxfp4_append", {pages, k_data, v_data});
-  const int64_t rows = ntoken * 2 * num_kv_heads;
-  hipLaunchKernelGGL(mxfp4_append_kernel, blocks_for("mxfp4_append", rows * (head_dim / 8)), dim3(256), 0, as_stream(stream),
-                     static_cast<uint8_t*>(pages), static_cast<const half_t*>(k_data), static_cast<const half_t*>(v_data),
-                     position_map, rows, num_kv_heads, page_size, head_dim);
-  KV_LAUNCH_CHECK();
+  for_row_pieces(head_dim, ntoken, num_kv_heads, [&](auto dim, int64_t first, uint32_t rows, dim3 grid) {
+    constexpr int D = decltype(dim)::value;
+    const int64_t at = first * num_kv_heads * D;
+    hipLaunchKernelGGL(mxfp4_append_kernel<D>, grid, dim3(256), 0, as_stream(stream), static_cast<uint8_t*>(pages),
+                       static_cast<const half_t*>(k_data) + at, static_cast<const half_t*>(v_data) + at, position_map + first, rows,
+                       static_cast<uint32_t>(num_kv_heads), static_cast<uint32_t>(page_size));
+  });
   KV_API_END();
 }
 
@@ -943,11 +979,13 @@ int tvmkv_mxfp4_read_kv(const void* pages, const int32_t* position_map, void* k_
   if (ntoken == 0) return TVMKV_OK;
   KV_CHECK(pages && k_data && v_data && position_map) << "mxfp4_read_kv: NULL tensor";
   check_aligned("mxfp4_read_kv", {pages, k_data, v_data});
-  const int64_t rows = ntoken * 2 * num_kv_heads;
-  hipLaunchKernelGGL(mxfp4_read_kernel, blocks_for("mxfp4_read_kv", rows * (head_dim / 8)), dim3(256), 0, as_stream(stream),
-                     static_cast<const uint8_t*>(pages), static_cast<half_t*>(k_data), static_cast<half_t*>(v_data), position_map,
-                     rows, num_kv_heads, page_size, head_dim);
-  KV_LAUNCH_CHECK();
+  for_row_pieces(head_dim, ntoken, num_kv_heads, [&](auto dim, int64_t first, uint32_t rows, dim3 grid) {
+    constexpr int D = decltype(dim)::value;
+    const int64_t at = first * num_kv_heads * D;
+    hipLaunchKernelGGL(mxfp4_read_kernel<D>, grid, dim3(256), 0, as_stream(stream), static_cast<const uint8_t*>(pages),
+                       static_cast<half_t*>(k_data) + at, static_cast<half_t*>(v_data) + at, position_map + first, rows,
+                       static_cast<uint32_t>(num_kv_heads), static_cast<uint32_t>(page_size));
+  });
   KV_API_END();
 }
 
