@@ -40,28 +40,29 @@ __device__ __forceinline__ half8_t dequantise8(uint32_t codes, float scale) {
   return half8_t{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
-// Where a work item of the append and the read kernel is: a thread has 8 elements of K and of V of a (token, head), its
-// neighbours the next 8, so that the fp16 rows of a workgroup are one stretch of memory.  All 32 bits: the launchers cut
-// calls of more than 2^31 threads into several.
+// Where a thread of the append and the read kernel is: it has 8 elements of K and of V of a (token, head), its neighbours
+// the next 8, then come the other tokens of 16, then the heads: the tokens of a call mostly follow one another in their
+// pages, where the codes of a head's tokens do, so that a workgroup's part of the cache is whole lines.  32 bits: the
+// launchers cut calls of more than 2^30 threads into several.
 struct RowPiece {
   bool there;
   uint32_t piece;    // of 8 elements
-  uint32_t row;      // token * h_kv + head
+  uint64_t at;       // of its elements in the fp16 rows
   int32_t position;  // slot of the token
   uint8_t* k;        // slab of the page's K and of its V
   uint8_t* v;
   uint32_t codes, scale;  // offsets of the piece's codes and of its block's scale
 };
 template <int D>
-__device__ __forceinline__ RowPiece row_piece(uint8_t* pages, const int32_t* position_map, uint32_t rows, uint32_t h_kv, uint32_t page_size) {
+__device__ __forceinline__ RowPiece row_piece(uint8_t* pages, const int32_t* position_map, uint32_t tokens, uint32_t h_kv, uint32_t page_size) {
   constexpr uint32_t kPieces = D / 8;
   const uint32_t gid = blockIdx.x * 256 + threadIdx.x;
   RowPiece x;
-  x.row = gid / kPieces;
+  const uint32_t row = gid / kPieces, sixteen = (row / 16) / h_kv, head = row / 16 - sixteen * h_kv;
   x.piece = gid % kPieces;
-  x.there = x.row < rows;
-  x.row = min(x.row, rows - 1);
-  const uint32_t token = x.row / h_kv, head = x.row - token * h_kv;
+  x.there = sixteen * 16 + row % 16 < tokens;
+  const uint32_t token = min(sixteen * 16 + row % 16, tokens - 1);
+  x.at = (static_cast<uint64_t>(token) * h_kv + head) * D + x.piece * 8;
   x.position = position_map[token];
   const uint32_t at = max(x.position, 0), page = at / page_size, slot = at - page * page_size;
   const uint32_t slab = page_size * (17 * D / 32);
@@ -100,11 +101,10 @@ __device__ __forceinline__ void quantise8(const Vec16& x, uint32_t piece, uint32
 template <int D>
 __global__ __launch_bounds__(256) void mxfp4_append_kernel(uint8_t* __restrict__ pages, const half_t* __restrict__ k_data,
                                                            const half_t* __restrict__ v_data,
-                                                           const int32_t* __restrict__ position_map, uint32_t rows, uint32_t h_kv,
+                                                           const int32_t* __restrict__ position_map, uint32_t tokens, uint32_t h_kv,
                                                            uint32_t page_size) {
-  const RowPiece x = row_piece<D>(pages, position_map, rows, h_kv, page_size);
-  const uint64_t at = static_cast<uint64_t>(x.row) * D + x.piece * 8;
-  const Vec16 k = ld16_nt(k_data + at), v = ld16_nt(v_data + at);
+  const RowPiece x = row_piece<D>(pages, position_map, tokens, h_kv, page_size);
+  const Vec16 k = ld16_nt(k_data + x.at), v = ld16_nt(v_data + x.at);
   if (!x.there || x.position < 0) return;  // whole blocks: four lanes have the same token
   quantise8(k, x.piece, reinterpret_cast<uint32_t*>(x.k + x.codes), x.k + x.scale);
   quantise8(v, x.piece, reinterpret_cast<uint32_t*>(x.v + x.codes), x.v + x.scale);
@@ -116,9 +116,9 @@ __global__ __launch_bounds__(256) void mxfp4_append_kernel(uint8_t* __restrict__
 template <int D>
 __global__ __launch_bounds__(256) void mxfp4_read_kernel(const uint8_t* __restrict__ pages, half_t* __restrict__ k_data,
                                                          half_t* __restrict__ v_data,
-                                                         const int32_t* __restrict__ position_map, uint32_t rows, uint32_t h_kv,
+                                                         const int32_t* __restrict__ position_map, uint32_t tokens, uint32_t h_kv,
                                                          uint32_t page_size) {
-  const RowPiece x = row_piece<D>(const_cast<uint8_t*>(pages), position_map, rows, h_kv, page_size);
+  const RowPiece x = row_piece<D>(const_cast<uint8_t*>(pages), position_map, tokens, h_kv, page_size);
   Vec16 k = zero16(), v = zero16();
   if (x.position >= 0) {
     const uint32_t k_codes = *reinterpret_cast<const uint32_t*>(x.k + x.codes), v_codes = *reinterpret_cast<const uint32_t*>(x.v + x.codes);
@@ -127,9 +127,8 @@ __global__ __launch_bounds__(256) void mxfp4_read_kernel(const uint8_t* __restri
     v.h8 = dequantise8(v_codes, scale_of(v_scale));
   }
   if (!x.there) return;
-  const uint64_t at = static_cast<uint64_t>(x.row) * D + x.piece * 8;
-  st16(k_data + at, k);
-  st16(v_data + at, v);
+  st16(k_data + x.at, k);
+  st16(v_data + x.at, v);
 }
 
 // ------------------------------------------------------------------------------------------
@@ -769,18 +768,19 @@ static void check_aligned(const char* what, std::initializer_list<const void*> d
   for (const void* p : data) KV_CHECK(reinterpret_cast<uintptr_t>(p) % 16 == 0) << what << ": data must be aligned to 16 bytes";
 }
 
-// Launches over the (token, head) rows of a call: launch(head dim, first token, rows, grid), of at most 2^30 threads each.
+// Launches over the (token, head) rows of a call: launch(head dim, first token, tokens, grid), of at most 2^30 threads each.
 template <class Launch>
 static void for_row_pieces(int d, int64_t ntoken, int64_t h_kv, Launch&& launch) {
-  const int64_t most = std::max<int64_t>((int64_t{1} << 30) / (h_kv * (d / 8)), 1);
+  const int64_t sixteen = 16 * h_kv * (d / 8);  // threads of 16 tokens
+  const int64_t most = std::max<int64_t>((int64_t{1} << 30) / sixteen, 1) * 16;
   for (int64_t first = 0; first < ntoken; first += most) {
-    const int64_t rows = std::min(most, ntoken - first) * h_kv;
-    const dim3 grid(static_cast<unsigned>((rows * (d / 8) + 255) / 256));
+    const int64_t tokens = std::min(most, ntoken - first);
+    const dim3 grid(static_cast<unsigned>(((tokens + 15) / 16 * sixteen + 255) / 256));
     switch (d) {
-      case 64: launch(std::integral_constant<int, 64>{}, first, static_cast<uint32_t>(rows), grid); break;
-      case 96: launch(std::integral_constant<int, 96>{}, first, static_cast<uint32_t>(rows), grid); break;
-      case 128: launch(std::integral_constant<int, 128>{}, first, static_cast<uint32_t>(rows), grid); break;
-      default: launch(std::integral_constant<int, 256>{}, first, static_cast<uint32_t>(rows), grid); break;
+      case 64: launch(std::integral_constant<int, 64>{}, first, static_cast<uint32_t>(tokens), grid); break;
+      case 96: launch(std::integral_constant<int, 96>{}, first, static_cast<uint32_t>(tokens), grid); break;
+      case 128: launch(std::integral_constant<int, 128>{}, first, static_cast<uint32_t>(tokens), grid); break;
+      default: launch(std::integral_constant<int, 256>{}, first, static_cast<uint32_t>(tokens), grid); break;
     }
     KV_LAUNCH_CHECK();
   }
@@ -961,11 +961,11 @@ int tvmkv_mxfp4_append(void* pages, const void* k_data, const void* v_data, cons
   if (ntoken == 0) return TVMKV_OK;
   KV_CHECK(pages && k_data && v_data && position_map) << "mxfp4_append: NULL tensor";
   check_aligned("mxfp4_append", {pages, k_data, v_data});
-  for_row_pieces(head_dim, ntoken, num_kv_heads, [&](auto dim, int64_t first, uint32_t rows, dim3 grid) {
+  for_row_pieces(head_dim, ntoken, num_kv_heads, [&](auto dim, int64_t first, uint32_t tokens, dim3 grid) {
     constexpr int D = decltype(dim)::value;
     const int64_t at = first * num_kv_heads * D;
     hipLaunchKernelGGL(mxfp4_append_kernel<D>, grid, dim3(256), 0, as_stream(stream), static_cast<uint8_t*>(pages),
-                       static_cast<const half_t*>(k_data) + at, static_cast<const half_t*>(v_data) + at, position_map + first, rows,
+                       static_cast<const half_t*>(k_data) + at, static_cast<const half_t*>(v_data) + at, position_map + first, tokens,
                        static_cast<uint32_t>(num_kv_heads), static_cast<uint32_t>(page_size));
   });
   KV_API_END();
@@ -979,11 +979,11 @@ int tvmkv_mxfp4_read_kv(const void* pages, const int32_t* position_map, void* k_
   if (ntoken == 0) return TVMKV_OK;
   KV_CHECK(pages && k_data && v_data && position_map) << "mxfp4_read_kv: NULL tensor";
   check_aligned("mxfp4_read_kv", {pages, k_data, v_data});
-  for_row_pieces(head_dim, ntoken, num_kv_heads, [&](auto dim, int64_t first, uint32_t rows, dim3 grid) {
+  for_row_pieces(head_dim, ntoken, num_kv_heads, [&](auto dim, int64_t first, uint32_t tokens, dim3 grid) {
     constexpr int D = decltype(dim)::value;
     const int64_t at = first * num_kv_heads * D;
     hipLaunchKernelGGL(mxfp4_read_kernel<D>, grid, dim3(256), 0, as_stream(stream), static_cast<const uint8_t*>(pages),
-                       static_cast<half_t*>(k_data) + at, static_cast<half_t*>(v_data) + at, position_map + first, rows,
+                       static_cast<half_t*>(k_data) + at, static_cast<half_t*>(v_data) + at, position_map + first, tokens,
                        static_cast<uint32_t>(num_kv_heads), static_cast<uint32_t>(page_size));
   });
   KV_API_END();
