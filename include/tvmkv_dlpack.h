@@ -189,6 +189,21 @@ int tvmkv_dl_debug_get_kv_mla(const DLTensor* pages, const DLTensor* position_ma
 int tvmkv_dl_compact_kv_copy(const DLTensor* pages, const DLTensor* copy_length_indptr,
                              const DLTensor* copy_src_dst_pos, int64_t batch_size, void* stream);
 
+/* A cache held in 4 bits (tvmkv.h has its format): pages uint8 (num_pages, 2, h_kv, page_size,
+ * 17 * head_dim / 32), rows, q and out float16.  No counterparts among the reference's kernels; the arguments are those
+ * of slots 13, 26, 17 and 16 without the ones of in-kernel RoPE (keys are stored rotated). */
+int tvmkv_dl_mxfp4_append(const DLTensor* pages, const DLTensor* k_data, const DLTensor* v_data,
+                          const DLTensor* append_position_map, void* stream);
+int tvmkv_dl_mxfp4_read_kv(const DLTensor* pages, const DLTensor* position_map, const DLTensor* k_data,
+                           const DLTensor* v_data, void* stream);
+int tvmkv_dl_mxfp4_batch_decode_paged_kv(const DLTensor* q, const DLTensor* pages, const DLTensor* page_indptr,
+                                         const DLTensor* page_indices, const DLTensor* length_info,
+                                         const DLTensor* out, const DLTensor* lse, double sm_scale, void* stream);
+int tvmkv_dl_mxfp4_batch_prefill_paged_kv(const DLTensor* q, const DLTensor* qo_indptr, const DLTensor* pages,
+                                          const DLTensor* page_indptr, const DLTensor* page_indices,
+                                          const DLTensor* length_info, const DLTensor* out, const DLTensor* lse,
+                                          int64_t causal, double sm_scale, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -384,3 +384,38 @@ def test_results_do_not_depend_on_the_run():
     for _ in range(5):
         again = decode(q, pool, 0.1)
         assert np.array_equal(first[0], again[0]) and np.array_equal(first[1], again[1])
+
+
+def test_tensor_level_entry_points_read_views_of_a_merged_buffer():
+    """The index arrays at offsets of one buffer, as the cache's are; the same bits as by the Python functions."""
+    from tvm_amd import dlpack as dl
+
+    rng = np.random.default_rng(17)
+    pool = Pool(rng, [300, 17, 90], 2, 16, 128)
+    pages, indptr, ids, info = pool.device()
+    k, v = rows_like(rng, 3, 2, 128), rows_like(rng, 3, 2, 128)
+    slots = np.array([pool.slot(b, n - 1) for b, n in enumerate((300, 17, 90))], np.int32)
+    merged = torch.zeros(1024, dtype=torch.int32, device=DEV)
+    views, at = [], 4
+    for values in (pool.indptr, pool.ids, pool.info, slots, np.array([0, 4, 5, 7], np.int32)):
+        merged[at:at + len(values)] = i32(values)
+        views.append(dl.view(merged, 4 * at, (len(values),)))
+        at += -(-len(values) // 4) * 4
+    d_indptr, d_ids, d_info, d_slots, d_q_indptr = views
+    dl.call("mxfp4_append", dl.tensor(pages), dl.tensor(dev(k)), dl.tensor(dev(v)), d_slots)
+    pool.pages = mxfp4.append(pool.pages, k, v, slots)
+    assert np.array_equal(host(pages), pool.pages)
+    back = [torch.empty((3, 2, 128), dtype=torch.float16, device=DEV) for _ in range(2)]
+    dl.call("mxfp4_read_kv", dl.tensor(pages), d_slots, dl.tensor(back[0]), dl.tensor(back[1]))
+    assert np.array_equal(host(back[0]).astype(np.float64), mxfp4.rounded(k)) and np.array_equal(host(back[1]).astype(np.float64), mxfp4.rounded(v))
+    q = rng.standard_normal((7, 8, 128)).astype(np.float16)
+    d_q = dev(q)
+    out, lse = torch.empty((7, 8, 128), dtype=torch.float16, device=DEV), torch.empty((7, 8), device=DEV)
+    dl.call("mxfp4_batch_prefill_paged_kv", dl.tensor(d_q), d_q_indptr, dl.tensor(pages), d_indptr, d_ids, d_info, dl.tensor(out), dl.tensor(lse),
+            1, 0.1)
+    again = prefill(q, [4, 1, 2], pool, 1, 0.1)
+    assert np.array_equal(host(out), again[0]) and np.array_equal(host(lse), again[1])
+    dl.call("mxfp4_batch_decode_paged_kv", dl.tensor(d_q[:3]), dl.tensor(pages), d_indptr, d_ids, d_info, dl.tensor(out[:3]), dl.tensor(lse[:3]),
+            0.1)
+    again = decode(q[:3], pool, 0.1)
+    assert np.array_equal(host(out[:3]), again[0]) and np.array_equal(host(lse[:3]), again[1])

@@ -158,3 +158,39 @@ def test_python_entry_points_check_their_tensors():
             kernels.mxfp4_batch_decode_paged_kv(*bad)
     with pytest.raises(KVError, match="q_indptr has shape"):
         kernels.mxfp4_batch_prefill_paged_kv(q, i32(3), pages, i32(2), i32(1), i32(1), q, lse, 1, 1.0)
+
+
+def test_tensor_level_entry_points_check_their_tensors():
+    torch = pytest.importorskip("torch")
+    from tvm_amd import KVError
+    from tvm_amd import dlpack as dl
+
+    f16, i32, f32, u8 = torch.float16, torch.int32, torch.float32, torch.uint8
+
+    def z(*shape, dtype=f16):
+        return dl.tensor(torch.zeros(*shape, dtype=dtype))
+
+    pages = z(10, 2, 2, 16, 68, dtype=u8)
+    append = dict(pages=pages, k=z(3, 2, 128), v=z(3, 2, 128), pos=z(3, dtype=i32))
+    decode = dict(q=z(3, 8, 128), pages=pages, indptr=z(4, dtype=i32), indices=z(7, dtype=i32), info=z(3, dtype=i32), out=z(3, 8, 128),
+                  lse=z(3, 8, dtype=f32))
+    prefill = dict(q=z(9, 8, 128), q_indptr=z(4, dtype=i32), pages=pages, indptr=z(4, dtype=i32), indices=z(7, dtype=i32),
+                   info=z(3, dtype=i32), out=z(9, 8, 128), lse=z(9, 8, dtype=f32))
+
+    def fails(name, args, text, *scalars):
+        with pytest.raises(KVError) as e:
+            dl.call(name, *args.values(), *scalars, stream=0)
+        assert e.value.code == -1 and text in str(e.value), str(e.value)
+
+    fails("mxfp4_append", {**append, "pages": z(10, 2, 2, 16, 128)}, "pages must be uint8")
+    fails("mxfp4_append", {**append, "pages": z(10, 2, 2, 16, 64, dtype=u8)}, "pages has shape (10, 2, 2, 16, 64), expected")
+    fails("mxfp4_append", {**append, "k": z(3, 2, 128, dtype=f32)}, "k_data must be float16")
+    fails("mxfp4_append", {**append, "v": z(2, 2, 128)}, "v_data has shape (2, 2, 128)")
+    fails("mxfp4_append", {**append, "pos": None}, "append_position_map is NULL")
+    back = {"pages": pages, "pos": append["pos"], "k": append["k"], "v": z(3, 1, 128)}
+    fails("mxfp4_read_kv", back, "v_data has shape (3, 1, 128)")
+    fails("mxfp4_batch_decode_paged_kv", {**decode, "q": z(4, 8, 128), "out": z(4, 8, 128), "lse": z(4, 8, dtype=f32)}, "q has shape", 0.1)
+    fails("mxfp4_batch_decode_paged_kv", {**decode, "info": z(2, 3, dtype=i32)}, "length_info has shape (2, 3), expected (3, batch)", 0.1)
+    fails("mxfp4_batch_decode_paged_kv", {**decode, "lse": z(3, 4, dtype=f32)}, "lse has shape (3, 4)", 0.1)
+    fails("mxfp4_batch_prefill_paged_kv", {**prefill, "q_indptr": z(5, dtype=i32)}, "qo_indptr has shape (5), expected (batch + 1,)", 1, 0.1)
+    fails("mxfp4_batch_prefill_paged_kv", {**prefill, "out": z(9, 8, 64)}, "out has shape", 1, 0.1)

@@ -128,6 +128,10 @@ SIGNATURES = {
     "tvmkv_dl_debug_get_kv": [c_vp] * 4 + [c_i64, c_vp],
     "tvmkv_dl_debug_get_kv_mla": [c_vp] * 3 + [c_i64, c_vp],
     "tvmkv_dl_compact_kv_copy": [c_vp] * 3 + [c_i64, c_vp],
+    "tvmkv_dl_mxfp4_append": [c_vp] * 5,
+    "tvmkv_dl_mxfp4_read_kv": [c_vp] * 5,
+    "tvmkv_dl_mxfp4_batch_decode_paged_kv": [c_vp] * 7 + [c_f64, c_vp],
+    "tvmkv_dl_mxfp4_batch_prefill_paged_kv": [c_vp] * 8 + [c_i64, c_f64, c_vp],
 }
 
 # include/tvmkv_bench.h: the measurement aids of bench.py, a library of their own

@@ -13,10 +13,11 @@ namespace tvmkv {
 namespace {
 
 // kStorage: the storage type of an MHA cache, float16 or float32 (the reference builds its kernels for either)
-enum Kind { kF16, kF32, kI32, kStorage };
+// kBytes: the pages of a 4-bit cache
+enum Kind { kF16, kF32, kI32, kStorage, kBytes };
 
 const char* KindName(Kind kind) {
-  return kind == kF16 ? "float16" : kind == kF32 ? "float32" : kind == kI32 ? "int32" : "float16 or float32";
+  return kind == kBytes ? "uint8" : kind == kF16 ? "float16" : kind == kF32 ? "float32" : kind == kI32 ? "int32" : "float16 or float32";
 }
 
 // One validated tensor argument.
@@ -36,9 +37,9 @@ Arg Take(const DLTensor* t, const char* name, Kind kind, std::initializer_list<i
   KV_CHECK(t->device.device_type == kDLROCM)
       << name << " must be a ROCm device tensor (device_type " << static_cast<int>(kDLROCM) << "), got device_type "
       << t->device.device_type;
-  const uint8_t code = kind == kI32 ? kDLInt : kDLFloat;
-  const uint8_t bits = kind == kF16 ? 16 : kind == kStorage ? t->dtype.bits : 32;
-  KV_CHECK(t->dtype.code == code && t->dtype.bits == bits && (bits == 16 || bits == 32) && t->dtype.lanes == 1)
+  const uint8_t code = kind == kI32 ? kDLInt : kind == kBytes ? kDLUInt : kDLFloat;
+  const uint8_t bits = kind == kF16 ? 16 : kind == kStorage ? t->dtype.bits : kind == kBytes ? 8 : 32;
+  KV_CHECK(t->dtype.code == code && t->dtype.bits == bits && (bits == 16 || bits == 32 || kind == kBytes) && t->dtype.lanes == 1)
       << name << " must be " << KindName(kind) << ", got dtype (code " << static_cast<int>(t->dtype.code) << ", bits "
       << static_cast<int>(t->dtype.bits) << ", lanes " << t->dtype.lanes << ")";
   bool ndim_ok = false;
@@ -62,7 +63,7 @@ Arg Take(const DLTensor* t, const char* name, Kind kind, std::initializer_list<i
   }
   KV_CHECK(elements == 0 || t->data != nullptr) << name << " has no data";
   const uintptr_t address = reinterpret_cast<uintptr_t>(t->data) + t->byte_offset;
-  const uintptr_t alignment = (kind == kF16 || kind == kStorage) ? 16 : 4;  // K/V/q rows are read 16 bytes at a time
+  const uintptr_t alignment = (kind == kF16 || kind == kStorage || kind == kBytes) ? 16 : 4;  // K/V/q rows are read 16 bytes at a time
   KV_CHECK(address % alignment == 0) << name << " (data + byte_offset) must be aligned to " << alignment << " bytes";
   return Arg{t, name};
 }
@@ -149,6 +150,29 @@ PagedShapes CheckPaged(const Arg& q, const Arg& pages, const Arg& page_indptr, c
   s.sliding = SlidingForm(length_info, s.batch);
   Expect(k_rope_pos_offset.dim(0) == s.batch, k_rope_pos_offset, "(batch,)");
   Expect(q_rope_position.dim(0) >= s.rows, q_rope_position, "(at least the rows of q,)");
+  Expect(out.dim(0) == s.rows && out.dim(1) == s.h_q && out.dim(2) == s.d, out, "the shape of q");
+  Expect(lse.dim(0) == s.rows && lse.dim(1) == s.h_q, lse, "(rows of q, h_q)");
+  return s;
+}
+
+// Pages of a 4-bit cache whose rows have d elements: (num_pages, 2, h_kv, page_size, 17 d / 32).
+void CheckMxfp4Pages(const Arg& pages, int64_t d) {
+  Expect(pages.dim(1) == 2 && pages.dim(4) * 32 == 17 * d, pages, "(num_pages, 2, h_kv, page_size, 17 * head_dim / 32)");
+}
+PagedShapes CheckMxfp4(const Arg& q, const Arg& pages, const Arg& page_indptr, const Arg& page_indices, const Arg& length_info,
+                       const Arg& out, const Arg& lse) {
+  PagedShapes s;
+  s.rows = q.dim(0);
+  s.h_q = static_cast<int32_t>(q.dim(1));
+  s.d = static_cast<int32_t>(q.dim(2));
+  CheckMxfp4Pages(pages, s.d);
+  s.num_pages = pages.dim(0);
+  s.h_kv = static_cast<int32_t>(pages.dim(2));
+  s.page_size = static_cast<int32_t>(pages.dim(3));
+  Expect(page_indptr.dim(0) >= 1, page_indptr, "(batch + 1,)");
+  s.batch = page_indptr.dim(0) - 1;
+  s.nnz_pages = page_indices.dim(0);
+  s.sliding = SlidingForm(length_info, s.batch);
   Expect(out.dim(0) == s.rows && out.dim(1) == s.h_q && out.dim(2) == s.d, out, "the shape of q");
   Expect(lse.dim(0) == s.rows && lse.dim(1) == s.h_q, lse, "(rows of q, h_q)");
   return s;
@@ -632,6 +656,72 @@ int tvmkv_dl_batch_tree_attn(const DLTensor* q, const DLTensor* qo_indptr, const
                              double sm_scale, void* stream) {
   return tvmkv_dl_batch_tree_attn_scaled(q, qo_indptr, k, v, kv_indptr, q_rope_position, tree_attn_mn_indptr, tree_attn_mask,
                                          out, lse, rotary_mode, rope_scale, rope_theta, sm_scale, nullptr, stream);
+}
+
+int tvmkv_dl_mxfp4_append(const DLTensor* pages_, const DLTensor* k_, const DLTensor* v_, const DLTensor* pos_, void* stream) {
+  KV_API_BEGIN();
+  Arg pages = Take(pages_, "pages", kBytes, {5}), k = Take(k_, "k_data", kF16, {3}), v = Take(v_, "v_data", kF16, {3});
+  Arg pos = Take(pos_, "append_position_map", kI32, {1});
+  const int device = SameDevice({pages, k, v, pos});
+  CheckMxfp4Pages(pages, k.dim(2));
+  const int64_t rows = pos.dim(0);
+  Expect(k.dim(0) >= rows && k.dim(1) == pages.dim(2), k, "(at least the length of append_position_map, h_kv of pages, head_dim)");
+  Expect(v.dim(0) >= rows && v.dim(1) == k.dim(1) && v.dim(2) == k.dim(2), v, "the shape of k_data");
+  Launch(device, [&] { return tvmkv_mxfp4_append(pages.ptr(), k.ptr(), v.ptr(), pos.i32(), rows, pages.dim(0),
+                                                 static_cast<int32_t>(pages.dim(2)), static_cast<int32_t>(pages.dim(3)),
+                                                 static_cast<int32_t>(k.dim(2)), stream); });
+  KV_API_END();
+}
+
+int tvmkv_dl_mxfp4_read_kv(const DLTensor* pages_, const DLTensor* pos_, const DLTensor* k_, const DLTensor* v_, void* stream) {
+  KV_API_BEGIN();
+  Arg pages = Take(pages_, "pages", kBytes, {5}), k = Take(k_, "k_data", kF16, {3}), v = Take(v_, "v_data", kF16, {3});
+  Arg pos = Take(pos_, "position_map", kI32, {1});
+  const int device = SameDevice({pages, k, v, pos});
+  CheckMxfp4Pages(pages, k.dim(2));
+  const int64_t rows = pos.dim(0);
+  Expect(k.dim(0) >= rows && k.dim(1) == pages.dim(2), k, "(at least the length of position_map, h_kv of pages, head_dim)");
+  Expect(v.dim(0) >= rows && v.dim(1) == k.dim(1) && v.dim(2) == k.dim(2), v, "the shape of k_data");
+  Launch(device, [&] { return tvmkv_mxfp4_read_kv(pages.ptr(), pos.i32(), k.ptr(), v.ptr(), rows, pages.dim(0),
+                                                  static_cast<int32_t>(pages.dim(2)), static_cast<int32_t>(pages.dim(3)),
+                                                  static_cast<int32_t>(k.dim(2)), stream); });
+  KV_API_END();
+}
+
+int tvmkv_dl_mxfp4_batch_decode_paged_kv(const DLTensor* q_, const DLTensor* pages_, const DLTensor* page_indptr_,
+                                         const DLTensor* page_indices_, const DLTensor* length_info_, const DLTensor* out_,
+                                         const DLTensor* lse_, double sm_scale, void* stream) {
+  KV_API_BEGIN();
+  Arg q = Take(q_, "q", kF16, {3}), pages = Take(pages_, "pages", kBytes, {5});
+  Arg page_indptr = Take(page_indptr_, "page_indptr", kI32, {1}), page_indices = Take(page_indices_, "page_indices", kI32, {1});
+  Arg length_info = Take(length_info_, "length_info", kI32, {1, 2});
+  Arg out = Take(out_, "out", kF16, {3}), lse = Take(lse_, "lse", kF32, {2});
+  const int device = SameDevice({q, pages, page_indptr, page_indices, length_info, out, lse});
+  const PagedShapes s = CheckMxfp4(q, pages, page_indptr, page_indices, length_info, out, lse);
+  Expect(s.rows == s.batch, q, "(batch, h_q, head_dim): one query token a sequence");
+  Launch(device, [&] { return tvmkv_mxfp4_batch_decode_paged_kv(q.ptr(), pages.ptr(), page_indptr.i32(), page_indices.i32(),
+                                                                length_info.i32(), out.ptr(), lse.f32(), sm_scale,
+                                                                static_cast<int32_t>(s.batch), s.nnz_pages, s.num_pages, s.h_q, s.h_kv,
+                                                                s.d, s.page_size, s.sliding, stream); });
+  KV_API_END();
+}
+
+int tvmkv_dl_mxfp4_batch_prefill_paged_kv(const DLTensor* q_, const DLTensor* qo_indptr_, const DLTensor* pages_,
+                                          const DLTensor* page_indptr_, const DLTensor* page_indices_, const DLTensor* length_info_,
+                                          const DLTensor* out_, const DLTensor* lse_, int64_t causal, double sm_scale, void* stream) {
+  KV_API_BEGIN();
+  Arg q = Take(q_, "q", kF16, {3}), qo_indptr = Take(qo_indptr_, "qo_indptr", kI32, {1}), pages = Take(pages_, "pages", kBytes, {5});
+  Arg page_indptr = Take(page_indptr_, "page_indptr", kI32, {1}), page_indices = Take(page_indices_, "page_indices", kI32, {1});
+  Arg length_info = Take(length_info_, "length_info", kI32, {1, 2});
+  Arg out = Take(out_, "out", kF16, {3}), lse = Take(lse_, "lse", kF32, {2});
+  const int device = SameDevice({q, qo_indptr, pages, page_indptr, page_indices, length_info, out, lse});
+  const PagedShapes s = CheckMxfp4(q, pages, page_indptr, page_indices, length_info, out, lse);
+  Expect(qo_indptr.dim(0) == s.batch + 1, qo_indptr, "(batch + 1,)");
+  Launch(device, [&] { return tvmkv_mxfp4_batch_prefill_paged_kv(q.ptr(), qo_indptr.i32(), pages.ptr(), page_indptr.i32(),
+                                                                 page_indices.i32(), length_info.i32(), out.ptr(), lse.f32(), causal,
+                                                                 sm_scale, static_cast<int32_t>(s.batch), s.rows, s.nnz_pages,
+                                                                 s.num_pages, s.h_q, s.h_kv, s.d, s.page_size, s.sliding, stream); });
+  KV_API_END();
 }
 
 }  // extern "C"

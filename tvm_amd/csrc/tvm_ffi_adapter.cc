@@ -242,6 +242,27 @@ TVM_FFI_STATIC_INIT_BLOCK() {
       // slot 27 f_compact_copy
       .def("tvmkv.compact_kv_copy", [](Tensor pages, Tensor copy_length_indptr, Tensor copy_src_dst_pos, int64_t batch_size) {
         Check(tvmkv_dl_compact_kv_copy(T(pages), T(copy_length_indptr), T(copy_src_dst_pos), batch_size, StreamOf(pages)));
-      });
+      })
+      // a cache held in 4 bits: append, read back, decode, prefill
+      .def("tvmkv.mxfp4_append",
+           [](Tensor pages, Tensor k_data, Tensor v_data, Tensor position_map) {
+             Check(tvmkv_dl_mxfp4_append(T(pages), T(k_data), T(v_data), T(position_map), StreamOf(pages)));
+           })
+      .def("tvmkv.mxfp4_read_kv",
+           [](Tensor pages, Tensor position_map, Tensor k_data, Tensor v_data) {
+             Check(tvmkv_dl_mxfp4_read_kv(T(pages), T(position_map), T(k_data), T(v_data), StreamOf(pages)));
+           })
+      .def("tvmkv.mxfp4_batch_decode_paged_kv",
+           [](Tensor q, Tensor pages, Tensor page_indptr, Tensor page_indices, Tensor length_info, Tensor out, Tensor lse,
+              double sm_scale) {
+             Check(tvmkv_dl_mxfp4_batch_decode_paged_kv(T(q), T(pages), T(page_indptr), T(page_indices), T(length_info), T(out), T(lse),
+                                                        sm_scale, StreamOf(q)));
+           })
+      .def("tvmkv.mxfp4_batch_prefill_paged_kv",
+           [](Tensor q, Tensor qo_indptr, Tensor pages, Tensor page_indptr, Tensor page_indices, Tensor length_info, Tensor out,
+              Tensor lse, int64_t causal, double sm_scale) {
+             Check(tvmkv_dl_mxfp4_batch_prefill_paged_kv(T(q), T(qo_indptr), T(pages), T(page_indptr), T(page_indices), T(length_info),
+                                                         T(out), T(lse), causal, sm_scale, StreamOf(q)));
+           });
 }
 #endif  // TVMKV_HAVE_TVM_FFI

@@ -10,7 +10,7 @@ import ctypes
 from ._lib import check, lib
 
 kDLROCM = 10
-kDLInt, kDLFloat = 0, 2
+kDLInt, kDLUInt, kDLFloat = 0, 1, 2
 
 
 class DLDevice(ctypes.Structure):
@@ -51,7 +51,7 @@ class RopeScaling(ctypes.Structure):
 def _dtype_of(torch_dtype):
     import torch
     table = {torch.float16: (kDLFloat, 16), torch.float32: (kDLFloat, 32), torch.int32: (kDLInt, 32),
-             torch.int64: (kDLInt, 64), torch.bfloat16: (4, 16)}
+             torch.int64: (kDLInt, 64), torch.bfloat16: (4, 16), torch.uint8: (kDLUInt, 8)}
     code, bits = table[torch_dtype]
     return DLDataType(code, bits, 1)
 
