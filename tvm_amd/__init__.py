@@ -10,3 +10,11 @@ kernel launchers with the argument order of the reference's kernel slots.
 """
 from ._lib import LIB_PATH, KVError, decode_split_plan, lib, set_option  # noqa: F401
 from .runtime import AttnKind, RopeMode, Shape, get_global_func  # noqa: F401
+
+
+def __getattr__(name):
+    """Mxfp4KVCache imports torch, which the host-only use of this package does without."""
+    if name == "Mxfp4KVCache":
+        from .mxfp4_cache import Mxfp4KVCache
+        return Mxfp4KVCache
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

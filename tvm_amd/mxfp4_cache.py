@@ -1,0 +1,143 @@
+"""A paged KV cache held in 4 bits, with the verbs of the fp16 cache.
+
+The page pool, the block tree and the step's index arrays are those of the library's cache object in its host-only form
+(``vm.builtin.paged_attention_kv_cache_create`` without a device); the rows live in uint8 pools (``kernels.mxfp4_pages``)
+that the 4-bit kernels write and read: 4.25 bits an element, 3.76 times the tokens of an fp16 pool of the same size.
+
+    cache = Mxfp4KVCache([64, 1 << 20, 4096, 16, 0], layers, 32, 8, 128)
+    cache.add_sequence(0)
+    cache.begin_forward([0], [prompt_length])
+    for layer in range(layers):
+        cache.attention_with_fused_qkv(layer, 128 ** -0.5, qkv[layer], out[layer])   # appends, attends
+    cache.end_forward()
+"""
+import torch
+
+from . import kernels
+from .runtime import KVError, RopeMode, get_global_func
+
+
+class Mxfp4KVCache:
+    """cache_config: the reference's (max batch, max total tokens, prefill chunk, page size, sliding windows), page size
+    a multiple of 16.  A step that appends one token to every sequence writes it first and attends to the cache alone; in
+    the others the new tokens attend to each other's fp16 rows and to the cached 4-bit ones, and are written afterwards.
+    Calls run on torch's current stream; token trees are not built."""
+
+    def __init__(self, cache_config, num_layers, num_qo_heads, num_kv_heads, head_dim, rope_mode=RopeMode.NORMAL, rope_scale=1.0,
+                 rope_theta=1e4, device="cuda"):
+        if rope_mode == RopeMode.INLINE:
+            raise KVError(-2, "a 4-bit cache stores rotated keys: rope_mode INLINE is not built")
+        self.num_layers, self.num_qo_heads, self.num_kv_heads, self.head_dim = num_layers, num_qo_heads, num_kv_heads, head_dim
+        self.rope = (rope_mode == RopeMode.NORMAL, float(rope_scale), float(rope_theta))
+        self.sliding_windows = bool(cache_config[4])
+        self._host = get_global_func("vm.builtin.paged_attention_kv_cache_create")(
+            list(cache_config), [0, num_layers], num_qo_heads, num_kv_heads, head_dim, head_dim, [0] * num_layers, False,
+            int(rope_mode), rope_scale, rope_theta, None, "host")
+        num_pages, page_size = self._host.flags()["num_total_pages"], cache_config[3]
+        self.pages = [kernels.mxfp4_pages(num_pages, num_kv_heads, page_size, head_dim, device) for _ in range(num_layers)]
+        self.device = self.pages[0].device
+        self._copied = 0  # entries of the host cache's copy log that have been done
+        self._step = None
+
+    # ---- sequences -----------------------------------------------------------------------------------------------
+    def _verb(self, name, *args):
+        return get_global_func("vm.builtin." + name)(self._host, *args)
+
+    def clear(self):
+        self._verb("kv_state_clear")
+        self._copied = 0
+
+    def add_sequence(self, seq_id):
+        self._verb("kv_state_add_sequence", seq_id)
+
+    def remove_sequence(self, seq_id):
+        self._verb("kv_state_remove_sequence", seq_id)
+
+    def fork_sequence(self, parent_id, child_id, fork_pos=-1):
+        self._verb("kv_state_fork_sequence", parent_id, child_id, fork_pos)
+        self._copy_pages()
+
+    def _copy_pages(self):
+        """What the host cache asked for since the last time: pages that a sequence no longer shares from some token on."""
+        log = self._host.copy_log()
+        for source, target, _ in log[self._copied:]:
+            for pages in self.pages:
+                pages[target].copy_(pages[source])
+        self._copied = len(log)
+
+    def popn(self, seq_id, n):
+        self._verb("kv_state_popn", seq_id, n)
+        self._copy_pages()  # a sequence that ends inside rows that others share is forked anew
+
+    def enable_sliding_window_for_seq(self, seq_id, window, sinks):
+        self._verb("attention_kv_cache_enable_sliding_window_for_seq", seq_id, window, sinks)
+
+    def get_num_available_pages(self):
+        return self._verb("attention_kv_cache_get_num_available_pages")
+
+    # ---- a step --------------------------------------------------------------------------------------------------
+    def begin_forward(self, seq_ids, append_lengths):
+        self._verb("kv_state_begin_forward", seq_ids, append_lengths)
+        aux, flags = self._host.aux, self._host.flags()
+        values, places = [], []
+
+        def upload(array):
+            values.extend([0] * (-len(values) % 4))
+            places.append((len(values), len(array)))
+            values.extend(array)
+            return len(places) - 1
+
+        names = ["last_page_len"] + (["sliding_window_offset", "sink_size"] if self.sliding_windows else [])
+        depths = []
+        for d in range(flags["num_depths"]):
+            qo_indptr, ids = aux("qo_indptr", d), aux("page_indices", d)
+            if not ids:
+                continue
+            info = [x for name in names for x in aux(name, d)]
+            one_each = all(b - a == 1 for a, b in zip(qo_indptr, qo_indptr[1:]))
+            depths.append((one_each, upload(qo_indptr), upload(aux("page_indptr", d)), upload(ids), upload(info)))
+        rest = [upload(aux(name)) for name in ("q_rope_position_map", "append_position_map", "cur_append_lengths_indptr",
+                                               "k_ragged_rope_pos_offset")]
+        merged = torch.tensor(values, dtype=torch.int32, device=self.device)
+        array = [merged[at:at + n] for at, n in places]
+        self._step = {
+            "rows": sum(append_lengths), "append_first": bool(flags["append_before_attn"]),
+            "depths": [(one, array[q], array[p], array[i], array[f].view(3, -1) if self.sliding_windows else array[f])
+                       for one, q, p, i, f in depths],
+            "positions": array[rest[0]], "slots": array[rest[1]], "indptr": array[rest[2]], "key_positions": array[rest[3]]}
+
+    def end_forward(self):
+        self._verb("kv_state_end_forward")
+        self._step = None
+
+    def attention_with_fused_qkv(self, layer_id, sm_scale, qkv, out):
+        """qkv (rows, num_qo_heads + 2 num_kv_heads, head_dim) of the step's tokens: rotates, appends to the layer's pages and
+        attends, into out (rows, num_qo_heads, head_dim)."""
+        step = self._step
+        if step is None:
+            raise KVError(-1, "attention_with_fused_qkv belongs between begin_forward and end_forward")
+        rows, hq, hkv, d = step["rows"], self.num_qo_heads, self.num_kv_heads, self.head_dim
+        for name, t, heads in (("qkv", qkv, hq + 2 * hkv), ("out", out, hq)):
+            if tuple(t.shape) != (rows, heads, d):
+                raise KVError(-1, f"{name} has shape {tuple(t.shape)}, expected {(rows, heads, d)}")
+        pages = self.pages[layer_id]
+        q, k, v = (torch.empty((rows, heads, d), dtype=torch.float16, device=self.device) for heads in (hq, hkv, hkv))
+        kernels.fused_rope(qkv, step["positions"], q, k, v, *self.rope)
+        lse = torch.empty((rows, hq), dtype=torch.float32, device=self.device)
+        if step["append_first"]:
+            kernels.mxfp4_append(pages, k, v, step["slots"])
+        else:
+            kernels.batch_prefill_ragged_kv(q, step["indptr"], k, v, step["indptr"], step["positions"], step["key_positions"], out, lse, 1,
+                                            0, 1.0, 1e4, sm_scale)
+        first = step["append_first"]
+        for one_each, qo_indptr, page_indptr, page_ids, length_info in step["depths"]:
+            o, s = (out, lse) if first else (torch.empty_like(out), torch.empty_like(lse))
+            if one_each:
+                kernels.mxfp4_batch_decode_paged_kv(q, pages, page_indptr, page_ids, length_info, o, s, sm_scale)
+            else:
+                kernels.mxfp4_batch_prefill_paged_kv(q, qo_indptr, pages, page_indptr, page_ids, length_info, o, s, 0, sm_scale)
+            if not first:
+                kernels.merge_state_inplace(out, lse, o, s)
+            first = False
+        if not step["append_first"]:
+            kernels.mxfp4_append(pages, k, v, step["slots"])
