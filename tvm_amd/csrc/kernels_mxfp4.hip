@@ -357,18 +357,24 @@ struct SharedStates {
 constexpr int v_row(int d) { return d == 64 || d == 96 ? d + 8 : d + 24; }
 
 // Workgroups of a compute unit, by the registers of a work item of rb blocks of 16 rows.
-constexpr int mxfp4_waves(int d, int rb) { return d == 256 ? (rb == 1 ? 2 : 1) : rb == 1 ? 4 : d == 64 && rb == 2 ? 3 : 2; }
+constexpr int mxfp4_waves(int d, int rb) { return d == 256 ? 2 : rb == 1 ? 4 : d == 64 && rb == 2 ? 3 : 2; }
 
 template <int D, int RB, bool PREFILL, bool ONCE>
 __global__ __launch_bounds__(256, mxfp4_waves(D, RB)) void mxfp4_attn_kernel(Mxfp4Params p) {
   constexpr int CH = LaneRow<D>::CH;
   constexpr int DB = D / 16;
   constexpr int R = 16 * RB;
-  constexpr int VS = v_row(D);
-  static_assert(32 * VS * sizeof(half_t) >= 16 * D * sizeof(float), "the merge buffer takes the V tile's place");
+  constexpr int VH = D > 128 ? 2 : 1;  // V goes through the wave's tile in halves of 128 columns
+  constexpr int VW = D / VH;
+  constexpr int VS = v_row(VW);
+  static_assert(32 * VS * sizeof(half_t) >= 16 * VW * sizeof(float), "the merge buffer takes the V tile's place");
+  // Head dim 256 with two blocks of rows has registers for two waves a SIMD if q stays in LDS and one step's codes at a
+  // time in registers, the next ones loaded as soon as they are used up (one wave a SIMD: 540 TFLOP/s instead of 732).
+  constexpr bool LEAN = D == 256 && RB == 2;
   constexpr int kJoinBytes = (R * 64 + 4 * R) * sizeof(float) + 256 * sizeof(float4_t);  // the join of states, below
   constexpr int kTileHalfs = std::max<int>(32 * VS, kJoinBytes / 8);
   __shared__ __attribute__((aligned(16))) half_t v_tiles[4][kTileHalfs];
+  __shared__ half8_t q_lds[LEAN ? RB * CH * 64 : 1];
   __shared__ float sm_m[4][16], sm_l[4][16];
   __shared__ int sm_last;
 
@@ -441,7 +447,7 @@ __global__ __launch_bounds__(256, mxfp4_waves(D, RB)) void mxfp4_attn_kernel(Mxf
   if (run < run_hi) load_ids(run);
 
   int my_end[RB];
-  half8_t qf[RB][CH];
+  half8_t qf[LEAN ? 1 : RB][LEAN ? 1 : CH];
 #pragma unroll
   for (int r = 0; r < RB; ++r) {
     const int my_row = row0 + r * 16 + c16;
@@ -450,10 +456,12 @@ __global__ __launch_bounds__(256, mxfp4_waves(D, RB)) void mxfp4_attn_kernel(Mxf
     const half_t* q = p.q + (static_cast<int64_t>(q_begin + my_row / p.group) * p.h_q + kvh * p.group + my_row % p.group) * D;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
+      if (LEAN && (r * CH + c) % 4 != wave) continue;
       Vec16 x = there ? ld16(q + LaneRow<D>::chunk(g4, c) * 8) : zero16();
 #pragma unroll
       for (int i = 0; i < 4; ++i) x.w[i] ^= p.q_sign;
-      qf[r][c] = x.h8;
+      if constexpr (LEAN) q_lds[(r * CH + c) * 64 + lane] = x.h8;
+      else qf[r][c] = x.h8;
     }
   }
   float4_t o[RB][DB];
@@ -465,6 +473,11 @@ __global__ __launch_bounds__(256, mxfp4_waves(D, RB)) void mxfp4_attn_kernel(Mxf
     m[r] = kNoKey;
     l[r] = 0.f;
   }
+  if constexpr (LEAN) __syncthreads();
+  const auto q_at = [&](int r, int c) {
+    if constexpr (LEAN) return q_lds[(r * CH + c) * 64 + lane];
+    else return qf[r][c];
+  };
   uint32_t poisoned[RB] = {};  // 32-element parts of the output that are NaN, see below
 
   half_t* const vt = v_tiles[wave];
@@ -473,7 +486,7 @@ __global__ __launch_bounds__(256, mxfp4_waves(D, RB)) void mxfp4_attn_kernel(Mxf
   };
   const global_bytes_t pool = uniform_bytes(p.pages);
   const uint32_t v_slab = slab16 * p.h_kv * 16;  // from K to V of a page
-  const auto load = [&](int nth, Step& x) {  // the nth step of the 64 whose pages are here
+  const auto load = [&](int nth, Step& x, bool want_k, bool want_v) {  // of the nth step of the 64 whose pages are here
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       global_bytes_t k = pool + static_cast<uint64_t>(__builtin_amdgcn_readlane(codes16[h], nth)) * 16;
@@ -481,11 +494,11 @@ __global__ __launch_bounds__(256, mxfp4_waves(D, RB)) void mxfp4_attn_kernel(Mxf
       global_bytes_t v = k + v_slab, v_scales = k_scales + v_slab;
       // kept in scalar registers: added up with the lanes' offsets first, they cost a 64-bit vector addition a load
       asm volatile("" : "+s"(k), "+s"(v), "+s"(k_scales), "+s"(v_scales));
-      x.k[h].template load<ONCE>(k, k_scales, c16, g4);
-      x.v[h].template load<ONCE>(v, v_scales, v_token, v_quarter);
+      if (want_k) x.k[h].template load<ONCE>(k, k_scales, c16, g4);
+      if (want_v) x.v[h].template load<ONCE>(v, v_scales, v_token, v_quarter);
     }
   };
-  const auto work = [&](int t0, Step& x) {
+  const auto work = [&](int t0, Step& x, int next) {  // next: the step that takes this one's place (LEAN)
     const bool whole = t0 + 2 * kRun <= first_end && (t0 >= window || t0 + 2 * kRun <= sink);  // no key of the step is masked
     float4_t s[RB][2];
 #pragma unroll
@@ -496,9 +509,10 @@ __global__ __launch_bounds__(256, mxfp4_waves(D, RB)) void mxfp4_attn_kernel(Mxf
       for (int c = 0; c < CH; ++c) {
         const half8_t a = x.k[h].values(g4, c);
 #pragma unroll
-        for (int r = 0; r < RB; ++r) s[r][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qf[r][c], s[r][h], 0, 0, 0);
+        for (int r = 0; r < RB; ++r) s[r][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, q_at(r, c), s[r][h], 0, 0, 0);
       }
     }
+    if (LEAN) load(next, x, true, false);
     if (!whole) {
 #pragma unroll
       for (int r = 0; r < RB; ++r) {
@@ -533,12 +547,15 @@ __global__ __launch_bounds__(256, mxfp4_waves(D, RB)) void mxfp4_attn_kernel(Mxf
         }
       }
     }
+    const auto write_v = [&](int half) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+      for (int h = 0; h < 2; ++h) {
 #pragma unroll
-      for (int c = 0; c < CH; ++c)
-        *reinterpret_cast<half8_t*>(vt + (h * kRun + v_token) * VS + LaneRow<D>::chunk(v_quarter, c) * 8) = x.v[h].values(v_quarter, c);
-    }
+        for (int c = half * (CH / VH); c < (half + 1) * (CH / VH); ++c)
+          *reinterpret_cast<half8_t*>(vt + (h * kRun + v_token) * VS + LaneRow<D>::chunk(v_quarter, c) * 8 - half * VW) = x.v[h].values(v_quarter, c);
+      }
+    };
+    write_v(0);
     // Weights: the lane has 8 of the step's 32 keys of its row.  The reference point only has to keep them in fp16's
     // range: it moves when the row's maximum is 2^14 above it, to 2^-6 of that, and mostly stays after the first
     // steps, so that O is seldom rescaled; weights far below the maximum stay out of fp16's subnormal range.
@@ -566,41 +583,55 @@ __global__ __launch_bounds__(256, mxfp4_waves(D, RB)) void mxfp4_attn_kernel(Mxf
         }
       }
     }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
 #pragma unroll
-    for (int i = 0; i < DB; ++i) {
-      const half_t* src = vt + (4 * g4 + (c16 >> 2)) * VS + i * 16 + (c16 & 3) * 4;
-      const half4_t lo = lds_read_tr16(src), hi = lds_read_tr16(src + kRun * VS);
-      const half8_t a = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    for (int half = 0; half < VH; ++half) {
+      if (half > 0) write_v(half);
+      if (LEAN && half == VH - 1) load(next, x, false, true);
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
 #pragma unroll
-      for (int r = 0; r < RB; ++r) o[r][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, pf[r], o[r][i], 0, 0, 0);
+      for (int i = half * (DB / VH); i < (half + 1) * (DB / VH); ++i) {
+        const half_t* src = vt + (4 * g4 + (c16 >> 2)) * VS + i * 16 - half * VW + (c16 & 3) * 4;
+        const half4_t lo = lds_read_tr16(src), hi = lds_read_tr16(src + kRun * VS);
+        const half8_t a = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+#pragma unroll
+        for (int r = 0; r < RB; ++r) o[r][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, pf[r], o[r][i], 0, 0, 0);
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
     }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
   };
   if (run < run_hi) {
     // Two steps in flight, and every load is issued whether or not its step exists (past the end the last run is loaded
     // again): with a branch around them the compiler waits for the next step's loads in front of this one's work.
-    Step x, y;
-    load(0, x);
     int nth = 1;
-    const auto next = [&](Step& z) {
+    const auto next_ids = [&]() {
       if (nth == 64) {
         nth = 0;
         load_ids(run + 8);
 #pragma unroll
         for (int h = 0; h < 2; ++h) asm volatile("" : "+v"(codes16[h]), "+v"(scales16[h]));  // waited for in here
       }
-      load(nth++, z);
     };
-    while (true) {
-      next(y);
-      work(run * kRun, x);
-      if ((run += 8) >= run_hi) break;
-      next(x);
-      work(run * kRun, y);
-      if ((run += 8) >= run_hi) break;
+    Step x;
+    load(0, x, true, true);
+    if constexpr (LEAN) {
+      do {
+        next_ids();
+        work(run * kRun, x, nth++);
+      } while ((run += 8) < run_hi);
+    } else {
+      Step y;
+      while (true) {
+        next_ids();
+        load(nth++, y, true, true);
+        work(run * kRun, x, 0);
+        if ((run += 8) >= run_hi) break;
+        next_ids();
+        load(nth++, x, true, true);
+        work(run * kRun, y, 0);
+        if ((run += 8) >= run_hi) break;
+      }
     }
   }
 
@@ -635,28 +666,34 @@ __global__ __launch_bounds__(256, mxfp4_waves(D, RB)) void mxfp4_attn_kernel(Mxf
       sm_l[wave][c16] = l[r];
     }
     float* const mine = reinterpret_cast<float*>(vt);
-    if (r * 16 + c16 < rows_here) {
 #pragma unroll
-      for (int i = 0; i < DB; ++i) *reinterpret_cast<float4_t*>(mine + c16 * D + ((i * 4 + g4) ^ (c16 & 7)) * 4) = o[r][i];
-    }
-    __syncthreads();
-    for (int at = threadIdx.x; at < min(16, rows_here - r * 16) * (D / 4); at += 256) {
-      const int row = at / (D / 4), f = at % (D / 4) * 4;
-      const float most = fmaxf(fmaxf(sm_m[0][row], sm_m[1][row]), fmaxf(sm_m[2][row], sm_m[3][row]));
-      float sum = 0.f;
-      float4_t acc = {0.f, 0.f, 0.f, 0.f};
+    for (int half = 0; half < VH; ++half) {
+      if (half > 0) __syncthreads();
+      if (r * 16 + c16 < rows_here) {
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const float part = fast_exp2(sm_m[w][row] - most);
-        sum += sm_l[w][row] * part;
-        acc += *reinterpret_cast<const float4_t*>(reinterpret_cast<const float*>(v_tiles[w]) + row * D + (f / 4 ^ (row & 7)) * 4) * part;
+        for (int i = 0; i < DB / VH; ++i)
+          *reinterpret_cast<float4_t*>(mine + c16 * VW + ((i * 4 + g4) ^ (c16 & 7)) * 4) = o[r][half * (DB / VH) + i];
       }
-      if (chunks == 1) {
-        finish(r * 16 + row, f, most, sum, acc);
-      } else {
-        const uint32_t out = state + r * 16 + row;
-        part_o.store4(out * D + f, acc);
-        if (f == 0) part_ml.store2(out * 2, most, sum);
+      __syncthreads();
+      for (int at = threadIdx.x; at < min(16, rows_here - r * 16) * (VW / 4); at += 256) {
+        const int row = at / (VW / 4), f = at % (VW / 4) * 4;
+        const float most = fmaxf(fmaxf(sm_m[0][row], sm_m[1][row]), fmaxf(sm_m[2][row], sm_m[3][row]));
+        float sum = 0.f;
+        float4_t acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const float part = fast_exp2(sm_m[w][row] - most);
+          sum += sm_l[w][row] * part;
+          acc += *reinterpret_cast<const float4_t*>(reinterpret_cast<const float*>(v_tiles[w]) + row * VW + (f / 4 ^ (row & 7)) * 4) * part;
+        }
+        const int column = half * VW + f;
+        if (chunks == 1) {
+          finish(r * 16 + row, column, most, sum, acc);
+        } else {
+          const uint32_t out = state + r * 16 + row;
+          part_o.store4(out * D + column, acc);
+          if (column == 0) part_ml.store2(out * 2, most, sum);
+        }
       }
     }
   }
@@ -882,32 +919,33 @@ static int64_t pick_chunk_runs(int64_t runs, int64_t batch, int64_t per_slot, in
 // How a prefill launch is cut, from shapes alone: blocks of 16 rows that a work item takes, and work items that share the keys
 // of a row block.  An item turns a key's codes into fp16 once for all of its rows, so that more blocks are faster where the
 // chip is full (8 chunks of 2048 tokens on 4096 + 2048 keys, 32 / 8 heads of dim 128, TFLOP/s at 1 / 2 / 3 blocks: 660 / 838 /
-// 949; of dim 64: 512 / 682 / 730; 8 / 4 heads of dim 256: 471 / 540), and slower where it is not (40 tokens on 4000:
-// 20.3 / 22.2 / 25.9 us).  What the rows of a sequence, the rounds that the items take and the steps of an item come to is
-// estimated in us: an item's start and end 4 + 2 a block, a step t_idle to t_full with the room that is taken (measured), the
-// join of the shares.
+// 949; of dim 64: 512 / 682 / 730; 8 / 4 heads of dim 256: 471 / 732), and slower where it is not (40 tokens on 4000:
+// 20.3 / 22.2 / 25.9 us).  Estimated in us: a compute unit takes its items `waves` at a time; an item's start and end cost 4
+// and 2 a block, a step t_idle alone on its compute unit and t_full where that is full (measured); joining the shares of a
+// row costs 1.5 and 0.12 a share and block.  (Two chunks of 216 tokens on 26000 keys, 16 / 2 heads of dim 256, 1 / 2 / 3 / 5 / 8
+// shares: 387 / 350 / 396 / 319 / 316 us, estimated 385 / 313 / 346 / 343 / 309.)
 struct Cut {
   int row_blocks;
   int shares;
 };
 static Cut cut_prefill(int cus, int64_t rows, int64_t batch, int64_t h_kv, int64_t runs, int d) {
-  const double t_full[4][3] = {{1.05, 1.18, 1.10}, {1.35, 1.23, 1.40}, {1.63, 1.28, 1.70}, {2.28, 2.00, 0}};
+  const double t_full[4][3] = {{1.05, 1.18, 1.10}, {1.35, 1.23, 1.40}, {1.63, 1.28, 1.70}, {2.28, 2.94, 0}};
   const int64_t forced = option(kOptPrefillKvSplits);
   const int64_t sequence = (rows + batch - 1) / batch;  // rows of one
   Cut best = {1, 1};
   double least = 1e30;
   for (int blocks = 1; blocks <= (d == 256 ? 2 : 3); ++blocks) {
     const int64_t items = (sequence + 16 * blocks - 1) / (16 * blocks) * batch * h_kv;
-    const int64_t resident = resident_items(cus, d, blocks);
-    const double idle = (0.35 + 0.15 * blocks) * (d == 256 ? 1.6 : 1.0);
+    const int waves = mxfp4_waves(d, blocks);
+    const double idle = (0.35 + 0.15 * blocks) * (d == 256 ? 2.8 : 1.0), start = 4.0 + 2.0 * blocks;
     const double full = t_full[d == 64 ? 0 : d == 96 ? 1 : d == 128 ? 2 : 3][blocks - 1];
-    const int64_t most = forced > 0 ? forced : items >= 2 * resident ? 1 : std::min<int64_t>(std::max<int64_t>(runs / 8, 1), 64);
+    const int64_t most = forced > 0 ? forced : items >= 2 * waves * cus ? 1 : std::min<int64_t>(std::max<int64_t>(runs / 8, 1), 64);
     for (int64_t n = forced > 0 ? forced : 1; n <= most; ++n) {
-      const double rounds = static_cast<double>((items * n + resident - 1) / resident);
-      const double room = std::min(1.0, static_cast<double>(items * n) / static_cast<double>(resident));
-      const double step = idle + (full - idle) * room;
+      const int64_t load = (items * n + cus - 1) / cus, rest = load % waves;  // items of a compute unit
       const double steps = static_cast<double>((runs + 8 * n - 1) / (8 * n));
-      const double us = rounds * (4.0 + 2.0 * blocks + step * steps) + (n > 1 ? 1.5 + 0.12 * blocks * static_cast<double>(n) : 0.0);
+      double us = static_cast<double>(load / waves) * (start + full * steps);
+      if (rest > 0) us += start + (idle + (full - idle) * static_cast<double>(rest - 1) / (waves - 1)) * steps;
+      if (n > 1) us += 1.5 + 0.12 * blocks * static_cast<double>(n);
       if (us < least) {
         least = us;
         best = {blocks, static_cast<int>(n)};
