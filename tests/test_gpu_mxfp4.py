@@ -174,6 +174,34 @@ def test_decode_of_many_short_sequences():
     compare(q, [1] * 300, pool, False, out, lse, 0.125)
 
 
+@pytest.mark.parametrize("batch", [64, 65, 130, 512, 513, 700])
+def test_batches_of_every_search_path(batch):
+    """A work item finds its sequence by one lane a sequence, by some sequences a lane, or by a search over all."""
+    rng = np.random.default_rng(batch)
+    stored = (rng.integers(0, 40, batch) * (rng.random(batch) < 0.8)).tolist()
+    stored[0], stored[-1] = 0, 33
+    pool = Pool(rng, stored, 1, 16, 64)
+    q = rng.standard_normal((batch, 2, 64)).astype(np.float16)
+    out, lse = decode(q, pool, 0.125)
+    compare(q, [1] * batch, pool, False, out, lse, 0.125)
+    q_lens = rng.integers(0, 4, batch).tolist()
+    q = rng.standard_normal((sum(q_lens), 2, 64)).astype(np.float16)
+    out, lse = prefill(q, q_lens, pool, 1, 0.125)
+    compare(q, q_lens, pool, True, out, lse, 0.125)
+
+
+@pytest.mark.parametrize("sm_scale", [-0.1, 0.0, 1.0])
+def test_scales_of_either_sign_and_none(sm_scale):
+    rng = np.random.default_rng(18)
+    pool = Pool(rng, [70, 1, 300], 2, 16, 128)
+    q = (0.3 * rng.standard_normal((3, 8, 128))).astype(np.float16)
+    out, lse = decode(q, pool, sm_scale)
+    compare(q, [1] * 3, pool, False, out, lse, sm_scale)
+    q = (0.3 * rng.standard_normal((40, 8, 128))).astype(np.float16)
+    out, lse = prefill(q, [30, 1, 9], pool, 1, sm_scale)
+    compare(q, [30, 1, 9], pool, True, out, lse, sm_scale)
+
+
 def test_decode_with_sharp_and_flat_weights():
     """Scores far apart (one key takes all) and all equal; the running maximum rises at the very end of a sequence."""
     rng = np.random.default_rng(9)
@@ -374,6 +402,21 @@ def test_a_step_can_be_captured():
             kernels.mxfp4_batch_decode_paged_kv(q, pages, indptr, ids, info, out, lse, 0.1)
         torch.cuda.synchronize()
         assert np.array_equal(host(out), replayed[0]) and np.array_equal(host(lse), replayed[1])
+
+
+def test_shapes_that_need_more_and_less_scratch_in_turn():
+    """The join's counters are where the next launch of other shapes, or of more rows, looks for them."""
+    rng = np.random.default_rng(19)
+    pools = [Pool(rng, [6000], 2, 16, 128), Pool(rng, [3000, 2000, 40], 1, 16, 64), Pool(rng, [2500] * 5, 2, 32, 256)]
+    qs = [rng.standard_normal((len(p.info), 4 * p.pages.shape[2], p.d)).astype(np.float16) for p in pools]
+    for _ in range(2):
+        for q, pool in zip(qs, pools):
+            out, lse = decode(q, pool, 0.1)
+            compare(q, [1] * len(q), pool, False, out, lse, 0.1)
+            few = [3] * len(q)
+            rows = np.repeat(q, 3, 0)
+            out, lse = prefill(rows, few, pool, 1, 0.1)
+            compare(rows, few, pool, True, out, lse, 0.1)
 
 
 def test_results_do_not_depend_on_the_run():

@@ -257,11 +257,20 @@ __device__ __forceinline__ Sequence sequence_of(const Mxfp4Params& p, int slot, 
   const int q = PREFILL ? p.q_indptr[at] : at, next_q = PREFILL ? p.q_indptr[at + 1] : at + 1;
   if (p.batch <= 64) {
     const int count = lane < p.batch ? (PREFILL ? items_of(q, next_q) : items_of(page, next_page)) : 0;
-    const int upto = prefix_sum(count);
-    const int lanes = __popcll(__ballot(upto <= slot));
-    found = lanes < p.batch;
-    who = min(lanes, p.batch - 1);
-    begin = __builtin_amdgcn_readlane(upto - count, who);
+    int mine;  // the lane's first item
+    if constexpr (PREFILL) {
+      // the sequences with the most keys first, so that the last items to start are short ones (eight chunks on up to 4096
+      // cached tokens 321 -> 307 us)
+      const int key = min(next_page - page, (1 << 24) - 1) * 64 + 63 - lane;  // (unlike from lane to lane)
+      mine = 0;
+      for (int j = 0; j < p.batch; ++j) mine += __builtin_amdgcn_readlane(key, j) > key ? __builtin_amdgcn_readlane(count, j) : 0;
+    } else {
+      mine = prefix_sum(count) - count;
+    }
+    const uint64_t hit = __ballot(slot >= mine && slot < mine + count);
+    found = hit != 0;
+    who = found ? __ffsll(static_cast<long long>(hit)) - 1 : 0;
+    begin = __builtin_amdgcn_readlane(mine, who);
   }
   const auto of = [&](int x) { return __builtin_amdgcn_readlane(x, who); };
   const int index = p.batch <= 64 ? who : __builtin_amdgcn_readfirstlane(at);
@@ -861,7 +870,8 @@ static void launch_attention(const Mxfp4Params& p, int d, int row_blocks, dim3 g
   }
 }
 
-// Scratch memory of a launch: arrival counters (0 when it is allocated and after every launch), then the states.
+// Scratch memory of a launch: arrival counters (0 when it is allocated and, since the last to arrive wraps its counter, after
+// every launch), then the states.
 constexpr int64_t kMaxCounters = 1 << 18;
 static bool states_fit(int64_t states, int d) { return states * d < int64_t{1} << 30; }  // 32-bit addresses of bytes
 static ScratchLease lease_states(const char* what, Mxfp4Params& p, hipStream_t s, int64_t states, int d) {
@@ -869,7 +879,10 @@ static ScratchLease lease_states(const char* what, Mxfp4Params& p, hipStream_t s
   KV_CHECK(states_fit(states, d)) << what << ": too many work items";
   constexpr size_t counter_bytes = kMaxCounters * sizeof(unsigned);
   const size_t o_bytes = static_cast<size_t>(states) * d * sizeof(float);
-  ScratchLease ws = lease_scratch(kScratchMxfp4, s, counter_bytes + o_bytes + static_cast<size_t>(states) * 2 * sizeof(float), counter_bytes);
+  // the first buffer holds the states of any launch whose items fill the chip once, so that a stream that has run one that
+  // shares keys can capture the others
+  const size_t at_least = counter_bytes + static_cast<size_t>(2048) * 16 * (d + 2) * sizeof(float);
+  ScratchLease ws = lease_scratch(kScratchMxfp4, s, counter_bytes + o_bytes + static_cast<size_t>(states) * 2 * sizeof(float), counter_bytes, at_least);
   p.arrivals = reinterpret_cast<unsigned*>(ws.ptr);
   p.part_o = reinterpret_cast<float*>(ws.ptr + counter_bytes);
   p.part_ml = reinterpret_cast<float*>(ws.ptr + counter_bytes + o_bytes);
@@ -890,11 +903,13 @@ static int decode_row_blocks(int cus, int64_t group, int64_t runs, int64_t h_kv,
 // Keys of a work item in runs, a multiple of 8 (a step of its four waves), from shapes alone: `avg` runs a sequence, per_slot
 // items for the same keys, `resident` items that the chip holds at once.
 //  * Never under sqrt(2 avg): a step takes a work item 0.47 us on an idle chip, a further state its row 0.12 us.
+//  * Sequences of up to five steps are left whole (nothing to join).
 //  * Small launches, whose items can all start at once with half of the chip's room to themselves: that many.
 //  * Long sequences: all of that room, once.
 //  * Between them sequences of unlike lengths leave workgroups over at the end: about two items a sequence.
 // Measured in us, 32 / 8 heads of dim 128 unless said, runs an item -> time, * = this rule:
-//   1 x 2000 tokens       8: 8.7   16*: 8.4   32: 9.3   64: 12.0       1 x 32768    32: 19.1  64*: 16.2  128: 19.0
+//   1 x 500 tokens        8: 7.2   40*: 6.8                            24 x U[500,2500], 40 / 40 of dim 64   48: 37  96*: 32
+//   1 x 2000              8: 8.7   16*: 8.4   32: 9.3   64: 12.0       1 x 32768    32: 19.1  64*: 16.2  128: 19.0
 //   1 x 131072           64: 39.8  128*: 33.9  256: 33.4               8 x U[2000,6000]      24: 14.4  40*: 14.2  96: 15.5
 //   16 x U[100,4000]     24: 14.6  48*: 15.1  96: 15.8  256: 25.5      64 x U[64,512]  16: 13.5  96*: 9.6  256: 9.7
 //   64 x U[1024,8192]    64: 64.1  96: 61.2  160*: 57.3  256: 62.8     8 x U[32768,131072], 64 / 8   96: 141  328*: 123
@@ -911,7 +926,8 @@ static int64_t pick_chunk_runs(int64_t runs, int64_t batch, int64_t per_slot, in
   const int64_t least = steps(static_cast<int64_t>(std::sqrt(2.0 * static_cast<double>(avg))));
   const int64_t small = for_items(resident / 2), full = for_items(resident);
   int64_t chunk = std::max<int64_t>(96, steps(avg * 5 / 8));
-  if (small <= 48) chunk = std::max(small, least);
+  if (avg <= 40) chunk = std::max<int64_t>(small, 40);
+  else if (small <= 48) chunk = std::max(small, least);
   else if (avg >= 4 * full) chunk = std::max(full, least);
   return std::min<int64_t>(chunk, 1 << 20);
 }
