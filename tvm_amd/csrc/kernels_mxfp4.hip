@@ -571,25 +571,47 @@ __global__ __launch_bounds__(256, mxfp4_waves(D, RB)) void mxfp4_attn_kernel(Mxf
     half8_t pf[RB];
 #pragma unroll
     for (int r = 0; r < RB; ++r) {
-      float top = fmaxf(fmaxf(fmaxf(s[r][0][0], s[r][0][1]), fmaxf(s[r][0][2], s[r][0][3])),
-                        fmaxf(fmaxf(s[r][1][0], s[r][1][1]), fmaxf(s[r][1][2], s[r][1][3])));
-      top = max_xor32(max_xor16(top)) * p.scale_log2;
-      if (__ballot(top > m[r] + 14.f) != 0) {
-        const float to = top > m[r] + 14.f ? top - 6.f : m[r];
+      float e[8], top = 0.f;
+      const auto exponents = [&]() {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) e[i] = fmaf(s[r][i / 4][i % 4], p.scale_log2, -m[r]);
+      };
+      const auto highest = [&]() {
+        top = s[r][0][0];
+#pragma unroll
+        for (int i = 1; i < 8; ++i) top = fmaxf(top, s[r][i / 4][i % 4]);
+        top = max_xor32(max_xor16(top)) * p.scale_log2;
+      };
+      // Prefill, which the vector ALU holds up, takes the maximum of the exponents: one of what comes from a matrix instruction
+      // costs another instruction a score (the compiler quiets it first; head dim 64 720 -> 750 TFLOP/s).  Decode has no register
+      // for it.
+      bool moves;
+      if constexpr (PREFILL) {
+        exponents();
+        float over = e[0];
+#pragma unroll
+        for (int i = 1; i < 8; ++i) over = fmaxf(over, e[i]);
+        moves = max_xor32(max_xor16(over)) > 14.f;
+      } else {
+        highest();
+        moves = top > m[r] + 14.f;
+      }
+      if (__ballot(moves) != 0) {
+        if constexpr (PREFILL) highest();
+        const float to = moves ? top - 6.f : m[r];
         const float alpha = fast_exp2(m[r] - to);
         m[r] = to;
         l[r] *= alpha;
 #pragma unroll
         for (int i = 0; i < DB; ++i) o[r][i] *= alpha;
+        if constexpr (PREFILL) exponents();
       }
+      if constexpr (!PREFILL) exponents();
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float w = fast_exp2(fmaf(s[r][h][i], p.scale_log2, -m[r]));
-          l[r] += w;
-          pf[r][h * 4 + i] = static_cast<half_t>(w);
-        }
+      for (int i = 0; i < 8; ++i) {
+        const float w = fast_exp2(e[i]);
+        l[r] += w;
+        pf[r][i] = static_cast<half_t>(w);
       }
     }
 #pragma unroll
