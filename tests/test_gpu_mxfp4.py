@@ -156,6 +156,18 @@ def test_decode_over_windows_with_sinks(d, page, sinks, evicted):
     compare(q, [1] * len(stored), pool, False, out, lse, d ** -0.5)
 
 
+def test_more_sinks_than_stored_tokens_are_all_of_them():
+    rng = np.random.default_rng(11)
+    stored = [5, 1, 40]
+    pool = Pool(rng, stored, 2, 16, 128, 0, 0)
+    q = rng.standard_normal((3, 8, 128)).astype(np.float16)
+    want, want_lse = decode(q, pool, 0.1)
+    for window in (0, 5, 40):
+        pool.info = np.stack((pool.info[0], np.minimum(window, stored), np.full(3, 1000))).astype(np.int32)
+        out, lse = decode(q, pool, 0.1)
+        assert np.array_equal(out, want) and np.array_equal(lse, want_lse), window
+
+
 @pytest.mark.parametrize("stored", [[20000], [9000, 1, 7000], [4100] * 3])
 def test_decode_of_long_sequences_is_split_and_joined(stored):
     rng = np.random.default_rng(len(stored))

@@ -96,6 +96,7 @@ ENTRIES = {"mxfp4_append": append_args, "mxfp4_read_kv": lambda **c: [append_arg
     (dict(d=512), -2, "head_dim 512 is not built"),
     (dict(page=24), -2, "page_size must be a multiple of 16, got 24"),
     (dict(page=0), -2, "page_size must be a multiple of 16, got 0"),
+    (dict(page=1 << 26, h_kv=4), -2, "a page of 8 GiB or more is not built"),
     (dict(h_kv=0), -1, "bad shape"),
     (dict(pages=None), -1, "NULL tensor"),
     (dict(pages=SOME + 8), -1, "aligned to 16 bytes"),
@@ -125,6 +126,20 @@ def test_refused(entry, changes, text):
     lib = tvm_amd.lib()
     assert getattr(lib, "tvmkv_" + entry)(*ENTRIES[entry](**changes)) == -1
     assert text in lib.tvmkv_last_error().decode()
+
+
+@pytest.mark.parametrize("entry", ["mxfp4_batch_decode_paged_kv", "mxfp4_batch_prefill_paged_kv"])
+def test_attention_refuses_pools_it_cannot_address(entry):
+    pages_of_64_gib = (1 << 36) // (2 * 2 * 16 * 68) + 1
+    lib = tvm_amd.lib()
+    assert getattr(lib, "tvmkv_" + entry)(*ENTRIES[entry](num_pages=pages_of_64_gib)) == -2
+    assert "a pool of 64 GiB or more is not built" in lib.tvmkv_last_error().decode()
+
+
+def test_more_work_items_than_a_launch_has_are_refused():
+    lib = tvm_amd.lib()
+    assert lib.tvmkv_mxfp4_batch_prefill_paged_kv(*prefill_args(total_q=1 << 30)) == -1
+    assert "too many work items" in lib.tvmkv_last_error().decode()
 
 
 @pytest.mark.parametrize("entry, changes", [("mxfp4_append", dict(n=0, pages=None)), ("mxfp4_read_kv", dict(n=0, pages=None)),

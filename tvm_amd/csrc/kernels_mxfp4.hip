@@ -152,7 +152,7 @@ __global__ __launch_bounds__(256) void mxfp4_read_kernel(const uint8_t* __restri
 //                              transposing read takes it; P stays in registers.  Decode loads it in the order of memory
 //                              (sixteen lanes touch 256 bytes instead of 16 rows: 10 % of a launch at head dim 64);
 //                              prefill, which waits for LDS rather than for memory, as K (at head dim 64 the other order
-//                              writes with conflicts, 640 instead of 733 TFLOP/s).
+//                              writes with conflicts, 13 % slower).
 // The codes of a wave's next step are on their way while it works on one.
 // ------------------------------------------------------------------------------------------
 struct Mxfp4Params {
@@ -378,7 +378,7 @@ __global__ __launch_bounds__(256, mxfp4_waves(D, RB)) void mxfp4_attn_kernel(Mxf
   constexpr int VS = v_row(VW);
   static_assert(32 * VS * sizeof(half_t) >= 16 * VW * sizeof(float), "the merge buffer takes the V tile's place");
   // Head dim 256 with two blocks of rows has registers for two waves a SIMD if q stays in LDS and one step's codes at a
-  // time in registers, the next ones loaded as soon as they are used up (one wave a SIMD: 540 TFLOP/s instead of 732).
+  // time in registers, the next ones loaded as soon as they are used up (one wave a SIMD: 540 TFLOP/s instead of 729).
   constexpr bool LEAN = D == 256 && RB == 2;
   constexpr int kJoinBytes = (R * 64 + 4 * R) * sizeof(float) + 256 * sizeof(float4_t);  // the join of states, below
   constexpr int kTileHalfs = std::max<int>(32 * VS, kJoinBytes / 8);
@@ -413,8 +413,9 @@ __global__ __launch_bounds__(256, mxfp4_waves(D, RB)) void mxfp4_attn_kernel(Mxf
         return static_cast<int>(static_cast<uint32_t>(first) * p.runs_per_page / p.chunk_runs) + i;
       });
   if (seq.index < 0) return;  // a spare slot
-  const int b = seq.index, page_begin = seq.page_begin, sink = seq.sink, window = seq.window;
+  const int b = seq.index, page_begin = seq.page_begin, window = seq.window;
   const int stored = seq.num_pages > 0 ? (seq.num_pages - 1) * p.page_size + seq.last_page_len : 0;
+  const int sink = min(seq.sink, stored);  // (so that no key is looked for behind the stored ones)
   const int keys = stored - window + sink;
   const int q_begin = seq.q_begin, q_len = seq.q_len;
   const int rows = q_len * p.group;
@@ -583,7 +584,7 @@ __global__ __launch_bounds__(256, mxfp4_waves(D, RB)) void mxfp4_attn_kernel(Mxf
         top = max_xor32(max_xor16(top)) * p.scale_log2;
       };
       // Prefill, which the vector ALU holds up, takes the maximum of the exponents: one of what comes from a matrix instruction
-      // costs another instruction a score (the compiler quiets it first; head dim 64 720 -> 750 TFLOP/s).  Decode has no register
+      // costs another instruction a score (the compiler quiets it first; head dim 64 730 -> 773 TFLOP/s).  Decode has no register
       // for it.
       bool moves;
       if constexpr (PREFILL) {
@@ -829,10 +830,14 @@ __global__ __launch_bounds__(256, mxfp4_waves(D, RB)) void mxfp4_attn_kernel(Mxf
   }
 }
 
+static double page_bytes(int32_t h_kv, int32_t page_size, int32_t d) { return 2.0 * h_kv * page_size * (17 * d / 32); }
+
 static void check_mxfp4(const char* what, int32_t h_kv, int32_t page_size, int32_t d) {
   KV_CHECK(h_kv > 0) << what << ": bad shape";
   KV_UNSUPPORTED(d != 64 && d != 96 && d != 128 && d != 256) << what << ": head_dim " << d << " is not built (64, 96, 128, 256)";
   KV_UNSUPPORTED(page_size <= 0 || page_size % kRun != 0) << what << ": page_size must be a multiple of 16, got " << page_size;
+  // offsets within K or V of a page are 32-bit numbers
+  KV_UNSUPPORTED(page_bytes(h_kv, page_size, d) >= 8589934592.0) << what << ": a page of 8 GiB or more is not built";
 }
 
 static void check_aligned(const char* what, std::initializer_list<const void*> data) {
@@ -895,6 +900,7 @@ static void launch_attention(const Mxfp4Params& p, int d, int row_blocks, dim3 g
 // Scratch memory of a launch: arrival counters (0 when it is allocated and, since the last to arrive wraps its counter, after
 // every launch), then the states.
 constexpr int64_t kMaxCounters = 1 << 18;
+constexpr int64_t kMaxItems = (int64_t{1} << 24) - 1;  // a launch has fewer than 2^32 threads
 static bool states_fit(int64_t states, int d) { return states * d < int64_t{1} << 30; }  // 32-bit addresses of bytes
 static ScratchLease lease_states(const char* what, Mxfp4Params& p, hipStream_t s, int64_t states, int d) {
   if (states == 0) return {};  // no row's keys are shared
@@ -956,8 +962,8 @@ static int64_t pick_chunk_runs(int64_t runs, int64_t batch, int64_t per_slot, in
 
 // How a prefill launch is cut, from shapes alone: blocks of 16 rows that a work item takes, and work items that share the keys
 // of a row block.  An item turns a key's codes into fp16 once for all of its rows, so that more blocks are faster where the
-// chip is full (8 chunks of 2048 tokens on 4096 + 2048 keys, 32 / 8 heads of dim 128, TFLOP/s at 1 / 2 / 3 blocks: 660 / 838 /
-// 949; of dim 64: 512 / 682 / 730; 8 / 4 heads of dim 256: 471 / 732), and slower where it is not (40 tokens on 4000:
+// chip is full (8 chunks of 2048 tokens on 4096 + 2048 keys, 32 / 8 heads of dim 128, TFLOP/s at 1 / 2 / 3 blocks: 680 / 840 /
+// 968; of dim 64: 526 / 716 / 773; 8 / 4 heads of dim 256: 470 / 729), and slower where it is not (40 tokens on 4000:
 // 20.3 / 22.2 / 25.9 us).  Estimated in us: a compute unit takes its items `waves` at a time; an item's start and end cost 4
 // and 2 a block, a step t_idle alone on its compute unit and t_full where that is full (measured); joining the shares of a
 // row costs 1.5 and 0.12 a share and block.  (Two chunks of 216 tokens on 26000 keys, 16 / 2 heads of dim 256, 1 / 2 / 3 / 5 / 8
@@ -999,9 +1005,8 @@ static Mxfp4Params attn_params(const char* what, const void* q, const void* page
                                int32_t page_size, int32_t sliding_window) {
   KV_CHECK(batch >= 0 && nnz_pages >= 0 && h_q > 0 && h_kv > 0 && h_q % h_kv == 0) << what << ": bad shape";
   check_mxfp4(what, h_kv, page_size, d);
-  // 36-bit addresses within the pool; K of a page is less than 4 GiB in front of its V
-  const double page_bytes = 2.0 * h_kv * page_size * (17 * d / 32);
-  KV_UNSUPPORTED(num_pages * page_bytes >= 68719476736.0 || page_bytes >= 8589934592.0) << what << ": a pool of 64 GiB or more is not built";
+  // 36-bit addresses within the pool
+  KV_UNSUPPORTED(num_pages * page_bytes(h_kv, page_size, d) >= 68719476736.0) << what << ": a pool of 64 GiB or more is not built";
   Mxfp4Params p = {};
   p.q = static_cast<const half_t*>(q);
   p.pages = static_cast<const uint8_t*>(pages);
@@ -1086,10 +1091,10 @@ int tvmkv_mxfp4_batch_decode_paged_kv(const void* q, const void* pages, const in
   p.row_blocks = (p.group + rows - 1) / rows;
   const int64_t per_slot = static_cast<int64_t>(h_kv) * p.row_blocks;
   KV_CHECK(runs < (int64_t{1} << 31)) << what << ": too many pages";
-  p.chunk_runs = batch_size * per_slot > kMaxCounters ? 1 << 30
-                                                      : static_cast<uint32_t>(pick_chunk_runs(runs, batch_size, per_slot, resident_items(cus, head_dim, row_blocks)));
+  p.chunk_runs = static_cast<uint32_t>(pick_chunk_runs(runs, batch_size, per_slot, resident_items(cus, head_dim, row_blocks)));
+  if (batch_size * per_slot > kMaxCounters || !states_fit((runs / p.chunk_runs + batch_size) * per_slot * rows, head_dim)) p.chunk_runs = 1 << 30;
   const int64_t slots = runs / p.chunk_runs + batch_size;
-  KV_CHECK(slots * per_slot < (int64_t{1} << 31)) << what << ": too many work items";
+  KV_CHECK(slots * per_slot <= kMaxItems) << what << ": too many work items";
   const hipStream_t s = as_stream(stream);
   const ScratchLease ws = lease_states(what, p, s, runs > p.chunk_runs ? slots * per_slot * rows : 0, head_dim);
   launch_attention<false>(p, head_dim, row_blocks, dim3(static_cast<unsigned>(slots * per_slot)), s);
@@ -1110,13 +1115,14 @@ int tvmkv_mxfp4_batch_prefill_paged_kv(const void* q, const int32_t* q_indptr, c
   KV_CHECK(q && q_indptr && pages && page_indptr && length_info && output && lse) << what << ": NULL tensor";
   KV_CHECK(nnz_pages == 0 || page_values) << what << ": NULL page table";
   check_aligned(what, {q, pages, output});
+  // (total_q group / 16 + batch) h_kv, the most that any cut makes
+  KV_CHECK(total_q <= (kMaxItems - static_cast<int64_t>(batch_size) * h_kv) / h_q * 16) << what << ": too many work items";
   p.q_indptr = q_indptr;
   p.causal = causal != 0;
   const hipStream_t s = as_stream(stream);
   const Cut cut = cut_prefill(compute_units(), total_q * p.group, batch_size, h_kv, nnz_pages * p.runs_per_page / batch_size, head_dim);
   const int row_blocks = cut.row_blocks, rows = 16 * row_blocks;
   const int64_t slots = total_q * p.group / rows + batch_size;
-  KV_CHECK(slots * h_kv < (int64_t{1} << 31)) << what << ": too many work items";
   p.shares = cut.shares;
   if (slots * h_kv > kMaxCounters || !states_fit(slots * p.shares * h_kv * rows, head_dim)) p.shares = 1;
   const ScratchLease ws = lease_states(what, p, s, p.shares > 1 ? slots * p.shares * h_kv * rows : 0, head_dim);
