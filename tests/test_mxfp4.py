@@ -209,3 +209,21 @@ def test_tensor_level_entry_points_check_their_tensors():
     fails("mxfp4_batch_decode_paged_kv", {**decode, "lse": z(3, 4, dtype=f32)}, "lse has shape (3, 4)", 0.1)
     fails("mxfp4_batch_prefill_paged_kv", {**prefill, "q_indptr": z(5, dtype=i32)}, "qo_indptr has shape (5), expected (batch + 1,)", 1, 0.1)
     fails("mxfp4_batch_prefill_paged_kv", {**prefill, "out": z(9, 8, 64)}, "out has shape", 1, 0.1)
+
+
+def test_forks_past_the_end_of_a_long_copy_log():
+    cache = tvm_amd.Mxfp4KVCache([4, 256, 64, 16, 0], 1, 4, 2, 64, device="cpu")
+    pages = cache.pages[0]
+    cache.add_sequence(0)
+    cache.begin_forward([0], [20])
+    cache.end_forward()
+    for i in range(4200):  # the host cache keeps the last 1024 of its copies when they become more than 8192
+        cache.fork_sequence(0, 1, 5)
+        source, target, _ = cache._host.copies_since(10**9)[0][0]
+        pages[source, 0, 0, :8] = i % 251
+        cache.remove_sequence(1)
+        pages[target] = 255
+        cache.fork_sequence(0, 1, 5)
+        source, again, _ = cache._host.copies_since(10**9)[0][0]
+        assert again == target and pages[target].equal(pages[source]), i
+        cache.remove_sequence(1)

@@ -36,7 +36,7 @@ class Mxfp4KVCache:
         num_pages, page_size = self._host.flags()["num_total_pages"], cache_config[3]
         self.pages = [kernels.mxfp4_pages(num_pages, num_kv_heads, page_size, head_dim, device) for _ in range(num_layers)]
         self.device = self.pages[0].device
-        self._copied = 0  # entries of the host cache's copy log that have been done
+        self._copied = 0  # length of the host cache's copy log when its copies were done last
         self._step = None
 
     # ---- sequences -----------------------------------------------------------------------------------------------
@@ -59,11 +59,10 @@ class Mxfp4KVCache:
 
     def _copy_pages(self):
         """What the host cache asked for since the last time: pages that a sequence no longer shares from some token on."""
-        log = self._host.copy_log()
-        for source, target, _ in log[self._copied:]:
+        copies, self._copied = self._host.copies_since(self._copied)
+        for source, target, _ in copies:
             for pages in self.pages:
                 pages[target].copy_(pages[source])
-        self._copied = len(log)
 
     def popn(self, seq_id, n):
         self._verb("kv_state_popn", seq_id, n)

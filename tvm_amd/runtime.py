@@ -133,10 +133,21 @@ class PagedAttentionKVCache:
         return {"free_page_ids": free_pages, "free_block_idx": free_blocks, "blocks": blocks, "seqs": seqs}
 
     def copy_log(self):
+        data, n = self._copy_log()
+        return [(int(data[3 * i]), int(data[3 * i + 1]), int(data[3 * i + 2])) for i in range(n)]
+
+    def copies_since(self, length):
+        """The page copies of the one verb since the log had ``length`` entries, and its length now.  (A verb asks for one
+        copy at most, and a long log has lost its oldest entries when it has become shorter.)"""
+        data, n = self._copy_log()
+        first = length if n >= length else n - 1
+        return [tuple(data[3 * i:3 * i + 3]) for i in range(first, n)], n
+
+    def _copy_log(self):
         data = ctypes.POINTER(ctypes.c_int64)()
         n = ctypes.c_int64()
         check(lib().tvmkv_cache_get_copy_log(self.handle, ctypes.byref(data), ctypes.byref(n)))
-        return [(int(data[3 * i]), int(data[3 * i + 1]), int(data[3 * i + 2])) for i in range(n.value)]
+        return data, n.value
 
     def pages_ptr(self, local_layer):
         ptr = ctypes.c_void_p()
