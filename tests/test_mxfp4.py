@@ -217,13 +217,12 @@ def test_forks_past_the_end_of_a_long_copy_log():
     cache.add_sequence(0)
     cache.begin_forward([0], [20])
     cache.end_forward()
-    for i in range(4200):  # the host cache keeps the last 1024 of its copies when they become more than 8192
+    target = None
+    for i in range(8300):  # the host cache keeps the last 1024 of its copies when they become more than 8192
+        if target is not None:
+            pages[source, 0, 0, :8] = i % 251
+            pages[target] = 255
         cache.fork_sequence(0, 1, 5)
-        source, target, _ = cache._host.copies_since(10**9)[0][0]
-        pages[source, 0, 0, :8] = i % 251
-        cache.remove_sequence(1)
-        pages[target] = 255
-        cache.fork_sequence(0, 1, 5)
-        source, again, _ = cache._host.copies_since(10**9)[0][0]
-        assert again == target and pages[target].equal(pages[source]), i
+        (source, target, _), = cache._host.copies_since(10**9)[0]
+        assert pages[target].equal(pages[source]), i
         cache.remove_sequence(1)
