@@ -11,6 +11,8 @@ that the 4-bit kernels write and read: 4.25 bits an element, 3.76 times the toke
         cache.attention_with_fused_qkv(layer, 128 ** -0.5, qkv[layer], out[layer])   # appends, attends
     cache.end_forward()
 """
+import ctypes
+
 import torch
 
 from . import kernels
@@ -77,33 +79,41 @@ class Mxfp4KVCache:
     # ---- a step --------------------------------------------------------------------------------------------------
     def begin_forward(self, seq_ids, append_lengths):
         self._verb("kv_state_begin_forward", seq_ids, append_lengths)
-        aux, flags = self._host.aux, self._host.flags()
-        values, places = [], []
+        flags, total, places = self._host.flags(), 0, []
 
-        def upload(array):
-            values.extend([0] * (-len(values) % 4))
-            places.append((len(values), len(array)))
-            values.extend(array)
+        def place(*arrays):  # one behind the other, the first at a multiple of 16 bytes
+            nonlocal total
+            total = -(-total // 4) * 4
+            places.append((total, [self._host.aux_data(*a) for a in arrays]))
+            total += sum(n for _, n in places[-1][1])
             return len(places) - 1
 
-        names = ["last_page_len"] + (["sliding_window_offset", "sink_size"] if self.sliding_windows else [])
+        info = ["last_page_len"] + (["sliding_window_offset", "sink_size"] if self.sliding_windows else [])
         depths = []
         for d in range(flags["num_depths"]):
-            qo_indptr, ids = aux("qo_indptr", d), aux("page_indices", d)
-            if not ids:
-                continue
-            info = [x for name in names for x in aux(name, d)]
-            one_each = all(b - a == 1 for a, b in zip(qo_indptr, qo_indptr[1:]))
-            depths.append((one_each, upload(qo_indptr), upload(aux("page_indptr", d)), upload(ids), upload(info)))
-        rest = [upload(aux(name)) for name in ("q_rope_position_map", "append_position_map", "cur_append_lengths_indptr",
-                                               "k_ragged_rope_pos_offset")]
-        merged = torch.tensor(values, dtype=torch.int32, device=self.device)
-        array = [merged[at:at + n] for at, n in places]
+            qo_indptr = place(("qo_indptr", d))
+            ids = place(("page_indices", d))
+            if places[ids][1][0][1] > 0:
+                depths.append((qo_indptr, place(("page_indptr", d)), ids, place(*((name, d) for name in info))))
+        rest = [place((name,)) for name in ("q_rope_position_map", "append_position_map", "cur_append_lengths_indptr",
+                                            "k_ragged_rope_pos_offset")]
+        merged = torch.empty(total, dtype=torch.int32, pin_memory=self.device.type == "cuda")
+        for at, arrays in places:
+            for data, n in arrays:
+                ctypes.memmove(merged.data_ptr() + 4 * at, data, 4 * n)
+                at += n
+        one_each = [bool((merged[at:at + n].diff() == 1).all()) for at, n in self._spans(places, [q for q, *_ in depths])]
+        merged = merged.to(self.device, non_blocking=True)
+        array = [merged[at:at + n] for at, n in self._spans(places, range(len(places)))]
         self._step = {
             "rows": sum(append_lengths), "append_first": bool(flags["append_before_attn"]),
             "depths": [(one, array[q], array[p], array[i], array[f].view(3, -1) if self.sliding_windows else array[f])
-                       for one, q, p, i, f in depths],
+                       for one, (q, p, i, f) in zip(one_each, depths)],
             "positions": array[rest[0]], "slots": array[rest[1]], "indptr": array[rest[2]], "key_positions": array[rest[3]]}
+
+    @staticmethod
+    def _spans(places, which):
+        return [(places[i][0], sum(n for _, n in places[i][1])) for i in which]
 
     def end_forward(self):
         self._verb("kv_state_end_forward")

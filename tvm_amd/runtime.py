@@ -86,10 +86,15 @@ class PagedAttentionKVCache:
 
     # ---- introspection used by the parity tests -------------------------------------------
     def aux(self, name, depth=0):
+        data, size = self.aux_data(name, depth)
+        return [data[i] for i in range(size)]
+
+    def aux_data(self, name, depth=0):
+        """The array itself, which stays as it is until the next call on the cache: int32 pointer, elements."""
         data = ctypes.POINTER(ctypes.c_int32)()
         size = ctypes.c_int64()
         check(lib().tvmkv_cache_get_aux(self.handle, name.encode(), depth, ctypes.byref(data), ctypes.byref(size)))
-        return [data[i] for i in range(size.value)]
+        return data, size.value
 
     def flags(self):
         buf = (ctypes.c_int64 * 11)()
