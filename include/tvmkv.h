@@ -465,7 +465,8 @@ int tvmkv_mxfp4_batch_decode_paged_kv(const void* q, const void* pages, const in
 /* Prefill: q_indptr (batch + 1) query tokens of each sequence, q and output (total_q, h_q, head_dim), lse
  * (total_q, h_q).  causal: the last query sees all keys, one before it one fewer, and so on (a sequence's new
  * tokens are in the cache already); otherwise every query sees all keys (e.g. new rows apart from the cache, joined
- * with tvmkv_merge_state_inplace).  A query without keys: output 0, lse -5e4. */
+ * with tvmkv_merge_state_inplace).  A query without keys: output 0, lse -5e4.  Scratch memory as above, where few
+ * rows share long sequences between work items.  Both refuse pools of 64 GiB or more. */
 int tvmkv_mxfp4_batch_prefill_paged_kv(const void* q, const int32_t* q_indptr, const void* pages,
                                        const int32_t* page_indptr, const int32_t* page_values,
                                        const int32_t* length_info, void* output, float* lse, int64_t causal,
