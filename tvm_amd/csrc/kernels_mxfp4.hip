@@ -178,7 +178,9 @@ struct Mxfp4Params {
   int causal;
   int page_size;
   uint32_t runs_per_page;
-  uint32_t run_magic;  // 2^32 / runs_per_page, rounded up (0: 1)
+  uint32_t run_magic;   // 2^32 / runs_per_page, rounded up, or 0 for 1
+  uint32_t run_mask;    // all bits for 1
+  float inv_group;
   uint32_t chunk_runs;  // decode: most keys of a work item, in runs; a multiple of 8
   int shares;           // prefill: work items that share the keys of a row block
   float scale_log2;     // > 0: |sm_scale| log2(e), never 0
@@ -387,6 +389,11 @@ __global__ __launch_bounds__(256, mxfp4_waves(D, RB)) void mxfp4_attn_kernel(Mxf
   __shared__ float sm_m[4][16], sm_l[4][16];
   __shared__ int sm_last;
 
+  // The arguments in one trip; read where they are used they are a dozen, one behind the other.
+  asm volatile("" ::"s"(p.q), "s"(p.pages), "s"(p.page_indptr), "s"(p.page_values), "s"(p.last_page_len), "s"(p.batch), "s"(p.h_q),
+               "s"(p.h_kv), "s"(p.group), "s"(p.page_size), "s"(p.runs_per_page), "s"(p.run_magic), "s"(p.run_mask), "s"(p.scale_log2),
+               "s"(p.q_sign));
+  if constexpr (PREFILL) asm volatile("" ::"s"(p.q_indptr), "s"(p.causal), "s"(p.shares));
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
   const int c16 = lane & 15;
@@ -423,11 +430,14 @@ __global__ __launch_bounds__(256, mxfp4_waves(D, RB)) void mxfp4_attn_kernel(Mxf
   const int row0 = block * R;
   if (row0 >= rows) return;  // a spare slot
   const int rows_here = min(R, rows - row0);
+  // Rows: the token and head of row0, then small numbers, which a product with 1 / group divides exactly.
+  const int token0 = row0 / p.group, head0 = row0 - token0 * p.group;
+  const auto token_of = [&](int r) { return static_cast<int>((static_cast<float>(head0 + r) + 0.5f) * p.inv_group); };  // from token0 on
   // stored tokens [0, end) hold the first n keys; token t of them is one iff t < sink or t >= window
   const auto end_of = [&](int n) { return n <= sink ? n : n - sink + window; };
-  const auto end_of_row = [&](int r) { return end_of(p.causal ? min(max(keys - q_len + 1 + r / p.group, 0), keys) : keys); };
-  const int first_end = end_of_row(row0);                 // every row sees the keys in front of it
-  const int last_end = end_of_row(row0 + rows_here - 1);  // no row sees a key behind it
+  const auto end_of_row = [&](int token) { return end_of(p.causal ? min(max(keys - q_len + 1 + token, 0), keys) : keys); };
+  const int first_end = end_of_row(token0);                             // every row sees the keys in front of it
+  const int last_end = end_of_row(token0 + token_of(rows_here - 1));  // no row sees a key behind it
   const int all_runs = (last_end + kRun - 1) / kRun;
   const int chunk = PREFILL ? static_cast<int>(blockIdx.z) : slot - seq.begin;
   // chunks of one length: whole ones and a rest end at different times (64 sequences of 1024-8192 tokens: 62 us, 57 so)
@@ -442,38 +452,50 @@ __global__ __launch_bounds__(256, mxfp4_waves(D, RB)) void mxfp4_attn_kernel(Mxf
   // (slabs are a multiple of that, and so are a run's codes and scales).
   const uint32_t slab16 = static_cast<uint32_t>(p.page_size) / kRun * (17 * D / 32);
   uint32_t codes16[2], scales16[2];
+  const auto sign_q = [&](half8_t q) {
+    Vec16 x;
+    x.h8 = q;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x.w[i] ^= p.q_sign;
+    return x.h8;
+  };
   const auto load_ids = [&](int run) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const uint32_t at = min(run + 8 * lane + h, run_hi - 1);
-      const uint32_t nth = p.run_magic != 0 ? __umulhi(at, p.run_magic) : at;
-      const uint32_t in_page = at - nth * p.runs_per_page;
-      const uint32_t slab = (p.page_values[page_begin + nth] * 2u * p.h_kv + kvh) * slab16;
+      const uint32_t nth = __umulhi(at, p.run_magic) + (at & p.run_mask);
+      codes16[h] = p.page_values[page_begin + nth];
+      scales16[h] = at - nth * p.runs_per_page;
+    }
+  };
+  const auto place_ids = [&]() {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t slab = (codes16[h] * 2u * p.h_kv + kvh) * slab16, in_page = scales16[h];
       codes16[h] = slab + in_page * (D / 2);
       scales16[h] = slab + p.runs_per_page * (D / 2) + in_page * (D / 32);
     }
   };
   int run = run_lo + 2 * wave;
-  if (run < run_hi) load_ids(run);
-
+  const bool works = run < run_hi;
   int my_end[RB];
   half8_t qf[LEAN ? 1 : RB][LEAN ? 1 : CH];
+  const auto load_q = [&]() {
 #pragma unroll
-  for (int r = 0; r < RB; ++r) {
-    const int my_row = row0 + r * 16 + c16;
-    const bool there = r * 16 + c16 < rows_here;
-    my_end[r] = there ? (PREFILL ? end_of_row(my_row) : last_end) : 0;
-    const half_t* q = p.q + (static_cast<int64_t>(q_begin + my_row / p.group) * p.h_q + kvh * p.group + my_row % p.group) * D;
+    for (int r = 0; r < RB; ++r) {
+      const int row = min(r * 16 + c16, rows_here - 1);  // (a row that isn't there computes as the last one and is not written)
+      const int token = token_of(row);
+      my_end[r] = PREFILL ? end_of_row(token0 + token) : last_end;
+      const half_t* q = p.q + (static_cast<int64_t>(q_begin + token0 + token) * p.h_q + kvh * p.group + head0 + row - token * p.group) * D;
 #pragma unroll
-    for (int c = 0; c < CH; ++c) {
-      if (LEAN && (r * CH + c) % 4 != wave) continue;
-      Vec16 x = there ? ld16(q + LaneRow<D>::chunk(g4, c) * 8) : zero16();
-#pragma unroll
-      for (int i = 0; i < 4; ++i) x.w[i] ^= p.q_sign;
-      if constexpr (LEAN) q_lds[(r * CH + c) * 64 + lane] = x.h8;
-      else qf[r][c] = x.h8;
+      for (int c = 0; c < CH; ++c) {
+        if (LEAN && (r * CH + c) % 4 != wave) continue;
+        const half8_t x = ld16(q + LaneRow<D>::chunk(g4, c) * 8).h8;
+        if constexpr (LEAN) q_lds[(r * CH + c) * 64 + lane] = sign_q(x);
+        else qf[r][c] = x;
+      }
     }
-  }
+  };
   float4_t o[RB][DB];
   float m[RB], l[RB];
 #pragma unroll
@@ -483,7 +505,10 @@ __global__ __launch_bounds__(256, mxfp4_waves(D, RB)) void mxfp4_attn_kernel(Mxf
     m[r] = kNoKey;
     l[r] = 0.f;
   }
-  if constexpr (LEAN) __syncthreads();
+  if constexpr (LEAN) {
+    load_q();
+    __syncthreads();
+  }
   const auto q_at = [&](int r, int c) {
     if constexpr (LEAN) return q_lds[(r * CH + c) * 64 + lane];
     else return qf[r][c];
@@ -633,7 +658,12 @@ __global__ __launch_bounds__(256, mxfp4_waves(D, RB)) void mxfp4_attn_kernel(Mxf
       __builtin_amdgcn_wave_barrier();
     }
   };
-  if (run < run_hi) {
+  if (works) {
+    // Page ids, q, then codes, each waited for when the next are on their way.
+    load_ids(run);
+    if constexpr (!LEAN) load_q();
+    __builtin_amdgcn_sched_barrier(0);
+    place_ids();
     // Two steps in flight, and every load is issued whether or not its step exists (past the end the last run is loaded
     // again): with a branch around them the compiler waits for the next step's loads in front of this one's work.
     int nth = 1;
@@ -641,6 +671,7 @@ __global__ __launch_bounds__(256, mxfp4_waves(D, RB)) void mxfp4_attn_kernel(Mxf
       if (nth == 64) {
         nth = 0;
         load_ids(run + 8);
+        place_ids();
 #pragma unroll
         for (int h = 0; h < 2; ++h) asm volatile("" : "+v"(codes16[h]), "+v"(scales16[h]));  // waited for in here
       }
@@ -653,6 +684,12 @@ __global__ __launch_bounds__(256, mxfp4_waves(D, RB)) void mxfp4_attn_kernel(Mxf
         work(run * kRun, x, nth++);
       } while ((run += 8) < run_hi);
     } else {
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int r = 0; r < RB; ++r) {
+#pragma unroll
+        for (int c = 0; c < CH; ++c) qf[r][c] = sign_q(qf[r][c]);
+      }
       Step y;
       while (true) {
         next_ids();
@@ -671,8 +708,8 @@ __global__ __launch_bounds__(256, mxfp4_waves(D, RB)) void mxfp4_attn_kernel(Mxf
   const uint32_t state = ((static_cast<uint32_t>(PREFILL ? slot * p.shares + chunk : slot) * blocks + (PREFILL ? 0 : block)) * p.h_kv + kvh) * R;
   SharedStates part_o(p.part_o), part_ml(p.part_ml);
   const auto finish = [&](int r, int f, float most, float sum, float4_t acc) {  // elements f.. f + 3 of row r
-    const int row = row0 + r;
-    const int64_t out = static_cast<int64_t>(q_begin + row / p.group) * p.h_q + kvh * p.group + row % p.group;
+    const int token = token_of(r);
+    const int64_t out = static_cast<int64_t>(q_begin + token0 + token) * p.h_q + kvh * p.group + head0 + r - token * p.group;
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
     half4_t h;
 #pragma unroll
@@ -1023,6 +1060,8 @@ static Mxfp4Params attn_params(const char* what, const void* q, const void* page
   p.group = h_q / h_kv;
   p.page_size = page_size;
   p.runs_per_page = page_size / kRun;
+  p.run_mask = p.runs_per_page == 1 ? ~0u : 0;
+  p.inv_group = 1.f / static_cast<float>(p.group);
   p.run_magic = p.runs_per_page == 1 ? 0 : static_cast<uint32_t>(((uint64_t{1} << 32) + p.runs_per_page - 1) / p.runs_per_page);
   // The kernel takes maxima of scores that are not scaled yet and masks with -inf: a scale below 0 goes to q, and one of
   // 0 (all weights equal) becomes one that is as good as 0.
