@@ -177,6 +177,16 @@ def test_decode_of_long_sequences_is_split_and_joined(stored):
     compare(q, [1] * len(stored), pool, False, out, lse, 0.1)
 
 
+@pytest.mark.parametrize("heads, d, stored", [
+    (64, 64, [3000, 5000, 100, 0]), (64, 64, [1, 9000]), (64, 64, [2500, 2500, 2500]), (16, 128, [17, 20000, 1, 9000, 4000]),  # chunks that the lengths decide
+    (128, 64, [1500, 1600, 1550, 1500]), (128, 64, [1500, 3100, 200, 1500])])  # sequences left whole, and not
+def test_decode_whose_chunks_the_device_chooses(heads, d, stored):
+    rng = np.random.default_rng(sum(stored))
+    pool = Pool(rng, stored, heads, 16, d)
+    q = rng.standard_normal((len(stored), heads, d)).astype(np.float16)
+    compare(q, [1] * len(stored), pool, False, *decode(q, pool, d ** -0.5), d ** -0.5)
+
+
 def test_decode_of_many_short_sequences():
     rng = np.random.default_rng(8)
     stored = rng.integers(0, 40, 300)

@@ -182,6 +182,8 @@ struct Mxfp4Params {
   uint32_t run_mask;    // all bits for 1
   float inv_group;
   uint32_t chunk_runs;  // decode: most keys of a work item, in runs; a multiple of 8
+  int fit_items;        // decode: > 0: chunks as short as leave so many items a row block and kv head, chunk_runs at most
+  uint32_t whole_runs;  // decode: where no sequence has more runs than these, sequences are left whole
   int shares;           // prefill: work items that share the keys of a row block
   float scale_log2;     // > 0: |sm_scale| log2(e), never 0
   uint32_t q_sign;      // of sm_scale, at the sign bits of two fp16
@@ -406,8 +408,32 @@ __global__ __launch_bounds__(256, mxfp4_waves(D, RB)) void mxfp4_attn_kernel(Mxf
   const int slot = blockIdx.x / (p.h_kv * blocks);
   // Decode: items for a sequence's chunks, by what its pages could hold, and one for a sequence without pages (the launcher
   // makes sure that the runs of all pages are a 31-bit number).  Prefill: items for the blocks of its rows.
+  // Two items a compute unit, started together, are what large launches run best with, and only the device has the lengths.
+  uint32_t chunk_runs = p.chunk_runs;
+  if (!PREFILL && (p.whole_runs > 0 || p.fit_items > 0)) {
+    const int i = min(lane, p.batch - 1);
+    const uint32_t runs = static_cast<uint32_t>(p.page_indptr[i + 1] - p.page_indptr[i]) * p.runs_per_page;
+    if (p.whole_runs > 0) {
+      const uint32_t longest = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(wave_max(static_cast<float>(runs))));
+      if (longest <= p.whole_runs) chunk_runs = max(chunk_runs, (longest + 7) & ~7u);
+    } else {
+      // five halvings of what lies between one item for every sequence and an equal share of all keys, in steps
+      const uint32_t own = lane < p.batch ? runs : 0;
+      const uint32_t total = __builtin_amdgcn_readlane(prefix_sum(static_cast<int>(own)), 63);
+      uint32_t lo = min(total / (8 * p.fit_items), chunk_runs / 8 - 1), hi = chunk_runs / 8;
+      for (int k = 0; k < 5 && hi - lo > 1; ++k) {
+        const uint32_t mid = (lo + hi) / 2;
+        // (a rounded-up quotient more than an item holds is only one item too many)
+        const int items = lane < p.batch ? max(static_cast<int>(ceilf(static_cast<float>(own) * (1.0000005f / static_cast<float>(8 * mid)))), 1) : 0;
+        const bool fits = static_cast<int>(__builtin_amdgcn_readlane(prefix_sum(items), 63)) <= p.fit_items;
+        hi = fits ? mid : hi;
+        lo = fits ? lo : mid;
+      }
+      chunk_runs = hi * 8;
+    }
+  }
   const auto chunks_of = [&](int pages) {
-    return max(static_cast<int>((static_cast<uint32_t>(pages) * p.runs_per_page + p.chunk_runs - 1) / p.chunk_runs), 1);
+    return max(static_cast<int>((static_cast<uint32_t>(pages) * p.runs_per_page + chunk_runs - 1) / chunk_runs), 1);
   };
   const Sequence seq = sequence_of<PREFILL>(
       p, slot, lane,
@@ -417,7 +443,7 @@ __global__ __launch_bounds__(256, mxfp4_waves(D, RB)) void mxfp4_attn_kernel(Mxf
       },
       [&](int i, int first) {
         if constexpr (PREFILL) return static_cast<int>(static_cast<int64_t>(first) * p.group / R) + i;
-        return static_cast<int>(static_cast<uint32_t>(first) * p.runs_per_page / p.chunk_runs) + i;
+        return static_cast<int>(static_cast<uint32_t>(first) * p.runs_per_page / chunk_runs) + i;
       });
   if (seq.index < 0) return;  // a spare slot
   const int b = seq.index, page_begin = seq.page_begin, window = seq.window;
@@ -965,23 +991,31 @@ static int decode_row_blocks(int cus, int64_t group, int64_t runs, int64_t h_kv,
   return runs * h_kv > 24 * resident_items(cus, d, static_cast<int>(fewest)) ? static_cast<int>(fewest) : 1;
 }
 
+static int64_t forced_chunk() {
+  const int64_t forced = option(kOptDecodeChunkPages);
+  return forced >= 8 && forced % 8 == 0 ? forced : 0;
+}
+
 // Keys of a work item in runs, a multiple of 8 (a step of its four waves), from shapes alone: `avg` runs a sequence, per_slot
 // items for the same keys, `resident` items that the chip holds at once.
 //  * Never under sqrt(2 avg): a step takes a work item 0.47 us on an idle chip, a further state its row 0.12 us.
 //  * Sequences of up to five steps are left whole (nothing to join).
 //  * Small launches, whose items can all start at once with half of the chip's room to themselves: that many.
-//  * Long sequences: all of that room, once.
-//  * Between them sequences of unlike lengths leave workgroups over at the end: about two items a sequence.
+//  * Few sequences, long: the shortest chunks with which there are two items a compute unit, as the device finds from the lengths
+//    (fit_items).  Two read faster than the four that fit, and a few items more than two, all started together, give some units
+//    three (32 x U[2048,16384]: 67, with chunks of 360 runs 87; 8 x 81920, 64 / 8: 125, with four a unit 135).
+//  * Many, long: all of the room, once.
+//  * Between them sequences of unlike lengths leave workgroups over at the end: about two items a sequence.  Where none is
+//    longer than its share, sequences are left whole (whole_runs: 64 x 4096 57 -> 51, 64 x 8192 of dim 64 66 -> 62).
 // Measured in us, 32 / 8 heads of dim 128 unless said, runs an item -> time, * = this rule:
 //   1 x 500 tokens        8: 7.2   40*: 6.8                            24 x U[500,2500], 40 / 40 of dim 64   48: 37  96*: 32
 //   1 x 2000              8: 8.7   16*: 8.4   32: 9.3   64: 12.0       1 x 32768    32: 19.1  64*: 16.2  128: 19.0
 //   1 x 131072           64: 39.8  128*: 33.9  256: 33.4               8 x U[2000,6000]      24: 14.4  40*: 14.2  96: 15.5
 //   16 x U[100,4000]     24: 14.6  48*: 15.1  96: 15.8  256: 25.5      64 x U[64,512]  16: 13.5  96*: 9.6  256: 9.7
-//   64 x U[1024,8192]    64: 64.1  96: 61.2  160*: 57.3  256: 62.8     8 x U[32768,131072], 64 / 8   96: 141  328*: 123
+//   64 x U[1024,8192]    64: 64.1  96: 61.2  160*: 57.3  256: 62.8     8 x U[32768,131072], 64 / 8   96: 144  found*: 123
 //   32 x U[1000,3000], 32 / 1   8: 23.7  24*: 13.9  64: 14.6           20 x U[1500,2500], 16 / 2 of dim 256   8: 25.4  24*: 15.0
-static int64_t pick_chunk_runs(int64_t runs, int64_t batch, int64_t per_slot, int64_t resident) {
-  const int64_t forced = option(kOptDecodeChunkPages);
-  if (forced >= 8 && forced % 8 == 0) return forced;
+static int64_t pick_chunk_runs(int64_t runs, int64_t batch, int64_t per_slot, int64_t resident, int64_t two_each, int* fit_items) {
+  if (forced_chunk() > 0) return forced_chunk();
   const auto steps = [](int64_t n) { return std::max<int64_t>((n + 7) / 8 * 8, 8); };
   const auto for_items = [&](int64_t items) {  // the shortest that leaves at most so many items
     const int64_t slots = items / per_slot - batch;
@@ -989,11 +1023,14 @@ static int64_t pick_chunk_runs(int64_t runs, int64_t batch, int64_t per_slot, in
   };
   const int64_t avg = runs / batch;
   const int64_t least = steps(static_cast<int64_t>(std::sqrt(2.0 * static_cast<double>(avg))));
-  const int64_t small = for_items(resident / 2), full = for_items(resident);
+  const int64_t small = for_items(resident / 2), full = for_items(resident), two = for_items(two_each);
   int64_t chunk = std::max<int64_t>(96, steps(avg * 5 / 8));
   if (avg <= 40) chunk = std::max<int64_t>(small, 40);
   else if (small <= 48) chunk = std::max(small, least);
-  else if (avg >= 4 * full) chunk = std::max(full, least);
+  else if (batch <= 64 && 2 * batch * per_slot <= two_each && two <= 1 << 20) {
+    chunk = two;
+    *fit_items = static_cast<int>(two_each / per_slot);
+  } else if (avg >= 4 * full) chunk = std::max(full, least);
   return std::min<int64_t>(chunk, 1 << 20);
 }
 
@@ -1130,12 +1167,19 @@ int tvmkv_mxfp4_batch_decode_paged_kv(const void* q, const void* pages, const in
   p.row_blocks = (p.group + rows - 1) / rows;
   const int64_t per_slot = static_cast<int64_t>(h_kv) * p.row_blocks;
   KV_CHECK(runs < (int64_t{1} << 31)) << what << ": too many pages";
-  p.chunk_runs = static_cast<uint32_t>(pick_chunk_runs(runs, batch_size, per_slot, resident_items(cus, head_dim, row_blocks)));
-  if (batch_size * per_slot > kMaxCounters || !states_fit((runs / p.chunk_runs + batch_size) * per_slot * rows, head_dim)) p.chunk_runs = 1 << 30;
-  const int64_t slots = runs / p.chunk_runs + batch_size;
+  p.chunk_runs = static_cast<uint32_t>(pick_chunk_runs(runs, batch_size, per_slot, resident_items(cus, head_dim, row_blocks), 2 * cus, &p.fit_items));
+  if (batch_size * per_slot > kMaxCounters || !states_fit((runs / p.chunk_runs + batch_size) * per_slot * rows, head_dim)) {
+    p.chunk_runs = 1 << 30;
+    p.fit_items = 0;
+  }
+  if (batch_size <= 64 && forced_chunk() == 0 && p.fit_items == 0) {
+    const int64_t whole = runs * per_slot * 11 / (20 * cus);  // an equal share of two items a compute unit, and a tenth
+    if (whole > p.chunk_runs) p.whole_runs = static_cast<uint32_t>(std::min<int64_t>(whole, 1 << 20));
+  }
+  const int64_t slots = p.fit_items > 0 ? p.fit_items : runs / p.chunk_runs + batch_size;
   KV_CHECK(slots * per_slot <= kMaxItems) << what << ": too many work items";
   const hipStream_t s = as_stream(stream);
-  const ScratchLease ws = lease_states(what, p, s, runs > p.chunk_runs ? slots * per_slot * rows : 0, head_dim);
+  const ScratchLease ws = lease_states(what, p, s, runs > p.chunk_runs || p.fit_items > 0 ? slots * per_slot * rows : 0, head_dim);
   launch_attention<false>(p, head_dim, row_blocks, dim3(static_cast<unsigned>(slots * per_slot)), s);
   KV_API_END();
 }
