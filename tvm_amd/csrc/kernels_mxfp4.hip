@@ -1004,9 +1004,9 @@ static int64_t forced_chunk() {
 //  * Few sequences, long: the shortest chunks with which there are two items a compute unit, as the device finds from the lengths
 //    (fit_items).  Two read faster than the four that fit, and a few items more than two, all started together, give some units
 //    three (32 x U[2048,16384]: 67, with chunks of 360 runs 87; 8 x 81920, 64 / 8: 125, with four a unit 135).
-//  * Many, long: all of the room, once.
-//  * Between them sequences of unlike lengths leave workgroups over at the end: about two items a sequence.  Where none is
-//    longer than its share, sequences are left whole (whole_runs: 64 x 4096 57 -> 51, 64 x 8192 of dim 64 66 -> 62).
+//  * More of them: sequences of unlike lengths leave workgroups over at the end, so that each has about two items, of 256 runs
+//    at most (48 x U[20000,60000]: 355, with 900 runs 420; 64 x U[2048,16384]: 133, with 392 runs 141).  Where none is longer
+//    than its share, sequences are left whole (whole_runs: 64 x 4096 57 -> 51, 64 x 8192 of dim 64 66 -> 62).
 // Measured in us, 32 / 8 heads of dim 128 unless said, runs an item -> time, * = this rule:
 //   1 x 500 tokens        8: 7.2   40*: 6.8                            24 x U[500,2500], 40 / 40 of dim 64   48: 37  96*: 32
 //   1 x 2000              8: 8.7   16*: 8.4   32: 9.3   64: 12.0       1 x 32768    32: 19.1  64*: 16.2  128: 19.0
@@ -1023,14 +1023,14 @@ static int64_t pick_chunk_runs(int64_t runs, int64_t batch, int64_t per_slot, in
   };
   const int64_t avg = runs / batch;
   const int64_t least = steps(static_cast<int64_t>(std::sqrt(2.0 * static_cast<double>(avg))));
-  const int64_t small = for_items(resident / 2), full = for_items(resident), two = for_items(two_each);
-  int64_t chunk = std::max<int64_t>(96, steps(avg * 5 / 8));
+  const int64_t small = for_items(resident / 2), two = for_items(two_each);
+  int64_t chunk = std::min<int64_t>(std::max<int64_t>(96, steps(avg * 5 / 8)), 256);
   if (avg <= 40) chunk = std::max<int64_t>(small, 40);
   else if (small <= 48) chunk = std::max(small, least);
   else if (batch <= 64 && 2 * batch * per_slot <= two_each && two <= 1 << 20) {
     chunk = two;
     *fit_items = static_cast<int>(two_each / per_slot);
-  } else if (avg >= 4 * full) chunk = std::max(full, least);
+  }
   return std::min<int64_t>(chunk, 1 << 20);
 }
 
