@@ -22,6 +22,7 @@
 
 #include "kernels_common.cuh"
 #include "runtime_support.h"
+#include "exact_division.h"
 
 namespace tvmkv {
 
@@ -178,8 +179,7 @@ struct Mxfp4Params {
   int causal;
   int page_size;
   uint32_t runs_per_page;
-  uint32_t run_magic;   // 2^32 / runs_per_page, rounded up, or 0 for 1
-  uint32_t run_mask;    // all bits for 1
+  ExactDivision page_of_run;  // by runs_per_page
   float inv_group;
   uint32_t chunk_runs;  // decode: most keys of a work item, in runs; a multiple of 8
   int fit_items;        // decode: > 0: chunks as short as leave so many items a row block and kv head, chunk_runs at most
@@ -393,8 +393,8 @@ __global__ __launch_bounds__(256, mxfp4_waves(D, RB)) void mxfp4_attn_kernel(Mxf
 
   // The arguments in one trip; read where they are used they are a dozen, one behind the other.
   asm volatile("" ::"s"(p.q), "s"(p.pages), "s"(p.page_indptr), "s"(p.page_values), "s"(p.last_page_len), "s"(p.batch), "s"(p.h_q),
-               "s"(p.h_kv), "s"(p.group), "s"(p.page_size), "s"(p.runs_per_page), "s"(p.run_magic), "s"(p.run_mask), "s"(p.scale_log2),
-               "s"(p.q_sign));
+               "s"(p.h_kv), "s"(p.group), "s"(p.page_size), "s"(p.runs_per_page), "s"(p.page_of_run.magic), "s"(p.page_of_run.shift),
+               "s"(p.page_of_run.mask), "s"(p.scale_log2), "s"(p.q_sign));
   if constexpr (PREFILL) asm volatile("" ::"s"(p.q_indptr), "s"(p.causal), "s"(p.shares));
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
@@ -489,7 +489,7 @@ __global__ __launch_bounds__(256, mxfp4_waves(D, RB)) void mxfp4_attn_kernel(Mxf
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const uint32_t at = min(run + 8 * lane + h, run_hi - 1);
-      const uint32_t nth = __umulhi(at, p.run_magic) + (at & p.run_mask);
+      const uint32_t nth = p.page_of_run(at);
       codes16[h] = p.page_values[page_begin + nth];
       scales16[h] = at - nth * p.runs_per_page;
     }
@@ -1097,9 +1097,8 @@ static Mxfp4Params attn_params(const char* what, const void* q, const void* page
   p.group = h_q / h_kv;
   p.page_size = page_size;
   p.runs_per_page = page_size / kRun;
-  p.run_mask = p.runs_per_page == 1 ? ~0u : 0;
+  p.page_of_run = ExactDivision::by(p.runs_per_page);
   p.inv_group = 1.f / static_cast<float>(p.group);
-  p.run_magic = p.runs_per_page == 1 ? 0 : static_cast<uint32_t>(((uint64_t{1} << 32) + p.runs_per_page - 1) / p.runs_per_page);
   // The kernel takes maxima of scores that are not scaled yet and masks with -inf: a scale below 0 goes to q, and one of
   // 0 (all weights equal) becomes one that is as good as 0.
   p.scale_log2 = std::max(std::fabs(static_cast<float>(sm_scale)) * kLog2e, 1e-30f);
