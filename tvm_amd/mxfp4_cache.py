@@ -46,6 +46,7 @@ class Mxfp4KVCache:
         return get_global_func("vm.builtin." + name)(self._host, *args)
 
     def clear(self):
+        self._step = None
         self._verb("kv_state_clear")
         self._copied = 0
 
@@ -78,6 +79,7 @@ class Mxfp4KVCache:
 
     # ---- a step --------------------------------------------------------------------------------------------------
     def begin_forward(self, seq_ids, append_lengths):
+        self._step = None  # until the new one is complete
         self._verb("kv_state_begin_forward", seq_ids, append_lengths)
         flags, total, places = self._host.flags(), 0, []
 
@@ -116,8 +118,8 @@ class Mxfp4KVCache:
         return [(places[i][0], sum(n for _, n in places[i][1])) for i in which]
 
     def end_forward(self):
-        self._verb("kv_state_end_forward")
         self._step = None
+        self._verb("kv_state_end_forward")
 
     def attention_with_fused_qkv(self, layer_id, sm_scale, qkv, out):
         """qkv (rows, num_qo_heads + 2 num_kv_heads, head_dim) of the step's tokens: rotates, appends to the layer's pages and
