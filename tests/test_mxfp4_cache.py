@@ -45,3 +45,12 @@ def test_no_step_is_left_after_end_forward():
     cache.begin_forward([0], [3])
     cache.end_forward()
     refuses_attention(cache, 3)
+
+
+@pytest.mark.parametrize("layer", [-1, 2])
+def test_a_layer_that_the_cache_does_not_have_is_refused(layer):
+    cache = cache_of()
+    cache.add_sequence(0)
+    cache.begin_forward([0], [3])
+    with pytest.raises(KVError, match="layer id .* out of range"):
+        attend(cache, 3, layer)

@@ -127,6 +127,8 @@ class Mxfp4KVCache:
         step = self._step
         if step is None:
             raise KVError(-1, "attention_with_fused_qkv belongs between begin_forward and end_forward")
+        if not 0 <= layer_id < self.num_layers:
+            raise KVError(-1, f"layer id {layer_id} out of range")
         rows, hq, hkv, d = step["rows"], self.num_qo_heads, self.num_kv_heads, self.head_dim
         for name, t, heads in (("qkv", qkv, hq + 2 * hkv), ("out", out, hq)):
             if tuple(t.shape) != (rows, heads, d):
