@@ -54,3 +54,14 @@ def test_a_layer_that_the_cache_does_not_have_is_refused(layer):
     cache.begin_forward([0], [3])
     with pytest.raises(KVError, match="layer id .* out of range"):
         attend(cache, 3, layer)
+
+
+@pytest.mark.parametrize("changes, text", [
+    (dict(head_dim=80), "head_dim 80 is not built"),
+    (dict(cache_config=[4, 256, 64, 24, 0]), "page_size must be a multiple of 16, got 24"),
+    (dict(num_qo_heads=5), "5 query heads"),
+    (dict(num_layers=0), "0 layers"),
+])
+def test_shapes_that_the_kernels_do_not_have_are_refused_before_memory_is_taken(changes, text):
+    with pytest.raises(KVError, match=text):
+        cache_of(**changes)

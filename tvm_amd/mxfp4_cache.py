@@ -29,6 +29,12 @@ class Mxfp4KVCache:
                  rope_theta=1e4, device="cuda"):
         if rope_mode == RopeMode.INLINE:
             raise KVError(-2, "a 4-bit cache stores rotated keys: rope_mode INLINE is not built")
+        if head_dim not in (64, 96, 128, 256):
+            raise KVError(-2, f"a 4-bit cache: head_dim {head_dim} is not built (64, 96, 128, 256)")
+        if cache_config[3] <= 0 or cache_config[3] % 16 != 0:
+            raise KVError(-2, f"a 4-bit cache: page_size must be a multiple of 16, got {cache_config[3]}")
+        if num_layers <= 0 or num_kv_heads <= 0 or num_qo_heads <= 0 or num_qo_heads % num_kv_heads != 0:
+            raise KVError(-1, f"a 4-bit cache: bad shape: {num_layers} layers, {num_qo_heads} query heads, {num_kv_heads} kv heads")
         self.num_layers, self.num_qo_heads, self.num_kv_heads, self.head_dim = num_layers, num_qo_heads, num_kv_heads, head_dim
         self.rope = (rope_mode == RopeMode.NORMAL, float(rope_scale), float(rope_theta))
         self.sliding_windows = bool(cache_config[4])
