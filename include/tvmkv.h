@@ -516,6 +516,10 @@ int tvmkv_release_scratch(void* stream);
  * are tagged with the low 32 bits of that count; the tests set it just below 2^32 and run launches across
  * the wrap. */
 int tvmkv_debug_set_scratch_launches(uint64_t launches);
+/* Test aid (no counterpart in the reference): leaves the arrival counters of every pooled scratch buffer of the current
+ * device, by a kernel on the buffer's stream, as a last launch that was abandoned after so many arrivals at each of them
+ * leaves them. */
+int tvmkv_debug_abandon_scratch_launches(uint32_t arrivals);
 /* The same arithmetic on the host alone: advances *launches and returns the epoch of that launch (never
  * 0); *wrapped = 1 when the epochs started over, which is when the launchers clear the counters. */
 uint32_t tvmkv_debug_next_scratch_epoch(uint64_t* launches, int32_t* wrapped);

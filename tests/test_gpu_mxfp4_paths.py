@@ -4,10 +4,12 @@ import numpy as np
 import pytest
 import torch
 
+import tvm_amd
 from oracle import mxfp4
 from tests.gpu_util import DEV, dev, host, i32
 from tests.test_gpu_mxfp4 import Pool, compare, rows_like
 from tvm_amd import kernels
+from tvm_amd._lib import check
 
 pytestmark = pytest.mark.gpu
 
@@ -31,3 +33,40 @@ def test_pages_of_many_runs(page):
     compare(q, [3], small, True, host(out), host(lse), 0.125)
     kernels.mxfp4_batch_decode_paged_kv(dev(q[:1]), pool, i32([0, 3]), i32(ids), info, out[:1], lse[:1], 0.125)
     compare(q[:1], [1], small, False, host(out[:1]), host(lse[:1]), 0.125)
+
+
+@pytest.mark.parametrize("arrivals", [1, 2, 5])
+def test_launches_after_an_abandoned_one_join_all_their_states(arrivals):
+    """Counters that an earlier launch left half way, at every buffer of the stream, of the fp16 decode kernel as well."""
+    rng = np.random.default_rng(arrivals)
+    pool = Pool(rng, [3000, 40, 1700], 2, 16, 128)
+    pages, indptr, ids, info = pool.device()
+    q = rng.standard_normal((3, 8, 128)).astype(np.float16)
+    rows = np.repeat(q, 2, 0)
+    d_q, d_rows = dev(q), dev(rows)
+    others = -d_q, -d_rows
+    fp16_pages = torch.randn((len(pool.pages), 2, 2, 16, 128), device=DEV).half()
+    zeros = torch.zeros(3, dtype=torch.int32, device=DEV)
+
+    def run(d_q=d_q, d_rows=d_rows):
+        o, s = ([torch.full((n, 8, *rest), 7.0, dtype=t, device=DEV) for n in (3, 3, 6)] for rest, t in (((128,), torch.float16), ((), torch.float32)))
+        kernels.batch_decode_paged_kv(d_q, fp16_pages, indptr, ids, info, zeros, zeros, o[0], s[0], 0, 1.0, 1e4, 0.1)
+        kernels.mxfp4_batch_decode_paged_kv(d_q, pages, indptr, ids, info, o[1], s[1], 0.1)
+        kernels.mxfp4_batch_prefill_paged_kv(d_rows, i32([0, 2, 4, 6]), pages, indptr, ids, info, o[2], s[2], 0, 0.1)
+        return [host(t) for t in o + s]
+
+    previous = [tvm_amd.set_option(name, value) for name, value in (("decode_chunk_pages", 8), ("prefill_kv_splits", 7))]
+    try:
+        run()
+        check(tvm_amd.lib().tvmkv_debug_abandon_scratch_launches(0))  # whole, whatever the tests before left
+        want = run()
+        for _ in range(3):
+            run(*others)  # what is joined too early is these rows' states
+            torch.cuda.synchronize()
+            check(tvm_amd.lib().tvmkv_debug_abandon_scratch_launches(arrivals))
+            assert all(np.array_equal(a, b) for a, b in zip(run(), want))
+        compare(q, [1] * 3, pool, False, want[1], want[4], 0.1)
+        compare(rows, [2] * 3, pool, False, want[2], want[5], 0.1)
+    finally:
+        for name, value in zip(("decode_chunk_pages", "prefill_kv_splits"), previous):
+            tvm_amd.set_option(name, value)

@@ -170,7 +170,7 @@ struct Mxfp4Params {
   // states of work items that have only some of a row's keys: (slot, row block, kv head, row of the block)
   float* part_o;   // D each, not normalised
   float* part_ml;  // reference point, sum
-  unsigned* arrivals;  // of the work items of some rows; 0 between launches
+  unsigned long long* arrivals;  // of the work items of some rows: epoch << 32 | those that have delivered their states
   int batch;
   int h_q;
   int h_kv;
@@ -185,6 +185,7 @@ struct Mxfp4Params {
   int fit_items;        // decode: > 0: chunks as short as leave so many items a row block and kv head, chunk_runs at most
   uint32_t whole_runs;  // decode: where no sequence has more runs than these, sequences are left whole
   int shares;           // prefill: work items that share the keys of a row block
+  uint32_t epoch;       // of the launch, if its work items share rows
   float scale_log2;     // > 0: |sm_scale| log2(e), never 0
   uint32_t q_sign;      // of sm_scale, at the sign bits of two fp16
 };
@@ -733,6 +734,10 @@ __global__ __launch_bounds__(256, mxfp4_waves(D, RB)) void mxfp4_attn_kernel(Mxf
   // ---- the four waves' states become one ------------------------------------------------------
   const uint32_t state = ((static_cast<uint32_t>(PREFILL ? slot * p.shares + chunk : slot) * blocks + (PREFILL ? 0 : block)) * p.h_kv + kvh) * R;
   SharedStates part_o(p.part_o), part_ml(p.part_ml);
+  unsigned long long* const counter = p.arrivals + static_cast<int64_t>(PREFILL ? slot : b * blocks + block) * p.h_kv + kvh;
+  // A word that an older launch left, also one that was abandoned half way, becomes (epoch, 0); on its way while the states merge.
+  if (chunks > 1 && threadIdx.x == 0)
+    __hip_atomic_fetch_max(counter, static_cast<unsigned long long>(p.epoch) << 32, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   const auto finish = [&](int r, int f, float most, float sum, float4_t acc) {  // elements f.. f + 3 of row r
     const int token = token_of(r);
     const int64_t out = static_cast<int64_t>(q_begin + token0 + token) * p.h_q + kvh * p.group + head0 + r - token * p.group;
@@ -800,9 +805,10 @@ __global__ __launch_bounds__(256, mxfp4_waves(D, RB)) void mxfp4_attn_kernel(Mxf
   wait_vmcnt<0>();
   __syncthreads();
   if (threadIdx.x == 0) {
-    // the counter goes back to 0 by itself when the last one arrives
-    unsigned* counter = p.arrivals + (PREFILL ? slot : b * blocks + block) * p.h_kv + kvh;
-    sm_last = __builtin_amdgcn_atomic_inc32(counter, chunks - 1, __ATOMIC_RELAXED, "agent") == static_cast<unsigned>(chunks - 1);
+    const unsigned long long before = __hip_atomic_fetch_add(counter, 1ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    sm_last = static_cast<uint32_t>(before) == static_cast<uint32_t>(chunks - 1);
+    // nobody of this launch touches the counter again: back to (epoch, 0), from which a replay of the launch counts
+    if (sm_last) __hip_atomic_store(counter, static_cast<unsigned long long>(p.epoch) << 32, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
   __syncthreads();
   if (!sm_last) return;
@@ -960,21 +966,21 @@ static void launch_attention(const Mxfp4Params& p, int d, int row_blocks, dim3 g
   }
 }
 
-// Scratch memory of a launch: arrival counters (0 when it is allocated and, since the last to arrive wraps its counter, after
-// every launch), then the states.
+// Scratch memory of a launch: arrival counters, which need no clearing between launches (runtime_support.h), then the states.
 constexpr int64_t kMaxCounters = 1 << 18;
 constexpr int64_t kMaxItems = (int64_t{1} << 24) - 1;  // a launch has fewer than 2^32 threads
 static bool states_fit(int64_t states, int d) { return states * d < int64_t{1} << 30; }  // 32-bit addresses of bytes
 static ScratchLease lease_states(const char* what, Mxfp4Params& p, hipStream_t s, int64_t states, int d) {
   if (states == 0) return {};  // no row's keys are shared
   KV_CHECK(states_fit(states, d)) << what << ": too many work items";
-  constexpr size_t counter_bytes = kMaxCounters * sizeof(unsigned);
+  constexpr size_t counter_bytes = kMaxCounters * sizeof(unsigned long long);
   const size_t o_bytes = static_cast<size_t>(states) * d * sizeof(float);
   // the first buffer holds the states of any launch whose items fill the chip once, so that a stream that has run one that
   // shares keys can capture the others
   const size_t at_least = counter_bytes + static_cast<size_t>(2048) * 16 * (d + 2) * sizeof(float);
   ScratchLease ws = lease_scratch(kScratchMxfp4, s, counter_bytes + o_bytes + static_cast<size_t>(states) * 2 * sizeof(float), counter_bytes, at_least);
-  p.arrivals = reinterpret_cast<unsigned*>(ws.ptr);
+  p.arrivals = reinterpret_cast<unsigned long long*>(ws.ptr);
+  p.epoch = ws.epoch;
   p.part_o = reinterpret_cast<float*>(ws.ptr + counter_bytes);
   p.part_ml = reinterpret_cast<float*>(ws.ptr + counter_bytes + o_bytes);
   return ws;

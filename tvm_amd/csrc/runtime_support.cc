@@ -52,10 +52,10 @@ std::map<std::tuple<int, hipStream_t, int>, Scratch> g_scratch;
 // Buffers that a captured graph may still name after their entry has grown: kept until the process ends.
 std::vector<char*> g_retired;
 
-__global__ void zero_words_kernel(unsigned long long* words, size_t count) {
+__global__ void fill_words_kernel(unsigned long long* words, size_t count, unsigned long long value) {
   for (size_t i = blockIdx.x * static_cast<size_t>(blockDim.x) + threadIdx.x; i < count;
        i += static_cast<size_t>(gridDim.x) * blockDim.x) {
-    words[i] = 0ull;
+    words[i] = value;
   }
 }
 
@@ -82,12 +82,13 @@ uint32_t next_scratch_epoch(uint64_t* launches, bool* wrapped) {
   return static_cast<uint32_t>(*launches);
 }
 
-void zero_scratch_counters(char* ptr, size_t counter_bytes, hipStream_t stream) {
+static void fill_scratch_counters(char* ptr, size_t counter_bytes, unsigned long long value, hipStream_t stream) {
   if (counter_bytes == 0) return;
   const size_t words = counter_bytes / sizeof(unsigned long long);
-  hipLaunchKernelGGL(zero_words_kernel, dim3(64), dim3(256), 0, stream, reinterpret_cast<unsigned long long*>(ptr), words);
+  hipLaunchKernelGGL(fill_words_kernel, dim3(64), dim3(256), 0, stream, reinterpret_cast<unsigned long long*>(ptr), words, value);
   HIP_CHECK(hipGetLastError());
 }
+void zero_scratch_counters(char* ptr, size_t counter_bytes, hipStream_t stream) { fill_scratch_counters(ptr, counter_bytes, 0, stream); }
 
 ScratchLease lease_scratch(ScratchUser user, hipStream_t stream, size_t bytes, size_t counter_bytes, size_t at_least) {
   int dev = 0;
@@ -167,6 +168,17 @@ void count_joint_launch() { g_joint_launches.fetch_add(1, std::memory_order_rela
 void debug_set_scratch_launches(uint64_t launches) {
   std::lock_guard<std::recursive_mutex> lock(g_scratch_mutex);
   for (auto& entry : g_scratch) entry.second.launches = launches;
+}
+
+void debug_abandon_scratch_launches(uint32_t arrivals) {
+  int dev = 0;
+  HIP_CHECK(hipGetDevice(&dev));
+  std::lock_guard<std::recursive_mutex> lock(g_scratch_mutex);
+  for (auto& [key, s] : g_scratch) {
+    if (std::get<0>(key) != dev || s.ptr == nullptr) continue;
+    const unsigned long long epoch = static_cast<uint32_t>(s.launches);
+    fill_scratch_counters(s.ptr, s.counter_bytes, epoch << 32 | arrivals, std::get<1>(key));
+  }
 }
 
 // Work items of a decode launch: every item pays ~2 us of fixed cost (locating its sequence, q, the
@@ -340,6 +352,12 @@ uint32_t tvmkv_debug_next_scratch_epoch(uint64_t* launches, int32_t* wrapped) {
   const uint32_t epoch = tvmkv::next_scratch_epoch(launches, &w);
   *wrapped = w ? 1 : 0;
   return epoch;
+}
+
+int tvmkv_debug_abandon_scratch_launches(uint32_t arrivals) {
+  KV_API_BEGIN();
+  tvmkv::debug_abandon_scratch_launches(arrivals);
+  KV_API_END();
 }
 
 int tvmkv_debug_joint_launches(uint64_t* launches) {

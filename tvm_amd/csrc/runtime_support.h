@@ -90,6 +90,9 @@ void zero_scratch_counters(char* ptr, size_t counter_bytes, hipStream_t stream);
 void count_joint_launch();
 // Test aid: sets the launch count of every pooled buffer (to run a launch across the epoch wrap).
 void debug_set_scratch_launches(uint64_t launches);
+// Test aid: leaves the counters of every pooled buffer of the current device as a last launch that was abandoned after so many
+// arrivals at each of them leaves them.
+void debug_abandon_scratch_launches(uint32_t arrivals);
 
 // A kernel that is launched with more dynamic shared memory than every function may have by itself (48 KB): said once per
 // kernel, which is a template argument so that kernels of one type do not share the flag, and again after a call that failed.
