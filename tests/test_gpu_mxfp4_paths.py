@@ -70,3 +70,29 @@ def test_launches_after_an_abandoned_one_join_all_their_states(arrivals):
     finally:
         for name, value in zip(("decode_chunk_pages", "prefill_kv_splits"), previous):
             tvm_amd.set_option(name, value)
+
+
+@pytest.mark.parametrize("begin, batch", [(90, 40), (90, 400), (90, 560)])
+def test_some_sequences_of_a_larger_table(begin, batch):
+    """page_indptr and q_indptr that do not begin at 0: the rest of the tables stays where it is."""
+    rng = np.random.default_rng(batch)
+    stored, q_lens = rng.integers(1, 50, 660).tolist(), rng.integers(0, 4, 660).tolist()
+    pool = Pool(rng, stored, 1, 16, 64)
+    pages, indptr, ids, info = pool.device()
+    some = slice(begin, begin + batch)
+    q = rng.standard_normal((660, 2, 64)).astype(np.float16)
+    out, lse = torch.zeros((batch, 2, 64), dtype=torch.float16, device=DEV), torch.zeros((batch, 2), device=DEV)
+    kernels.mxfp4_batch_decode_paged_kv(dev(q[some]), pages, indptr[begin:begin + batch + 1], ids, info[some], out, lse, 0.125)
+    whole = Pool.__new__(Pool)
+    whole.__dict__.update(pool.__dict__, indptr=pool.indptr[begin:begin + batch + 1], info=pool.info[some])
+    compare(q[some], [1] * batch, whole, False, host(out), host(lse), 0.125)
+    q_indptr = np.concatenate(([0], np.cumsum(q_lens)))
+    q = rng.standard_normal((q_indptr[-1], 2, 64)).astype(np.float16)
+    out, lse = torch.full(q.shape, 7.0, dtype=torch.float16, device=DEV), torch.full(q.shape[:2], 7.0, device=DEV)
+    kernels.mxfp4_batch_prefill_paged_kv(dev(q), i32(q_indptr[begin:begin + batch + 1]), pages, indptr[begin:begin + batch + 1], ids, info[some],
+                                         out, lse, 1, 0.125)
+    rows = slice(q_indptr[begin], q_indptr[begin + batch])
+    compare(q[rows], q_lens[some], whole, True, host(out)[rows], host(lse)[rows], 0.125)
+    others = np.ones(len(q), bool)
+    others[rows] = False
+    assert (host(out)[others] == 7).all() and (host(lse)[others] == 7).all()

@@ -205,7 +205,7 @@ __device__ __forceinline__ int prefix_sum(int x) {
 // items, one behind the other without gaps: the launch has more workgroups than items, since only the device knows the
 // lengths, and spare ones between the others put the real ones on some of the compute units (64 sequences of 4096 tokens, 512
 // items: 79 us with a spare one beside every real one, 50 without).  The wave adds the items up, a sequence a lane, or up
-// to 8 neighbours a lane; with more sequences each has a fixed range of items instead, spare_begin(i, indptr[i]) onwards, and
+// to 8 neighbours a lane; with more sequences each has a fixed range of items instead, spare_begin(i, indptr[i] - indptr[0]) onwards, and
 // the wave looks for the last that begins at or before the slot.
 struct Sequence {
   int index, begin;  // begin: its first work item
@@ -242,16 +242,17 @@ __device__ __forceinline__ Sequence sequence_of(const Mxfp4Params& p, int slot, 
       at = min(n, p.batch - 1);
     } else {
       int lo = 0, n = p.batch;
+      const int base = indptr[0];  // (of a part of a larger table it need not be 0)
       while (n > 1) {
         const int stride = (n + 63) >> 6;
         const int i = lo + lane * stride;
-        const bool hit = i < lo + n && spare_begin(i, indptr[i]) <= slot;
+        const bool hit = i < lo + n && spare_begin(i, indptr[i] - base) <= slot;
         const int first = lo + (max(static_cast<int>(__popcll(__ballot(hit))), 1) - 1) * stride;
         n = min(stride, lo + n - first);
         lo = first;
       }
       at = lo;
-      begin = spare_begin(at, indptr[at]);
+      begin = spare_begin(at, indptr[at] - base);
     }
     who = 0;
   } else {
