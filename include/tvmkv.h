@@ -488,6 +488,10 @@ int tvmkv_mxfp4_batch_prefill_paged_kv(const void* q, const int32_t* q_indptr, c
  *   step_route             > 0: the route of the cache object's prefill steps instead of the one that an estimate
  *                          from the lengths prefers, where a step can take it: 1 the general launches, 2 prompts
  *                          and decoding sequences apart, 3 over gathered keys (tests, measurements).
+ *   mxfp4_row_blocks       > 0: blocks of 16 rows (query token, query head of a group) that a work item of the
+ *                          4-bit attention launches takes, at most 3, at head dim 256 at most 2; 0 = from the shapes.
+ *                          Of these options they also follow decode_chunk_pages (in runs of 16 tokens, whatever the
+ *                          page size) and prefill_kv_splits.
  *   no_fused_decode_step   != 0: the cache object runs a plain decode step as two launches (split + RoPE +
  *                          append, then decode attention) instead of tvmkv_fused_decode_step */
 int tvmkv_set_option(const char* name, int64_t value);

@@ -1,5 +1,7 @@
 """The kernels of the 4-bit cache on the paths that small launches do not take by themselves, against the definition in 64 bits
 (oracle/mxfp4.py) within the bounds that tests/test_gpu_mxfp4.py derives."""
+import contextlib
+
 import numpy as np
 import pytest
 import torch
@@ -7,7 +9,7 @@ import torch
 import tvm_amd
 from oracle import mxfp4
 from tests.gpu_util import DEV, dev, host, i32
-from tests.test_gpu_mxfp4 import Pool, compare, rows_like
+from tests.test_gpu_mxfp4 import Pool, bound, compare, decode, prefill, rows_like
 from tvm_amd import kernels
 from tvm_amd._lib import check
 
@@ -96,3 +98,163 @@ def test_some_sequences_of_a_larger_table(begin, batch):
     others = np.ones(len(q), bool)
     others[rows] = False
     assert (host(out)[others] == 7).all() and (host(lse)[others] == 7).all()
+
+
+# ---- every number of rows that a work item takes ------------------------------------------------------------------------
+
+EVERY_ITEM = [(d, blocks) for d in (64, 96, 128, 256) for blocks in (1, 2, 3) if d < 256 or blocks < 3]
+
+
+@contextlib.contextmanager
+def options(**values):
+    previous = {name: tvm_amd.set_option(name, value) for name, value in values.items()}
+    try:
+        yield
+    finally:
+        for name, value in previous.items():
+            tvm_amd.set_option(name, value)
+
+
+def compare_where_finite(q, q_lens, pool, causal, out, lse, sm_scale):
+    """NaN exactly where the definition has NaN, and elsewhere within the bound."""
+    rows = mxfp4.rows_of(pool.pages, pool.d)
+    want, want_lse = mxfp4.attention(q, q_lens, rows, pool.indptr, pool.ids, pool.info, causal, sm_scale)
+    assert np.array_equal(np.isnan(out), np.isnan(want)) and np.array_equal(np.isnan(lse), np.isnan(want_lse))
+    off = np.abs(out.astype(np.float64) - want) - bound(q, q_lens, pool, causal, sm_scale)
+    assert np.nanmax(off, initial=-1.0) <= 0
+    assert np.nanmax(np.abs(lse - want_lse), initial=0.0) <= 5e-5
+
+
+@pytest.mark.parametrize("d, blocks", EVERY_ITEM)
+@pytest.mark.parametrize("chunk", [0, 8])
+def test_decode_of_every_item(d, blocks, chunk):
+    """Groups of 40 and 17 heads: whole and partly filled blocks of rows; sequences whole and in chunks of 128 tokens."""
+    rng = np.random.default_rng(d + blocks)
+    for group, stored in ((40, [0, 1, 33, 129, 700, 1500]), (17, [16, 300, 2]), (3, [500, 31])):
+        pool = Pool(rng, stored, 2, 16, d)
+        q = (1.5 * rng.standard_normal((len(stored), 2 * group, d))).astype(np.float16)
+        with options(mxfp4_row_blocks=blocks, decode_chunk_pages=chunk):
+            out, lse = decode(q, pool, d ** -0.5)
+        compare(q, [1] * len(stored), pool, False, out, lse, d ** -0.5)
+
+
+@pytest.mark.parametrize("d, blocks", EVERY_ITEM)
+@pytest.mark.parametrize("causal, shares", [(1, 1), (0, 1), (1, 3)])
+def test_prefill_of_every_item(d, blocks, causal, shares):
+    """Prompts that end in every part of an item of 16, 32 or 48 rows, with and without keys in front of them."""
+    rng = np.random.default_rng(d + blocks + shares)
+    stored, q_lens = [130, 5, 40, 0, 470, 70, 33, 16, 3], [130, 5, 17, 2, 11, 0, 33, 16, 6]
+    for group in (1, 5):
+        pool = Pool(rng, stored, 2, 32, d)
+        q = (1.5 * rng.standard_normal((sum(q_lens), 2 * group, d))).astype(np.float16)
+        with options(mxfp4_row_blocks=blocks, prefill_kv_splits=shares):
+            out, lse = prefill(q, q_lens, pool, causal, d ** -0.5)
+        compare(q, q_lens, pool, causal, out, lse, d ** -0.5)
+
+
+@pytest.mark.parametrize("d, blocks", EVERY_ITEM)
+def test_windows_with_sinks_of_every_item(d, blocks):
+    rng = np.random.default_rng(7 * d + blocks)
+    stored, q_lens = [120, 7, 45, 400, 60, 3], [40, 7, 30, 1, 44, 3]
+    for sinks, evicted, shares, chunk in ((4, 13, 1, 0), (20, 50, 2, 8)):
+        pool = Pool(rng, stored, 1, 16, d, sinks, evicted)
+        for causal in (1, 0):
+            q = (1.5 * rng.standard_normal((sum(q_lens), 6, d))).astype(np.float16)
+            with options(mxfp4_row_blocks=blocks, prefill_kv_splits=shares):
+                out, lse = prefill(q, q_lens, pool, causal, d ** -0.5)
+            compare(q, q_lens, pool, causal, out, lse, d ** -0.5)
+        q = (1.5 * rng.standard_normal((len(stored), 20, d))).astype(np.float16)
+        with options(mxfp4_row_blocks=blocks, decode_chunk_pages=chunk):
+            out, lse = decode(q, pool, d ** -0.5)
+        compare(q, [1] * len(stored), pool, False, out, lse, d ** -0.5)
+
+
+@pytest.mark.parametrize("d, blocks", EVERY_ITEM)
+@pytest.mark.parametrize("split", [False, True])
+def test_what_is_not_finite_stays_with_its_rows_in_every_item(d, blocks, split):
+    """NaN keys and values behind the end, among evicted tokens and behind some of an item's queries reach the rows that see
+    them and no others; so do NaN and infinite queries."""
+    rng = np.random.default_rng(3 * d + blocks)
+    stored, q_lens = [330, 100, 75], [60, 9, 40]
+    pool = Pool(rng, stored, 1, 16, d, 4, 20)
+    nan = np.full((1, 1, d), np.nan, np.float16)
+    for b, t in ((0, 330), (1, 100), (1, 5), (1, 23), (2, 79)):  # seen by nobody
+        pool.pages = mxfp4.append(pool.pages, nan, nan, [pool.slot(b, t)])
+    for b, t, what in ((0, 300, "v"), (0, 317, "k"), (2, 50, "v"), (2, 72, "kv")):  # by the later queries
+        k, v = rows_like(rng, 1, 1, d), rows_like(rng, 1, 1, d)
+        if "k" in what:
+            k[0, 0, 3] = np.inf
+        if "v" in what:
+            v[0, 0, d - 20] = np.nan
+        pool.pages = mxfp4.append(pool.pages, k, v, [pool.slot(b, t)])
+    q = rng.standard_normal((sum(q_lens), 5, d)).astype(np.float16)
+    q[62, 1, 9] = np.nan
+    with options(mxfp4_row_blocks=blocks, prefill_kv_splits=3 if split else 1, decode_chunk_pages=8 if split else 0):
+        for causal in (1, 0):
+            out, lse = prefill(q, q_lens, pool, causal, 0.1)
+            compare_where_finite(q, q_lens, pool, causal, out, lse, 0.1)
+        q = rng.standard_normal((3, 20, d)).astype(np.float16)
+        q[1, 18] = np.nan
+        out, lse = decode(q, pool, 0.1)
+        compare_where_finite(q, [1] * 3, pool, False, out, lse, 0.1)
+
+
+@pytest.mark.parametrize("d, blocks", EVERY_ITEM)
+def test_items_of_more_than_512_runs(d, blocks):
+    """A wave's page ids are those of 64 steps of eight runs: it reads more of them on the way."""
+    rng = np.random.default_rng(d * blocks)
+    stored = [8193, 17000, 5]
+    pool = Pool(rng, stored, 1, 16, d)
+    q = (1.5 * rng.standard_normal((3, 18, d))).astype(np.float16)
+    with options(mxfp4_row_blocks=blocks, decode_chunk_pages=2048, prefill_kv_splits=1):
+        out, lse = decode(q, pool, d ** -0.5)
+        compare(q, [1] * 3, pool, False, out, lse, d ** -0.5)
+        q = (1.5 * rng.standard_normal((7, 6, d))).astype(np.float16)
+        out, lse = prefill(q, [3, 3, 1], pool, 1, d ** -0.5)
+        compare(q, [3, 3, 1], pool, True, out, lse, d ** -0.5)
+
+
+@pytest.mark.parametrize("d, blocks", EVERY_ITEM)
+def test_rows_of_more_than_64_states(d, blocks):
+    """Joined 64 at a time: of 80, 129 and 64 chunks of 128 tokens."""
+    rng = np.random.default_rng(d * blocks + 1)
+    stored = [80 * 128, 128 * 128 + 1, 100, 64 * 128]
+    pool = Pool(rng, stored, 1, 16, d)
+    q = (1.5 * rng.standard_normal((4, 19, d))).astype(np.float16)
+    with options(mxfp4_row_blocks=blocks, decode_chunk_pages=8):
+        out, lse = decode(q, pool, d ** -0.5)
+    compare(q, [1] * 4, pool, False, out, lse, d ** -0.5)
+
+
+@pytest.mark.parametrize("batch", [64, 65, 130, 512, 513, 700])
+@pytest.mark.parametrize("blocks", [1, 3])
+def test_batches_whose_sequences_have_several_items(batch, blocks):
+    """Long sequences and prompts of several blocks at both ends of a batch and among the others, on every search path."""
+    rng = np.random.default_rng(batch + blocks)
+    stored = (rng.integers(0, 40, batch) * (rng.random(batch) < 0.8)).tolist()
+    for b in (0, 1, 7, 8, 9, batch // 2, batch - 2, batch - 1):
+        stored[b] = int(rng.integers(200, 1500))
+    pool = Pool(rng, stored, 1, 16, 64)
+    q = rng.standard_normal((batch, 20, 64)).astype(np.float16)
+    with options(mxfp4_row_blocks=blocks, decode_chunk_pages=8):
+        out, lse = decode(q, pool, 0.125)
+    compare(q, [1] * batch, pool, False, out, lse, 0.125)
+    q_lens = rng.integers(0, 3, batch).tolist()
+    for b in (0, 3, 4, batch // 2, batch - 1):
+        q_lens[b] = int(rng.integers(20, 70))
+    q = rng.standard_normal((sum(q_lens), 3, 64)).astype(np.float16)
+    for shares in (1, 2):
+        with options(mxfp4_row_blocks=blocks, prefill_kv_splits=shares):
+            out, lse = prefill(q, q_lens, pool, 1, 0.125)
+        compare(q, q_lens, pool, True, out, lse, 0.125)
+
+
+def test_more_row_blocks_than_there_are():
+    """More blocks than there are kernels for give the largest there is."""
+    rng = np.random.default_rng(2)
+    for d in (128, 256):
+        pool = Pool(rng, [100, 30], 1, 16, d)
+        q = rng.standard_normal((2, 50, d)).astype(np.float16)
+        with options(mxfp4_row_blocks=100):
+            compare(q, [1, 1], pool, False, *decode(q, pool, 0.1), 0.1)
+            compare(q, [1, 1], pool, True, *prefill(q, [1, 1], pool, 1, 0.1), 0.1)

@@ -991,8 +991,13 @@ static ScratchLease lease_states(const char* what, Mxfp4Params& p, hipStream_t s
 // dim 256: two at one): for few keys one, which starts and ends sooner; where they fill the chip the fewest items for the
 // group, of equal size.  32 sequences of U[1000,3000] tokens, 32 heads on one: 14.2 us with one block, 17.4 with two; 64 of
 // U[20000,40000]: 102 and 74.
+static int max_row_blocks(int d) { return d == 256 ? 2 : 3; }
+static int forced_row_blocks(int d) {
+  return static_cast<int>(std::min<int64_t>(std::max<int64_t>(option(kOptMxfp4RowBlocks), 0), max_row_blocks(d)));
+}
 static int decode_row_blocks(int cus, int64_t group, int64_t runs, int64_t h_kv, int d) {
-  const int64_t blocks = (group + 15) / 16, most = d == 256 ? 2 : 3;
+  if (forced_row_blocks(d) > 0) return forced_row_blocks(d);
+  const int64_t blocks = (group + 15) / 16, most = max_row_blocks(d);
   const int64_t items = (blocks + most - 1) / most;
   const int64_t fewest = (blocks + items - 1) / items;
   return runs * h_kv > 24 * resident_items(cus, d, static_cast<int>(fewest)) ? static_cast<int>(fewest) : 1;
@@ -1059,7 +1064,8 @@ static Cut cut_prefill(int cus, int64_t rows, int64_t batch, int64_t h_kv, int64
   const int64_t sequence = (rows + batch - 1) / batch;  // rows of one
   Cut best = {1, 1};
   double least = 1e30;
-  for (int blocks = 1; blocks <= (d == 256 ? 2 : 3); ++blocks) {
+  const int forced_blocks = forced_row_blocks(d);
+  for (int blocks = std::max(forced_blocks, 1); blocks <= (forced_blocks > 0 ? forced_blocks : max_row_blocks(d)); ++blocks) {
     const int64_t items = (sequence + 16 * blocks - 1) / (16 * blocks) * batch * h_kv;
     const int waves = mxfp4_waves(d, blocks);
     const double idle = (0.35 + 0.15 * blocks) * (d == 256 ? 2.8 : 1.0), start = 4.0 + 2.0 * blocks;

@@ -27,6 +27,7 @@ enum Option {
   kOptNoFusedDecodeStep,      // != 0: the cache object runs a decode step as split+RoPE+append and decode, two launches
   kOptStepRoute,              // > 0: the route of the cache object's steps instead of the one that the estimate prefers, where a
                               // step can take it: 1 the general launches, 2 prompts and decoding sequences apart, 3 gathered keys
+  kOptMxfp4RowBlocks,         // > 0: blocks of 16 rows of a work item of the 4-bit attention kernels, 0 = derived from the shapes
   kNumOptions
 };
 bool stream_is_capturing(hipStream_t stream);
