@@ -258,3 +258,16 @@ def test_more_row_blocks_than_there_are():
         with options(mxfp4_row_blocks=100):
             compare(q, [1, 1], pool, False, *decode(q, pool, 0.1), 0.1)
             compare(q, [1, 1], pool, True, *prefill(q, [1, 1], pool, 1, 0.1), 0.1)
+
+
+def test_more_shares_than_there_are():
+    """More shares than the option has give the most there are, as in the fp16 launches."""
+    rng = np.random.default_rng(4)
+    pool = Pool(rng, [9000, 30], 1, 16, 128)
+    q = rng.standard_normal((4, 2, 128)).astype(np.float16)
+    with options(prefill_kv_splits=64):
+        want = prefill(q, [2, 2], pool, 1, 0.1)
+    with options(prefill_kv_splits=100000):
+        out = prefill(q, [2, 2], pool, 1, 0.1)
+    assert all(np.array_equal(a, b) for a, b in zip(out, want))
+    compare(q, [2, 2], pool, True, *out, 0.1)

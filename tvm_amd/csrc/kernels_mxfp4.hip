@@ -1060,7 +1060,7 @@ struct Cut {
 };
 static Cut cut_prefill(int cus, int64_t rows, int64_t batch, int64_t h_kv, int64_t runs, int d) {
   const double t_full[4][3] = {{1.05, 1.18, 1.10}, {1.35, 1.23, 1.40}, {1.63, 1.28, 1.70}, {2.28, 2.94, 0}};
-  const int64_t forced = option(kOptPrefillKvSplits);
+  const int64_t forced = std::min<int64_t>(option(kOptPrefillKvSplits), 64);
   const int64_t sequence = (rows + batch - 1) / batch;  // rows of one
   Cut best = {1, 1};
   double least = 1e30;
