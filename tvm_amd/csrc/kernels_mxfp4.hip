@@ -141,7 +141,9 @@ __global__ __launch_bounds__(256) void mxfp4_read_kernel(const uint8_t* __restri
 // ------------------------------------------------------------------------------------------
 // Attention.  With s = sm_scale log2(e) q.k the output of a row is sum 2^(s - m) v / sum 2^(s - m) and its
 // log-sum-exp (base 2) m + log2(sum), for any m; sums, statistics and outputs in float32, the weights rounded to fp16
-// for the second matrix product (11 bits, as the output itself).
+// for the second matrix product (11 bits, as the output itself).  Their sum is of the weights before that rounding: outputs are
+// off by 2.4e-4 to 3e-4 of their root mean square, 2.0e-4 of it the output's own rounding; the sum of the rounded weights gives
+// 2.4e-4, and cost 5 % of prefill.
 //
 // A row of a kv head is (query token, query head of its group), token-major.  A workgroup of four waves takes up to
 // 16 RB rows of a kv head and a range of the sequence's keys, a wave every fourth step of 32 keys (two runs of 16
@@ -371,7 +373,9 @@ struct SharedStates {
 // meets a bank twice.  (At 8 banks the writes did, and a third of the tile's LDS cycles were conflicts.)
 constexpr int v_row(int d) { return d == 64 || d == 96 ? d + 8 : d + 24; }
 
-// Workgroups of a compute unit, by the registers of a work item of rb blocks of 16 rows.
+// Workgroups of a compute unit, four waves each, that a work item of rb blocks of 16 rows leaves registers for: the bound that the
+// kernels are compiled for, and what the rules below count on.  At head dim 64 the compiler needs fewer (126 registers for two
+// blocks, 163 to 167 for three), so that the hardware holds one more there; the rules' times were measured so.
 constexpr int mxfp4_waves(int d, int rb) { return d == 256 ? 2 : rb == 1 ? 4 : d == 64 && rb == 2 ? 3 : 2; }
 
 template <int D, int RB, bool PREFILL, bool ONCE>
@@ -383,8 +387,9 @@ __global__ __launch_bounds__(256, mxfp4_waves(D, RB)) void mxfp4_attn_kernel(Mxf
   constexpr int VW = D / VH;
   constexpr int VS = v_row(VW);
   static_assert(32 * VS * sizeof(half_t) >= 16 * VW * sizeof(float), "the merge buffer takes the V tile's place");
-  // Head dim 256 with two blocks of rows has registers for two waves a SIMD if q stays in LDS and one step's codes at a
-  // time in registers, the next ones loaded as soon as they are used up (one wave a SIMD: 540 TFLOP/s instead of 729).
+  // Head dim 256 with two blocks of rows: two waves a SIMD, with q in LDS and one step's codes at a time in registers, the next
+  // ones loaded as soon as they are used up (one wave a SIMD: 540 TFLOP/s instead of 729).  256 registers do not hold all of the
+  // rest: prefill keeps 15 values in scratch memory, decode 22.
   constexpr bool LEAN = D == 256 && RB == 2;
   constexpr int kJoinBytes = (R * 64 + 4 * R) * sizeof(float) + 256 * sizeof(float4_t);  // the join of states, below
   constexpr int kTileHalfs = std::max<int>(32 * VS, kJoinBytes / 8);
