@@ -271,3 +271,28 @@ def test_more_shares_than_there_are():
         out = prefill(q, [2, 2], pool, 1, 0.1)
     assert all(np.array_equal(a, b) for a, b in zip(out, want))
     compare(q, [2, 2], pool, True, *out, 0.1)
+
+
+@pytest.mark.parametrize("d", [64, 96, 128, 256])
+@pytest.mark.parametrize("k_scale, q_scale, v_scale", [(-18, 12, -21), (-22, 14, -22), (12, -11, 12), (11, 3, 11)])
+def test_rows_of_every_magnitude(d, k_scale, q_scale, v_scale):
+    """Values among fp16's subnormal numbers and near its largest, in keys and in values; scores that leave one key."""
+    rng = np.random.default_rng(d + k_scale)
+    stored, q_lens = [300, 17, 64], [20, 17, 3]
+    pool = Pool(rng, stored, 2, 16, d)
+    n = len(pool.pages) * 16
+    k = (rng.uniform(-2, 2, (n, 2, d)) * 2.0 ** k_scale).astype(np.float16)
+    v = (rng.uniform(-2, 2, (n, 2, d)) * 2.0 ** v_scale).astype(np.float16)
+    pool.pages = mxfp4.append(pool.pages, k, v, np.arange(n))
+    q = (rng.uniform(-2, 2, (sum(q_lens), 6, d)) * 2.0 ** q_scale).astype(np.float16)
+    sm_scale = 2.0 ** min(0, -k_scale - q_scale) if k_scale < 0 else 1.0
+    rows = mxfp4.rows_of(pool.pages, d)
+    for q_here, lens, causal, (out, lse) in ((q, q_lens, 1, prefill(q, q_lens, pool, 1, sm_scale)), (q[:3], [1] * 3, 0, decode(q[:3], pool, sm_scale))):
+        want, want_lse = mxfp4.attention(q_here, lens, rows, pool.indptr, pool.ids, pool.info, causal, sm_scale)
+        # a score's float32 sum is off by up to D 2^-24 of the sum of its products' magnitudes, a weight by twice that part of itself
+        # (the keys' scores against the row's largest), and a row by twice that part of A, which bound() has 1.25 * 2^-10 of
+        most = d * np.abs(q_here.astype(np.float64)).max() * np.abs(rows[:, 0]).max() * sm_scale / np.log(2.0)
+        shaky = 2 * d * 2.0 ** -24 * most
+        limit = bound(q_here, lens, pool, causal, sm_scale) * (1 + 2 * shaky * 2.0 ** 10 / 1.25)
+        assert (np.abs(out.astype(np.float64) - want) <= np.minimum(limit, 2 * np.abs(rows[:, 1]).max())).all()
+        assert (np.abs(lse - want_lse) <= 5e-5 + shaky + 2.0 ** -22 * np.abs(want_lse)).all()
