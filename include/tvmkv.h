@@ -474,6 +474,53 @@ int tvmkv_mxfp4_batch_prefill_paged_kv(const void* q, const int32_t* q_indptr, c
                                        int64_t num_pages, int32_t h_q, int32_t h_kv, int32_t head_dim,
                                        int32_t page_size, int32_t sliding_window, void* stream);
 
+/* ---- eviction by attention weight (no counterpart among the reference's kernels) -------------------
+ *
+ * The attention calls below also add up what each stored token receives: with s the scaled scores of a query head (base 2) and
+ * lse their log-sum-exp, a key's weight is 2^(s - lse), and the sum of a (token, kv head) grows by the weights of the query heads
+ * of its group.  The sums are key_weights, float32 (num_weight_pages, h_kv, page_size), on pages of their own: entry i of
+ * weight_page_values has the sums of the tokens on page page_values[i].  Sequences may share K/V pages; their weight pages are all
+ * different (passing page_values for both is fine where no page is shared).  Sums of slots that hold no token stay as they are.
+ *
+ * Built for fp16 rows, pages of 16, 32, 64 or 128 tokens, head dims 64, 80, 96, 112, 128 and 256, any GQA group; keys are stored
+ * rotated, caches without sliding windows.  q, pages and output are aligned to 16 bytes. */
+
+/* tvmkv_batch_decode_paged_kv with the sums: one query token a sequence, q and output (batch, h_q, d), lse (batch, h_q),
+ * length_info (batch). */
+int tvmkv_batch_decode_paged_kv_weights(const void* q, const void* pages, const int32_t* page_indptr, const int32_t* page_values,
+                                        const int32_t* length_info, void* output, float* lse, float* key_weights,
+                                        const int32_t* weight_page_values, double sm_scale, int32_t batch_size, int64_t nnz_pages,
+                                        int64_t num_pages, int32_t h_q, int32_t h_kv, int32_t d, int32_t page_size, void* stream);
+
+/* tvmkv_batch_prefill_paged_kv with the sums: a sequence's new tokens are in the cache already, as its last; causal: the last query
+ * sees all keys, the one before it one fewer, and so on.  observed > 0: only the last `observed` queries of a sequence add to the
+ * sums; 0: all of them. */
+int tvmkv_batch_prefill_paged_kv_weights(const void* q, const int32_t* q_indptr, const void* pages, const int32_t* page_indptr,
+                                         const int32_t* page_values, const int32_t* length_info, void* output, float* lse,
+                                         float* key_weights, const int32_t* weight_page_values, int64_t causal, int64_t observed,
+                                         double sm_scale, int32_t batch_size, int64_t total_q, int64_t nnz_pages, int64_t num_pages,
+                                         int32_t h_q, int32_t h_kv, int32_t d, int32_t page_size, void* stream);
+
+/* Which tokens stay.  Of a sequence of L tokens n = min(L, keep[b], max_keep) do, for each kv head its own: the last
+ * min(num_recent, n), the first num_sinks as far as there is room, and of the others those with the largest sums (of equal ones the
+ * first; NaN is below everything).  kept (batch, h_kv, max_keep) names the token that each of the first n places takes, -1 behind
+ * them: the recent tokens have the last places, in order; in front of them a token that stays and has a place already keeps it, and
+ * the other places, from the front, take the others in order.  keep (batch) is in device memory.  A sequence that already has n
+ * tokens keeps all as they are.  More than 262144 tokens in all need scratch memory, kept as that of the decode entry point. */
+int tvmkv_select_kept_tokens(const float* key_weights, const int32_t* page_indptr, const int32_t* weight_page_values,
+                             const int32_t* length_info, const int32_t* keep, int32_t* kept, int64_t num_sinks, int64_t num_recent,
+                             int32_t batch_size, int64_t nnz_pages, int32_t h_kv, int32_t page_size, int32_t max_keep, void* stream);
+
+/* Moves the rows of the tokens kept (batch, h_kv, max_keep) to their places, K, V and, where key_weights is not NULL, the sums, in
+ * place.  Lists of the caller's own may name any token that is not in front of its place (an ascending list does); entries that
+ * name none behind it, or none of the sequence's pages, move nothing.  The sequence then has as many tokens as the list names, on
+ * the first of its pages.  Pages that other sequences share are copied first (tvmkv_copy_single_page).  Rows of d elements of
+ * dtype_bits (16 or 32), a multiple of 16 bytes; pages of 16, 32, 64 or 128 tokens. */
+int tvmkv_move_kept_tokens(void* pages, float* key_weights, const int32_t* page_indptr, const int32_t* page_values,
+                           const int32_t* weight_page_values, const int32_t* kept, int32_t batch_size, int64_t nnz_pages,
+                           int64_t num_pages, int32_t h_kv, int32_t page_size, int32_t d, int32_t dtype_bits, int32_t max_keep,
+                           void* stream);
+
 /* Tuning options (no counterpart in the reference).  Each starts from an environment variable read
  * once when the library is loaded (TVMKV_ + the upper-case name) and defaults to 0:
  *   decode_chunk_pages     pages per split-KV chunk of the decode kernel (a multiple of 8); 0 = from shapes

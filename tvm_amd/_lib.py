@@ -67,6 +67,11 @@ SIGNATURES = {
     "tvmkv_kv_cache_debug_get_kv": [c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_i32, c_i32, c_i32, c_vp],
     "tvmkv_kv_cache_debug_get_kv_mla": [c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_i32, c_i32, c_vp],
     "tvmkv_compact_kv_copy": [c_vp, c_vp, c_vp, c_i32, c_i32, c_i64, c_i32, c_i32, c_i32, c_vp],
+    "tvmkv_batch_decode_paged_kv_weights": [c_vp] * 9 + [c_f64, c_i32, c_i64, c_i64, c_i32, c_i32, c_i32, c_i32, c_vp],
+    "tvmkv_batch_prefill_paged_kv_weights": [c_vp] * 10 + [c_i64, c_i64, c_f64, c_i32, c_i64, c_i64, c_i64, c_i32, c_i32, c_i32,
+                                                           c_i32, c_vp],
+    "tvmkv_select_kept_tokens": [c_vp] * 6 + [c_i64, c_i64, c_i32, c_i64, c_i32, c_i32, c_i32, c_vp],
+    "tvmkv_move_kept_tokens": [c_vp] * 6 + [c_i32, c_i64, c_i64, c_i32, c_i32, c_i32, c_i32, c_i32, c_vp],
     "tvmkv_mxfp4_append": [c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_i32, c_i32, c_i32, c_vp],
     "tvmkv_mxfp4_read_kv": [c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_i32, c_i32, c_i32, c_vp],
     "tvmkv_mxfp4_batch_decode_paged_kv": [c_vp] * 7 + [c_f64, c_i32, c_i64, c_i64, c_i32, c_i32, c_i32, c_i32, c_i32, c_vp],
@@ -133,6 +138,10 @@ SIGNATURES = {
     "tvmkv_dl_mxfp4_read_kv": [c_vp] * 5,
     "tvmkv_dl_mxfp4_batch_decode_paged_kv": [c_vp] * 7 + [c_f64, c_vp],
     "tvmkv_dl_mxfp4_batch_prefill_paged_kv": [c_vp] * 8 + [c_i64, c_f64, c_vp],
+    "tvmkv_dl_batch_decode_paged_kv_weights": [c_vp] * 9 + [c_f64, c_vp],
+    "tvmkv_dl_batch_prefill_paged_kv_weights": [c_vp] * 10 + [c_i64, c_i64, c_f64, c_vp],
+    "tvmkv_dl_select_kept_tokens": [c_vp] * 6 + [c_i64, c_i64, c_vp],
+    "tvmkv_dl_move_kept_tokens": [c_vp] * 7,
 }
 
 # include/tvmkv_bench.h: the measurement aids of bench.py, a library of their own

@@ -155,6 +155,30 @@ PagedShapes CheckPaged(const Arg& q, const Arg& pages, const Arg& page_indptr, c
   return s;
 }
 
+// The attention calls that add up what stored tokens receive: as above without in-kernel RoPE and windows, and the sums on pages of
+// their own.
+PagedShapes CheckWeighed(const Arg& q, const Arg& pages, const Arg& page_indptr, const Arg& page_indices, const Arg& length_info,
+                         const Arg& out, const Arg& lse, const Arg& key_weights, const Arg& weight_page_indices) {
+  PagedShapes s;
+  s.rows = q.dim(0);
+  s.h_q = static_cast<int32_t>(q.dim(1));
+  s.d = static_cast<int32_t>(q.dim(2));
+  Expect(pages.dim(1) == 2 && pages.dim(4) == s.d, pages, "(num_pages, 2, h_kv, page_size, head_dim of q)");
+  s.num_pages = pages.dim(0);
+  s.h_kv = static_cast<int32_t>(pages.dim(2));
+  s.page_size = static_cast<int32_t>(pages.dim(3));
+  Expect(page_indptr.dim(0) >= 1, page_indptr, "(batch + 1,)");
+  s.batch = page_indptr.dim(0) - 1;
+  s.nnz_pages = page_indices.dim(0);
+  s.sliding = 0;
+  Expect(length_info.dim(0) == s.batch, length_info, "(batch,)");
+  Expect(out.dim(0) == s.rows && out.dim(1) == s.h_q && out.dim(2) == s.d, out, "the shape of q");
+  Expect(lse.dim(0) == s.rows && lse.dim(1) == s.h_q, lse, "(rows of q, h_q)");
+  Expect(key_weights.dim(1) == s.h_kv && key_weights.dim(2) == s.page_size, key_weights, "(num_weight_pages, h_kv, page_size of pages)");
+  Expect(weight_page_indices.dim(0) == s.nnz_pages, weight_page_indices, "the shape of page_indices");
+  return s;
+}
+
 // Pages of a 4-bit cache whose rows have d elements: (num_pages, 2, h_kv, page_size, 17 d / 32).
 void CheckMxfp4Pages(const Arg& pages, int64_t d) {
   Expect(pages.dim(1) == 2 && pages.dim(4) * 32 == 17 * d, pages, "(num_pages, 2, h_kv, page_size, 17 * head_dim / 32)");
@@ -721,6 +745,94 @@ int tvmkv_dl_mxfp4_batch_prefill_paged_kv(const DLTensor* q_, const DLTensor* qo
                                                                  page_indices.i32(), length_info.i32(), out.ptr(), lse.f32(), causal,
                                                                  sm_scale, static_cast<int32_t>(s.batch), s.rows, s.nnz_pages,
                                                                  s.num_pages, s.h_q, s.h_kv, s.d, s.page_size, s.sliding, stream); });
+  KV_API_END();
+}
+
+int tvmkv_dl_batch_decode_paged_kv_weights(const DLTensor* q_, const DLTensor* pages_, const DLTensor* page_indptr_,
+                                           const DLTensor* page_indices_, const DLTensor* length_info_, const DLTensor* out_,
+                                           const DLTensor* lse_, const DLTensor* key_weights_, const DLTensor* weight_page_indices_,
+                                           double sm_scale, void* stream) {
+  KV_API_BEGIN();
+  Arg q = Take(q_, "q", kF16, {3}), pages = Take(pages_, "pages", kF16, {5});
+  Arg page_indptr = Take(page_indptr_, "page_indptr", kI32, {1}), page_indices = Take(page_indices_, "page_indices", kI32, {1});
+  Arg length_info = Take(length_info_, "length_info", kI32, {1}), out = Take(out_, "out", kF16, {3}), lse = Take(lse_, "lse", kF32, {2});
+  Arg sums = Take(key_weights_, "key_weights", kF32, {3}), weight_pages = Take(weight_page_indices_, "weight_page_indices", kI32, {1});
+  const int device = SameDevice({q, pages, page_indptr, page_indices, length_info, out, lse, sums, weight_pages});
+  const PagedShapes s = CheckWeighed(q, pages, page_indptr, page_indices, length_info, out, lse, sums, weight_pages);
+  Expect(s.rows == s.batch, q, "(batch, h_q, head_dim): one query token a sequence");
+  Launch(device, [&] { return tvmkv_batch_decode_paged_kv_weights(q.ptr(), pages.ptr(), page_indptr.i32(), page_indices.i32(),
+                                                                  length_info.i32(), out.ptr(), lse.f32(), sums.f32(), weight_pages.i32(),
+                                                                  sm_scale, static_cast<int32_t>(s.batch), s.nnz_pages, s.num_pages, s.h_q,
+                                                                  s.h_kv, s.d, s.page_size, stream); });
+  KV_API_END();
+}
+
+int tvmkv_dl_batch_prefill_paged_kv_weights(const DLTensor* q_, const DLTensor* qo_indptr_, const DLTensor* pages_,
+                                            const DLTensor* page_indptr_, const DLTensor* page_indices_, const DLTensor* length_info_,
+                                            const DLTensor* out_, const DLTensor* lse_, const DLTensor* key_weights_,
+                                            const DLTensor* weight_page_indices_, int64_t causal, int64_t observed, double sm_scale,
+                                            void* stream) {
+  KV_API_BEGIN();
+  Arg q = Take(q_, "q", kF16, {3}), qo_indptr = Take(qo_indptr_, "qo_indptr", kI32, {1}), pages = Take(pages_, "pages", kF16, {5});
+  Arg page_indptr = Take(page_indptr_, "page_indptr", kI32, {1}), page_indices = Take(page_indices_, "page_indices", kI32, {1});
+  Arg length_info = Take(length_info_, "length_info", kI32, {1}), out = Take(out_, "out", kF16, {3}), lse = Take(lse_, "lse", kF32, {2});
+  Arg sums = Take(key_weights_, "key_weights", kF32, {3}), weight_pages = Take(weight_page_indices_, "weight_page_indices", kI32, {1});
+  const int device = SameDevice({q, qo_indptr, pages, page_indptr, page_indices, length_info, out, lse, sums, weight_pages});
+  const PagedShapes s = CheckWeighed(q, pages, page_indptr, page_indices, length_info, out, lse, sums, weight_pages);
+  Expect(qo_indptr.dim(0) == s.batch + 1, qo_indptr, "(batch + 1,)");
+  Launch(device, [&] { return tvmkv_batch_prefill_paged_kv_weights(q.ptr(), qo_indptr.i32(), pages.ptr(), page_indptr.i32(),
+                                                                   page_indices.i32(), length_info.i32(), out.ptr(), lse.f32(), sums.f32(),
+                                                                   weight_pages.i32(), causal, observed, sm_scale,
+                                                                   static_cast<int32_t>(s.batch), s.rows, s.nnz_pages, s.num_pages, s.h_q,
+                                                                   s.h_kv, s.d, s.page_size, stream); });
+  KV_API_END();
+}
+
+int tvmkv_dl_select_kept_tokens(const DLTensor* key_weights_, const DLTensor* page_indptr_, const DLTensor* weight_page_indices_,
+                                const DLTensor* length_info_, const DLTensor* keep_, const DLTensor* kept_, int64_t num_sinks,
+                                int64_t num_recent, void* stream) {
+  KV_API_BEGIN();
+  Arg sums = Take(key_weights_, "key_weights", kF32, {3}), page_indptr = Take(page_indptr_, "page_indptr", kI32, {1});
+  Arg weight_pages = Take(weight_page_indices_, "weight_page_indices", kI32, {1}), length_info = Take(length_info_, "length_info", kI32, {1});
+  Arg keep = Take(keep_, "keep", kI32, {1}), kept = Take(kept_, "kept", kI32, {3});
+  const int device = SameDevice({sums, page_indptr, weight_pages, length_info, keep, kept});
+  Expect(page_indptr.dim(0) >= 1, page_indptr, "(batch + 1,)");
+  const int64_t batch = page_indptr.dim(0) - 1;
+  Expect(length_info.dim(0) == batch, length_info, "(batch,)");
+  Expect(keep.dim(0) == batch, keep, "(batch,)");
+  Expect(kept.dim(0) == batch && kept.dim(1) == sums.dim(1) && kept.dim(2) <= INT32_MAX, kept, "(batch, h_kv of key_weights, max_keep)");
+  Launch(device, [&] { return tvmkv_select_kept_tokens(sums.f32(), page_indptr.i32(), weight_pages.i32(), length_info.i32(), keep.i32(),
+                                                       static_cast<int32_t*>(kept.ptr()), num_sinks, num_recent,
+                                                       static_cast<int32_t>(batch), weight_pages.dim(0), static_cast<int32_t>(sums.dim(1)),
+                                                       static_cast<int32_t>(sums.dim(2)), static_cast<int32_t>(kept.dim(2)), stream); });
+  KV_API_END();
+}
+
+int tvmkv_dl_move_kept_tokens(const DLTensor* pages_, const DLTensor* key_weights_, const DLTensor* page_indptr_,
+                              const DLTensor* page_indices_, const DLTensor* weight_page_indices_, const DLTensor* kept_, void* stream) {
+  KV_API_BEGIN();
+  Arg pages = Take(pages_, "pages", kStorage, {5}), page_indptr = Take(page_indptr_, "page_indptr", kI32, {1});
+  Arg page_indices = Take(page_indices_, "page_indices", kI32, {1}), kept = Take(kept_, "kept", kI32, {3});
+  const int device = SameDevice({pages, page_indptr, page_indices, kept});
+  Expect(page_indptr.dim(0) >= 1, page_indptr, "(batch + 1,)");
+  const int64_t batch = page_indptr.dim(0) - 1;
+  Expect(pages.dim(1) == 2, pages, "(num_pages, 2, h_kv, page_size, head_dim)");
+  Expect(kept.dim(0) == batch && kept.dim(1) == pages.dim(2) && kept.dim(2) <= INT32_MAX, kept, "(batch, h_kv of pages, max_keep)");
+  float* sums_at = nullptr;
+  const int32_t* weight_pages_at = nullptr;
+  if (key_weights_ != nullptr) {
+    Arg sums = Take(key_weights_, "key_weights", kF32, {3}), weight_pages = Take(weight_page_indices_, "weight_page_indices", kI32, {1});
+    SameDevice({pages, sums, weight_pages});
+    Expect(sums.dim(1) == pages.dim(2) && sums.dim(2) == pages.dim(3), sums, "(num_weight_pages, h_kv, page_size of pages)");
+    Expect(weight_pages.dim(0) == page_indices.dim(0), weight_pages, "the shape of page_indices");
+    sums_at = sums.f32();
+    weight_pages_at = weight_pages.i32();
+  }
+  Launch(device, [&] { return tvmkv_move_kept_tokens(pages.ptr(), sums_at, page_indptr.i32(), page_indices.i32(), weight_pages_at,
+                                                     kept.i32(), static_cast<int32_t>(batch), page_indices.dim(0), pages.dim(0),
+                                                     static_cast<int32_t>(pages.dim(2)), static_cast<int32_t>(pages.dim(3)),
+                                                     static_cast<int32_t>(pages.dim(4)), pages.t->dtype.bits,
+                                                     static_cast<int32_t>(kept.dim(2)), stream); });
   KV_API_END();
 }
 

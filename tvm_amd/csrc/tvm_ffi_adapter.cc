@@ -263,6 +263,31 @@ TVM_FFI_STATIC_INIT_BLOCK() {
               Tensor lse, int64_t causal, double sm_scale) {
              Check(tvmkv_dl_mxfp4_batch_prefill_paged_kv(T(q), T(qo_indptr), T(pages), T(page_indptr), T(page_indices), T(length_info),
                                                          T(out), T(lse), causal, sm_scale, StreamOf(q)));
+           })
+      // eviction by attention weight: decode and prefill that add up what stored tokens receive, the choice, the move
+      .def("tvmkv.batch_decode_paged_kv_weights",
+           [](Tensor q, Tensor pages, Tensor page_indptr, Tensor page_indices, Tensor length_info, Tensor out, Tensor lse,
+              Tensor key_weights, Tensor weight_page_indices, double sm_scale) {
+             Check(tvmkv_dl_batch_decode_paged_kv_weights(T(q), T(pages), T(page_indptr), T(page_indices), T(length_info), T(out), T(lse),
+                                                          T(key_weights), T(weight_page_indices), sm_scale, StreamOf(q)));
+           })
+      .def("tvmkv.batch_prefill_paged_kv_weights",
+           [](Tensor q, Tensor qo_indptr, Tensor pages, Tensor page_indptr, Tensor page_indices, Tensor length_info, Tensor out,
+              Tensor lse, Tensor key_weights, Tensor weight_page_indices, int64_t causal, int64_t observed, double sm_scale) {
+             Check(tvmkv_dl_batch_prefill_paged_kv_weights(T(q), T(qo_indptr), T(pages), T(page_indptr), T(page_indices), T(length_info),
+                                                           T(out), T(lse), T(key_weights), T(weight_page_indices), causal, observed,
+                                                           sm_scale, StreamOf(q)));
+           })
+      .def("tvmkv.select_kept_tokens",
+           [](Tensor key_weights, Tensor page_indptr, Tensor weight_page_indices, Tensor length_info, Tensor keep, Tensor kept,
+              int64_t num_sinks, int64_t num_recent) {
+             Check(tvmkv_dl_select_kept_tokens(T(key_weights), T(page_indptr), T(weight_page_indices), T(length_info), T(keep), T(kept),
+                                               num_sinks, num_recent, StreamOf(key_weights)));
+           })
+      .def("tvmkv.move_kept_tokens",
+           [](Tensor pages, Tensor key_weights, Tensor page_indptr, Tensor page_indices, Tensor weight_page_indices, Tensor kept) {
+             Check(tvmkv_dl_move_kept_tokens(T(pages), T(key_weights), T(page_indptr), T(page_indices), T(weight_page_indices), T(kept),
+                                             StreamOf(pages)));
            });
 }
 #endif  // TVMKV_HAVE_TVM_FFI

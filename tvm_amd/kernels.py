@@ -374,3 +374,112 @@ def mxfp4_batch_prefill_paged_kv(q, q_indptr, pages, page_indptr, page_values, l
     _shape(q_indptr, "q_indptr", (batch + 1,))
     _mxfp4_call(lib().tvmkv_mxfp4_batch_prefill_paged_kv, (q, q_indptr, pages, page_indptr, page_values, length_info, output, lse),
                 causal, sm_scale, batch, rows, *sizes)
+
+
+# ---- eviction by attention weight (include/tvmkv.h says what the calls compute) -----------------------------------
+
+
+def key_weight_pages(num_pages, h_kv, page_size, device="cuda"):
+    """Sums of the attention weights that stored tokens have received, for the *_weights calls: none yet."""
+    return torch.zeros((num_pages, h_kv, page_size), dtype=torch.float32, device=device)
+
+
+def _weights_call(entry, tensors, *rest):
+    """tensors: all on one device, which is the current one for the call; None: NULL."""
+    index = tensors[0].get_device()
+    for t in tensors:
+        if t is not None and (not t.is_cuda or not t.is_contiguous() or t.get_device() != index):
+            _p(t)
+            raise KVError(-1, f"kernel arguments must be on one device, got {t.device} and {tensors[0].device}")
+    pointers = [None if t is None else t.data_ptr() for t in tensors]
+    if index == torch.cuda.current_device():
+        check(entry(*pointers, *rest, _raw_stream(index)))
+    else:
+        with torch.cuda.device(index):
+            check(entry(*pointers, *rest, _raw_stream(index)))
+
+
+def _key_weights(key_weights, hkv, ps):
+    if key_weights.dtype != torch.float32:
+        raise KVError(-1, f"key_weights must be float32, got {key_weights.dtype}")
+    if key_weights.dim() != 3 or key_weights.shape[1] != hkv or key_weights.shape[2] != ps:
+        raise KVError(-1, f"key_weights has shape {tuple(key_weights.shape)}, expected (num_weight_pages, {hkv}, {ps})")
+
+
+def _weighed_attention(q, pages, page_indptr, page_values, length_info, output, lse, key_weights, weight_page_values):
+    _f16(q, pages, output)
+    _i32(page_indptr, page_values, length_info, weight_page_values)
+    if lse.dtype != torch.float32:
+        raise KVError(-1, f"lse must be float32, got {lse.dtype}")
+    rows, hq, d = q.shape
+    if pages.dim() != 5 or pages.shape[1] != 2 or pages.shape[4] != d:
+        raise KVError(-1, f"pages has shape {tuple(pages.shape)}, expected (num_pages, 2, h_kv, page_size, {d})")
+    num_pages, _, hkv, ps, _ = pages.shape
+    batch = page_indptr.shape[0] - 1
+    _shape(output, "output", (rows, hq, d))
+    _shape(lse, "lse", (rows, hq))
+    _shape(length_info, "length_info", (batch,))
+    _shape(weight_page_values, "weight_page_values", page_values.shape)
+    _key_weights(key_weights, hkv, ps)
+    return rows, batch, (page_values.shape[0], num_pages, hq, hkv, d, ps)
+
+
+def batch_decode_paged_kv_weights(q, pages, page_indptr, page_values, length_info, output, lse, key_weights, weight_page_values,
+                                  sm_scale):
+    """batch_decode_paged_kv, keys stored rotated, that also adds each stored token's attention weight to key_weights
+    (num_weight_pages, h_kv, page_size) on the pages weight_page_values, which lie beside page_values."""
+    rows, batch, sizes = _weighed_attention(q, pages, page_indptr, page_values, length_info, output, lse, key_weights,
+                                            weight_page_values)
+    if rows != batch:
+        raise KVError(-1, f"q has shape {tuple(q.shape)}, expected {(batch,) + tuple(q.shape[1:])}")
+    _weights_call(lib().tvmkv_batch_decode_paged_kv_weights,
+                  (q, pages, page_indptr, page_values, length_info, output, lse, key_weights, weight_page_values), sm_scale, batch, *sizes)
+
+
+def batch_prefill_paged_kv_weights(q, q_indptr, pages, page_indptr, page_values, length_info, output, lse, key_weights,
+                                   weight_page_values, causal, observed, sm_scale):
+    """batch_prefill_paged_kv, keys stored rotated, that also adds each stored token's attention weight to key_weights; observed > 0:
+    that of the last `observed` queries of each sequence only."""
+    rows, batch, sizes = _weighed_attention(q, pages, page_indptr, page_values, length_info, output, lse, key_weights,
+                                            weight_page_values)
+    _i32(q_indptr)
+    _shape(q_indptr, "q_indptr", (batch + 1,))
+    _weights_call(lib().tvmkv_batch_prefill_paged_kv_weights,
+                  (q, q_indptr, pages, page_indptr, page_values, length_info, output, lse, key_weights, weight_page_values), int(causal),
+                  int(observed), sm_scale, batch, rows, *sizes)
+
+
+def select_kept_tokens(key_weights, page_indptr, weight_page_values, length_info, keep, kept, num_sinks, num_recent):
+    """Which tokens stay, into kept (batch, h_kv, max_keep): of each sequence keep[b] at most, for each kv head its first num_sinks,
+    its last num_recent and those with the largest sums; kept names the token that each place takes, -1 behind the last."""
+    _i32(page_indptr, weight_page_values, length_info, keep, kept)
+    batch = page_indptr.shape[0] - 1
+    if key_weights.dim() != 3 or key_weights.dtype != torch.float32:
+        raise KVError(-1, f"key_weights must be float32 (num_weight_pages, h_kv, page_size), got {key_weights.dtype} of shape "
+                          f"{tuple(key_weights.shape)}")
+    _, hkv, ps = key_weights.shape
+    _shape(length_info, "length_info", (batch,))
+    _shape(keep, "keep", (batch,))
+    if kept.dim() != 3 or kept.shape[:2] != (batch, hkv):
+        raise KVError(-1, f"kept has shape {tuple(kept.shape)}, expected ({batch}, {hkv}, max_keep)")
+    _weights_call(lib().tvmkv_select_kept_tokens, (key_weights, page_indptr, weight_page_values, length_info, keep, kept), int(num_sinks),
+                  int(num_recent), batch, weight_page_values.shape[0], hkv, ps, kept.shape[2])
+
+
+def move_kept_tokens(pages, key_weights, page_indptr, page_values, weight_page_values, kept):
+    """Moves the rows of the tokens `kept`, K, V and (key_weights not None) their sums, to their places at the front of each sequence's
+    pages; float16 or float32 pages."""
+    _i32(page_indptr, page_values, weight_page_values, kept)
+    if pages.dtype not in (torch.float16, torch.float32):
+        raise KVError(-2, f"only float16 and float32 rows are built, got {pages.dtype}")
+    if pages.dim() != 5 or pages.shape[1] != 2:
+        raise KVError(-1, f"pages has shape {tuple(pages.shape)}, expected (num_pages, 2, h_kv, page_size, head_dim)")
+    num_pages, _, hkv, ps, d = pages.shape
+    batch = page_indptr.shape[0] - 1
+    if key_weights is not None:
+        _key_weights(key_weights, hkv, ps)
+        _shape(weight_page_values, "weight_page_values", page_values.shape)
+    if kept.dim() != 3 or kept.shape[:2] != (batch, hkv):
+        raise KVError(-1, f"kept has shape {tuple(kept.shape)}, expected ({batch}, {hkv}, max_keep)")
+    _weights_call(lib().tvmkv_move_kept_tokens, (pages, key_weights, page_indptr, page_values, weight_page_values, kept), batch,
+                  page_values.shape[0], num_pages, hkv, ps, d, 8 * pages.element_size(), kept.shape[2])
