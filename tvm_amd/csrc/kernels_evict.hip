@@ -151,10 +151,15 @@ __global__ __launch_bounds__(256) void key_weights_kernel(KeyWeightsParams p) {
 }
 
 // ------------------------------------------------------------------------------------------
-// The choice.  A workgroup has the tokens of one (sequence, kv head); weights are compared as integers that order like them
-// (NaN below everything, -0 as 0).  Four passes of 8 bits find the smallest weight that stays, T, and how many of the weights
-// equal to it do: counts, exact whatever their order.  Then a bit a token says which ones stay, in shared memory or, for longer
-// sequences, in scratch memory, and running counts of free places and of tokens without one pair them.
+// The choice.  A workgroup has the tokens of one (sequence, kv head).  As integers that order like them (NaN below everything, -0
+// as 0) the weights go through passes of 8 bits that find the smallest one that stays, T, and how many of the weights equal to it
+// do: counts, exact whatever their order.  Then a bit a token says which ones stay, and running counts of free places and of tokens
+// without one pair them.
+// A wave takes blocks of 256 tokens, four neighbouring ones a lane; bit l of the block's four words of 64 is token 4 l + (0..3)'s,
+// as a comparison leaves them.  Up to 4 blocks a wave are loaded once and kept in registers.  Longer sequences are read twice: the
+// passes over some of their tokens, evenly spaced, say between which two weights T lies but for a chance that counts show, the
+// weights between them go to shared memory, and the passes over those find T.  Where it does not lie there, or they are too many,
+// every pass reads the whole sequence.  Bits and counts of more than BLOCKS blocks are in scratch memory.
 // ------------------------------------------------------------------------------------------
 struct SelectParams {
   const float* key_weights;
@@ -163,7 +168,7 @@ struct SelectParams {
   const int32_t* last_page_len;
   const int32_t* keep;
   int32_t* kept;
-  uint64_t* words;  // scratch memory: 64 tokens each, and as many counts; NULL where no sequence can be longer than kLdsWords
+  uint64_t* words;  // scratch memory: four words a block, and a count; NULL where no sequence can need it
   int32_t* counts;
   int h_kv;
   int max_keep;
@@ -171,48 +176,86 @@ struct SelectParams {
   int recent;
   int page_shift;
 };
-constexpr int kSelectThreads = 1024;
-constexpr int kSelectWaves = kSelectThreads / 64;
-constexpr int kLdsWords = 4096;  // 262144 tokens
+typedef float float4_any_t __attribute__((ext_vector_type(4), aligned(4)));
+typedef int int4_any_t __attribute__((ext_vector_type(4), aligned(4)));
 
+constexpr uint32_t kOrderOfMinusInf = 0x007fffff, kOrderOfInf = 0xff800000;
 __device__ __forceinline__ uint32_t weight_order(float w) {
   if (w != w) return 0;
   const uint32_t bits = __float_as_uint(w + 0.f);  // -0 + 0 = 0
   return bits & 0x80000000u ? ~bits : bits | 0x80000000u;
 }
-// The nth set bit of x, which has more than n.
-__device__ __forceinline__ int nth_bit(uint64_t x, int n) {
-  int at = 0;
-#pragma unroll
-  for (int width = 32; width > 0; width >>= 1) {
-    const int below = __popcll(x >> at & ((uint64_t{1} << width) - 1));
-    const bool up = n >= below;
-    n -= up ? below : 0;
-    at += up ? width : 0;
-  }
-  return at;
+// The smallest weight of this order or a larger one (but NaN): w >= weight_from(x) is weight_order(w) >= x for x > 0.
+__device__ __forceinline__ float weight_from(uint32_t x) {
+  x = min(max(x, kOrderOfMinusInf), kOrderOfInf);
+  return __uint_as_float(x & 0x80000000u ? x ^ 0x80000000u : ~x);
 }
-// Sum of what the waves in front of this one bring, and of all.
-__device__ __forceinline__ int sum_before_wave(int* shared, int value, int wave, int lane, int* total) {
-  __syncthreads();
-  if (lane == 0) shared[wave] = value;
-  __syncthreads();
-  int before = 0, all = 0;
+__device__ __forceinline__ uint64_t low_bits(int n) { return n >= 64 ? ~uint64_t{0} : (uint64_t{1} << n) - 1; }
+// Sum of x over the lanes up to this one.
+__device__ __forceinline__ int sum_of_lanes_up_to(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // from 1, 2, 4 and 8 lanes below in the row of 16
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // the row below's last to rows 1 and 3
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // lane 31's to rows 2 and 3
+  return x;
+}
+// Of a word that all lanes have: the lane's bit, the set bits of the lanes below it.
+__device__ __forceinline__ bool bit_of_lane(uint64_t word) { return __builtin_amdgcn_inverse_ballot_w64(word); }
+__device__ __forceinline__ int bits_below(uint64_t word, int and_these) {
+  return __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(word >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(word), and_these));
+}
+// The four words of a block, of 256 tokens.
+struct BlockBits {
+  uint64_t w[4];
+  __device__ __forceinline__ int count() const { return __popcll(w[0]) + __popcll(w[1]) + __popcll(w[2]) + __popcll(w[3]); }
+  // set bits of the tokens in front of the lane's, where all lanes have the block
+  __device__ __forceinline__ int before() const { return bits_below(w[3], bits_below(w[2], bits_below(w[1], bits_below(w[0], 0)))); }
+  // those of the tokens in front of the nth, or the others
+  __device__ __forceinline__ BlockBits first(int n, bool others = false) const {
+    BlockBits x;
 #pragma unroll
-  for (int i = 0; i < kSelectWaves; ++i) {
-    before += i < wave ? shared[i] : 0;
-    all += shared[i];
+    for (int i = 0; i < 4; ++i) {
+      const uint64_t mask = low_bits(max(n - i + 3, 0) >> 2);
+      x.w[i] = w[i] & (others ? ~mask : mask);
+    }
+    return x;
   }
-  *total = all;
-  return before;
+  __device__ __forceinline__ BlockBits inverse() const { return {{~w[0], ~w[1], ~w[2], ~w[3]}}; }
+  // the token of the nth set bit
+  __device__ __forceinline__ int nth(int n) const {
+    int token = 0;
+#pragma unroll
+    for (int step = 128; step > 0; step >>= 1) token += first(token + step).count() <= n ? step : 0;
+    return token;
+  }
+};
+template <class Words>
+__device__ __forceinline__ BlockBits load_block(Words words, int block) {
+  BlockBits x;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint64_t word = words[block * 4 + i];
+    x.w[i] = static_cast<uint64_t>(__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(word >> 32))) << 32 | static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(word)));
+  }
+  return x;
 }
 
-__global__ __launch_bounds__(kSelectThreads) void select_kept_kernel(SelectParams p) {
-  __shared__ uint64_t lds_words[kLdsWords];
-  __shared__ int32_t lds_counts[kLdsWords];
-  __shared__ uint32_t histogram[256];
-  __shared__ int per_wave[kSelectWaves];
-  __shared__ uint32_t chosen_digit, left_over, as_many;
+template <int THREADS, int BLOCKS, int NEAR, int COPIES>
+__global__ __launch_bounds__(THREADS) void select_kept_kernel(SelectParams p) {
+  constexpr int WAVES = THREADS / 64;
+  constexpr int HELD = 4;             // blocks a wave keeps in registers
+  constexpr int SAMPLES = 2;          // of their lanes' neighbouring four tokens, in longer sequences
+  constexpr int MINE = NEAR / WAVES;  // weights near T that a wave finds
+  __shared__ uint64_t lds_words[BLOCKS * 4];
+  __shared__ int32_t lds_counts[BLOCKS];
+  __shared__ uint32_t near[NEAR];                // weights near T; later the tokens without a place
+  __shared__ uint32_t histogram[256 * COPIES];   // lanes take turns: most weights fall into a few of the first pass's bins
+  __shared__ uint32_t bins[256];
+  __shared__ int per_wave[2][WAVES];
+  __shared__ uint32_t found[3];
+  __shared__ int num_homeless;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int kvh = blockIdx.x, b = blockIdx.y;
   const int page_begin = p.page_indptr[b], num_pages = p.page_indptr[b + 1] - page_begin;
@@ -221,104 +264,345 @@ __global__ __launch_bounds__(kSelectThreads) void select_kept_kernel(SelectParam
   int32_t* const kept = p.kept + (static_cast<int64_t>(b) * p.h_kv + kvh) * p.max_keep;
   const int recent = min(p.recent, n), sinks = min(p.sinks, n - recent), places = n - recent;
   const int gone = stored - n;
-  for (int i = places + tid; i < p.max_keep; i += kSelectThreads) kept[i] = i < n ? i + gone : -1;
+  for (int i = places + tid; i < p.max_keep; i += THREADS) kept[i] = i < n ? i + gone : -1;
   if (gone == 0 || places == sinks) {
-    for (int i = tid; i < places; i += kSelectThreads) kept[i] = i;
+    for (int i = tid; i < places; i += THREADS) kept[i] = i;
     return;
   }
-  const auto order_of = [&](int t) {
-    const int page = p.weight_page_values[page_begin + (t >> p.page_shift)];
-    return weight_order(p.key_weights[((static_cast<int64_t>(page) * p.h_kv + kvh) << p.page_shift) + (t & ((1 << p.page_shift) - 1))]);
-  };
   const int end = stored - recent;  // candidates: tokens [sinks, end), of which `need` stay and at least one does not
-  uint32_t least = 0, need = places - sinks;
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    for (int i = tid; i < 256; i += kSelectThreads) histogram[i] = 0;
-    __syncthreads();
-    for (int t = sinks + tid; t < end; t += kSelectThreads) {
-      const uint32_t x = order_of(t);
-      if (shift == 24 || x >> (shift + 8) == least) atomicAdd(&histogram[x >> shift & 255], 1u);
-    }
-    __syncthreads();
-    if (tid == 0) {
-      uint32_t above = 0;
-      int digit = 255;
-      while (digit > 0 && above + histogram[digit] < need) above += histogram[digit--];
-      chosen_digit = digit;
-      left_over = need - above;
-      as_many = histogram[digit];
-    }
-    __syncthreads();
-    least = least << 8 | chosen_digit;
-    need = left_over;
+  const int num_blocks = (end + 255) >> 8, num_groups = (end + 3) >> 2;  // groups: of four tokens
+  // A group behind the end is the last one (its tokens are none).
+  const auto page_of = [&](int group) { return p.weight_page_values[page_begin + (min(group, num_groups - 1) >> (p.page_shift - 2))]; };
+  const auto weights_of = [&](int page, int group) {
+    const int in_page = min(group, num_groups - 1) * 4 & ((1 << p.page_shift) - 1);
+    return *reinterpret_cast<const float4_any_t*>(p.key_weights + ((static_cast<int64_t>(page) * p.h_kv + kvh) << p.page_shift) + in_page);
+  };
+  float4_any_t held[HELD];  // of blocks wave, wave + WAVES, ..; of a longer sequence the sample
+  const bool in_registers = num_blocks <= WAVES * HELD;
+  {
+    // groups of the sample: evenly spaced
+    const int spacing = in_registers ? 1 : num_groups / (SAMPLES * THREADS);
+    int page[HELD];
+#pragma unroll
+    for (int u = 0; u < HELD; ++u) page[u] = page_of((tid + u * THREADS) * spacing);
+#pragma unroll
+    for (int u = 0; u < HELD; ++u) held[u] = weights_of(page[u], (tid + u * THREADS) * spacing);
   }
-  // Bits of the tokens in front of the recent ones, a range of words a wave.  Of the as_many weights equal to T the first
-  // `need` stay.
-  const int num_words = (end + 63) >> 6;
-  uint64_t* const words = num_words <= kLdsWords ? lds_words : p.words + (((static_cast<int64_t>(page_begin - p.page_indptr[0]) << p.page_shift) >> 6) + b) * p.h_kv + static_cast<int64_t>(kvh) * num_words;
-  int32_t* const counts = num_words <= kLdsWords ? lds_counts : p.counts + (words - p.words);
-  const int per = (num_words + kSelectWaves - 1) / kSelectWaves, word_lo = min(wave * per, num_words), word_hi = min(word_lo + per, num_words);
-  int equal_before = 0, total;
-  if (need < as_many) {
-    int equal = 0;
-    for (int w = word_lo; w < word_hi; ++w) {
-      const int t = w * 64 + lane;
-      equal += __popcll(__ballot(t >= sinks && t < end && order_of(t) == least));
-    }
-    equal_before = sum_before_wave(per_wave, equal, wave, lane, &total);
-  }
-  const int boundary = places >> 6;  // the word with the first token behind the places; holes up to it, tokens without a place from it on
-  const uint64_t in_places = (uint64_t{1} << (places & 63)) - 1;  // of its bits
-  int holes = 0, homeless = 0;
-  for (int w = word_lo; w < word_hi; ++w) {
-    const int t = w * 64 + lane;
-    bool stays = t < sinks;
-    if (t >= sinks && t < end) {
-      const uint32_t x = order_of(t);
-      const uint64_t equal = __ballot(x == least);
-      stays = x > least || (x == least && equal_before + static_cast<int>(__popcll(equal & ((uint64_t{1} << lane) - 1))) < static_cast<int>(need));
-      equal_before += __popcll(equal);
-    }
-    const uint64_t word = __ballot(stays);
-    if (lane == 0) words[w] = word;
-    holes += __popcll(~word & (w < boundary ? ~uint64_t{0} : w == boundary ? in_places : 0));
-    homeless += __popcll(word & (w > boundary ? ~uint64_t{0} : w == boundary ? ~in_places : 0));
-  }
-  int holes_before = sum_before_wave(per_wave, holes, wave, lane, &total);
-  int homeless_before = sum_before_wave(per_wave, homeless, wave, lane, &total);
-  // counts of a word: up to the boundary the holes in front of it, behind it the tokens without a place in front of it
-  for (int w = word_lo; w < word_hi; ++w) {
-    const uint64_t word = words[w];
-    if (lane == 0) counts[w] = w <= boundary ? holes_before : homeless_before;
-    holes_before += __popcll(~word & (w < boundary ? ~uint64_t{0} : 0));
-    homeless_before += __popcll(word & (w > boundary ? ~uint64_t{0} : w == boundary ? ~in_places : 0));
-  }
-  __syncthreads();
-  const uint64_t first_homeless = boundary < num_words ? words[boundary] & ~in_places : 0;
-  for (int i = tid; i < places; i += kSelectThreads) {
-    const uint64_t word = words[i >> 6];
-    int from = i;
-    if (!(word >> (i & 63) & 1)) {
-      const int rank = counts[i >> 6] + __popcll(~word & ((uint64_t{1} << (i & 63)) - 1));
-      if (rank < static_cast<int>(__popcll(first_homeless))) {
-        from = boundary * 64 + nth_bit(first_homeless, rank);
-      } else {
-        int lo = boundary + 1, hi = num_words - 1;  // the last word that begins at or in front of the rank
-        while (lo < hi) {
-          const int mid = (lo + hi + 1) >> 1;
-          if (counts[mid] <= rank) lo = mid; else hi = mid - 1;
+  // f(block, the lane's weights) for every block; all lanes of a wave take the same steps
+  const auto every_block = [&](auto&& f) {
+    if (in_registers) {
+#pragma unroll
+      for (int u = 0; u < HELD; ++u) {
+        if (u * WAVES + wave < num_blocks) f(u * WAVES + wave, held[u]);
+      }
+    } else {
+      constexpr int U = 8;
+      int page[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) page[u] = page_of(tid + u * THREADS);
+      for (int k0 = wave; k0 < num_blocks; k0 += U * WAVES) {
+        float4_any_t w[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) w[u] = weights_of(page[u], (k0 + u * WAVES) * 64 + lane);
+#pragma unroll
+        for (int u = 0; u < U; ++u) page[u] = page_of((k0 + (U + u) * WAVES) * 64 + lane);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          if (k0 + u * WAVES < num_blocks) f(k0 + u * WAVES, w[u]);
         }
-        from = lo * 64 + nth_bit(words[lo], rank - counts[lo]);
       }
     }
-    kept[i] = from;
+  };
+  // the block's candidates for which `is` holds
+  const auto candidates = [&](int block, float4_any_t w, auto&& is) {
+    BlockBits x;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x.w[i] = __ballot(is(w[i]));
+    if (block * 256 < sinks || block * 256 + 256 > end) x = x.first(end - block * 256).first(sinks - block * 256, true);
+    return x;
+  };
+
+  // One pass: `each` hands its weights, those whose bits above the `width` from `shift` on are those of least, to the histogram; the
+  // digit in which the need-th largest of them lies becomes part of least, need what is left of it there.  True: all weights of
+  // that digit do.
+  const auto pass = [&](auto&& each, int shift, int width, bool first, uint32_t& least, uint32_t& need) {
+    for (int i = tid; i < 256 * COPIES; i += THREADS) histogram[i] = 0;
+    __syncthreads();
+    const uint32_t digits = (1u << width) - 1;
+    each([&](uint32_t x) {
+      if (first || ((x ^ least) >> shift) <= digits) atomicAdd(&histogram[(x >> shift & digits) * COPIES + (lane & (COPIES - 1))], 1u);
+    });
+    __syncthreads();
+    constexpr int SHARE = THREADS / 256;  // threads that add a bin's copies up
+    static_assert(SHARE == 1 || SHARE == 4, "a thread or four lanes");
+    uint32_t copies = 0;
+#pragma unroll
+    for (int c = 0; c < COPIES / SHARE; ++c) copies += histogram[tid / SHARE * COPIES + ((tid % SHARE * (COPIES / SHARE) + c + tid / SHARE) & (COPIES - 1))];
+    if (SHARE == 4) {
+      copies += __builtin_amdgcn_update_dpp(0, copies, kDppXor1, 0xf, 0xf, true);
+      copies += __builtin_amdgcn_update_dpp(0, copies, kDppXor2, 0xf, 0xf, true);
+    }
+    if (tid % SHARE == 0) bins[255 - tid / SHARE] = copies;  // the largest digit first
+    __syncthreads();
+    if (wave == 0) {
+      uint32_t mine[4], sum = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sum += mine[i] = bins[lane * 4 + i];
+      uint32_t above = sum_of_lanes_up_to(sum) - sum;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (above < need && need <= above + mine[i]) {
+          found[0] = 255 - (lane * 4 + i);
+          found[1] = need - above;
+          found[2] = mine[i];
+        }
+        above += mine[i];
+      }
+    }
+    __syncthreads();
+    least |= found[0] << shift;
+    need = found[1];
+    return found[1] == found[2];
+  };
+
+  uint32_t least = 0, need = places - sinks;  // of T; how many of the weights equal to it stay
+  bool cut = true;                            // not all of them
+  const auto passes = [&](auto&& each, int bits) {
+    for (int left = bits; left > 0 && cut; left -= 8) cut = !pass(each, max(left - 8, 0), min(left, 8), left == bits, least, need);
+  };
+  const auto all_candidates = [&](auto&& add) {
+    every_block([&](int block, float4_any_t w) {
+      const int t = block * 256 + lane * 4;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (t + i >= sinks && t + i < end) add(weight_order(w[i]));
+      }
+    });
+  };
+  if (in_registers) {
+    passes(all_candidates, 32);
+  } else {
+    // The number of samples over T deviates by sqrt(samples) / 2 at most; nearly nine times that leave T between the two weights also
+    // where neighbouring tokens' weights are alike.
+    constexpr int kSamples = SAMPLES * THREADS * 4, kMargin = 400;
+    static_assert(kSamples <= 8192, "the margin");
+    const auto sampled = [&](auto&& add) {
+#pragma unroll
+      for (int u = 0; u < SAMPLES; ++u) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) add(weight_order(held[u][i]));
+      }
+    };
+    const int middle = static_cast<int>(static_cast<int64_t>(need) * kSamples / (end - sinks));
+    uint32_t upper = kOrderOfInf, lower = 0;  // weights above the first stay, none under the second does
+    if (middle - kMargin >= 1) {
+      uint32_t to = 0, left = middle - kMargin;
+      pass(sampled, 24, 8, true, to, left);
+      pass(sampled, 16, 8, false, to, left);
+      upper = min(max(to | 0xffff, kOrderOfMinusInf), kOrderOfInf);
+    }
+    if (middle + kMargin <= kSamples) {
+      uint32_t left = middle + kMargin;
+      pass(sampled, 24, 8, true, lower, left);
+      pass(sampled, 16, 8, false, lower, left);
+    }
+    const float highest = weight_from(upper), lowest = weight_from(lower);
+    int above = 0, mine = 0;
+    every_block([&](int block, float4_any_t w) {
+      const BlockBits over = candidates(block, w, [&](float x) { return x > highest; });
+      above += over.count();
+      const BlockBits here = candidates(block, w, [&](float x) { return !(x > highest) && (lower == 0 || x >= lowest); });
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int place = bits_below(here.w[i], mine);
+        if (bit_of_lane(here.w[i]) && place < MINE) near[wave * MINE + place] = __float_as_uint(w[i]);
+        mine += __popcll(here.w[i]);
+      }
+    });
+    __syncthreads();
+    if (lane == 0) {
+      per_wave[0][wave] = above;
+      per_wave[1][wave] = mine;
+    }
+    __syncthreads();
+    int all_above = 0, all_near = 0;
+    bool fits = true;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+      all_above += per_wave[0][w];
+      all_near += per_wave[1][w];
+      fits &= per_wave[1][w] <= MINE;
+    }
+    if (fits && all_above < static_cast<int>(need) && static_cast<int>(need) <= all_above + all_near) {
+      need -= all_above;
+      passes([&](auto&& add) {
+        for (int i = lane; i < mine; i += 256) {
+          uint32_t x[4];
+#pragma unroll
+          for (int u = 0; u < 4; ++u) x[u] = near[wave * MINE + min(i + u * 64, mine - 1)];
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            if (i + u * 64 < mine) add(weight_order(__uint_as_float(x[u])) - lower);
+          }
+        }
+      }, max(32 - __clz(upper - lower), 1));
+      least += lower;
+    } else {
+      passes(all_candidates, 32);
+    }
+  }
+
+  const float smallest = weight_from(least);
+  const auto is_equal = [&](float x) { return least == 0 ? x != x : x == smallest; };
+  const auto stays = [&](float x) { return least == 0 || x >= smallest; };
+  // A range of blocks a thread, for the running counts: two sums over the blocks in front of it.
+  const int per = (num_blocks + THREADS - 1) / THREADS, block_lo = min(tid * per, num_blocks), block_hi = min(block_lo + per, num_blocks);
+  const auto sums_in_front = [&](int a, int c) {
+    const int a_to = sum_of_lanes_up_to(a), c_to = sum_of_lanes_up_to(c);
+    __syncthreads();
+    if (lane == 63) {
+      per_wave[0][wave] = a_to;
+      per_wave[1][wave] = c_to;
+    }
+    __syncthreads();
+    int2 front = make_int2(a_to - a, c_to - c);
+#pragma unroll
+    for (int w = 0; w < WAVES - 1; ++w) {
+      front.x += w < wave ? per_wave[0][w] : 0;
+      front.y += w < wave ? per_wave[1][w] : 0;
+    }
+    return front;
+  };
+  const auto finish = [&](auto* words, auto* counts) {
+    if (cut) {  // weights equal to T in front of each block
+      every_block([&](int block, float4_any_t w) {
+        const BlockBits equal = candidates(block, w, is_equal);
+        if (lane == 0) counts[block] = equal.count();
+      });
+      __syncthreads();
+      int equal = 0;
+      for (int k = block_lo; k < block_hi; ++k) equal += counts[k];
+      int front = sums_in_front(equal, 0).x;
+      for (int k = block_lo; k < block_hi; ++k) {
+        const int here = counts[k];
+        counts[k] = front;
+        front += here;
+      }
+      __syncthreads();
+    }
+    every_block([&](int block, float4_any_t w) {
+      BlockBits x = candidates(block, w, stays);
+      if (cut) {
+        const BlockBits equal = candidates(block, w, is_equal);
+        int rank = counts[block] + equal.before();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const bool mine = bit_of_lane(equal.w[i]);
+          x.w[i] &= ~__ballot(mine && rank >= static_cast<int>(need));
+          rank += mine;
+        }
+      }
+      if (block * 256 < sinks) {
+        const BlockBits first = BlockBits{{~uint64_t{0}, ~uint64_t{0}, ~uint64_t{0}, ~uint64_t{0}}}.first(sinks - block * 256);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x.w[i] |= first.w[i];
+      }
+      if (lane < 4) words[block * 4 + lane] = lane == 0 ? x.w[0] : lane == 1 ? x.w[1] : lane == 2 ? x.w[2] : x.w[3];
+    });
+    __syncthreads();
+    // Free places up to the block with the first token behind the places, tokens without a place from that block on.
+    const int boundary = places >> 8;
+    const auto holes_in = [&](const BlockBits& x, int block) {
+      return block < boundary ? x.inverse() : x.inverse().first(block == boundary ? places & 255 : 0);
+    };
+    const auto homeless_in = [&](const BlockBits& x, int block) {
+      return block > boundary ? x : x.first(block == boundary ? places & 255 : 256, true);
+    };
+    const auto any_block = [&](int block) { return BlockBits{{words[block * 4], words[block * 4 + 1], words[block * 4 + 2], words[block * 4 + 3]}}; };
+    int holes = 0, homeless = 0;
+    for (int k = block_lo; k < block_hi; ++k) {
+      const BlockBits x = any_block(k);
+      holes += holes_in(x, k).count();
+      homeless += homeless_in(x, k).count();
+    }
+    int2 front = sums_in_front(holes, homeless);
+    // counts of a block: up to the boundary the holes in front of it, behind it the tokens without a place in front of it
+    for (int k = block_lo; k < block_hi; ++k) {
+      counts[k] = k <= boundary ? front.x : front.y;
+      const BlockBits x = any_block(k);
+      front.x += holes_in(x, k).count();
+      front.y += homeless_in(x, k).count();
+    }
+    if (tid == THREADS - 1) num_homeless = front.y;
+    __syncthreads();
+    // Tokens without a place, in order, where they are few enough; else a place looks for its own.
+    const bool listed = num_homeless <= NEAR;
+    if (listed) {
+      for (int k = boundary + wave; k < num_blocks; k += WAVES) {
+        const BlockBits x = homeless_in(load_block(words, k), k);
+        int rank = (k == boundary ? 0 : counts[k]) + x.before();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const bool mine = bit_of_lane(x.w[i]);
+          if (mine) near[rank] = k * 256 + lane * 4 + i;
+          rank += mine;
+        }
+      }
+      __syncthreads();
+    }
+    for (int k = wave; k * 256 < places; k += WAVES) {
+      const BlockBits x = holes_in(load_block(words, k), k);
+      const int t = k * 256 + lane * 4;
+      int rank = counts[k] + x.before();
+      int4_any_t from;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        from[i] = t + i;
+        if (bit_of_lane(x.w[i])) {
+          if (listed) {
+            from[i] = near[rank];
+          } else {
+            const BlockBits first = homeless_in(any_block(boundary), boundary);
+            if (rank < first.count()) {
+              from[i] = boundary * 256 + first.nth(rank);
+            } else {
+              int lo = boundary + 1, hi = num_blocks - 1;  // the last block that begins at or in front of the rank
+              while (lo < hi) {
+                const int mid = (lo + hi + 1) >> 1;
+                if (counts[mid] <= rank) lo = mid; else hi = mid - 1;
+              }
+              from[i] = lo * 256 + homeless_in(any_block(lo), lo).nth(rank - counts[lo]);
+            }
+          }
+          ++rank;
+        }
+      }
+      if (t + 4 <= places) {
+        *reinterpret_cast<int4_any_t*>(kept + t) = from;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (t + i < places) kept[t + i] = from[i];
+        }
+      }
+    }
+  };
+  if (num_blocks <= BLOCKS) {
+    finish(lds_words, lds_counts);
+  } else {
+    const int64_t at = (((static_cast<int64_t>(page_begin - p.page_indptr[0]) << p.page_shift) >> 8) + b) * p.h_kv + static_cast<int64_t>(kvh) * num_blocks;
+    finish(p.words + at * 4, p.counts + at);
   }
 }
 
 // ------------------------------------------------------------------------------------------
-// The move: row kept[i] to place i, in place.  kept[i] is never in front of i, so that places filled in order never overwrite a row
-// that a later one needs: a workgroup has the rows of one of K, V or the sums of a (sequence, kv head), reads those of a few
-// places, waits until all have, and writes.  Entries that name no token behind their place are passed over.
+// The move: row kept[i] to place i, in place; kept[i] is never in front of i, so that rows taken in order are still there when they
+// are needed.  Where there are many lists (sequence, kv head), a workgroup fills all places of one, with a part of each row's bytes:
+// it reads the rows of a few places, waits until all its waves have theirs, and writes.  Where there are few, a range of places is a
+// workgroup's, in two launches: with n entries in the list and s the first place that is also a source (n if none is), the places in
+// front of s can be filled in any order, none of the rows that they need is written meanwhile, and the first launch does it.  The
+// second fills the others: in any order again if none of them is the source of one of them, else (recent tokens that move by fewer
+// places than they are) in order as above.  Entries that name no token behind their place are passed over.
 // ------------------------------------------------------------------------------------------
 struct MoveParams {
   uint8_t* pages;
@@ -330,66 +614,166 @@ struct MoveParams {
   int h_kv;
   int max_keep;
   int page_shift;
-  int pieces;  // of 16 bytes in a row
-  ExactDivision by_pieces;
+  int pieces;            // of 16 bytes in the rows of K and V together
+  int slices;            // parts of them that workgroups have which fill places in order
+  ExactDivision by_row;  // pieces, pieces / slices
+  ExactDivision by_slice;
 };
 constexpr int kMoveThreads = 256;
+constexpr int kMoveWaves = kMoveThreads / 64;
+
+__device__ __forceinline__ int smallest_of_workgroup(int x, int* shared, int wave, int lane) {
+  x = min(x, __builtin_amdgcn_update_dpp(x, x, kDppXor1, 0xf, 0xf, false));
+  x = min(x, __builtin_amdgcn_update_dpp(x, x, kDppXor2, 0xf, 0xf, false));
+  x = min(x, __builtin_amdgcn_update_dpp(x, x, kDppRowHalfMirror, 0xf, 0xf, false));
+  x = min(x, __builtin_amdgcn_update_dpp(x, x, kDppRowMirror, 0xf, 0xf, false));
+  x = min(min(__builtin_amdgcn_readlane(x, 0), __builtin_amdgcn_readlane(x, 16)), min(__builtin_amdgcn_readlane(x, 32), __builtin_amdgcn_readlane(x, 48)));
+  __syncthreads();
+  if (lane == 0) shared[wave] = x;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kMoveWaves; ++w) x = min(x, shared[w]);
+  return x;
+}
+
+enum MoveLaunch { kMoveInOrder, kMoveFirst, kMoveSecond };
+template <MoveLaunch LAUNCH>
 __global__ __launch_bounds__(kMoveThreads) void move_kept_kernel(MoveParams p) {
-  __shared__ int places[kMoveThreads], sources[kMoveThreads];
-  __shared__ int per_wave[kMoveThreads / 64];
+  constexpr int EACH = 8;  // places a thread looks at before their rows are moved
+  __shared__ int2 list[kMoveThreads * EACH];  // place, source
+  __shared__ int per_wave[EACH][kMoveWaves];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int part = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z;
+  const int part = blockIdx.x, parts = gridDim.x, kvh = blockIdx.y, b = blockIdx.z;
   const int page_begin = p.page_indptr[b], capacity = (p.page_indptr[b + 1] - page_begin) << p.page_shift;
   const int32_t* const kept = p.kept + (static_cast<int64_t>(b) * p.h_kv + kvh) * p.max_keep;
   const int in_page = (1 << p.page_shift) - 1;
+  const auto moves = [&](int i, int from) { return from > i && from < capacity; };
+  int lo = 0, hi = min(p.max_keep, capacity);
+  bool in_order = LAUNCH == kMoveInOrder;
+  if constexpr (LAUNCH != kMoveInOrder) {
+    // what the list says: its smallest source, the place behind its last one that a row moves to
+    int least = INT32_MAX, last = 0;
+    const auto look = [&](int begin, int end) {
+      for (int i0 = begin + tid * 4; i0 < end; i0 += EACH * kMoveThreads * 4) {
+        int4_any_t from[EACH];
+#pragma unroll
+        for (int u = 0; u < EACH; ++u) {
+          const int i = i0 + u * kMoveThreads * 4;
+          if (i + 4 <= end) {
+            from[u] = *reinterpret_cast<const int4_any_t*>(kept + i);
+          } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) from[u][k] = i + k < end ? kept[i + k] : -1;
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < EACH; ++u) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int i = i0 + u * kMoveThreads * 4 + k;
+            if (moves(i, from[u][k])) {
+              least = min(least, from[u][k]);
+              last = max(last, i + 1);
+            }
+          }
+        }
+      }
+    };
+    look(0, hi);
+    const int n = -smallest_of_workgroup(-last, per_wave[0], wave, lane);
+    hi = min(smallest_of_workgroup(least, per_wave[0], wave, lane), n);
+    if constexpr (LAUNCH == kMoveSecond) {
+      lo = hi;
+      hi = n;
+      if (lo >= hi) return;
+      least = INT32_MAX;
+      look(lo, hi);
+      in_order = smallest_of_workgroup(least, per_wave[0], wave, lane) < n;
+    }
+  }
+  int y0 = 0, width = p.pieces;
+  const ExactDivision by_width = in_order ? p.by_slice : p.by_row;
+  if (in_order) {
+    if (part >= p.slices) return;
+    width = p.pieces / p.slices;
+    y0 = part * width;
+  } else {
+    const int each = (hi - lo + parts - 1) / parts;
+    lo += part * each;
+    hi = min(lo + each, hi);
+  }
+  const bool with_sums = p.key_weights != nullptr && y0 == 0;
   const auto sum_at = [&](int t) {
     const int page = p.weight_page_values[page_begin + (t >> p.page_shift)];
     return p.key_weights + ((static_cast<int64_t>(page) * p.h_kv + kvh) << p.page_shift) + (t & in_page);
   };
-  const auto row_at = [&](int t) {
+  const int half = p.pieces >> 1;  // a row's pieces of K, then those of V
+  const auto piece_at = [&](int t, int y) {
     const int page = p.page_values[page_begin + (t >> p.page_shift)];
-    return p.pages + ((((static_cast<int64_t>(page) * 2 + part) * p.h_kv + kvh) << p.page_shift) + (t & in_page)) * (p.pieces * 16);
+    const bool v = y >= half;
+    return p.pages + (((((static_cast<int64_t>(page) * 2 + v) * p.h_kv + kvh) << p.page_shift) + (t & in_page)) * half + (y - (v ? half : 0))) * 16;
   };
-  const int limit = min(p.max_keep, capacity);
-  for (int i0 = 0; i0 < limit; i0 += kMoveThreads) {
-    const int i = i0 + tid;
-    const int from = i < limit ? kept[i] : -1;
-    const bool moves = from > i && from < capacity;
-    if (part == 2) {
-      float x = 0.f;
-      if (moves) x = *sum_at(from);
+  // Loads are complete, not only issued, where a workgroup goes on to overwrite what they read.
+  const auto all_have_read = [&] {
+    if (in_order) {
+      wait_vmcnt<0>();
       __syncthreads();
-      if (moves) *sum_at(i) = x;
-      continue;
     }
-    const uint64_t who = __ballot(moves);
-    if (lane == 0) per_wave[wave] = __popcll(who);
-    __syncthreads();
-    int at = __popcll(who & ((uint64_t{1} << lane) - 1)), count = 0;
+  };
+  for (int i0 = lo; i0 < hi; i0 += kMoveThreads * EACH) {
+    int from[EACH], at[EACH];
 #pragma unroll
-    for (int w = 0; w < kMoveThreads / 64; ++w) {
-      at += w < wave ? per_wave[w] : 0;
-      count += per_wave[w];
+    for (int u = 0; u < EACH; ++u) {
+      const int i = i0 + u * kMoveThreads + tid;
+      from[u] = i < hi ? kept[i] : -1;
     }
-    if (moves) {
-      places[at] = i;
-      sources[at] = from;
+#pragma unroll
+    for (int u = 0; u < EACH; ++u) {
+      if (!moves(i0 + u * kMoveThreads + tid, from[u])) from[u] = -1;
+      const uint64_t who = __ballot(from[u] >= 0);
+      at[u] = __popcll(who & ((uint64_t{1} << lane) - 1));
+      if (lane == 0) per_wave[u][wave] = __popcll(who);
     }
     __syncthreads();
-    constexpr int U = 4;
-    const int total = count * p.pieces;  // at most 256 rows of 64 pieces
+    int count = 0;
+#pragma unroll
+    for (int u = 0; u < EACH; ++u) {
+#pragma unroll
+      for (int w = 0; w < kMoveWaves; ++w) {
+        at[u] += w == wave ? count : 0;
+        count += per_wave[u][w];
+      }
+      if (from[u] >= 0) list[at[u]] = make_int2(i0 + u * kMoveThreads + tid, from[u]);
+    }
+    __syncthreads();
+    if (with_sums) {
+      float sum[EACH];
+#pragma unroll
+      for (int u = 0; u < EACH; ++u) {
+        const int x = u * kMoveThreads + tid;
+        if (x < count) sum[u] = *sum_at(list[x].y);
+      }
+      all_have_read();
+#pragma unroll
+      for (int u = 0; u < EACH; ++u) {
+        const int x = u * kMoveThreads + tid;
+        if (x < count) *sum_at(list[x].x) = sum[u];
+      }
+    }
+    constexpr int U = 8;
+    const int total = count * width;
     for (int x0 = 0; x0 < total; x0 += kMoveThreads * U) {
       Vec16 v[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int x = x0 + u * kMoveThreads + tid, row = p.by_pieces(x);
-        if (x < total) v[u] = ld16(row_at(sources[row]) + (x - row * p.pieces) * 16);
+        const int x = x0 + u * kMoveThreads + tid, row = by_width(x);
+        if (x < total) v[u] = ld16_nt(piece_at(list[row].y, y0 + x - row * width));
       }
-      __syncthreads();
+      all_have_read();
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int x = x0 + u * kMoveThreads + tid, row = p.by_pieces(x);
-        if (x < total) st16(row_at(places[row]) + (x - row * p.pieces) * 16, v[u]);
+        const int x = x0 + u * kMoveThreads + tid, row = by_width(x);
+        if (x < total) st16(piece_at(list[row].x, y0 + x - row * width), v[u]);
       }
     }
     __syncthreads();  // the list has been read
@@ -541,14 +925,20 @@ int tvmkv_select_kept_tokens(const float* key_weights, const int32_t* page_indpt
   p.words = nullptr;
   p.counts = nullptr;
   const int64_t tokens = nnz_pages << p.page_shift;
+  const bool small = tokens <= static_cast<int64_t>(batch_size) * 4096;
+  const int blocks_in_lds = small ? 256 : 1024;
   ScratchLease ws{};
-  if (tokens > kLdsWords * 64) {
-    const size_t words = static_cast<size_t>((tokens >> 6) + batch_size) * h_kv;
-    ws = lease_scratch(kScratchEvict, s, words * (sizeof(uint64_t) + sizeof(int32_t)), 0);
+  if (tokens > static_cast<int64_t>(blocks_in_lds) * 256) {
+    const size_t blocks = static_cast<size_t>((tokens >> 8) + batch_size) * h_kv;
+    ws = lease_scratch(kScratchEvict, s, blocks * (4 * sizeof(uint64_t) + sizeof(int32_t)), 0);
     p.words = reinterpret_cast<uint64_t*>(ws.ptr);
-    p.counts = reinterpret_cast<int32_t*>(p.words + words);
+    p.counts = reinterpret_cast<int32_t*>(p.words + blocks * 4);
   }
-  hipLaunchKernelGGL(select_kept_kernel, dim3(h_kv, batch_size), dim3(kSelectThreads), 0, s, p);
+  if (small) {
+    hipLaunchKernelGGL((select_kept_kernel<256, 256, 2048, 8>), dim3(h_kv, batch_size), dim3(256), 0, s, p);
+  } else {
+    hipLaunchKernelGGL((select_kept_kernel<1024, 1024, 20480, 32>), dim3(h_kv, batch_size), dim3(1024), 0, s, p);
+  }
   KV_LAUNCH_CHECK();
   KV_API_END();
 }
@@ -577,9 +967,25 @@ int tvmkv_move_kept_tokens(void* pages, float* key_weights, const int32_t* page_
   p.kept = kept;
   p.h_kv = h_kv;
   p.max_keep = max_keep;
-  p.pieces = d * dtype_bits / 128;
-  p.by_pieces = ExactDivision::by(p.pieces);
-  hipLaunchKernelGGL(move_kept_kernel, dim3(key_weights != nullptr ? 3 : 2, h_kv, batch_size), dim3(kMoveThreads), 0, as_stream(stream), p);
+  p.pieces = 2 * (d * dtype_bits / 128);
+  const int64_t lists = static_cast<int64_t>(batch_size) * h_kv;
+  // In one launch and in order, in parts of 128 bytes at least, where that makes four workgroups a compute unit, or lists are short.
+  const auto cut_rows = [&](int64_t most, int least_pieces) {
+    p.slices = 1;
+    while (p.slices * 2 <= most && p.pieces % (p.slices * 2) == 0 && p.pieces / (p.slices * 2) >= least_pieces) p.slices *= 2;
+    p.by_row = ExactDivision::by(p.pieces);
+    p.by_slice = ExactDivision::by(p.pieces / p.slices);
+  };
+  const int wanted = 4 * compute_units();
+  cut_rows(std::max<int64_t>(wanted / lists, 1), 8);
+  if (lists * p.slices >= wanted || max_keep <= 1024) {
+    hipLaunchKernelGGL(move_kept_kernel<kMoveInOrder>, dim3(p.slices, h_kv, batch_size), dim3(kMoveThreads), 0, as_stream(stream), p);
+  } else {
+    const int parts = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>((max_keep + 63) / 64, wanted / lists)));
+    cut_rows(parts, 4);
+    hipLaunchKernelGGL(move_kept_kernel<kMoveFirst>, dim3(parts, h_kv, batch_size), dim3(kMoveThreads), 0, as_stream(stream), p);
+    hipLaunchKernelGGL(move_kept_kernel<kMoveSecond>, dim3(parts, h_kv, batch_size), dim3(kMoveThreads), 0, as_stream(stream), p);
+  }
   KV_LAUNCH_CHECK();
   KV_API_END();
 }
