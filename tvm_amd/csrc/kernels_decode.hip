@@ -87,6 +87,9 @@ struct DecodeParams {
   int rope_inverse;
   int rope_halves_differ;
   float rope_magnitude;
+  // decode_mfma_kernel<..., KEEP = true>: the scaled scores (base 2) of all keys, float32 (16-token run of the page table, kv head,
+  // head of the group, 16 tokens)
+  float* scores;
 };
 
 // Same answer as find_sequence for more than 64 sequences, computed by one wavefront as a 64-ary search: the lanes
@@ -317,6 +320,8 @@ struct DecodeRopeRunning : DecodeRopeDivisors {
 // state of that one key instead of the empty one, so that a step whose new rows may not be in the pages yet (windows,
 // steps that mix prompts and decoding sequences) needs neither a self-attention launch nor a merge.
 //
+// KEEP (plain cache, groups of one block): the scores also go to memory, for the sums of attention weights (kernels_evict.hip).
+//
 // decode_items works on items first_item, first_item + stride, ... below num_items.
 template <int D, bool FUSED, bool RUNNING>
 struct DecodeShared {
@@ -326,7 +331,8 @@ struct DecodeShared {
   alignas(16) half_t own[FUSED ? 2 * D : 8];  // the new token's rotated k row and its v row
   alignas(16) float rope[RUNNING ? 5 : 1][RUNNING ? D / 2 : 1];
 };
-template <bool EXT, int D, bool REREAD, int HB = 1, bool FUSED = false, bool PAD = false, bool VARIANT = false, bool SELF = false>
+template <bool EXT, int D, bool REREAD, int HB = 1, bool FUSED = false, bool PAD = false, bool VARIANT = false, bool SELF = false,
+          bool KEEP = false>
 __device__ __forceinline__ void decode_items(const DecodeParams& p, const int group, const int num_items,
                                              const std::conditional_t<EXT && !VARIANT, DecodeRopeRunning, DecodeRopeDivisors>& div,
                                              const int first_item, const int stride, DecodeShared<D, FUSED, EXT && !VARIANT>& shared) {
@@ -334,6 +340,7 @@ __device__ __forceinline__ void decode_items(const DecodeParams& p, const int gr
   static_assert(!(FUSED && EXT), "the fused step exists for the plain cache");
   static_assert(!SELF || (EXT && !VARIANT), "the new-token form: an extended kernel with the default frequencies");
   static_assert(!PAD || (!EXT && !FUSED), "padded head dims: plain cache, no in-kernel RoPE");
+  static_assert(!KEEP || (!EXT && !FUSED && HB == 1), "kept scores: plain cache, one block of heads");
   const int dm = PAD ? p.d_mem : D;  // elements per row in memory
   constexpr int PS = DM_PS;
   constexpr int KS = D / 32;                // k-steps of the score product
@@ -853,6 +860,18 @@ __device__ __forceinline__ void decode_items(const DecodeParams& p, const int gr
           mx = fmaxf(mx, v);
         }
       }
+      if constexpr (KEEP) {
+        if (c16 < heads) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            if (pi + h >= page_hi) break;
+            float* to = p.scores + (((static_cast<int64_t>(pbeg) << psh) + pi + h) * p.h_kv + kvh) * (group * 16) + c16 * 16 + 2 * g4;
+            static_assert(!KEEP || KLINE, "a lane's tokens");
+            *reinterpret_cast<float2*>(to) = make_float2(s[j][h][0], s[j][h][1]);
+            *reinterpret_cast<float2*>(to + 8) = make_float2(s[j][h][2], s[j][h][3]);
+          }
+        }
+      }
       mx = max_xor32(max_xor16(mx));
       // the reference point moves only when the maximum exceeds it by more than 2^8 (p stays <= 256):
       // after the first steps almost no step rescales O
@@ -999,11 +1018,12 @@ __device__ __forceinline__ void decode_items(const DecodeParams& p, const int gr
   }  // items
 }
 
-template <bool EXT, int D, bool REREAD, int HB = 1, bool FUSED = false, bool PAD = false, bool VARIANT = false, bool SELF = false>
+template <bool EXT, int D, bool REREAD, int HB = 1, bool FUSED = false, bool PAD = false, bool VARIANT = false, bool SELF = false,
+          bool KEEP = false>
 __global__ __launch_bounds__(256, D > 128 ? 1 : ((EXT || HB > 1) ? 2 : 3)) void decode_mfma_kernel(DecodeParams p, int group, int num_items,
     std::conditional_t<EXT && !VARIANT, DecodeRopeRunning, DecodeRopeDivisors> div) {
   __shared__ DecodeShared<D, FUSED, EXT && !VARIANT> shared;
-  decode_items<EXT, D, REREAD, HB, FUSED, PAD, VARIANT, SELF>(p, group, num_items, div, blockIdx.x, gridDim.x, shared);
+  decode_items<EXT, D, REREAD, HB, FUSED, PAD, VARIANT, SELF, KEEP>(p, group, num_items, div, blockIdx.x, gridDim.x, shared);
 }
 
 // The decoding sequences of a step and its prompts in one launch.  Behind each other, the prompts' row tiles wait for the
@@ -1125,6 +1145,7 @@ struct FusedStep {
   const int32_t* page_begin = nullptr;
   int64_t q_stride = 0, new_stride = 0;
   const PromptLaunch* beside = nullptr;
+  float* scores = nullptr;  // where a plain call of groups of at most 16 heads keeps its scores
 };
 
 // Body of the decode entry point.  lease(bytes, at_least) hands out the scratch memory of the call: arrival
@@ -1197,6 +1218,7 @@ static void decode_entry(Lease&& lease, const FusedStep& fused_step, const void*
   p.v_new = static_cast<const half_t*>(fused_step.v_new);
   p.rows = fused_step.rows;
   p.page_begin = fused_step.page_begin;
+  p.scores = fused_step.scores;
   p.q_stride = fused_step.q_stride;
   p.new_stride = fused_step.new_stride;
   const int64_t slots = nnz_pages / p.chunk_pages + batch_size;
@@ -1256,7 +1278,9 @@ static void decode_entry(Lease&& lease, const FusedStep& fused_step, const void*
       hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(grid_x)), dim3(256), 0, s, p, group, static_cast<int>(num_items),
                          static_cast<const DecodeRopeDivisors&>(div));
     };
-    if (head_blocks > 1) {
+    if (p.scores != nullptr) {
+      launch_padded(decode_mfma_kernel<false, 128, false, 1, false, true, false, false, true>);
+    } else if (head_blocks > 1) {
       launch_padded(decode_mfma_kernel<false, 128, true, 2, false, true>);
     } else if (heads_per_item == 32) {
       launch_padded(decode_mfma_kernel<false, 128, false, 2, false, true>);
@@ -1278,7 +1302,9 @@ static void decode_entry(Lease&& lease, const FusedStep& fused_step, const void*
     constexpr int kWide = kD <= 128 ? 2 : 1;  // head blocks per item for groups of more than 16 heads
     const bool wide = heads_per_item == 32;
     const bool reread = head_blocks > 1;       // several items read the same K/V rows
-    if (fused_step.beside != nullptr) {
+    if (p.scores != nullptr) {
+      launch(decode_mfma_kernel<false, kD, false, 1, false, false, false, false, true>);
+    } else if (fused_step.beside != nullptr) {
       if constexpr (kD <= 128) launch_beside_prefill<kD>(p, group, num_items, div, *fused_step.beside, s);
     } else if (fused_launch) {
       if (reread) {
@@ -1489,6 +1515,21 @@ int tvmkv::decode_with_shared_prefix(const SharedPrefixDecode& a, void* stream) 
     KV_API_END();
   };
   return prefill_shared_prefix(a, own, stream);
+}
+
+// Decode attention that also keeps its scores (typed_kernels.h)
+int tvmkv::decode_keeping_scores(const void* q, const void* pages, const int32_t* page_indptr, const int32_t* page_values,
+                                 const int32_t* length_info, void* output, float* lse, float* scores, double sm_scale, int32_t batch_size,
+                                 int64_t nnz_pages, int64_t num_pages, int32_t h_q, int32_t h_kv, int32_t d, int32_t page_size, void* stream) {
+  KV_API_BEGIN();
+  KV_CHECK(h_kv > 0 && h_q <= 16 * h_kv) << "decode_keeping_scores: more than 16 query heads a kv head";
+  hipStream_t s = as_stream(stream);
+  FusedStep step;
+  step.scores = scores;
+  decode_entry([&](size_t bytes, size_t at_least) { return lease_scratch(kScratchDecode, s, bytes, kArrivalBytes, at_least); }, step, q, pages, page_indptr,
+               page_values, length_info, nullptr, nullptr, output, lse, 0, 1.0, 1e4, sm_scale, batch_size, nnz_pages, num_pages, h_q, h_kv, d,
+               page_size, 0, stream);
+  KV_API_END();
 }
 
 // The same entry point for callers that must not allocate (code under HIP graph capture, serving

@@ -17,6 +17,9 @@
 
 namespace tvmkv {
 
+typedef float float4_any_t __attribute__((ext_vector_type(4), aligned(4)));
+typedef int int4_any_t __attribute__((ext_vector_type(4), aligned(4)));
+
 // Where work items begin: sequence b of x_b = tokens that its pages hold owns the slots [X_b / per + b, ...), X_b the tokens of
 // the pages in front of it; the grid, sized from shapes alone, has X_batch / per + batch slots.
 struct SequenceOf {
@@ -151,6 +154,65 @@ __global__ __launch_bounds__(256) void key_weights_kernel(KeyWeightsParams p) {
 }
 
 // ------------------------------------------------------------------------------------------
+// Weights from kept scores: decode's, which are few (4 bytes for each of the group's heads, where K has 2 D).  A wave has 256 tokens
+// of a kv head, a lane four neighbouring ones of every head.
+// ------------------------------------------------------------------------------------------
+struct KeptScoresParams {
+  const float* scores;  // (16-token run of the page table, kv head, head of the group, 16 tokens)
+  const int32_t* page_indptr;
+  const int32_t* weight_page_values;
+  const int32_t* last_page_len;
+  const float* lse;
+  float* key_weights;
+  int batch;
+  int h_kv;
+  int group;
+  int page_shift;
+};
+constexpr int kKeptTokensShift = 10;  // of a workgroup
+__global__ __launch_bounds__(256) void kept_scores_kernel(KeptScoresParams p) {
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int kvh = blockIdx.x % p.h_kv, slot = blockIdx.x / p.h_kv;
+  const SequenceOf s = sequence_of_slot(p.page_indptr, p.last_page_len, p.batch, p.page_shift, kKeptTokensShift, slot, lane);
+  const int stored = s.stored(p.page_shift);
+  const int t0 = ((slot - s.slot_begin) << kKeptTokensShift) + wave * 256, t = t0 + lane * 4;
+  if (t >= stored) return;
+  const int run = (s.page_begin << (p.page_shift - 4)) + (t >> 4);
+  const float* at = p.scores + ((static_cast<int64_t>(run) * p.h_kv + kvh) * p.group) * 16 + (t & 15);
+  const float* lse = p.lse + (static_cast<int64_t>(s.index) * p.h_kv + kvh) * p.group;
+  const int page = p.weight_page_values[s.page_begin + (t >> p.page_shift)];
+  float* const to = p.key_weights + ((static_cast<int64_t>(page) * p.h_kv + kvh) << p.page_shift) + (t & ((1 << p.page_shift) - 1));
+  const float4_any_t before = *reinterpret_cast<const float4_any_t*>(to);
+  float4_any_t sum = {0.f, 0.f, 0.f, 0.f};  // of this call's alone, so that what is there already rounds it once
+  for (int g = 0; g < p.group; g += 4) {
+    float4_t x[4];
+    float of[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int h = min(g + i, p.group - 1);
+      x[i] = *reinterpret_cast<const float4_t*>(at + h * 16);
+      of[i] = lse[h];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (g + i < p.group) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) sum[k] += fast_exp2(x[i][k] - of[i]);
+      }
+    }
+  }
+  sum += before;
+  if (t + 4 <= stored) {
+    *reinterpret_cast<float4_any_t*>(to) = sum;
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (t + k < stored) to[k] = sum[k];
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------
 // The choice.  A workgroup has the tokens of one (sequence, kv head).  As integers that order like them (NaN below everything, -0
 // as 0) the weights go through passes of 8 bits that find the smallest one that stays, T, and how many of the weights equal to it
 // do: counts, exact whatever their order.  Then a bit a token says which ones stay, and running counts of free places and of tokens
@@ -176,9 +238,6 @@ struct SelectParams {
   int recent;
   int page_shift;
 };
-typedef float float4_any_t __attribute__((ext_vector_type(4), aligned(4)));
-typedef int int4_any_t __attribute__((ext_vector_type(4), aligned(4)));
-
 constexpr uint32_t kOrderOfMinusInf = 0x007fffff, kOrderOfInf = 0xff800000;
 __device__ __forceinline__ uint32_t weight_order(float w) {
   if (w != w) return 0;
@@ -799,6 +858,8 @@ static void check_aligned16(const char* what, std::initializer_list<const void*>
     KV_CHECK(reinterpret_cast<uintptr_t>(t) % 16 == 0) << what << ": q, pages and output must be aligned to 16 bytes";
 }
 
+constexpr size_t kMostKept = size_t{1} << 29;  // bytes of a decode call's kept scores; more than that is computed again
+
 static void add_key_weights(const char* what, const void* q, const int32_t* q_indptr, const void* pages, const int32_t* page_indptr,
                             const int32_t* page_values, const int32_t* length_info, const float* lse, float* key_weights,
                             const int32_t* weight_page_values, bool causal, int64_t observed, double sm_scale, int32_t batch_size,
@@ -870,6 +931,29 @@ int tvmkv_batch_decode_paged_kv_weights(const void* q, const void* pages, const 
   check_attention(what, q, pages, page_indptr, page_values, length_info, output, lse, key_weights, weight_page_values, batch_size, nnz_pages,
                   h_q, h_kv, d, page_size);
   if (batch_size == 0) return TVMKV_OK;
+  const size_t kept = static_cast<size_t>(nnz_pages) * page_size * h_q * sizeof(float);
+  if (nnz_pages > 0 && h_q <= 16 * h_kv && kept <= kMostKept) {
+    const hipStream_t s = as_stream(stream);
+    const ScratchLease ws = lease_scratch(kScratchEvict, s, kept, 0);
+    KeptScoresParams p;
+    p.scores = reinterpret_cast<const float*>(ws.ptr);
+    p.page_indptr = page_indptr;
+    p.weight_page_values = weight_page_values;
+    p.last_page_len = length_info;
+    p.lse = lse;
+    p.key_weights = key_weights;
+    p.batch = batch_size;
+    p.h_kv = h_kv;
+    p.group = h_q / h_kv;
+    p.page_shift = shift_of_page(what, page_size);
+    const int64_t items = (((nnz_pages << p.page_shift) >> kKeptTokensShift) + batch_size) * h_kv;
+    KV_CHECK(items < (int64_t{1} << 31)) << what << ": too many work items";
+    run(decode_keeping_scores(q, pages, page_indptr, page_values, length_info, output, lse, reinterpret_cast<float*>(ws.ptr), sm_scale, batch_size,
+                              nnz_pages, num_pages, h_q, h_kv, d, page_size, stream));
+    hipLaunchKernelGGL(kept_scores_kernel, dim3(static_cast<unsigned>(items)), dim3(256), 0, s, p);
+    KV_LAUNCH_CHECK();
+    return TVMKV_OK;
+  }
   run(tvmkv_batch_decode_paged_kv(q, pages, page_indptr, page_values, length_info, nullptr, nullptr, output, lse, 0, 1.0, 1e4, sm_scale,
                                   batch_size, nnz_pages, num_pages, h_q, h_kv, d, page_size, 0, stream));
   add_key_weights(what, q, nullptr, pages, page_indptr, page_values, length_info, lse, key_weights, weight_page_values, false, 0, sm_scale,

@@ -157,6 +157,12 @@ struct NewTokenDecode {
   int32_t batch = 0, h_q = 0, h_kv = 0, d = 0, page_size = 0;
   int32_t sliding = 0;
 };
+// tvmkv_batch_decode_paged_kv over a plain cache, at most 16 query heads a kv head, that also writes the scaled scores (base 2) of all
+// keys: scores (16-token run of the page table, kv head, head of the group, 16 tokens).  What a run holds behind the last token is not
+// written or of no use.
+int decode_keeping_scores(const void* q, const void* pages, const int32_t* page_indptr, const int32_t* page_values, const int32_t* length_info,
+                          void* output, float* lse, float* scores, double sm_scale, int32_t batch_size, int64_t nnz_pages, int64_t num_pages,
+                          int32_t h_q, int32_t h_kv, int32_t d, int32_t page_size, void* stream);
 struct PromptLaunch;
 // beside: prompts to run in the same launch (kernels_decode.hip), or NULL
 int decode_with_new_token(const NewTokenDecode& args, void* stream, const PromptLaunch* beside = nullptr);
