@@ -87,9 +87,10 @@ struct DecodeParams {
   int rope_inverse;
   int rope_halves_differ;
   float rope_magnitude;
-  // decode_mfma_kernel<..., KEEP = true>: the scaled scores (base 2) of all keys, float32 (16-token run of the page table, kv head,
-  // head of the group, 16 tokens)
+  // decode_mfma_kernel<..., KEEP = true>: the scaled scores (base 2) of all keys, float32 (kv head, 16-token run of the page table,
+  // head of the group, 16 tokens in the order that kept_score_token gives)
   float* scores;
+  int64_t scores_of_head;  // of a kv head
 };
 
 // Same answer as find_sequence for more than 64 sequences, computed by one wavefront as a 64-ary search: the lanes
@@ -860,18 +861,6 @@ __device__ __forceinline__ void decode_items(const DecodeParams& p, const int gr
           mx = fmaxf(mx, v);
         }
       }
-      if constexpr (KEEP) {
-        if (c16 < heads) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            if (pi + h >= page_hi) break;
-            float* to = p.scores + (((static_cast<int64_t>(pbeg) << psh) + pi + h) * p.h_kv + kvh) * (group * 16) + c16 * 16 + 2 * g4;
-            static_assert(!KEEP || KLINE, "a lane's tokens");
-            *reinterpret_cast<float2*>(to) = make_float2(s[j][h][0], s[j][h][1]);
-            *reinterpret_cast<float2*>(to + 8) = make_float2(s[j][h][2], s[j][h][3]);
-          }
-        }
-      }
       mx = max_xor32(max_xor16(mx));
       // the reference point moves only when the maximum exceeds it by more than 2^8 (p stays <= 256):
       // after the first steps almost no step rescales O
@@ -899,6 +888,16 @@ __device__ __forceinline__ void decode_items(const DecodeParams& p, const int gr
     // vmcnt reaches 0, and the reads below are done before the MFMAs that use them are issued,
     // which is before the next step's copies in program order.
     wait_vmcnt<0>();
+    if constexpr (KEEP) {  // behind that wait, which would take their way to memory too (64 sequences of 1024-4096 tokens 134 us)
+      static_assert(!KEEP || KLINE, "a lane's tokens");
+      if (c16 < heads) {
+        float* const to = p.scores + kvh * p.scores_of_head + ((static_cast<int64_t>(pbeg) << psh) + pi) * (group * 16) + c16 * 16 + 4 * g4;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (pi + h < page_hi) *reinterpret_cast<float4_t*>(to + h * (group * 16)) = s[0][h];
+        }
+      }
+    }
     const bool gap = EXT && __builtin_amdgcn_readfirstlane(pi * PS < win_lo && (pi + 2) * PS > sink);
 #pragma unroll
     for (int db = 0; db < DB; ++db) {
@@ -1219,6 +1218,7 @@ static void decode_entry(Lease&& lease, const FusedStep& fused_step, const void*
   p.rows = fused_step.rows;
   p.page_begin = fused_step.page_begin;
   p.scores = fused_step.scores;
+  p.scores_of_head = (nnz_pages << p.page_shift) * group * 16;
   p.q_stride = fused_step.q_stride;
   p.new_stride = fused_step.new_stride;
   const int64_t slots = nnz_pages / p.chunk_pages + batch_size;

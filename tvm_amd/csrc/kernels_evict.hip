@@ -18,6 +18,7 @@
 namespace tvmkv {
 
 typedef float float4_any_t __attribute__((ext_vector_type(4), aligned(4)));
+typedef float float2_any_t __attribute__((ext_vector_type(2), aligned(4)));
 typedef int int4_any_t __attribute__((ext_vector_type(4), aligned(4)));
 
 // Where work items begin: sequence b of x_b = tokens that its pages hold owns the slots [X_b / per + b, ...), X_b the tokens of
@@ -155,16 +156,17 @@ __global__ __launch_bounds__(256) void key_weights_kernel(KeyWeightsParams p) {
 
 // ------------------------------------------------------------------------------------------
 // Weights from kept scores: decode's, which are few (4 bytes for each of the group's heads, where K has 2 D).  A wave has 256 tokens
-// of a kv head, a lane four neighbouring ones of every head.
+// of a kv head, a lane the four of a run of 16 that a lane of the decode kernel had.
 // ------------------------------------------------------------------------------------------
 struct KeptScoresParams {
-  const float* scores;  // (16-token run of the page table, kv head, head of the group, 16 tokens)
+  const float* scores;  // (kv head, 16-token run of the page table, head of the group, 16 tokens in the order of kept_score_token)
   const int32_t* page_indptr;
   const int32_t* weight_page_values;
   const int32_t* last_page_len;
   const float* lse;
   float* key_weights;
   int batch;
+  int nnz_pages;
   int h_kv;
   int group;
   int page_shift;
@@ -175,15 +177,17 @@ __global__ __launch_bounds__(256) void kept_scores_kernel(KeptScoresParams p) {
   const int kvh = blockIdx.x % p.h_kv, slot = blockIdx.x / p.h_kv;
   const SequenceOf s = sequence_of_slot(p.page_indptr, p.last_page_len, p.batch, p.page_shift, kKeptTokensShift, slot, lane);
   const int stored = s.stored(p.page_shift);
-  const int t0 = ((slot - s.slot_begin) << kKeptTokensShift) + wave * 256, t = t0 + lane * 4;
-  if (t >= stored) return;
-  const int run = (s.page_begin << (p.page_shift - 4)) + (t >> 4);
-  const float* at = p.scores + ((static_cast<int64_t>(run) * p.h_kv + kvh) * p.group) * 16 + (t & 15);
+  const int run = (((slot - s.slot_begin) << kKeptTokensShift) + wave * 256) / 16 + (lane >> 2);  // of the sequence
+  if (run * 16 >= stored) return;
+  const float* at = p.scores + (((kvh * static_cast<int64_t>(p.nnz_pages) + s.page_begin) << (p.page_shift - 4)) + run) * (p.group * 16) + 4 * (lane & 3);
   const float* lse = p.lse + (static_cast<int64_t>(s.index) * p.h_kv + kvh) * p.group;
-  const int page = p.weight_page_values[s.page_begin + (t >> p.page_shift)];
-  float* const to = p.key_weights + ((static_cast<int64_t>(page) * p.h_kv + kvh) << p.page_shift) + (t & ((1 << p.page_shift) - 1));
-  const float4_any_t before = *reinterpret_cast<const float4_any_t*>(to);
-  float4_any_t sum = {0.f, 0.f, 0.f, 0.f};  // of this call's alone, so that what is there already rounds it once
+  const int page = p.weight_page_values[s.page_begin + (run >> (p.page_shift - 4))];
+  float* const to = p.key_weights + ((static_cast<int64_t>(page) * p.h_kv + kvh) << p.page_shift) + (run * 16 & ((1 << p.page_shift) - 1));
+  // the lane's tokens are two pairs of neighbours
+  static_assert(kept_score_token(1) == kept_score_token(0) + 1 && kept_score_token(2) == kept_score_token(0) + 8 && kept_score_token(4) == 2, "pairs");
+  const int first = 2 * (lane & 3);
+  const float2_any_t before[2] = {*reinterpret_cast<const float2_any_t*>(to + first), *reinterpret_cast<const float2_any_t*>(to + first + 8)};
+  float sum[4] = {0.f, 0.f, 0.f, 0.f};  // of this call's weights alone, so that what is there already rounds it once
   for (int g = 0; g < p.group; g += 4) {
     float4_t x[4];
     float of[4];
@@ -201,14 +205,12 @@ __global__ __launch_bounds__(256) void kept_scores_kernel(KeptScoresParams p) {
       }
     }
   }
-  sum += before;
-  if (t + 4 <= stored) {
-    *reinterpret_cast<float4_any_t*>(to) = sum;
-  } else {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      if (t + k < stored) to[k] = sum[k];
-    }
+  for (int k = 0; k < 2; ++k) {
+    const int token = first + 8 * k, left = stored - (run * 16 + token);
+    const float2_any_t x = {before[k][0] + sum[2 * k], before[k][1] + sum[2 * k + 1]};
+    if (left >= 2) *reinterpret_cast<float2_any_t*>(to + token) = x;
+    if (left == 1) to[token] = x[0];
   }
 }
 
@@ -943,6 +945,7 @@ int tvmkv_batch_decode_paged_kv_weights(const void* q, const void* pages, const 
     p.lse = lse;
     p.key_weights = key_weights;
     p.batch = batch_size;
+    p.nnz_pages = static_cast<int>(nnz_pages);
     p.h_kv = h_kv;
     p.group = h_q / h_kv;
     p.page_shift = shift_of_page(what, page_size);

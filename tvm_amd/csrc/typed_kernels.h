@@ -158,8 +158,10 @@ struct NewTokenDecode {
   int32_t sliding = 0;
 };
 // tvmkv_batch_decode_paged_kv over a plain cache, at most 16 query heads a kv head, that also writes the scaled scores (base 2) of all
-// keys: scores (16-token run of the page table, kv head, head of the group, 16 tokens).  What a run holds behind the last token is not
-// written or of no use.
+// keys: scores (kv head, 16-token run of the page table, head of the group, 16 places).  What a run holds behind the last token is not
+// written or of no use.  A lane of the kernel has two tokens of either half of a run, and writes them together: place p of a run is
+// token kept_score_token(p).
+constexpr int kept_score_token(int place) { return 8 * (place >> 1 & 1) + 2 * (place >> 2) + (place & 1); }
 int decode_keeping_scores(const void* q, const void* pages, const int32_t* page_indptr, const int32_t* page_values, const int32_t* length_info,
                           void* output, float* lse, float* scores, double sm_scale, int32_t batch_size, int64_t nnz_pages, int64_t num_pages,
                           int32_t h_q, int32_t h_kv, int32_t d, int32_t page_size, void* stream);
