@@ -55,6 +55,7 @@ __device__ __forceinline__ SequenceOf sequence_of_slot(const int32_t* page_indpt
 // Weights from q, K and lse.  A wave keeps 32 TB tokens' K in registers as the A operand of the 32x32x16 matrix instruction and
 // walks the rows (query token, query head of the group) that count, 32 at a time as the B operand: S^T[token, row] has a
 // row a lane, so that a lane subtracts one lse, and its 16 sums a block are tokens'.  The lanes' sums are added at the end.
+// The four waves share the rows, which asynchronous copies bring to shared memory kStages - 1 tiles ahead, with the rows' lse.
 // ------------------------------------------------------------------------------------------
 struct KeyWeightsParams {
   const half_t* q;
@@ -77,27 +78,48 @@ struct KeyWeightsParams {
   float scale_log2;
 };
 
+// copy16_to_lds of 4 bytes a lane
+__device__ __forceinline__ void copy4_to_lds(const void* src_base, uint32_t byte_off, uint32_t lds_addr) {
+  lds_addr = __builtin_amdgcn_readfirstlane(lds_addr);
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(byte_off), "s"(src_base), "s"(lds_addr) : "memory");
+}
+
+template <int D>
+struct WeightTiles {
+  static constexpr int kRow = D == 64 ? 64 : D <= 128 ? 128 : 256;  // halfs of a row in shared memory
+  static constexpr int kPieces = kRow / 8;
+  static constexpr int kCopies = 32 * kPieces / 256;  // copy instructions of a wave for a tile of 32 rows
+  static constexpr int kStages = 4;
+  // Piece c of row r is at c ^ swizzle(r): 16 lanes read the same piece of 16 neighbouring rows, 256 bytes in all banks.
+  static __device__ __forceinline__ int swizzle(int row) { return kRow == 64 ? row >> 1 & 7 : row & 15; }
+};
+
 template <int D, int TB>
-__global__ __launch_bounds__(256) void key_weights_kernel(KeyWeightsParams p) {
-  constexpr int KS = D / 16;
+__global__ __launch_bounds__(256, 2) void key_weights_kernel(KeyWeightsParams p) {
+  using Tiles = WeightTiles<D>;
+  constexpr int KS = D / 16, PIECES = Tiles::kPieces, COPIES = Tiles::kCopies, STAGES = Tiles::kStages;
   constexpr int T = 128 * TB;
+  static_assert(TB == 1 || TB == 2, "the shift below");
+  __shared__ __attribute__((aligned(16))) half_t rows_lds[STAGES][32 * Tiles::kRow];
+  __shared__ float lse_lds[STAGES][4][64];  // a copy for each wave, of 32 rows
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
   const int col = lane & 31;
   const int half = lane >> 5;
   const int kvh = blockIdx.x % p.h_kv, slot = blockIdx.x / p.h_kv;
   const SequenceOf s = sequence_of_slot(p.page_indptr, p.last_page_len, p.batch, p.page_shift, TB == 1 ? 7 : 8, slot, lane);
-  static_assert(TB == 1 || TB == 2, "the shift above");
   const int stored = s.stored(p.page_shift);
-  const int t0 = (slot - s.slot_begin) * T + wave * 32 * TB;  // the wave's first token
-  if (t0 >= stored) return;
+  const int tile_t0 = (slot - s.slot_begin) * T, t0 = tile_t0 + wave * 32 * TB;  // the workgroup's and the wave's first token
+  if (tile_t0 >= stored) return;
   const int q_begin = p.q_indptr != nullptr ? p.q_indptr[s.index] : s.index;
   const int q_len = p.q_indptr != nullptr ? p.q_indptr[s.index + 1] - q_begin : 1;
   const int first_counted = p.observed > 0 ? max(q_len - p.observed, 0) : 0;
   const int in_front = stored - q_len;  // query i sees the keys up to in_front + i
-  const int row_end = q_len * p.group;
-  const int row_begin = first_counted * p.group;
-  const int first_row = max(first_counted, p.causal ? t0 - in_front : 0) * p.group;  // no row in front of it sees the wave's tokens
+  const int row_begin = first_counted * p.group, row_end = q_len * p.group;
+  const auto end_of = [&](int token) { return p.causal ? min(in_front + token + 1, stored) : stored; };
+  // no row in front of the first tile's sees a token of the workgroup's
+  const int first_tile = max(first_counted, p.causal ? tile_t0 - in_front : 0) * p.group >> 5, num_tiles = (row_end + 31) >> 5;
+  if (first_tile >= num_tiles) return;
 
   half8_t k[TB][KS];
 #pragma unroll
@@ -114,29 +136,82 @@ __global__ __launch_bounds__(256) void key_weights_kernel(KeyWeightsParams p) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) sum[b][i] = 0.f;
   }
-  for (int r0 = first_row & ~31; r0 < row_end; r0 += 32) {
-    const int row = min(r0 + col, row_end - 1);
-    const int token = p.by_group(row);
-    const int64_t at = static_cast<int64_t>(q_begin + token) * p.h_q + kvh * p.group + row - token * p.group;
-    const bool counts = r0 + col < row_end && row >= row_begin;
-    const int end = p.causal ? min(in_front + token + 1, stored) : stored;
-    const float lse = p.lse[at];
+
+  const int64_t head0 = static_cast<int64_t>(q_begin) * p.h_q + kvh * p.group;  // (query, head) of row 0
+  // Tile by tile, tiles behind the last one as that one, so that a tile is always so many copies behind the next.
+  const auto issue = [&](int tile) {
+    const int r0 = min(tile, num_tiles - 1) * 32, token0 = p.by_group(r0), stage = tile % STAGES;
+    const int64_t at0 = head0 + static_cast<int64_t>(token0) * p.h_q;
+    const auto offset_of = [&](int r) {  // in heads, from the first head of the tile's first query
+      const int row = min(r0 + r, row_end - 1), token = p.by_group(row);
+      return static_cast<uint32_t>((token - token0) * p.h_q + row - token * p.group);
+    };
+    const uint32_t rows_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_ptr_t)rows_lds[stage]));
+#pragma unroll
+    for (int i = 0; i < COPIES; ++i) {
+      const int nth = (wave * COPIES + i) * 64, r = (nth + lane) / PIECES;
+      const int piece = min(((nth + lane) % PIECES) ^ Tiles::swizzle(r), D / 8 - 1);
+      copy16_to_lds(p.q + at0 * D, offset_of(r) * (D * 2) + piece * 16, rows_at + nth * 16);
+    }
+    copy4_to_lds(p.lse + at0, offset_of(col) * 4, static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_ptr_t)lse_lds[stage][wave])));
+  };
+  wait_vmcnt<0>();  // K is there: from here on only the copies count
+#pragma unroll
+  for (int i = 0; i < STAGES - 1; ++i) issue(first_tile + i);
+  for (int tile = first_tile; tile < num_tiles; ++tile) {
+    // The wave's part of the tile has landed where no more than the later tiles' copies are outstanding; behind the barrier everyone's
+    // has, and every wave is done with the stage that the next copies overwrite.
+    wait_vmcnt<(STAGES - 2) * (COPIES + 1)>();
+    __syncthreads();
+    issue(tile + STAGES - 1);
+    const int r0 = tile * 32;
+    if (end_of(p.by_group(min(r0 + 31, row_end - 1))) <= t0) continue;  // no row of the tile sees a token of the wave's
+    const half_t* const rows = rows_lds[tile % STAGES];
+    const float lse = lse_lds[tile % STAGES][wave][col];
     half8_t q[KS];
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) q[ks] = ld16(p.q + at * D + half * 8 + ks * 16).h8;
-#pragma unroll
-    for (int b = 0; b < TB; ++b) {
+    for (int ks = 0; ks < KS; ++ks)
+      q[ks] = *reinterpret_cast<const half8_t*>(rows + col * Tiles::kRow + (((ks * 2 + half) ^ Tiles::swizzle(col)) * 8));
+    const auto product = [&](int b) {
       float16_t x = {};
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) x = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[b][ks], q[ks], x, 0, 0, 0);
+      return x;
+    };
+    // every row counts and sees all of the wave's tokens (those behind the last stored one are not written)
+    if (r0 >= row_begin && r0 + 32 <= row_end && end_of(p.by_group(r0)) >= min(t0 + 32 * TB, stored)) {
+      const auto add = [&](int b, const float16_t& x) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int t = t0 + b * 32 + (i & 3) + 8 * (i >> 2) + 4 * half;
-        const float w = fast_exp2(fmaf(x[i], p.scale_log2, -lse));
-        sum[b][i] += counts && t < end ? w : 0.f;
+        for (int i = 0; i < 16; ++i) sum[b][i] += fast_exp2(fmaf(x[i], p.scale_log2, -lse));
+      };
+      __builtin_amdgcn_sched_barrier(0);
+      const float16_t x0 = product(0);
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (TB == 2) {
+        const float16_t x1 = product(TB - 1);
+        add(0, x0);
+        interleave_mfma_valu<KS>();
+        __builtin_amdgcn_sched_barrier(0);
+        add(TB - 1, x1);
+      } else {
+        add(0, x0);
+      }
+    } else {
+      const int row = min(r0 + col, row_end - 1);
+      const int end = r0 + col < row_end && row >= row_begin ? end_of(p.by_group(row)) : 0;
+#pragma unroll
+      for (int b = 0; b < TB; ++b) {
+        const float16_t x = product(b);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int t = t0 + b * 32 + (i & 3) + 8 * (i >> 2) + 4 * half;
+          const float w = fast_exp2(fmaf(x[i], p.scale_log2, -lse));
+          sum[b][i] += t < end ? w : 0.f;
+        }
       }
     }
   }
+  wait_vmcnt<0>();  // no copy is on its way into memory that is another workgroup's then
   // lane i of 32 takes the sum of its half's i-th token of a block
 #pragma unroll
   for (int b = 0; b < TB; ++b) {
@@ -865,7 +940,7 @@ constexpr size_t kMostKept = size_t{1} << 29;  // bytes of a decode call's kept 
 static void add_key_weights(const char* what, const void* q, const int32_t* q_indptr, const void* pages, const int32_t* page_indptr,
                             const int32_t* page_values, const int32_t* length_info, const float* lse, float* key_weights,
                             const int32_t* weight_page_values, bool causal, int64_t observed, double sm_scale, int32_t batch_size,
-                            int64_t nnz_pages, int32_t h_q, int32_t h_kv, int32_t d, int page_shift, hipStream_t stream) {
+                            int64_t total_q, int64_t nnz_pages, int32_t h_q, int32_t h_kv, int32_t d, int page_shift, hipStream_t stream) {
   if (batch_size == 0 || nnz_pages == 0) return;
   KeyWeightsParams p;
   p.q = static_cast<const half_t*>(q);
@@ -886,17 +961,23 @@ static void add_key_weights(const char* what, const void* q, const int32_t* q_in
   p.observed = static_cast<int>(std::min<int64_t>(observed, INT32_MAX));
   p.page_shift = page_shift;
   p.scale_log2 = static_cast<float>(sm_scale) * kLog2e;
-  const int64_t items = (((nnz_pages << page_shift) >> 7) + batch_size) * h_kv;
-  KV_CHECK(items < (int64_t{1} << 31)) << what << ": too many work items";
-  const auto launch = [&](auto dim) {
-    hipLaunchKernelGGL((key_weights_kernel<decltype(dim)::value, 1>), dim3(static_cast<unsigned>(items)), dim3(256), 0, stream, p);
+  const int64_t rows = std::min<int64_t>(total_q, observed > 0 ? observed * batch_size : total_q) * p.group;  // that count, at most
+  const auto launch = [&](auto dim, auto blocks) {
+    constexpr int D = decltype(dim)::value, TB = decltype(blocks)::value;
+    const int64_t items = (((nnz_pages << page_shift) / (128 * TB)) + batch_size) * h_kv;
+    KV_CHECK(items < (int64_t{1} << 31)) << what << ": too many work items";
+    hipLaunchKernelGGL((key_weights_kernel<D, TB>), dim3(static_cast<unsigned>(items)), dim3(256), 0, stream, p);
   };
-  if (d == 64) launch(std::integral_constant<int, 64>{});
-  if (d == 80) launch(std::integral_constant<int, 80>{});
-  if (d == 96) launch(std::integral_constant<int, 96>{});
-  if (d == 112) launch(std::integral_constant<int, 112>{});
-  if (d == 128) launch(std::integral_constant<int, 128>{});
-  if (d == 256) launch(std::integral_constant<int, 256>{});
+  const bool many_rows = rows >= int64_t{256} * batch_size;
+  const auto launch_blocks = [&](auto dim) {
+    if (many_rows) launch(dim, std::integral_constant<int, 2>{}); else launch(dim, std::integral_constant<int, 1>{});
+  };
+  if (d == 64) launch_blocks(std::integral_constant<int, 64>{});
+  if (d == 80) launch_blocks(std::integral_constant<int, 80>{});
+  if (d == 96) launch_blocks(std::integral_constant<int, 96>{});
+  if (d == 112) launch_blocks(std::integral_constant<int, 112>{});
+  if (d == 128) launch_blocks(std::integral_constant<int, 128>{});
+  if (d == 256) launch(std::integral_constant<int, 256>{}, std::integral_constant<int, 1>{});
   KV_LAUNCH_CHECK();
 }
 
@@ -960,7 +1041,7 @@ int tvmkv_batch_decode_paged_kv_weights(const void* q, const void* pages, const 
   run(tvmkv_batch_decode_paged_kv(q, pages, page_indptr, page_values, length_info, nullptr, nullptr, output, lse, 0, 1.0, 1e4, sm_scale,
                                   batch_size, nnz_pages, num_pages, h_q, h_kv, d, page_size, 0, stream));
   add_key_weights(what, q, nullptr, pages, page_indptr, page_values, length_info, lse, key_weights, weight_page_values, false, 0, sm_scale,
-                  batch_size, nnz_pages, h_q, h_kv, d, shift_of_page(what, page_size), as_stream(stream));
+                  batch_size, batch_size, nnz_pages, h_q, h_kv, d, shift_of_page(what, page_size), as_stream(stream));
   KV_API_END();
 }
 
@@ -981,7 +1062,7 @@ int tvmkv_batch_prefill_paged_kv_weights(const void* q, const int32_t* q_indptr,
   run(tvmkv_batch_prefill_paged_kv(q, q_indptr, pages, page_indptr, page_values, length_info, nullptr, nullptr, output, lse, causal, 0, 1.0, 1e4,
                                    sm_scale, batch_size, total_q, nnz_pages, num_pages, h_q, h_kv, d, page_size, 0, 0, stream));
   add_key_weights(what, q, q_indptr, pages, page_indptr, page_values, length_info, lse, key_weights, weight_page_values, causal != 0, observed,
-                  sm_scale, batch_size, nnz_pages, h_q, h_kv, d, shift_of_page(what, page_size), as_stream(stream));
+                  sm_scale, batch_size, total_q, nnz_pages, h_q, h_kv, d, shift_of_page(what, page_size), as_stream(stream));
   KV_API_END();
 }
 
