@@ -56,6 +56,7 @@ __device__ __forceinline__ SequenceOf sequence_of_slot(const int32_t* page_indpt
 // walks the rows (query token, query head of the group) that count, 32 at a time as the B operand: S^T[token, row] has a
 // row a lane, so that a lane subtracts one lse, and its 16 sums a block are tokens'.  The lanes' sums are added at the end.
 // The four waves share the rows, which asynchronous copies bring to shared memory kStages - 1 tiles ahead, with the rows' lse.
+// A block's products run under the exponentials of the block before it.
 // ------------------------------------------------------------------------------------------
 struct KeyWeightsParams {
   const half_t* q;
@@ -72,11 +73,31 @@ struct KeyWeightsParams {
   int h_kv;
   int group;
   ExactDivision by_group;
+  uint32_t inv_group;  // 2^16 / group, rounded up: divides numbers below 128 by groups below 64
   int causal;
   int observed;    // > 0: queries at a sequence's end that count
   int page_shift;  // pages hold 1 << page_shift tokens
   float scale_log2;
 };
+
+// The sequence of a slot where they are few: those with the most rows that count first, so that the last workgroups to start have the
+// least to do, each with as many slots as it has tiles of T tokens.
+__device__ __forceinline__ SequenceOf sequence_by_rows(const KeyWeightsParams& p, int T, int slot, int lane) {
+  const int at = min(lane, p.batch - 1);
+  const int page = p.page_indptr[at], num_pages = p.page_indptr[at + 1] - page, last = p.last_page_len[at];
+  int rows = p.q_indptr != nullptr ? p.q_indptr[at + 1] - p.q_indptr[at] : 1;
+  if (p.observed > 0) rows = min(rows, p.observed);
+  const int stored = num_pages > 0 ? ((num_pages - 1) << p.page_shift) + last : 0;
+  const int tiles = lane < p.batch && rows > 0 ? (stored + T - 1) / T : 0;
+  const int key = min(rows, (1 << 24) - 1) * 64 + 63 - lane;  // unlike from lane to lane
+  int begin = 0;
+  for (int j = 0; j < p.batch; ++j) begin += __builtin_amdgcn_readlane(key, j) > key ? __builtin_amdgcn_readlane(tiles, j) : 0;
+  const uint64_t hit = __ballot(slot >= begin && slot < begin + tiles);
+  if (hit == 0) return {-1, 0, 0, 0, 0};
+  const int who = __ffsll(static_cast<long long>(hit)) - 1;
+  const auto of = [&](int x) { return __builtin_amdgcn_readlane(x, who); };
+  return {who, of(begin), of(page), of(num_pages), of(last)};
+}
 
 // copy16_to_lds of 4 bytes a lane
 __device__ __forceinline__ void copy4_to_lds(const void* src_base, uint32_t byte_off, uint32_t lds_addr) {
@@ -84,30 +105,33 @@ __device__ __forceinline__ void copy4_to_lds(const void* src_base, uint32_t byte
   asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(byte_off), "s"(src_base), "s"(lds_addr) : "memory");
 }
 
-template <int D>
+template <int D, int TB>
 struct WeightTiles {
   static constexpr int kRow = D == 64 ? 64 : D <= 128 ? 128 : 256;  // halfs of a row in shared memory
   static constexpr int kPieces = kRow / 8;
-  static constexpr int kCopies = 32 * kPieces / 256;  // copy instructions of a wave for a tile of 32 rows
-  static constexpr int kStages = 4;
+  static constexpr int kRows = TB == 2 ? 64 : 32;        // of a tile
+  static constexpr int kCopies = kRows * kPieces / 256;  // copy instructions of a wave for a tile
+  static constexpr int kStages = TB == 2 ? 3 : 4;
   // Piece c of row r is at c ^ swizzle(r): 16 lanes read the same piece of 16 neighbouring rows, 256 bytes in all banks.
   static __device__ __forceinline__ int swizzle(int row) { return kRow == 64 ? row >> 1 & 7 : row & 15; }
 };
 
 template <int D, int TB>
 __global__ __launch_bounds__(256, 2) void key_weights_kernel(KeyWeightsParams p) {
-  using Tiles = WeightTiles<D>;
-  constexpr int KS = D / 16, PIECES = Tiles::kPieces, COPIES = Tiles::kCopies, STAGES = Tiles::kStages;
+  using Tiles = WeightTiles<D, TB>;
+  constexpr int KS = D / 16, PIECES = Tiles::kPieces, COPIES = Tiles::kCopies, STAGES = Tiles::kStages, R = Tiles::kRows;
   constexpr int T = 128 * TB;
   static_assert(TB == 1 || TB == 2, "the shift below");
-  __shared__ __attribute__((aligned(16))) half_t rows_lds[STAGES][32 * Tiles::kRow];
-  __shared__ float lse_lds[STAGES][4][64];  // a copy for each wave, of 32 rows
+  __shared__ __attribute__((aligned(16))) half_t rows_lds[STAGES][R * Tiles::kRow];
+  __shared__ float lse_lds[STAGES][4][64];  // a copy for each wave
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
   const int col = lane & 31;
   const int half = lane >> 5;
   const int kvh = blockIdx.x % p.h_kv, slot = blockIdx.x / p.h_kv;
-  const SequenceOf s = sequence_of_slot(p.page_indptr, p.last_page_len, p.batch, p.page_shift, TB == 1 ? 7 : 8, slot, lane);
+  const SequenceOf s = p.batch <= 64 ? sequence_by_rows(p, T, slot, lane)
+                                     : sequence_of_slot(p.page_indptr, p.last_page_len, p.batch, p.page_shift, TB == 1 ? 7 : 8, slot, lane);
+  if (s.index < 0) return;  // a spare slot
   const int stored = s.stored(p.page_shift);
   const int tile_t0 = (slot - s.slot_begin) * T, t0 = tile_t0 + wave * 32 * TB;  // the workgroup's and the wave's first token
   if (tile_t0 >= stored) return;
@@ -118,7 +142,7 @@ __global__ __launch_bounds__(256, 2) void key_weights_kernel(KeyWeightsParams p)
   const int row_begin = first_counted * p.group, row_end = q_len * p.group;
   const auto end_of = [&](int token) { return p.causal ? min(in_front + token + 1, stored) : stored; };
   // no row in front of the first tile's sees a token of the workgroup's
-  const int first_tile = max(first_counted, p.causal ? tile_t0 - in_front : 0) * p.group >> 5, num_tiles = (row_end + 31) >> 5;
+  const int first_tile = max(first_counted, p.causal ? tile_t0 - in_front : 0) * p.group / R, num_tiles = (row_end + R - 1) / R;
   if (first_tile >= num_tiles) return;
 
   half8_t k[TB][KS];
@@ -139,39 +163,59 @@ __global__ __launch_bounds__(256, 2) void key_weights_kernel(KeyWeightsParams p)
 
   const int64_t head0 = static_cast<int64_t>(q_begin) * p.h_q + kvh * p.group;  // (query, head) of row 0
   // Tile by tile, tiles behind the last one as that one, so that a tile is always so many copies behind the next.
-  const auto issue = [&](int tile) {
-    const int r0 = min(tile, num_tiles - 1) * 32, token0 = p.by_group(r0), stage = tile % STAGES;
-    const int64_t at0 = head0 + static_cast<int64_t>(token0) * p.h_q;
-    const auto offset_of = [&](int r) {  // in heads, from the first head of the tile's first query
-      const int row = min(r0 + r, row_end - 1), token = p.by_group(row);
-      return static_cast<uint32_t>((token - token0) * p.h_q + row - token * p.group);
-    };
-    const uint32_t rows_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_ptr_t)rows_lds[stage]));
+  // Offsets of a lane's copies, in heads, from the first head of the tile's first query, row `rest` of it: row r of the tile.
+  const auto offset_of = [&](int r, int rest) {
+    const uint32_t nth = rest + r;  // below 64 + group
+    const uint32_t token = p.group >= 64 ? (nth >= static_cast<uint32_t>(p.group) ? 1 : 0) : __umul24(nth, p.inv_group) >> 16;
+    return __umul24(token, p.h_q - p.group) + nth;
+  };
+  const auto row_of = [&](int i) { return ((wave * COPIES + i) * 64 + lane) / PIECES; };
+  const auto piece_of = [&](int i) { return min((((wave * COPIES + i) * 64 + lane) % PIECES) ^ Tiles::swizzle(row_of(i)), D / 8 - 1) * 16; };
+  // the same for every whole tile where tiles begin with a query's first head
+  const bool regular = R % p.group == 0;
+  uint32_t whole[COPIES], whole_lse = offset_of(lane & (R - 1), 0) * 4;
 #pragma unroll
-    for (int i = 0; i < COPIES; ++i) {
-      const int nth = (wave * COPIES + i) * 64, r = (nth + lane) / PIECES;
-      const int piece = min(((nth + lane) % PIECES) ^ Tiles::swizzle(r), D / 8 - 1);
-      copy16_to_lds(p.q + at0 * D, offset_of(r) * (D * 2) + piece * 16, rows_at + nth * 16);
+  for (int i = 0; i < COPIES; ++i) whole[i] = offset_of(row_of(i), 0) * (D * 2) + piece_of(i);
+  const auto issue = [&](int tile, int stage) {
+    const int r0 = min(tile, num_tiles - 1) * R, token0 = p.by_group(r0);
+    const int64_t at0 = head0 + static_cast<int64_t>(token0) * p.h_q;
+    const half_t* const q = p.q + at0 * D;
+    const float* const lse = p.lse + at0;
+    const uint32_t rows_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_ptr_t)rows_lds[stage])) + wave * (COPIES * 1024);
+    const uint32_t lse_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_ptr_t)lse_lds[stage][wave]));
+    if (regular && r0 + R <= row_end) {
+#pragma unroll
+      for (int i = 0; i < COPIES; ++i) copy16_to_lds(q, whole[i], rows_at + i * 1024);
+      copy4_to_lds(lse, whole_lse, lse_at);
+    } else {
+      const int rest = r0 - token0 * p.group, last = row_end - 1 - r0;
+#pragma unroll
+      for (int i = 0; i < COPIES; ++i) copy16_to_lds(q, offset_of(min(row_of(i), last), rest) * (D * 2) + piece_of(i), rows_at + i * 1024);
+      copy4_to_lds(lse, offset_of(min(lane & (R - 1), last), rest) * 4, lse_at);
     }
-    copy4_to_lds(p.lse + at0, offset_of(col) * 4, static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_ptr_t)lse_lds[stage][wave])));
   };
   wait_vmcnt<0>();  // K is there: from here on only the copies count
 #pragma unroll
-  for (int i = 0; i < STAGES - 1; ++i) issue(first_tile + i);
-  for (int tile = first_tile; tile < num_tiles; ++tile) {
+  for (int i = 0; i < STAGES - 1; ++i) issue(first_tile + i, i);
+  int stage = 0, next_stage = STAGES - 1;
+  for (int tile = first_tile; tile < num_tiles; ++tile, stage = stage + 1 < STAGES ? stage + 1 : 0) {
     // The wave's part of the tile has landed where no more than the later tiles' copies are outstanding; behind the barrier everyone's
     // has, and every wave is done with the stage that the next copies overwrite.
     wait_vmcnt<(STAGES - 2) * (COPIES + 1)>();
     __syncthreads();
-    issue(tile + STAGES - 1);
-    const int r0 = tile * 32;
-    if (end_of(p.by_group(min(r0 + 31, row_end - 1))) <= t0) continue;  // no row of the tile sees a token of the wave's
-    const half_t* const rows = rows_lds[tile % STAGES];
-    const float lse = lse_lds[tile % STAGES][wave][col];
+    issue(tile + STAGES - 1, next_stage);
+    next_stage = next_stage + 1 < STAGES ? next_stage + 1 : 0;
+    const int r0 = tile * R;
+    if (end_of(p.by_group(min(r0 + R - 1, row_end - 1))) <= t0) continue;  // no row of the tile sees a token of the wave's
+    const half_t* const rows = rows_lds[stage];
     half8_t q[KS];
+    float lse;
+    const auto read = [&](int h) {
+      lse = lse_lds[stage][wave][h * 32 + col];
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks)
-      q[ks] = *reinterpret_cast<const half8_t*>(rows + col * Tiles::kRow + (((ks * 2 + half) ^ Tiles::swizzle(col)) * 8));
+      for (int ks = 0; ks < KS; ++ks)
+        q[ks] = *reinterpret_cast<const half8_t*>(rows + (h * 32 + col) * Tiles::kRow + (((ks * 2 + half) ^ Tiles::swizzle(h * 32 + col)) * 8));
+    };
     const auto product = [&](int b) {
       float16_t x = {};
 #pragma unroll
@@ -179,34 +223,46 @@ __global__ __launch_bounds__(256, 2) void key_weights_kernel(KeyWeightsParams p)
       return x;
     };
     // every row counts and sees all of the wave's tokens (those behind the last stored one are not written)
-    if (r0 >= row_begin && r0 + 32 <= row_end && end_of(p.by_group(r0)) >= min(t0 + 32 * TB, stored)) {
-      const auto add = [&](int b, const float16_t& x) {
+    if (r0 >= row_begin && r0 + R <= row_end && end_of(p.by_group(r0)) >= min(t0 + 32 * TB, stored)) {
+      const auto add = [&](int b, const float16_t& x, float of) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) sum[b][i] += fast_exp2(fmaf(x[i], p.scale_log2, -lse));
+        for (int i = 0; i < 16; ++i) sum[b][i] += fast_exp2(fmaf(x[i], p.scale_log2, -of));
       };
-      __builtin_amdgcn_sched_barrier(0);
-      const float16_t x0 = product(0);
-      __builtin_amdgcn_sched_barrier(0);
-      if constexpr (TB == 2) {
-        const float16_t x1 = product(TB - 1);
-        add(0, x0);
-        interleave_mfma_valu<KS>();
-        __builtin_amdgcn_sched_barrier(0);
-        add(TB - 1, x1);
-      } else {
-        add(0, x0);
+      float16_t x;
+      float x_lse;
+#pragma unroll
+      for (int h = 0; h < R / 32; ++h) {
+        read(h);
+#pragma unroll
+        for (int b = 0; b < TB; ++b) {
+          __builtin_amdgcn_sched_barrier(0);
+          const float16_t y = product(b);
+          if (h > 0 || b > 0) {
+            add((b + TB - 1) % TB, x, x_lse);
+            interleave_mfma_valu<KS>();
+          }
+          x = y;
+          x_lse = lse;
+        }
       }
+      __builtin_amdgcn_sched_barrier(0);
+      add(TB - 1, x, x_lse);
     } else {
-      const int row = min(r0 + col, row_end - 1);
-      const int end = r0 + col < row_end && row >= row_begin ? end_of(p.by_group(row)) : 0;
 #pragma unroll
-      for (int b = 0; b < TB; ++b) {
-        const float16_t x = product(b);
+      for (int h = 0; h < R / 32; ++h) {
+        if (r0 + h * 32 >= row_end) break;
+        read(h);
+        const int row = min(r0 + h * 32 + col, row_end - 1);
+        const int end = r0 + h * 32 + col < row_end && row >= row_begin ? end_of(p.by_group(row)) : 0;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int t = t0 + b * 32 + (i & 3) + 8 * (i >> 2) + 4 * half;
-          const float w = fast_exp2(fmaf(x[i], p.scale_log2, -lse));
-          sum[b][i] += t < end ? w : 0.f;
+        for (int b = 0; b < TB; ++b) {
+          const float16_t x = product(b);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int t = t0 + b * 32 + (i & 3) + 8 * (i >> 2) + 4 * half;
+            const float w = fast_exp2(fmaf(x[i], p.scale_log2, -lse));
+            sum[b][i] += t < end ? w : 0.f;
+          }
         }
       }
     }
@@ -957,6 +1013,7 @@ static void add_key_weights(const char* what, const void* q, const int32_t* q_in
   p.h_kv = h_kv;
   p.group = h_q / h_kv;
   p.by_group = ExactDivision::by(p.group);
+  p.inv_group = (65536 + p.group - 1) / p.group;
   p.causal = causal;
   p.observed = static_cast<int>(std::min<int64_t>(observed, INT32_MAX));
   p.page_shift = page_shift;
