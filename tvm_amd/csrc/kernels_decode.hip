@@ -24,6 +24,7 @@
 #include <mutex>
 #include <type_traits>
 
+#include "kept_scores.cuh"
 #include "launch_mix.h"
 #include "prefill_kernel.cuh"
 #include "runtime_support.h"
@@ -90,7 +91,9 @@ struct DecodeParams {
   // decode_mfma_kernel<..., KEEP = true>: the scaled scores (base 2) of all keys, float32 (kv head, 16-token run of the page table,
   // head of the group, 16 tokens in the order that kept_score_token gives)
   float* scores;
-  int64_t scores_of_head;  // of a kv head
+  uint32_t scores_of_head;  // of a kv head
+  float* key_weights;       // not NULL: the launch adds the weights to these sums, (weight page, kv head, token of the page)
+  const int32_t* weight_page_values;
 };
 
 // Same answer as find_sequence for more than 64 sequences, computed by one wavefront as a 64-ary search: the lanes
@@ -321,7 +324,8 @@ struct DecodeRopeRunning : DecodeRopeDivisors {
 // state of that one key instead of the empty one, so that a step whose new rows may not be in the pages yet (windows,
 // steps that mix prompts and decoding sequences) needs neither a self-attention launch nor a merge.
 //
-// KEEP (plain cache, groups of one block): the scores also go to memory, for the sums of attention weights (kernels_evict.hip).
+// KEEP (plain cache, groups of one block): the scores also go to memory, for the sums of attention weights (kernels_evict.hip).  In
+// small launches the workgroup that has the last state of a (sequence, kv head) also adds the weights of its keys to the sums.
 //
 // decode_items works on items first_item, first_item + stride, ... below num_items.
 template <int D, bool FUSED, bool RUNNING>
@@ -891,10 +895,15 @@ __device__ __forceinline__ void decode_items(const DecodeParams& p, const int gr
     if constexpr (KEEP) {  // behind that wait, which would take their way to memory too (64 sequences of 1024-4096 tokens 134 us)
       static_assert(!KEEP || KLINE, "a lane's tokens");
       if (c16 < heads) {
-        float* const to = p.scores + kvh * p.scores_of_head + ((static_cast<int64_t>(pbeg) << psh) + pi) * (group * 16) + c16 * 16 + 4 * g4;
+        const uint32_t to = kvh * p.scores_of_head + ((pbeg << psh) + pi) * (group * 16) + c16 * 16 + 4 * g4;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          if (pi + h < page_hi) *reinterpret_cast<float4_t*>(to + h * (group * 16)) = s[0][h];
+          if (pi + h >= page_hi) break;
+          if (p.key_weights != nullptr) {  // (read again in this launch: 2 % slower than a plain store)
+            store_kept(p.scores, to + h * (group * 16), s[0][h]);
+          } else {
+            *reinterpret_cast<float4_t*>(p.scores + to + h * (group * 16)) = s[0][h];
+          }
         }
       }
     }
@@ -1011,6 +1020,22 @@ __device__ __forceinline__ void decode_items(const DecodeParams& p, const int gr
     __syncthreads();
     if (sm_last) {
       for (int g = wave; g < heads; g += 4) merge_row<D, true, SELF>(p, b, hq0 + g, nchunks, lane);
+    }
+  }
+  if constexpr (KEEP) {
+    if (p.key_weights != nullptr && (single_chunk || sm_last)) {
+      wait_vmcnt<0>();
+      __syncthreads();  // the log-sum-exps are in memory
+      const int part = tid & 3;
+      const float* const lse = p.lse + static_cast<int64_t>(token) * p.h_q + hq0;
+      const uint32_t scores = kvh * p.scores_of_head + (pbeg << psh) * (group * 16) + 4 * part;
+      for (int run = tid >> 2; run * PS < kv_len; run += 64) {
+        const float4_t x = kept_weights(
+            group, [&](int h) { return load_kept(p.scores, scores + (run * group + h) * 16); },
+            [&](int h) { return load_partial(lse + h, true); });
+        const int page = p.weight_page_values[pbeg + (run >> psh)];
+        add_to_sums(p.key_weights + (static_cast<int64_t>(page) * p.h_kv + kvh) * (PS << psh) + (run & ((1 << psh) - 1)) * PS, part, x, kv_len - run * PS);
+      }
     }
   }
   __syncthreads();  // the merge buffers are the next item's V tiles
@@ -1145,6 +1170,9 @@ struct FusedStep {
   int64_t q_stride = 0, new_stride = 0;
   const PromptLaunch* beside = nullptr;
   float* scores = nullptr;  // where a plain call of groups of at most 16 heads keeps its scores
+  float* key_weights = nullptr;  // and the sums that it adds the weights to, where the launch merges its chunks itself
+  const int32_t* weight_page_values = nullptr;
+  bool* added = nullptr;  // whether it has
 };
 
 // Body of the decode entry point.  lease(bytes, at_least) hands out the scratch memory of the call: arrival
@@ -1218,7 +1246,9 @@ static void decode_entry(Lease&& lease, const FusedStep& fused_step, const void*
   p.rows = fused_step.rows;
   p.page_begin = fused_step.page_begin;
   p.scores = fused_step.scores;
-  p.scores_of_head = (nnz_pages << p.page_shift) * group * 16;
+  p.scores_of_head = static_cast<uint32_t>((nnz_pages << p.page_shift) * group * 16);
+  p.key_weights = nullptr;
+  p.weight_page_values = fused_step.weight_page_values;
   p.q_stride = fused_step.q_stride;
   p.new_stride = fused_step.new_stride;
   const int64_t slots = nnz_pages / p.chunk_pages + batch_size;
@@ -1254,6 +1284,8 @@ static void decode_entry(Lease&& lease, const FusedStep& fused_step, const void*
   const bool fused = static_cast<size_t>(batch_size) * h_kv * head_blocks * sizeof(unsigned long long) <= kArrivalBytes &&
                      option(kOptDecodeSeparateMerge) == 0 && heads_per_item == 16;
   if (fused) p.arrivals = reinterpret_cast<unsigned long long*>(ws.ptr);
+  if (fused) p.key_weights = fused_step.key_weights;
+  if (fused_step.added != nullptr) *fused_step.added = p.key_weights != nullptr;
   DecodeRopeRunning div{};
   if (p.rotary || (fused_launch && p.apply_rope)) {
     const InlineRopeHost table = inline_rope_table(fused_launch ? nullptr : fused_step.rope_scaling, d, rope_theta);
@@ -1519,13 +1551,18 @@ int tvmkv::decode_with_shared_prefix(const SharedPrefixDecode& a, void* stream) 
 
 // Decode attention that also keeps its scores (typed_kernels.h)
 int tvmkv::decode_keeping_scores(const void* q, const void* pages, const int32_t* page_indptr, const int32_t* page_values,
-                                 const int32_t* length_info, void* output, float* lse, float* scores, double sm_scale, int32_t batch_size,
-                                 int64_t nnz_pages, int64_t num_pages, int32_t h_q, int32_t h_kv, int32_t d, int32_t page_size, void* stream) {
+                                 const int32_t* length_info, void* output, float* lse, float* scores, float* key_weights,
+                                 const int32_t* weight_page_values, bool* added, double sm_scale, int32_t batch_size, int64_t nnz_pages,
+                                 int64_t num_pages, int32_t h_q, int32_t h_kv, int32_t d, int32_t page_size, void* stream) {
   KV_API_BEGIN();
   KV_CHECK(h_kv > 0 && h_q <= 16 * h_kv) << "decode_keeping_scores: more than 16 query heads a kv head";
+  KV_CHECK(nnz_pages * page_size * h_q < (int64_t{1} << 30)) << "decode_keeping_scores: more scores than 32-bit offsets reach";
   hipStream_t s = as_stream(stream);
   FusedStep step;
   step.scores = scores;
+  step.key_weights = key_weights;
+  step.weight_page_values = weight_page_values;
+  step.added = added;
   decode_entry([&](size_t bytes, size_t at_least) { return lease_scratch(kScratchDecode, s, bytes, kArrivalBytes, at_least); }, step, q, pages, page_indptr,
                page_values, length_info, nullptr, nullptr, output, lse, 0, 1.0, 1e4, sm_scale, batch_size, nnz_pages, num_pages, h_q, h_kv, d,
                page_size, 0, stream);

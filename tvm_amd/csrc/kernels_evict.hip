@@ -10,6 +10,7 @@
 #include <initializer_list>
 #include <type_traits>
 
+#include "kept_scores.cuh"
 #include "kernels_common.cuh"
 #include "runtime_support.h"
 #include "typed_kernels.h"
@@ -18,7 +19,6 @@
 namespace tvmkv {
 
 typedef float float4_any_t __attribute__((ext_vector_type(4), aligned(4)));
-typedef float float2_any_t __attribute__((ext_vector_type(2), aligned(4)));
 typedef int int4_any_t __attribute__((ext_vector_type(4), aligned(4)));
 
 // Where work items begin: sequence b of x_b = tokens that its pages hold owns the slots [X_b / per + b, ...), X_b the tokens of
@@ -310,39 +310,13 @@ __global__ __launch_bounds__(256) void kept_scores_kernel(KeptScoresParams p) {
   const int stored = s.stored(p.page_shift);
   const int run = (((slot - s.slot_begin) << kKeptTokensShift) + wave * 256) / 16 + (lane >> 2);  // of the sequence
   if (run * 16 >= stored) return;
-  const float* at = p.scores + (((kvh * static_cast<int64_t>(p.nnz_pages) + s.page_begin) << (p.page_shift - 4)) + run) * (p.group * 16) + 4 * (lane & 3);
+  const int part = lane & 3;
+  const float* at = p.scores + (((kvh * static_cast<int64_t>(p.nnz_pages) + s.page_begin) << (p.page_shift - 4)) + run) * (p.group * 16) + 4 * part;
   const float* lse = p.lse + (static_cast<int64_t>(s.index) * p.h_kv + kvh) * p.group;
   const int page = p.weight_page_values[s.page_begin + (run >> (p.page_shift - 4))];
-  float* const to = p.key_weights + ((static_cast<int64_t>(page) * p.h_kv + kvh) << p.page_shift) + (run * 16 & ((1 << p.page_shift) - 1));
-  // the lane's tokens are two pairs of neighbours
-  static_assert(kept_score_token(1) == kept_score_token(0) + 1 && kept_score_token(2) == kept_score_token(0) + 8 && kept_score_token(4) == 2, "pairs");
-  const int first = 2 * (lane & 3);
-  const float2_any_t before[2] = {*reinterpret_cast<const float2_any_t*>(to + first), *reinterpret_cast<const float2_any_t*>(to + first + 8)};
-  float sum[4] = {0.f, 0.f, 0.f, 0.f};  // of this call's weights alone, so that what is there already rounds it once
-  for (int g = 0; g < p.group; g += 4) {
-    float4_t x[4];
-    float of[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int h = min(g + i, p.group - 1);
-      x[i] = *reinterpret_cast<const float4_t*>(at + h * 16);
-      of[i] = lse[h];
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (g + i < p.group) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) sum[k] += fast_exp2(x[i][k] - of[i]);
-      }
-    }
-  }
-#pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    const int token = first + 8 * k, left = stored - (run * 16 + token);
-    const float2_any_t x = {before[k][0] + sum[2 * k], before[k][1] + sum[2 * k + 1]};
-    if (left >= 2) *reinterpret_cast<float2_any_t*>(to + token) = x;
-    if (left == 1) to[token] = x[0];
-  }
+  const float4_t x = kept_weights(p.group, [&](int h) { return *reinterpret_cast<const float4_t*>(at + h * 16); }, [&](int h) { return lse[h]; });
+  add_to_sums(p.key_weights + ((static_cast<int64_t>(page) * p.h_kv + kvh) << p.page_shift) + (run * 16 & ((1 << p.page_shift) - 1)), part, x,
+              stored - run * 16);
 }
 
 // ------------------------------------------------------------------------------------------
@@ -1089,8 +1063,15 @@ int tvmkv_batch_decode_paged_kv_weights(const void* q, const void* pages, const 
     p.page_shift = shift_of_page(what, page_size);
     const int64_t items = (((nnz_pages << p.page_shift) >> kKeptTokensShift) + batch_size) * h_kv;
     KV_CHECK(items < (int64_t{1} << 31)) << what << ": too many work items";
-    run(decode_keeping_scores(q, pages, page_indptr, page_values, length_info, output, lse, reinterpret_cast<float*>(ws.ptr), sm_scale, batch_size,
-                              nnz_pages, num_pages, h_q, h_kv, d, page_size, stream));
+    // A launch of a few short sequences adds the weights itself (one of 500 tokens 12.9 -> 10.3 us); a sequence's are added by one
+    // workgroup, and longer ones take it longer than a second launch (41 of up to 2500 tokens 23.5 -> 26.4).
+    const int64_t tokens = nnz_pages * page_size;
+    const bool itself = tokens <= 16384 && tokens <= int64_t{1024} * batch_size;
+    bool added = false;
+    run(decode_keeping_scores(q, pages, page_indptr, page_values, length_info, output, lse, reinterpret_cast<float*>(ws.ptr),
+                              itself ? key_weights : nullptr, weight_page_values, &added, sm_scale, batch_size, nnz_pages, num_pages, h_q, h_kv, d,
+                              page_size, stream));
+    if (added) return TVMKV_OK;
     hipLaunchKernelGGL(kept_scores_kernel, dim3(static_cast<unsigned>(items)), dim3(256), 0, s, p);
     KV_LAUNCH_CHECK();
     return TVMKV_OK;
@@ -1116,8 +1097,9 @@ int tvmkv_batch_prefill_paged_kv_weights(const void* q, const int32_t* q_indptr,
                   h_q, h_kv, d, page_size);
   if (batch_size == 0) return TVMKV_OK;
   KV_CHECK(q_indptr) << what << ": NULL tensor";
-  run(tvmkv_batch_prefill_paged_kv(q, q_indptr, pages, page_indptr, page_values, length_info, nullptr, nullptr, output, lse, causal, 0, 1.0, 1e4,
-                                   sm_scale, batch_size, total_q, nnz_pages, num_pages, h_q, h_kv, d, page_size, 0, 0, stream));
+  // Shares of 128 keys: what launches of few rows on few keys take is the walk along them (five tokens on 700 keys 17.6 -> 11.3 us).
+  run(prefill_paged_in_float(q, q_indptr, pages, page_indptr, page_values, length_info, output, lse, causal, sm_scale, batch_size, total_q,
+                             nnz_pages, num_pages, h_q, h_kv, d, page_size, 128, stream));
   add_key_weights(what, q, q_indptr, pages, page_indptr, page_values, length_info, lse, key_weights, weight_page_values, causal != 0, observed,
                   sm_scale, batch_size, total_q, nnz_pages, h_q, h_kv, d, shift_of_page(what, page_size), as_stream(stream));
   KV_API_END();

@@ -308,7 +308,7 @@ int64_t prefill_workgroups(int64_t work_q, int group, int64_t work_seqs, int h_k
 //    2000-6000 keys, 512 workgroups: 0.171 ms unsplit, 0.183 with 2 shares; a 63-node tree per sequence,
 //    1008 workgroups, matrix-bound: 0.409 against 0.442).
 // No share shorter than 8 tiles on average, at most 64 shares.
-int prefill_kv_splits(int64_t work_q, int group, int64_t work_seqs, int h_kv, int64_t avg_keys, int cus) {
+int prefill_kv_splits(int64_t work_q, int group, int64_t work_seqs, int h_kv, int64_t avg_keys, int cus, int64_t least_keys) {
   const int64_t forced = option(kOptPrefillKvSplits);
   if (forced > 0) return static_cast<int>(std::min<int64_t>(forced, 64));
   const int64_t resident = static_cast<int64_t>(cus) * 2;
@@ -319,7 +319,7 @@ int prefill_kv_splits(int64_t work_q, int group, int64_t work_seqs, int h_kv, in
   } else if (workgroups <= resident && work_q * group * h_kv * 2 <= workgroups * 128) {
     want = 2;
   }
-  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(std::min(want, avg_keys / kMinShareKeys), 64)));
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(std::min(want, avg_keys / least_keys), 64)));
 }
 
 // Few row tiles against long page lists: split the keys over workgroups until the chip has ~16 workgroups per compute

@@ -160,11 +160,12 @@ struct NewTokenDecode {
 // tvmkv_batch_decode_paged_kv over a plain cache, at most 16 query heads a kv head, that also writes the scaled scores (base 2) of all
 // keys: scores (kv head, 16-token run of the page table, head of the group, 16 places).  What a run holds behind the last token is not
 // written or of no use.  A lane of the kernel has two tokens of either half of a run, and writes them together: place p of a run is
-// token kept_score_token(p).
+// token kept_score_token(p).  key_weights not NULL: the launch may add the weights to these sums itself; *added says whether it does.
 constexpr int kept_score_token(int place) { return 8 * (place >> 1 & 1) + 2 * (place >> 2) + (place & 1); }
 int decode_keeping_scores(const void* q, const void* pages, const int32_t* page_indptr, const int32_t* page_values, const int32_t* length_info,
-                          void* output, float* lse, float* scores, double sm_scale, int32_t batch_size, int64_t nnz_pages, int64_t num_pages,
-                          int32_t h_q, int32_t h_kv, int32_t d, int32_t page_size, void* stream);
+                          void* output, float* lse, float* scores, float* key_weights, const int32_t* weight_page_values, bool* added,
+                          double sm_scale, int32_t batch_size, int64_t nnz_pages, int64_t num_pages, int32_t h_q, int32_t h_kv, int32_t d,
+                          int32_t page_size, void* stream);
 struct PromptLaunch;
 // beside: prompts to run in the same launch (kernels_decode.hip), or NULL
 int decode_with_new_token(const NewTokenDecode& args, void* stream, const PromptLaunch* beside = nullptr);
@@ -206,6 +207,12 @@ int prefill_paged_with_lengths(const void* q, const int32_t* q_indptr, const voi
                                int64_t nnz_pages, int64_t num_pages, int32_t h_q, int32_t h_kv, int32_t d, int32_t page_size,
                                int32_t sliding_window, int32_t sliding_window_size, int32_t merge_into,
                                const tvmkv_rope_scaling* rope_scaling, int64_t longest, void* stream);
+
+// tvmkv_batch_prefill_paged_kv over a plain cache, the states of a split launch's shares in float32, least_keys keys a share at least
+int prefill_paged_in_float(const void* q, const int32_t* q_indptr, const void* pages, const int32_t* page_indptr, const int32_t* page_values,
+                           const int32_t* length_info, void* output, float* lse, int64_t causal, double sm_scale, int32_t batch_size,
+                           int64_t total_q, int64_t nnz_pages, int64_t num_pages, int32_t h_q, int32_t h_kv, int32_t d, int32_t page_size,
+                           int64_t least_keys, void* stream);
 
 // A decode step behind a shared prefix (fp16, plain cache): decode attention over the sequences' own pages, which writes
 // out and lse, and paged prefill attention of all queries over the prefix, merged into them.  One launch and the merge of
