@@ -274,12 +274,35 @@ def test_select(kind, page, sinks, recent):
 @pytest.mark.parametrize("stored, keep, heads", [([70000], [5000], 2), ([300000], [60000], 1), ([5, 270000, 3000], [9, 269000, 500], 1)])
 @pytest.mark.parametrize("kind", ["sums", "ties"])
 def test_select_of_long_sequences(stored, keep, heads, kind):
-    """Up to 262144 tokens the bits are in shared memory, for longer sequences in scratch memory."""
+    """In chunks, by several launches."""
     rng = np.random.default_rng(len(stored))
     total, table = table_of(rng, stored, 128)
     sums = values(rng, kind, (total, heads, 128))
     want = eviction.select(sums, table[0], table[2], table[1], keep, max(keep), 4, 700)
     assert np.array_equal(select(sums, table, keep, max(keep), 4, 700), want)
+
+
+@pytest.mark.parametrize("stored, keep", [([70000] + [1] * 20, 20000), ([40000] + [10] * 5, 30000), ([300000] + [1] * 30, 100000),
+                                          ([1000] * 9 + [0, 33000], 700)])
+@pytest.mark.parametrize("kind", ["sums", "ties", "any"])
+def test_select_of_a_long_sequence_among_short_ones(stored, keep, kind):
+    """A workgroup a list, whose tokens are more than its registers hold, their bits more than its shared memory does."""
+    rng = np.random.default_rng(len(stored))
+    total, table = table_of(rng, stored, 32)
+    sums = values(rng, kind, (total, 1, 32))
+    want = eviction.select(sums, table[0], table[2], table[1], [keep] * len(stored), keep, 4, 100)
+    assert np.array_equal(select(sums, table, [keep] * len(stored), keep, 4, 100), want)
+
+
+@pytest.mark.parametrize("kind", ["ties", "equal", "close", "any"])
+@pytest.mark.parametrize("stored, keep, sinks, recent", [([20000, 33000], [4096, 8192], 0, 0), ([50000], [49999], 4097, 4095), ([17000], [1], 0, 0),
+                                                         ([17000], [0], 0, 0), ([40000], [30000], 0, 0), ([4096 * 9 + 1], [4097], 3, 1)])
+def test_select_in_chunks(stored, keep, sinks, recent, kind):
+    rng = np.random.default_rng(sinks + recent)
+    total, table = table_of(rng, stored, 64)
+    sums = values(rng, kind, (total, 2, 64))
+    want = eviction.select(sums, table[0], table[2], table[1], keep, max(keep) + 5, sinks, recent)
+    assert np.array_equal(select(sums, table, keep, max(keep) + 5, sinks, recent), want)
 
 
 def test_select_of_many_sequences():

@@ -320,16 +320,24 @@ __global__ __launch_bounds__(256) void kept_scores_kernel(KeptScoresParams p) {
 }
 
 // ------------------------------------------------------------------------------------------
-// The choice.  A workgroup has the tokens of one (sequence, kv head).  As integers that order like them (NaN below everything, -0
-// as 0) the weights go through passes of 8 bits that find the smallest one that stays, T, and how many of the weights equal to it
-// do: counts, exact whatever their order.  Then a bit a token says which ones stay, and running counts of free places and of tokens
-// without one pair them.
-// A wave takes blocks of 256 tokens, four neighbouring ones a lane; bit l of the block's four words of 64 is token 4 l + (0..3)'s,
-// as a comparison leaves them.  Up to 4 blocks a wave are loaded once and kept in registers.  Longer sequences are read twice: the
-// passes over some of their tokens, evenly spaced, say between which two weights T lies but for a chance that counts show, the
-// weights between them go to shared memory, and the passes over those find T.  Where it does not lie there, or they are too many,
-// every pass reads the whole sequence.  Bits and counts of more than BLOCKS blocks are in scratch memory.
+// The choice.  As integers that order like them (NaN below everything, -0 as 0) the weights of a (sequence, kv head), a list from here
+// on, go through passes over some of their bits that find the smallest one that stays, T, and how many of the weights equal to it
+// do: counts, exact whatever their order.  Then a bit a token says which ones stay, and running counts of free places and of
+// tokens without one pair them.  A wave takes blocks of 256 tokens, four neighbouring ones a lane; bit l of the block's four words of
+// 64 is token 4 l + (0..3)'s, as a comparison leaves them.
+//
+// Lists of ordinary length are a workgroup's, in one launch: passes of 8 bits, the weights loaded once and kept in registers, up to
+// HELD blocks a wave (longer lists are read again in every pass, their bits in scratch memory).  Where all are long they are cut into
+// chunks of 4096 tokens, in six launches: the histograms of 11, 11 and 10 bits are added up in memory and the last of a list's
+// workgroups goes on to find the digit; then the bits; then the places.  (One list of 131072 tokens by a single workgroup, which
+// reads it with 25 GB/s, took 92 us, with T narrowed down by a sample first 60.)
 // ------------------------------------------------------------------------------------------
+struct SelectState {
+  uint32_t least;  // of T, the bits that are known
+  uint32_t need;   // how many of the weights that begin with them stay
+  uint32_t cut;    // not all of them
+  uint32_t unused;
+};
 struct SelectParams {
   const float* key_weights;
   const int32_t* page_indptr;
@@ -337,14 +345,21 @@ struct SelectParams {
   const int32_t* last_page_len;
   const int32_t* keep;
   int32_t* kept;
-  uint64_t* words;  // scratch memory: four words a block, and a count; NULL where no sequence can need it
-  int32_t* counts;
+  // scratch memory
+  uint64_t* words;  // four a block
+  int32_t* counts;  // one a block
+  SelectState* states;  // one a list
+  uint32_t* histograms;  // (list, pass, kBins)
+  unsigned long long* arrivals;  // (list, pass): epoch << 32 | workgroups that have added their histogram
+  uint32_t epoch;
+  int batch;
   int h_kv;
   int max_keep;
   int sinks;
   int recent;
   int page_shift;
 };
+
 constexpr uint32_t kOrderOfMinusInf = 0x007fffff, kOrderOfInf = 0xff800000;
 __device__ __forceinline__ uint32_t weight_order(float w) {
   if (w != w) return 0;
@@ -408,16 +423,134 @@ __device__ __forceinline__ BlockBits load_block(Words words, int block) {
   return x;
 }
 
-template <int THREADS, int BLOCKS, int NEAR, int COPIES>
+// What a list's lengths come to.
+struct List {
+  int page_begin, stored;
+  int n, recent, sinks, places;  // tokens that stay: all, the last ones, the first ones; places in front of the recent ones' 
+  int gone;
+  int end;  // candidates: tokens [sinks, end), of which places - sinks stay and at least one does not
+  __device__ __forceinline__ List(const SelectParams& p, int b, int page_begin, int stored) : page_begin(page_begin), stored(stored) {
+    n = min(stored, max(min(p.keep[b], p.max_keep), 0));
+    recent = min(p.recent, n);
+    sinks = min(p.sinks, n - recent);
+    places = n - recent;
+    gone = stored - n;
+    end = stored - recent;
+  }
+  __device__ __forceinline__ bool no_choice() const { return gone == 0 || places == sinks; }
+  __device__ __forceinline__ int num_blocks() const { return (end + 255) >> 8; }
+  // Four tokens' weights, by their group of four; a group behind the end is the last one (its tokens are none).
+  __device__ __forceinline__ int page_of(const SelectParams& p, int group) const {
+    return p.weight_page_values[page_begin + (min(group, (end - 1) >> 2) >> (p.page_shift - 2))];
+  }
+  __device__ __forceinline__ float4_any_t weights_of(const SelectParams& p, int kvh, int page, int group) const {
+    const int in_page = min(group, (end - 1) >> 2) * 4 & ((1 << p.page_shift) - 1);
+    return *reinterpret_cast<const float4_any_t*>(p.key_weights + ((static_cast<int64_t>(page) * p.h_kv + kvh) << p.page_shift) + in_page);
+  }
+  // a block's candidates for which `is` holds
+  template <class Is>
+  __device__ __forceinline__ BlockBits candidates(int block, float4_any_t w, Is is) const {
+    BlockBits x;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x.w[i] = __ballot(is(w[i]));
+    if (block * 256 < sinks || block * 256 + 256 > end) x = x.first(end - block * 256).first(sinks - block * 256, true);
+    return x;
+  }
+  template <class Add>
+  __device__ __forceinline__ void add_candidates(int block, float4_any_t w, int lane, Add add) const {
+    const int t = block * 256 + lane * 4;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (t + i >= sinks && t + i < end) add(weight_order(w[i]));
+    }
+  }
+  // Bits of the tokens in front of the recent ones that stay.  equal_before: weights equal to T in front of the block, where only the
+  // first `need` of them stay.
+  __device__ __forceinline__ BlockBits stay(int block, float4_any_t w, const SelectState& t, int equal_before) const {
+    const float smallest = weight_from(t.least);
+    BlockBits x = candidates(block, w, [&](float v) { return t.least == 0 || v >= smallest; });
+    if (t.cut) {
+      const BlockBits equal = equal_to(block, w, t);
+      int rank = equal_before + equal.before();
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const bool mine = bit_of_lane(equal.w[i]);
+        x.w[i] &= ~__ballot(mine && rank >= static_cast<int>(t.need));
+        rank += mine;
+      }
+    }
+    if (block * 256 < sinks) {
+      const BlockBits first = BlockBits{{~uint64_t{0}, ~uint64_t{0}, ~uint64_t{0}, ~uint64_t{0}}}.first(sinks - block * 256);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x.w[i] |= first.w[i];
+    }
+    return x;
+  }
+  __device__ __forceinline__ BlockBits equal_to(int block, float4_any_t w, const SelectState& t) const {
+    const float smallest = weight_from(t.least);
+    return candidates(block, w, [&](float v) { return t.least == 0 ? v != v : v == smallest; });
+  }
+  // Free places up to the block with the first token behind the places, tokens without a place from that block on.
+  __device__ __forceinline__ int boundary() const { return places >> 8; }
+  __device__ __forceinline__ BlockBits holes_in(const BlockBits& x, int block) const {
+    return block < boundary() ? x.inverse() : x.inverse().first(block == boundary() ? places & 255 : 0);
+  }
+  __device__ __forceinline__ BlockBits homeless_in(const BlockBits& x, int block) const {
+    return block > boundary() ? x : x.first(block == boundary() ? places & 255 : 256, true);
+  }
+};
+template <class Words>
+__device__ __forceinline__ BlockBits any_block(Words words, int block) {
+  return {{words[block * 4], words[block * 4 + 1], words[block * 4 + 2], words[block * 4 + 3]}};
+}
+// The token without a place of a rank; counts: up to the boundary anything, behind it such tokens in front of the block.
+template <class Words, class Counts>
+__device__ __forceinline__ int homeless_of_rank(const List& l, Words words, Counts counts, int rank) {
+  const BlockBits first = l.homeless_in(any_block(words, l.boundary()), l.boundary());
+  if (rank < first.count()) return l.boundary() * 256 + first.nth(rank);
+  int lo = l.boundary() + 1, hi = l.num_blocks() - 1;  // the last block that begins at or in front of the rank
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (counts[mid] <= rank) lo = mid; else hi = mid - 1;
+  }
+  return lo * 256 + any_block(words, lo).nth(rank - counts[lo]);
+}
+// Sums of two numbers over the threads in front of this one.
+template <int WAVES>
+__device__ __forceinline__ int2 sums_in_front(int (&shared)[2][WAVES], int a, int c, int wave, int lane) {
+  const int a_to = sum_of_lanes_up_to(a), c_to = sum_of_lanes_up_to(c);
+  __syncthreads();
+  if (lane == 63) {
+    shared[0][wave] = a_to;
+    shared[1][wave] = c_to;
+  }
+  __syncthreads();
+  int2 front = make_int2(a_to - a, c_to - c);
+#pragma unroll
+  for (int w = 0; w < WAVES - 1; ++w) {
+    front.x += w < wave ? shared[0][w] : 0;
+    front.y += w < wave ? shared[1][w] : 0;
+  }
+  return front;
+}
+// Where a list's blocks are in scratch memory: as many as the pages of the sequences in front could have.
+__device__ __forceinline__ int64_t blocks_at(const SelectParams& p, const List& l, int b, int kvh) {
+  return (((static_cast<int64_t>(l.page_begin - p.page_indptr[0]) << p.page_shift) >> 8) + b) * p.h_kv + static_cast<int64_t>(kvh) * l.num_blocks();
+}
+__device__ __forceinline__ void no_choice_made(const SelectParams& p, const List& l, int32_t* kept, int thread, int threads) {
+  for (int i = l.places + thread; i < p.max_keep; i += threads) kept[i] = i < l.n ? i + l.gone : -1;
+  if (l.no_choice()) {
+    for (int i = thread; i < l.places; i += threads) kept[i] = i;
+  }
+}
+
+template <int THREADS, int HELD, int BLOCKS, int LISTED, int COPIES>
 __global__ __launch_bounds__(THREADS) void select_kept_kernel(SelectParams p) {
   constexpr int WAVES = THREADS / 64;
-  constexpr int HELD = 4;             // blocks a wave keeps in registers
-  constexpr int SAMPLES = 2;          // of their lanes' neighbouring four tokens, in longer sequences
-  constexpr int MINE = NEAR / WAVES;  // weights near T that a wave finds
   __shared__ uint64_t lds_words[BLOCKS * 4];
   __shared__ int32_t lds_counts[BLOCKS];
-  __shared__ uint32_t near[NEAR];                // weights near T; later the tokens without a place
-  __shared__ uint32_t histogram[256 * COPIES];   // lanes take turns: most weights fall into a few of the first pass's bins
+  __shared__ int32_t homeless_lds[LISTED];
+  __shared__ uint32_t histogram[256 * COPIES];  // lanes take turns: most weights fall into a few of the first pass's bins
   __shared__ uint32_t bins[256];
   __shared__ int per_wave[2][WAVES];
   __shared__ uint32_t found[3];
@@ -425,78 +558,41 @@ __global__ __launch_bounds__(THREADS) void select_kept_kernel(SelectParams p) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int kvh = blockIdx.x, b = blockIdx.y;
   const int page_begin = p.page_indptr[b], num_pages = p.page_indptr[b + 1] - page_begin;
-  const int stored = num_pages > 0 ? ((num_pages - 1) << p.page_shift) + p.last_page_len[b] : 0;
-  const int n = min(stored, max(min(p.keep[b], p.max_keep), 0));
+  const List l(p, b, page_begin, num_pages > 0 ? ((num_pages - 1) << p.page_shift) + p.last_page_len[b] : 0);
   int32_t* const kept = p.kept + (static_cast<int64_t>(b) * p.h_kv + kvh) * p.max_keep;
-  const int recent = min(p.recent, n), sinks = min(p.sinks, n - recent), places = n - recent;
-  const int gone = stored - n;
-  for (int i = places + tid; i < p.max_keep; i += THREADS) kept[i] = i < n ? i + gone : -1;
-  if (gone == 0 || places == sinks) {
-    for (int i = tid; i < places; i += THREADS) kept[i] = i;
-    return;
-  }
-  const int end = stored - recent;  // candidates: tokens [sinks, end), of which `need` stay and at least one does not
-  const int num_blocks = (end + 255) >> 8, num_groups = (end + 3) >> 2;  // groups: of four tokens
-  // A group behind the end is the last one (its tokens are none).
-  const auto page_of = [&](int group) { return p.weight_page_values[page_begin + (min(group, num_groups - 1) >> (p.page_shift - 2))]; };
-  const auto weights_of = [&](int page, int group) {
-    const int in_page = min(group, num_groups - 1) * 4 & ((1 << p.page_shift) - 1);
-    return *reinterpret_cast<const float4_any_t*>(p.key_weights + ((static_cast<int64_t>(page) * p.h_kv + kvh) << p.page_shift) + in_page);
-  };
-  float4_any_t held[HELD];  // of blocks wave, wave + WAVES, ..; of a longer sequence the sample
-  const bool in_registers = num_blocks <= WAVES * HELD;
-  {
-    // groups of the sample: evenly spaced
-    const int spacing = in_registers ? 1 : num_groups / (SAMPLES * THREADS);
+  no_choice_made(p, l, kept, tid, THREADS);
+  if (l.no_choice()) return;
+  const int num_blocks = l.num_blocks();
+  float4_any_t held[HELD];  // of blocks wave, wave + WAVES, ..
+  const auto hold = [&](int k0) {
     int page[HELD];
 #pragma unroll
-    for (int u = 0; u < HELD; ++u) page[u] = page_of((tid + u * THREADS) * spacing);
+    for (int u = 0; u < HELD; ++u) page[u] = l.page_of(p, (k0 + u * WAVES) * 64 + lane);
 #pragma unroll
-    for (int u = 0; u < HELD; ++u) held[u] = weights_of(page[u], (tid + u * THREADS) * spacing);
-  }
+    for (int u = 0; u < HELD; ++u) held[u] = l.weights_of(p, kvh, page[u], (k0 + u * WAVES) * 64 + lane);
+  };
+  const bool in_registers = num_blocks <= WAVES * HELD;
+  hold(wave);
   // f(block, the lane's weights) for every block; all lanes of a wave take the same steps
   const auto every_block = [&](auto&& f) {
-    if (in_registers) {
+#pragma unroll 1
+    for (int k0 = wave; k0 < num_blocks; k0 += HELD * WAVES) {
+      if (!in_registers) hold(k0);
 #pragma unroll
       for (int u = 0; u < HELD; ++u) {
-        if (u * WAVES + wave < num_blocks) f(u * WAVES + wave, held[u]);
-      }
-    } else {
-      constexpr int U = 8;
-      int page[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u) page[u] = page_of(tid + u * THREADS);
-      for (int k0 = wave; k0 < num_blocks; k0 += U * WAVES) {
-        float4_any_t w[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) w[u] = weights_of(page[u], (k0 + u * WAVES) * 64 + lane);
-#pragma unroll
-        for (int u = 0; u < U; ++u) page[u] = page_of((k0 + (U + u) * WAVES) * 64 + lane);
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          if (k0 + u * WAVES < num_blocks) f(k0 + u * WAVES, w[u]);
-        }
+        if (k0 + u * WAVES < num_blocks) f(k0 + u * WAVES, held[u]);
       }
     }
   };
-  // the block's candidates for which `is` holds
-  const auto candidates = [&](int block, float4_any_t w, auto&& is) {
-    BlockBits x;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x.w[i] = __ballot(is(w[i]));
-    if (block * 256 < sinks || block * 256 + 256 > end) x = x.first(end - block * 256).first(sinks - block * 256, true);
-    return x;
-  };
-
-  // One pass: `each` hands its weights, those whose bits above the `width` from `shift` on are those of least, to the histogram; the
-  // digit in which the need-th largest of them lies becomes part of least, need what is left of it there.  True: all weights of
-  // that digit do.
-  const auto pass = [&](auto&& each, int shift, int width, bool first, uint32_t& least, uint32_t& need) {
+  SelectState t = {0, static_cast<uint32_t>(l.places - l.sinks), 1, 0};
+#pragma unroll 1
+  for (int shift = 24; shift >= 0 && t.cut; shift -= 8) {
     for (int i = tid; i < 256 * COPIES; i += THREADS) histogram[i] = 0;
     __syncthreads();
-    const uint32_t digits = (1u << width) - 1;
-    each([&](uint32_t x) {
-      if (first || ((x ^ least) >> shift) <= digits) atomicAdd(&histogram[(x >> shift & digits) * COPIES + (lane & (COPIES - 1))], 1u);
+    every_block([&](int block, float4_any_t w) {
+      l.add_candidates(block, w, lane, [&](uint32_t x) {
+        if (shift == 24 || ((x ^ t.least) >> shift) < 256) atomicAdd(&histogram[(x >> shift & 255) * COPIES + (lane & (COPIES - 1))], 1u);
+      });
     });
     __syncthreads();
     constexpr int SHARE = THREADS / 256;  // threads that add a bin's copies up
@@ -517,138 +613,32 @@ __global__ __launch_bounds__(THREADS) void select_kept_kernel(SelectParams p) {
       uint32_t above = sum_of_lanes_up_to(sum) - sum;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        if (above < need && need <= above + mine[i]) {
+        if (above < t.need && t.need <= above + mine[i]) {
           found[0] = 255 - (lane * 4 + i);
-          found[1] = need - above;
+          found[1] = t.need - above;
           found[2] = mine[i];
         }
         above += mine[i];
       }
     }
     __syncthreads();
-    least |= found[0] << shift;
-    need = found[1];
-    return found[1] == found[2];
-  };
-
-  uint32_t least = 0, need = places - sinks;  // of T; how many of the weights equal to it stay
-  bool cut = true;                            // not all of them
-  const auto passes = [&](auto&& each, int bits) {
-    for (int left = bits; left > 0 && cut; left -= 8) cut = !pass(each, max(left - 8, 0), min(left, 8), left == bits, least, need);
-  };
-  const auto all_candidates = [&](auto&& add) {
-    every_block([&](int block, float4_any_t w) {
-      const int t = block * 256 + lane * 4;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (t + i >= sinks && t + i < end) add(weight_order(w[i]));
-      }
-    });
-  };
-  if (in_registers) {
-    passes(all_candidates, 32);
-  } else {
-    // The number of samples over T deviates by sqrt(samples) / 2 at most; nearly nine times that leave T between the two weights also
-    // where neighbouring tokens' weights are alike.
-    constexpr int kSamples = SAMPLES * THREADS * 4, kMargin = 400;
-    static_assert(kSamples <= 8192, "the margin");
-    const auto sampled = [&](auto&& add) {
-#pragma unroll
-      for (int u = 0; u < SAMPLES; ++u) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) add(weight_order(held[u][i]));
-      }
-    };
-    const int middle = static_cast<int>(static_cast<int64_t>(need) * kSamples / (end - sinks));
-    uint32_t upper = kOrderOfInf, lower = 0;  // weights above the first stay, none under the second does
-    if (middle - kMargin >= 1) {
-      uint32_t to = 0, left = middle - kMargin;
-      pass(sampled, 24, 8, true, to, left);
-      pass(sampled, 16, 8, false, to, left);
-      upper = min(max(to | 0xffff, kOrderOfMinusInf), kOrderOfInf);
-    }
-    if (middle + kMargin <= kSamples) {
-      uint32_t left = middle + kMargin;
-      pass(sampled, 24, 8, true, lower, left);
-      pass(sampled, 16, 8, false, lower, left);
-    }
-    const float highest = weight_from(upper), lowest = weight_from(lower);
-    int above = 0, mine = 0;
-    every_block([&](int block, float4_any_t w) {
-      const BlockBits over = candidates(block, w, [&](float x) { return x > highest; });
-      above += over.count();
-      const BlockBits here = candidates(block, w, [&](float x) { return !(x > highest) && (lower == 0 || x >= lowest); });
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int place = bits_below(here.w[i], mine);
-        if (bit_of_lane(here.w[i]) && place < MINE) near[wave * MINE + place] = __float_as_uint(w[i]);
-        mine += __popcll(here.w[i]);
-      }
-    });
-    __syncthreads();
-    if (lane == 0) {
-      per_wave[0][wave] = above;
-      per_wave[1][wave] = mine;
-    }
-    __syncthreads();
-    int all_above = 0, all_near = 0;
-    bool fits = true;
-#pragma unroll
-    for (int w = 0; w < WAVES; ++w) {
-      all_above += per_wave[0][w];
-      all_near += per_wave[1][w];
-      fits &= per_wave[1][w] <= MINE;
-    }
-    if (fits && all_above < static_cast<int>(need) && static_cast<int>(need) <= all_above + all_near) {
-      need -= all_above;
-      passes([&](auto&& add) {
-        for (int i = lane; i < mine; i += 256) {
-          uint32_t x[4];
-#pragma unroll
-          for (int u = 0; u < 4; ++u) x[u] = near[wave * MINE + min(i + u * 64, mine - 1)];
-#pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            if (i + u * 64 < mine) add(weight_order(__uint_as_float(x[u])) - lower);
-          }
-        }
-      }, max(32 - __clz(upper - lower), 1));
-      least += lower;
-    } else {
-      passes(all_candidates, 32);
-    }
+    t.least |= found[0] << shift;
+    t.need = found[1];
+    t.cut = found[1] != found[2];  // otherwise all weights with these bits stay
   }
 
-  const float smallest = weight_from(least);
-  const auto is_equal = [&](float x) { return least == 0 ? x != x : x == smallest; };
-  const auto stays = [&](float x) { return least == 0 || x >= smallest; };
-  // A range of blocks a thread, for the running counts: two sums over the blocks in front of it.
+  // A range of blocks a thread, for the running counts.
   const int per = (num_blocks + THREADS - 1) / THREADS, block_lo = min(tid * per, num_blocks), block_hi = min(block_lo + per, num_blocks);
-  const auto sums_in_front = [&](int a, int c) {
-    const int a_to = sum_of_lanes_up_to(a), c_to = sum_of_lanes_up_to(c);
-    __syncthreads();
-    if (lane == 63) {
-      per_wave[0][wave] = a_to;
-      per_wave[1][wave] = c_to;
-    }
-    __syncthreads();
-    int2 front = make_int2(a_to - a, c_to - c);
-#pragma unroll
-    for (int w = 0; w < WAVES - 1; ++w) {
-      front.x += w < wave ? per_wave[0][w] : 0;
-      front.y += w < wave ? per_wave[1][w] : 0;
-    }
-    return front;
-  };
   const auto finish = [&](auto* words, auto* counts) {
-    if (cut) {  // weights equal to T in front of each block
+    if (t.cut) {  // weights equal to T in front of each block
       every_block([&](int block, float4_any_t w) {
-        const BlockBits equal = candidates(block, w, is_equal);
+        const BlockBits equal = l.equal_to(block, w, t);
         if (lane == 0) counts[block] = equal.count();
       });
       __syncthreads();
       int equal = 0;
       for (int k = block_lo; k < block_hi; ++k) equal += counts[k];
-      int front = sums_in_front(equal, 0).x;
+      int front = sums_in_front(per_wave, equal, 0, wave, lane).x;
       for (int k = block_lo; k < block_hi; ++k) {
         const int here = counts[k];
         counts[k] = front;
@@ -657,98 +647,58 @@ __global__ __launch_bounds__(THREADS) void select_kept_kernel(SelectParams p) {
       __syncthreads();
     }
     every_block([&](int block, float4_any_t w) {
-      BlockBits x = candidates(block, w, stays);
-      if (cut) {
-        const BlockBits equal = candidates(block, w, is_equal);
-        int rank = counts[block] + equal.before();
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const bool mine = bit_of_lane(equal.w[i]);
-          x.w[i] &= ~__ballot(mine && rank >= static_cast<int>(need));
-          rank += mine;
-        }
-      }
-      if (block * 256 < sinks) {
-        const BlockBits first = BlockBits{{~uint64_t{0}, ~uint64_t{0}, ~uint64_t{0}, ~uint64_t{0}}}.first(sinks - block * 256);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x.w[i] |= first.w[i];
-      }
+      const BlockBits x = l.stay(block, w, t, t.cut ? counts[block] : 0);
       if (lane < 4) words[block * 4 + lane] = lane == 0 ? x.w[0] : lane == 1 ? x.w[1] : lane == 2 ? x.w[2] : x.w[3];
     });
     __syncthreads();
-    // Free places up to the block with the first token behind the places, tokens without a place from that block on.
-    const int boundary = places >> 8;
-    const auto holes_in = [&](const BlockBits& x, int block) {
-      return block < boundary ? x.inverse() : x.inverse().first(block == boundary ? places & 255 : 0);
-    };
-    const auto homeless_in = [&](const BlockBits& x, int block) {
-      return block > boundary ? x : x.first(block == boundary ? places & 255 : 256, true);
-    };
-    const auto any_block = [&](int block) { return BlockBits{{words[block * 4], words[block * 4 + 1], words[block * 4 + 2], words[block * 4 + 3]}}; };
     int holes = 0, homeless = 0;
     for (int k = block_lo; k < block_hi; ++k) {
-      const BlockBits x = any_block(k);
-      holes += holes_in(x, k).count();
-      homeless += homeless_in(x, k).count();
+      const BlockBits x = any_block(words, k);
+      holes += l.holes_in(x, k).count();
+      homeless += l.homeless_in(x, k).count();
     }
-    int2 front = sums_in_front(holes, homeless);
+    int2 front = sums_in_front(per_wave, holes, homeless, wave, lane);
     // counts of a block: up to the boundary the holes in front of it, behind it the tokens without a place in front of it
     for (int k = block_lo; k < block_hi; ++k) {
-      counts[k] = k <= boundary ? front.x : front.y;
-      const BlockBits x = any_block(k);
-      front.x += holes_in(x, k).count();
-      front.y += homeless_in(x, k).count();
+      const BlockBits x = any_block(words, k);
+      counts[k] = k <= l.boundary() ? front.x : front.y;
+      front.x += l.holes_in(x, k).count();
+      front.y += l.homeless_in(x, k).count();
     }
     if (tid == THREADS - 1) num_homeless = front.y;
     __syncthreads();
     // Tokens without a place, in order, where they are few enough; else a place looks for its own.
-    const bool listed = num_homeless <= NEAR;
+    const bool listed = num_homeless <= LISTED;
     if (listed) {
-      for (int k = boundary + wave; k < num_blocks; k += WAVES) {
-        const BlockBits x = homeless_in(load_block(words, k), k);
-        int rank = (k == boundary ? 0 : counts[k]) + x.before();
+      for (int k = l.boundary() + wave; k < num_blocks; k += WAVES) {
+        const BlockBits x = l.homeless_in(load_block(words, k), k);
+        int rank = (k == l.boundary() ? 0 : counts[k]) + x.before();
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const bool mine = bit_of_lane(x.w[i]);
-          if (mine) near[rank] = k * 256 + lane * 4 + i;
+          if (mine) homeless_lds[rank] = k * 256 + lane * 4 + i;
           rank += mine;
         }
       }
       __syncthreads();
     }
-    for (int k = wave; k * 256 < places; k += WAVES) {
-      const BlockBits x = holes_in(load_block(words, k), k);
-      const int t = k * 256 + lane * 4;
+    for (int k = wave; k * 256 < l.places; k += WAVES) {
+      const BlockBits x = l.holes_in(load_block(words, k), k);
+      const int at = k * 256 + lane * 4;
       int rank = counts[k] + x.before();
       int4_any_t from;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        from[i] = t + i;
-        if (bit_of_lane(x.w[i])) {
-          if (listed) {
-            from[i] = near[rank];
-          } else {
-            const BlockBits first = homeless_in(any_block(boundary), boundary);
-            if (rank < first.count()) {
-              from[i] = boundary * 256 + first.nth(rank);
-            } else {
-              int lo = boundary + 1, hi = num_blocks - 1;  // the last block that begins at or in front of the rank
-              while (lo < hi) {
-                const int mid = (lo + hi + 1) >> 1;
-                if (counts[mid] <= rank) lo = mid; else hi = mid - 1;
-              }
-              from[i] = lo * 256 + homeless_in(any_block(lo), lo).nth(rank - counts[lo]);
-            }
-          }
-          ++rank;
-        }
+        const bool hole = bit_of_lane(x.w[i]);
+        from[i] = !hole ? at + i : listed ? homeless_lds[rank] : homeless_of_rank(l, words, counts, rank);
+        rank += hole;
       }
-      if (t + 4 <= places) {
-        *reinterpret_cast<int4_any_t*>(kept + t) = from;
+      if (at + 4 <= l.places) {
+        *reinterpret_cast<int4_any_t*>(kept + at) = from;
       } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          if (t + i < places) kept[t + i] = from[i];
+          if (at + i < l.places) kept[at + i] = from[i];
         }
       }
     }
@@ -756,8 +706,180 @@ __global__ __launch_bounds__(THREADS) void select_kept_kernel(SelectParams p) {
   if (num_blocks <= BLOCKS) {
     finish(lds_words, lds_counts);
   } else {
-    const int64_t at = (((static_cast<int64_t>(page_begin - p.page_indptr[0]) << p.page_shift) >> 8) + b) * p.h_kv + static_cast<int64_t>(kvh) * num_blocks;
+    const int64_t at = blocks_at(p, l, b, kvh);
     finish(p.words + at * 4, p.counts + at);
+  }
+}
+
+// Long lists, in chunks of 16 blocks.
+constexpr int kChunkShift = 12, kBins = 2048, kSelectPasses = 3;
+constexpr int64_t kMostChunkedBlocks = 8192;  // whose counts a workgroup of the last launch keeps
+__global__ __launch_bounds__(256) void select_clear_kernel(uint32_t* histograms, int64_t count) {
+  for (int64_t i = blockIdx.x * int64_t{256} + threadIdx.x; i < count; i += gridDim.x * int64_t{256}) histograms[i] = 0;
+}
+// The list and the chunk of a workgroup of the other launches; a list without a choice has no chunks.
+struct Chunk {
+  int b, kvh, first_block;
+  __device__ __forceinline__ Chunk(const SelectParams& p, int lane, SequenceOf& s) {
+    kvh = blockIdx.x % p.h_kv;
+    const int slot = blockIdx.x / p.h_kv;
+    s = sequence_of_slot(p.page_indptr, p.last_page_len, p.batch, p.page_shift, kChunkShift, slot, lane);
+    b = s.index;
+    first_block = (slot - s.slot_begin) << (kChunkShift - 8);
+  }
+};
+
+__global__ __launch_bounds__(256) void select_pass_kernel(SelectParams p, int nth) {
+  __shared__ uint32_t histogram[kBins];
+  __shared__ int per_wave[2][4];
+  __shared__ int is_last;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  SequenceOf s;
+  const Chunk c(p, lane, s);
+  const List l(p, c.b, s.page_begin, s.stored(p.page_shift));
+  if (l.no_choice() || c.first_block >= l.num_blocks()) return;
+  const int64_t list = static_cast<int64_t>(c.b) * p.h_kv + c.kvh;
+  SelectState t = {0, static_cast<uint32_t>(l.places - l.sinks), 1, 0};
+  if (nth > 0) t = p.states[list];
+  if (!t.cut) return;  // T is known well enough
+  const int shift = nth == 0 ? 21 : nth == 1 ? 10 : 0, digits = nth == 2 ? 1023 : 2047;
+  int page[4];
+  float4_any_t w[4];
+#pragma unroll
+  for (int u = 0; u < 4; ++u) page[u] = l.page_of(p, (c.first_block + wave + 4 * u) * 64 + lane);
+#pragma unroll
+  for (int u = 0; u < 4; ++u) w[u] = l.weights_of(p, c.kvh, page[u], (c.first_block + wave + 4 * u) * 64 + lane);
+  for (int i = tid; i < kBins; i += 256) histogram[i] = 0;
+  __syncthreads();
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    l.add_candidates(c.first_block + wave + 4 * u, w[u], lane, [&](uint32_t x) {
+      if (nth == 0 || (x ^ t.least) >> shift <= static_cast<uint32_t>(digits)) atomicAdd(&histogram[x >> shift & digits], 1u);
+    });
+  }
+  __syncthreads();
+  uint32_t* const all = p.histograms + (list * kSelectPasses + nth) * kBins;
+  for (int i = tid; i < kBins; i += 256) {
+    if (histogram[i] != 0) __hip_atomic_fetch_add(all + i, histogram[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  wait_vmcnt<0>();
+  __syncthreads();
+  if (tid == 0) {
+    // A word that an older launch left, also one that was abandoned half way, becomes (epoch, 0); back to that behind the last.
+    unsigned long long* const counter = p.arrivals + list * kSelectPasses + nth;
+    const unsigned long long none = static_cast<unsigned long long>(p.epoch) << 32;
+    __hip_atomic_fetch_max(counter, none, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const unsigned long long before = __hip_atomic_fetch_add(counter, 1ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const int chunks = (l.num_blocks() + 15) >> 4;
+    is_last = static_cast<uint32_t>(before) == static_cast<uint32_t>(chunks - 1);
+    if (is_last) __hip_atomic_store(counter, none, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __syncthreads();
+  if (!is_last) return;
+  constexpr int EACH = kBins / 256;
+  uint32_t mine[EACH], sum = 0;  // the largest digit first
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) mine[i] = __hip_atomic_load(all + kBins - 1 - (tid * EACH + i), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) sum += mine[i];
+  uint32_t above = sums_in_front(per_wave, static_cast<int>(sum), 0, wave, lane).x;
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    if (above < t.need && t.need <= above + mine[i]) {
+      const uint32_t left = t.need - above;
+      p.states[list] = {t.least | static_cast<uint32_t>(kBins - 1 - (tid * EACH + i)) << shift, left, left != mine[i], 0};
+    }
+    above += mine[i];
+  }
+}
+
+__global__ __launch_bounds__(256) void select_bits_kernel(SelectParams p) {
+  __shared__ int per_wave[4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  SequenceOf s;
+  const Chunk c(p, lane, s);
+  const List l(p, c.b, s.page_begin, s.stored(p.page_shift));
+  if (l.no_choice() || c.first_block >= l.num_blocks()) return;
+  const SelectState t = p.states[static_cast<int64_t>(c.b) * p.h_kv + c.kvh];
+  // (a wave has neighbouring blocks here)
+  const int block0 = c.first_block + 4 * wave;
+  int page[4];
+  float4_any_t w[4];
+#pragma unroll
+  for (int u = 0; u < 4; ++u) page[u] = l.page_of(p, (block0 + u) * 64 + lane);
+#pragma unroll
+  for (int u = 0; u < 4; ++u) w[u] = l.weights_of(p, c.kvh, page[u], (block0 + u) * 64 + lane);
+  int equal_before = 0;
+  if (t.cut) {  // weights equal to T in front of the wave's: its workgroup counts them in the chunks in front of its own
+    int equal = 0;
+    for (int k = wave; k < c.first_block; k += 4) {
+      const int group = k * 64 + lane;
+      equal += l.equal_to(k, l.weights_of(p, c.kvh, l.page_of(p, group), group), t).count();
+    }
+    int own = 0;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) own += block0 + u < l.num_blocks() ? l.equal_to(block0 + u, w[u], t).count() : 0;
+    if (lane == 0) per_wave[wave] = equal;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) equal_before += per_wave[i];
+    __syncthreads();
+    if (lane == 0) per_wave[wave] = own;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) equal_before += i < wave ? per_wave[i] : 0;
+  }
+  const int64_t at = blocks_at(p, l, c.b, c.kvh);
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    const int block = block0 + u;
+    if (block >= l.num_blocks()) break;
+    const BlockBits x = l.stay(block, w[u], t, equal_before);
+    if (t.cut) equal_before += l.equal_to(block, w[u], t).count();
+    if (lane < 4) p.words[(at + block) * 4 + lane] = lane == 0 ? x.w[0] : lane == 1 ? x.w[1] : lane == 2 ? x.w[2] : x.w[3];
+  }
+}
+
+// Places, a block of them a wave (each looks for its token: 23 us with four blocks a wave); lists without a choice, too.
+__global__ __launch_bounds__(256) void select_places_kernel(SelectParams p) {
+  __shared__ int32_t counts[kMostChunkedBlocks];
+  __shared__ int per_wave[2][4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int kvh = blockIdx.y, b = blockIdx.z;
+  const int page_begin = p.page_indptr[b], num_pages = p.page_indptr[b + 1] - page_begin;
+  const List l(p, b, page_begin, num_pages > 0 ? ((num_pages - 1) << p.page_shift) + p.last_page_len[b] : 0);
+  int32_t* const kept = p.kept + (static_cast<int64_t>(b) * p.h_kv + kvh) * p.max_keep;
+  no_choice_made(p, l, kept, blockIdx.x * 256 + tid, gridDim.x * 256);
+  const int first_block = blockIdx.x * 4;
+  if (l.no_choice() || first_block * 256 >= l.places) return;
+  const uint64_t* const words = p.words + blocks_at(p, l, b, kvh) * 4;
+  const int num_blocks = l.num_blocks();
+  const int per = (num_blocks + 255) / 256, block_lo = min(tid * per, num_blocks), block_hi = min(block_lo + per, num_blocks);
+  int holes = 0, homeless = 0;
+  for (int k = block_lo; k < block_hi; ++k) {
+    const BlockBits x = any_block(words, k);
+    holes += l.holes_in(x, k).count();
+    homeless += l.homeless_in(x, k).count();
+  }
+  int2 front = sums_in_front(per_wave, holes, homeless, wave, lane);
+  for (int k = block_lo; k < block_hi; ++k) {
+    const BlockBits x = any_block(words, k);
+    counts[k] = k <= l.boundary() ? front.x : front.y;
+    front.x += l.holes_in(x, k).count();
+    front.y += l.homeless_in(x, k).count();
+  }
+  __syncthreads();
+  const int k = first_block + wave;
+  if (k * 256 < l.places) {
+    const BlockBits x = l.holes_in(load_block(words, k), k);
+    const int at = k * 256 + lane * 4;
+    int rank = counts[k] + x.before();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const bool hole = bit_of_lane(x.w[i]);
+      if (at + i < l.places) kept[at + i] = hole ? homeless_of_rank(l, words, counts, rank) : at + i;
+      rank += hole;
+    }
   }
 }
 
@@ -949,6 +1071,8 @@ __global__ __launch_bounds__(kMoveThreads) void move_kept_kernel(MoveParams p) {
 // ------------------------------------------------------------------------------------------
 // Launches
 // ------------------------------------------------------------------------------------------
+constexpr size_t kSelectCounterBytes = 64 * 1024;  // of the scratch memory: arrival counters
+
 static int shift_of_page(const char* what, int32_t page_size) {
   KV_UNSUPPORTED(page_size < 16 || page_size > 128 || (page_size & (page_size - 1)) != 0)
       << what << ": page_size " << page_size << " is not built (16, 32, 64, 128)";
@@ -1048,7 +1172,7 @@ int tvmkv_batch_decode_paged_kv_weights(const void* q, const void* pages, const 
   const size_t kept = static_cast<size_t>(nnz_pages) * page_size * h_q * sizeof(float);
   if (nnz_pages > 0 && h_q <= 16 * h_kv && kept <= kMostKept) {
     const hipStream_t s = as_stream(stream);
-    const ScratchLease ws = lease_scratch(kScratchEvict, s, kept, 0);
+    const ScratchLease ws = lease_scratch(kScratchKept, s, kept, 0);
     KeptScoresParams p;
     p.scores = reinterpret_cast<const float*>(ws.ptr);
     p.page_indptr = page_indptr;
@@ -1110,7 +1234,7 @@ int tvmkv_select_kept_tokens(const float* key_weights, const int32_t* page_indpt
                              int32_t batch_size, int64_t nnz_pages, int32_t h_kv, int32_t page_size, int32_t max_keep, void* stream) {
   KV_API_BEGIN();
   const char* const what = "select_kept_tokens";
-  SelectParams p;
+  SelectParams p{};
   p.page_shift = shift_of_page(what, page_size);
   check_table(what, batch_size, nnz_pages, h_kv, page_size);
   KV_CHECK(num_sinks >= 0 && num_recent >= 0 && max_keep >= 0) << what << ": bad shape";
@@ -1129,22 +1253,40 @@ int tvmkv_select_kept_tokens(const float* key_weights, const int32_t* page_indpt
   p.max_keep = max_keep;
   p.sinks = static_cast<int>(std::min<int64_t>(num_sinks, INT32_MAX));
   p.recent = static_cast<int>(std::min<int64_t>(num_recent, INT32_MAX));
-  p.words = nullptr;
-  p.counts = nullptr;
-  const int64_t tokens = nnz_pages << p.page_shift;
+  p.batch = batch_size;
+  // Scratch memory: arrival counters, then what the launches leave for each other.  Of one workgroup a list it is the bits of lists that
+  // are longer than its shared memory has room for: none where all tokens together are few enough.
+  const int64_t tokens = nnz_pages << p.page_shift, lists = static_cast<int64_t>(batch_size) * h_kv;
   const bool small = tokens <= static_cast<int64_t>(batch_size) * 4096;
-  const int blocks_in_lds = small ? 256 : 1024;
+  // Long lists that are too few to fill the chip, a workgroup each.
+  const bool chunked = tokens > static_cast<int64_t>(batch_size) * 16384 && lists <= 4 * compute_units() && tokens <= kMostChunkedBlocks * 256 &&
+                       lists * kSelectPasses * sizeof(unsigned long long) <= kSelectCounterBytes;
+  const int64_t blocks_in_lds = small ? 256 : 1024;
   ScratchLease ws{};
-  if (tokens > static_cast<int64_t>(blocks_in_lds) * 256) {
-    const size_t blocks = static_cast<size_t>((tokens >> 8) + batch_size) * h_kv;
-    ws = lease_scratch(kScratchEvict, s, blocks * (4 * sizeof(uint64_t) + sizeof(int32_t)), 0);
-    p.words = reinterpret_cast<uint64_t*>(ws.ptr);
-    p.counts = reinterpret_cast<int32_t*>(p.words + blocks * 4);
+  if (chunked || tokens > blocks_in_lds * 256) {
+    const size_t blocks = static_cast<size_t>((tokens >> 8) + batch_size) * h_kv, bins = chunked ? static_cast<size_t>(lists) * kSelectPasses * kBins : 0;
+    const size_t states = chunked ? static_cast<size_t>(lists) : 0;
+    ws = lease_scratch(kScratchSelect, s,
+                       kSelectCounterBytes + blocks * 4 * sizeof(uint64_t) + states * sizeof(SelectState) + (blocks + bins) * sizeof(uint32_t),
+                       kSelectCounterBytes);
+    p.arrivals = reinterpret_cast<unsigned long long*>(ws.ptr);
+    p.epoch = ws.epoch;
+    p.words = reinterpret_cast<uint64_t*>(ws.ptr + kSelectCounterBytes);
+    p.states = reinterpret_cast<SelectState*>(p.words + blocks * 4);
+    p.counts = reinterpret_cast<int32_t*>(p.states + states);
+    p.histograms = reinterpret_cast<uint32_t*>(p.counts + blocks);
   }
-  if (small) {
-    hipLaunchKernelGGL((select_kept_kernel<256, 256, 2048, 8>), dim3(h_kv, batch_size), dim3(256), 0, s, p);
+  if (chunked) {
+    const int64_t bins = lists * kSelectPasses * kBins, items = ((tokens >> kChunkShift) + batch_size) * h_kv;
+    const dim3 grid(static_cast<unsigned>(items));
+    hipLaunchKernelGGL(select_clear_kernel, dim3(static_cast<unsigned>(std::min<int64_t>((bins + 255) / 256, 1024))), dim3(256), 0, s, p.histograms, bins);
+    for (int nth = 0; nth < kSelectPasses; ++nth) hipLaunchKernelGGL(select_pass_kernel, grid, dim3(256), 0, s, p, nth);
+    hipLaunchKernelGGL(select_bits_kernel, grid, dim3(256), 0, s, p);
+    hipLaunchKernelGGL(select_places_kernel, dim3((max_keep + 1023) / 1024, h_kv, batch_size), dim3(256), 0, s, p);
+  } else if (small) {
+    hipLaunchKernelGGL((select_kept_kernel<256, 4, 256, 2048, 8>), dim3(h_kv, batch_size), dim3(256), 0, s, p);
   } else {
-    hipLaunchKernelGGL((select_kept_kernel<1024, 1024, 20480, 32>), dim3(h_kv, batch_size), dim3(1024), 0, s, p);
+    hipLaunchKernelGGL((select_kept_kernel<1024, 4, 1024, 16384, 32>), dim3(h_kv, batch_size), dim3(1024), 0, s, p);
   }
   KV_LAUNCH_CHECK();
   KV_API_END();

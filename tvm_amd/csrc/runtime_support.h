@@ -78,7 +78,7 @@ struct ScratchLease {
   uint32_t epoch;   // never 0
   ScratchHold hold;
 };
-enum ScratchUser { kScratchDecode = 0, kScratchMla = 1, kScratchPrefill = 2, kScratchGeneric = 3, kScratchMxfp4 = 4, kScratchEvict = 5 };
+enum ScratchUser { kScratchDecode = 0, kScratchMla = 1, kScratchPrefill = 2, kScratchGeneric = 3, kScratchMxfp4 = 4, kScratchKept = 5, kScratchSelect = 6 };
 // at_least: what a buffer that has to be allocated gets in any case
 ScratchLease lease_scratch(ScratchUser user, hipStream_t stream, size_t bytes, size_t counter_bytes, size_t at_least = 0);
 // Frees the buffers of (current device, stream) after synchronising the stream; a buffer whose address
