@@ -160,6 +160,53 @@ def test_prefill_of_many_sequences():
     check_attention(q, q_lens, pool, 1, 4, prefill(q, q_lens, pool, 1, 4))
 
 
+@pytest.mark.parametrize("q_lens, stored", [([5, 3], [700, 2000]), ([40, 300], [900, 300])])
+def test_rows_and_sums_behind_the_last_sequence_stay_as_they_are(q_lens, stored):
+    """A padded batch: q, out and lse have rows that no sequence has, the page table entries that none has."""
+    rng = np.random.default_rng(q_lens[0])
+    pool = Pool(rng, stored, 2, 16, 128)
+    q = queries(rng, sum(q_lens) + 7, 8, 128)
+    pool.ids, pool.weight_ids = (np.concatenate((x, x[:1], x[:1])) for x in (pool.ids, pool.weight_ids))
+    out, lse, sums = prefill(q, q_lens, pool, 1)
+    n = sum(q_lens)
+    assert (out[n:] == 7.0).all() and (lse[n:] == 7.0).all()
+    check_attention(q[:n], q_lens, pool, True, 0, (out[:n], lse[:n], sums))
+
+
+def test_pools_of_more_than_4_gib():
+    """Offsets of rows and of sums that 32 bits do not hold."""
+    rng = np.random.default_rng(12)
+    pool = Pool(rng, [200, 90], 8, 128, 128)
+    high_pages, high_sums = 9000, 1 << 20  # 512 KiB a page, 4 KiB a page of sums
+    big = torch.zeros((high_pages + len(pool.pages), 2, 8, 128, 128), dtype=torch.float16, device=DEV)
+    big_sums = torch.zeros((high_sums + len(pool.sums), 8, 128), dtype=torch.float32, device=DEV)
+    big[high_pages:] = dev(pool.pages)
+    big_sums[high_sums:] = dev(pool.sums)
+    indptr, ids, info, weight_ids = pool.table()
+    ids, weight_ids = ids + high_pages, weight_ids + high_sums
+    for q_lens in ([1, 1], [40, 3]):
+        pool.sums = host(big_sums[high_sums:])
+        q = queries(rng, sum(q_lens), 16, 128)
+        out = torch.empty(q.shape, dtype=torch.float16, device=DEV)
+        lse = torch.empty(q.shape[:2], dtype=torch.float32, device=DEV)
+        if q_lens == [1, 1]:
+            kernels.batch_decode_paged_kv_weights(dev(q), big, indptr, ids, info, out, lse, big_sums, weight_ids, 128 ** -0.5)
+        else:
+            kernels.batch_prefill_paged_kv_weights(dev(q), i32([0, 40, 43]), big, indptr, ids, info, out, lse, big_sums, weight_ids, 1, 0,
+                                                   128 ** -0.5)
+        check_attention(q, q_lens, pool, True, 0, (host(out), host(lse), host(big_sums[high_sums:])))
+    sums = host(big_sums[high_sums:])
+    kept = torch.empty((2, 8, 80), dtype=torch.int32, device=DEV)
+    kernels.select_kept_tokens(big_sums, indptr, weight_ids, info, i32([80, 60]), kept, 2, 20)
+    want = eviction.select(sums, pool.indptr, pool.weight_ids, pool.info, [80, 60], 80, 2, 20)
+    assert np.array_equal(host(kept), want)
+    kernels.move_kept_tokens(big, big_sums, indptr, ids, weight_ids, kept)
+    want_pages, want_sums = eviction.move(pool.pages, sums, pool.indptr, pool.ids, pool.weight_ids, want)
+    assert np.array_equal(host(big[high_pages:]).view(np.uint16), want_pages.view(np.uint16))
+    assert np.array_equal(host(big_sums[high_sums:]), want_sums)
+    assert not big[:high_pages].any() and not big_sums[:high_sums].any()
+
+
 def test_weights_of_a_query_add_up_to_one():
     rng = np.random.default_rng(4)
     pool = Pool(rng, [777], 1, 16, 128)
@@ -181,7 +228,7 @@ def test_what_does_not_count_does_not_reach_the_sums(value):
     """Queries that are not observed, and the slots behind the last token."""
     rng = np.random.default_rng(6)
     pool = Pool(rng, [21, 40], 1, 32, 64)
-    pool.pages[pool.ids[0], :, :, 21:] = 65504.0
+    pool.pages[pool.ids[0], 0, :, 21:] = value
     q_lens = [5, 3]
     q = queries(rng, sum(q_lens), 4, 64)
     _, _, want, slack, _ = eviction.attention(q, q_lens, pool.pages, pool.indptr, pool.ids, pool.info, True, 64 ** -0.5, pool.sums,
@@ -468,6 +515,45 @@ def test_a_captured_step_replays():
         torch.cuda.synchronize()
         assert torch.equal(out, eager_out) and torch.equal(lse, eager_lse) and torch.equal(state["kept"], eager["kept"])
         assert torch.equal(state["sums"], eager["sums"]) and torch.equal(state["pages"].view(torch.int16), eager["pages"].view(torch.int16))
+
+
+def test_a_captured_choice_in_chunks_replays():
+    rng = np.random.default_rng(35)
+    stored, keep = [30000, 20000, 9], [5000, 300, 50]
+    total, (indptr, info, weight_ids) = table_of(rng, stored, 64)
+    sums, kept = torch.zeros((total, 2, 64), device=DEV), torch.zeros((3, 2, 5000), dtype=torch.int32, device=DEV)
+    args = (i32(indptr), i32(weight_ids), i32(info), i32(keep))
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        kernels.select_kept_tokens(sums, *args, kept, 4, 30)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            kernels.select_kept_tokens(sums, *args, kept, 4, 30)
+    for kind in ("sums", "ties", "any", "equal"):
+        fresh = values(rng, kind, (total, 2, 64))
+        torch.cuda.synchronize()
+        sums.copy_(dev(fresh))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert np.array_equal(host(kept), eviction.select(fresh, indptr, weight_ids, info, keep, 5000, 4, 30))
+        eager = torch.empty_like(kept)
+        kernels.select_kept_tokens(sums, *args, eager, 4, 30)
+        assert torch.equal(kept, eager)
+
+
+def test_scratch_counters_of_an_older_launch_do_not_count():
+    import ctypes
+
+    from tvm_amd._lib import check, lib
+    rng = np.random.default_rng(36)
+    total, table = table_of(rng, [30000, 40000], 64)
+    sums = values(rng, "sums", (total, 1, 64))
+    want = eviction.select(sums, table[0], table[2], table[1], [4000, 7000], 7000, 4, 30)
+    for arrivals in (1, 3, 7):
+        assert np.array_equal(select(sums, table, [4000, 7000], 7000, 4, 30), want)
+        check(lib().tvmkv_debug_abandon_scratch_launches(ctypes.c_uint32(arrivals)))
+    assert np.array_equal(select(sums, table, [4000, 7000], 7000, 4, 30), want)
 
 
 def test_two_streams_at_once():

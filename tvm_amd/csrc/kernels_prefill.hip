@@ -73,11 +73,12 @@ template <typename T, int DV>
 __global__ __launch_bounds__(256) void prefill_split_merge_kernel(const T* __restrict__ part_o,
                                                                   const float* __restrict__ part_lse, half_t* __restrict__ output,
                                                                   float* __restrict__ lse, int64_t rows, int splits,
-                                                                  int merge_into) {
+                                                                  int merge_into, const int32_t* __restrict__ q_end, int h_q) {
   constexpr int TPR = DV / 8;  // threads per row, 8 features each
   const int64_t row = static_cast<int64_t>(blockIdx.x) * (256 / TPR) + threadIdx.x / TPR;
   const int piece = threadIdx.x % TPR;
-  if (row >= rows) return;
+  // (rows behind the last sequence have no shares and stay as they are)
+  if (row >= min(rows, static_cast<int64_t>(*q_end) * h_q)) return;
   // the shares' loads do not depend on each other: unrolled, eight are in flight at once (64 shares of a
   // 64-token chunk: 35 us as a loop of dependent round trips)
   float s_max = kNegInit;
@@ -171,7 +172,7 @@ struct KvSplit {
     const unsigned rows_per_block = 256 / (dv / 8);
     const dim3 grid(static_cast<unsigned>((rows + rows_per_block - 1) / rows_per_block));
     auto merge = [&](auto kernel, const auto* shares) {
-      hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, shares, p.lse, output, lse, rows, splits, merge_into);
+      hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, shares, p.lse, output, lse, rows, splits, merge_into, p.q_indptr + p.batch_size, p.h_q);
     };
     auto merge_dim = [&](auto dim) {
       constexpr int kD = decltype(dim)::value;
