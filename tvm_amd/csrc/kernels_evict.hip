@@ -934,7 +934,7 @@ enum MoveLaunch { kMoveInOrder, kMoveFirst, kMoveSecond };
 template <MoveLaunch LAUNCH>
 __global__ __launch_bounds__(kMoveThreads) void move_kept_kernel(MoveParams p) {
   constexpr int EACH = 8;  // places a thread looks at before their rows are moved
-  __shared__ int2 list[kMoveThreads * EACH];  // place, source
+  __shared__ uint2 list[kMoveThreads * EACH];  // K's rows in the pool: of a place, of its source
   __shared__ int per_wave[EACH][kMoveWaves];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int part = blockIdx.x, parts = gridDim.x, kvh = blockIdx.y, b = blockIdx.z;
@@ -997,15 +997,13 @@ __global__ __launch_bounds__(kMoveThreads) void move_kept_kernel(MoveParams p) {
     hi = min(lo + each, hi);
   }
   const bool with_sums = p.key_weights != nullptr && y0 == 0;
-  const auto sum_at = [&](int t) {
-    const int page = p.weight_page_values[page_begin + (t >> p.page_shift)];
-    return p.key_weights + ((static_cast<int64_t>(page) * p.h_kv + kvh) << p.page_shift) + (t & in_page);
-  };
-  const int half = p.pieces >> 1;  // a row's pieces of K, then those of V
-  const auto piece_at = [&](int t, int y) {
-    const int page = p.page_values[page_begin + (t >> p.page_shift)];
+  const auto sum_at = [&](int page, int t) { return p.key_weights + ((static_cast<int64_t>(page) * p.h_kv + kvh) << p.page_shift) + (t & in_page); };
+  const auto row_at = [&](int page, int t) { return ((static_cast<uint32_t>(page) * 2 * p.h_kv + kvh) << p.page_shift) + (t & in_page); };
+  const int half = p.pieces >> 1;  // a row's pieces of K, then those of V, which are so many rows behind
+  const uint32_t to_v = static_cast<uint32_t>(p.h_kv) << p.page_shift;
+  const auto piece_at = [&](uint32_t row, int y) {
     const bool v = y >= half;
-    return p.pages + (((((static_cast<int64_t>(page) * 2 + v) * p.h_kv + kvh) << p.page_shift) + (t & in_page)) * half + (y - (v ? half : 0))) * 16;
+    return p.pages + (static_cast<int64_t>(row + (v ? to_v : 0)) * half + (y - (v ? half : 0))) * 16;
   };
   // Loads are complete, not only issued, where a workgroup goes on to overwrite what they read.
   const auto all_have_read = [&] {
@@ -1021,9 +1019,16 @@ __global__ __launch_bounds__(kMoveThreads) void move_kept_kernel(MoveParams p) {
       const int i = i0 + u * kMoveThreads + tid;
       from[u] = i < hi ? kept[i] : -1;
     }
+    // the pages of places and sources, of K / V and of the sums, where there is something to move
+    int page[EACH], page_from[EACH];
 #pragma unroll
     for (int u = 0; u < EACH; ++u) {
-      if (!moves(i0 + u * kMoveThreads + tid, from[u])) from[u] = -1;
+      const int i = i0 + u * kMoveThreads + tid;
+      if (!moves(i, from[u])) from[u] = -1;
+      if (from[u] >= 0) {
+        page[u] = p.page_values[page_begin + (i >> p.page_shift)];
+        page_from[u] = p.page_values[page_begin + (from[u] >> p.page_shift)];
+      }
       const uint64_t who = __ballot(from[u] >= 0);
       at[u] = __popcll(who & ((uint64_t{1} << lane) - 1));
       if (lane == 0) per_wave[u][wave] = __popcll(who);
@@ -1037,23 +1042,26 @@ __global__ __launch_bounds__(kMoveThreads) void move_kept_kernel(MoveParams p) {
         at[u] += w == wave ? count : 0;
         count += per_wave[u][w];
       }
-      if (from[u] >= 0) list[at[u]] = make_int2(i0 + u * kMoveThreads + tid, from[u]);
+      if (from[u] >= 0) list[at[u]] = make_uint2(row_at(page[u], i0 + u * kMoveThreads + tid), row_at(page_from[u], from[u]));
     }
-    __syncthreads();
     if (with_sums) {
+      float* to[EACH];
       float sum[EACH];
 #pragma unroll
       for (int u = 0; u < EACH; ++u) {
-        const int x = u * kMoveThreads + tid;
-        if (x < count) sum[u] = *sum_at(list[x].y);
+        if (from[u] >= 0) {
+          const int i = i0 + u * kMoveThreads + tid;
+          to[u] = sum_at(p.weight_page_values[page_begin + (i >> p.page_shift)], i);
+          sum[u] = *sum_at(p.weight_page_values[page_begin + (from[u] >> p.page_shift)], from[u]);
+        }
       }
       all_have_read();
 #pragma unroll
       for (int u = 0; u < EACH; ++u) {
-        const int x = u * kMoveThreads + tid;
-        if (x < count) *sum_at(list[x].x) = sum[u];
+        if (from[u] >= 0) *to[u] = sum[u];
       }
     }
+    __syncthreads();
     constexpr int U = 8;
     const int total = count * width;
     for (int x0 = 0; x0 < total; x0 += kMoveThreads * U) {
@@ -1310,6 +1318,8 @@ int tvmkv_move_kept_tokens(void* pages, float* key_weights, const int32_t* page_
   KV_UNSUPPORTED(dtype_bits != 16 && dtype_bits != 32) << what << ": rows of " << dtype_bits << " bits an element are not built (16, 32)";
   KV_UNSUPPORTED(d <= 0 || d > 256 || d * dtype_bits % 128 != 0) << what << ": head_dim " << d << " is not built";
   KV_CHECK(batch_size < 65536 && h_kv < 65536) << what << ": too many sequences or heads";  // dimensions of the grid
+  KV_CHECK(num_pages >= 0) << what << ": bad shape";
+  KV_UNSUPPORTED(num_pages >= (int64_t{1} << 32) / (2 * page_size) / h_kv) << what << ": a pool of 2^32 rows or more is not built";
   if (batch_size == 0 || max_keep == 0 || nnz_pages == 0) return TVMKV_OK;
   KV_CHECK(pages && page_indptr && kept) << what << ": NULL tensor";
   KV_CHECK(page_values && (key_weights == nullptr || weight_page_values)) << what << ": NULL page table";

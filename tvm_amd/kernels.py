@@ -384,15 +384,22 @@ def key_weight_pages(num_pages, h_kv, page_size, device="cuda"):
     return torch.zeros((num_pages, h_kv, page_size), dtype=torch.float32, device=device)
 
 
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
 def _weights_call(entry, tensors, *rest):
     """tensors: all on one device, which is the current one for the call; None: NULL."""
-    index = tensors[0].get_device()
+    index = tensors[0].get_device()  # -1: not in device memory
+    pointers = []
     for t in tensors:
-        if t is not None and (not t.is_cuda or not t.is_contiguous() or t.get_device() != index):
+        if t is None:
+            pointers.append(None)
+            continue
+        if t.get_device() != index or index < 0 or not t.is_contiguous():
             _p(t)
             raise KVError(-1, f"kernel arguments must be on one device, got {t.device} and {tensors[0].device}")
-    pointers = [None if t is None else t.data_ptr() for t in tensors]
-    if index == torch.cuda.current_device():
+        pointers.append(t.data_ptr())
+    if index == _current_device():
         check(entry(*pointers, *rest, _raw_stream(index)))
     else:
         with torch.cuda.device(index):
