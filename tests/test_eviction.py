@@ -155,3 +155,89 @@ def test_refused(entry, changes, code, text):
 ])
 def test_nothing_to_do(entry, changes):
     assert refusal(entry, changes)[0] == 0
+
+
+# ---- the Python face: its checks read shapes and types, so that host tensors do -------------------------------------
+
+
+def tensors(batch=2, rows=2, h_q=8, h_kv=2, d=64, page=16):
+    import torch
+    i32 = lambda *shape: torch.zeros(shape, dtype=torch.int32)
+    f16 = lambda *shape: torch.zeros(shape, dtype=torch.float16)
+    f32 = lambda *shape: torch.zeros(shape, dtype=torch.float32)
+    return {"q": f16(rows, h_q, d), "q_indptr": i32(batch + 1), "pages": f16(5, 2, h_kv, page, d), "page_indptr": i32(batch + 1), "page_values": i32(4),
+            "length_info": i32(batch), "output": f16(rows, h_q, d), "lse": f32(rows, h_q), "key_weights": f32(6, h_kv, page),
+            "weight_page_values": i32(4), "keep": i32(batch), "kept": i32(batch, h_kv, 8)}
+
+
+PYTHON = {
+    "batch_decode_paged_kv_weights": (["q", "pages", "page_indptr", "page_values", "length_info", "output", "lse", "key_weights",
+                                       "weight_page_values"], [0.125]),
+    "batch_prefill_paged_kv_weights": (["q", "q_indptr", "pages", "page_indptr", "page_values", "length_info", "output", "lse", "key_weights",
+                                        "weight_page_values"], [1, 0, 0.125]),
+    "select_kept_tokens": (["key_weights", "page_indptr", "weight_page_values", "length_info", "keep", "kept"], [1, 1]),
+    "move_kept_tokens": (["pages", "key_weights", "page_indptr", "page_values", "weight_page_values", "kept"], []),
+}
+
+
+def call(name, t):
+    from tvm_amd import kernels
+    order, rest = PYTHON[name]
+    getattr(kernels, name)(*[t[k] for k in order], *rest)
+
+
+@pytest.mark.parametrize("name", PYTHON)
+def test_host_tensors_are_refused(name):
+    with pytest.raises(tvm_amd.KVError, match="device memory"):
+        call(name, tensors())
+
+
+def changes():
+    import torch
+    attention = ("batch_decode_paged_kv_weights", "batch_prefill_paged_kv_weights")
+    for name in attention:
+        yield name, dict(q=torch.zeros(2, 8, 64)), "float16"
+        yield name, dict(page_values=torch.zeros(4, dtype=torch.int64)), "int32"
+        yield name, dict(lse=torch.zeros(2, 8, dtype=torch.float64)), "lse must be float32"
+        yield name, dict(lse=torch.zeros(2, 9)), "lse has shape"
+        yield name, dict(output=torch.zeros(3, 8, 64, dtype=torch.float16)), "output has shape"
+        yield name, dict(pages=torch.zeros(5, 2, 2, 16, 32, dtype=torch.float16)), "pages has shape"
+        yield name, dict(pages=torch.zeros(5, 2, 16, 64, dtype=torch.float16)), "pages has shape"
+        yield name, dict(length_info=torch.zeros(3, 2, dtype=torch.int32)), "length_info has shape"  # sliding windows
+        yield name, dict(weight_page_values=torch.zeros(3, dtype=torch.int32)), "weight_page_values has shape"
+        yield name, dict(key_weights=torch.zeros(6, 2, 16, dtype=torch.float16)), "key_weights must be float32"
+        yield name, dict(key_weights=torch.zeros(6, 2, 32)), "key_weights has shape"
+    yield attention[0], dict(tensors(rows=3), length_info=tensors()["length_info"]), "q has shape"
+    yield attention[1], dict(q_indptr=torch.zeros(2, dtype=torch.int32)), "q_indptr has shape"
+    yield "select_kept_tokens", dict(key_weights=torch.zeros(6, 2, 16, dtype=torch.float64)), "key_weights must be float32"
+    yield "select_kept_tokens", dict(keep=torch.zeros(3, dtype=torch.int32)), "keep has shape"
+    yield "select_kept_tokens", dict(length_info=torch.zeros(1, dtype=torch.int32)), "length_info has shape"
+    yield "select_kept_tokens", dict(kept=torch.zeros(2, 3, 8, dtype=torch.int32)), "kept has shape"
+    yield "select_kept_tokens", dict(kept=torch.zeros(2, 2, 8, dtype=torch.int64)), "int32"
+    yield "move_kept_tokens", dict(pages=torch.zeros(5, 2, 2, 16, 64, dtype=torch.bfloat16)), "only float16 and float32"
+    yield "move_kept_tokens", dict(pages=torch.zeros(5, 3, 2, 16, 64)), "pages has shape"
+    yield "move_kept_tokens", dict(key_weights=torch.zeros(6, 2, 32)), "key_weights has shape"
+    yield "move_kept_tokens", dict(weight_page_values=torch.zeros(5, dtype=torch.int32)), "weight_page_values has shape"
+    yield "move_kept_tokens", dict(kept=torch.zeros(1, 2, 8, dtype=torch.int32)), "kept has shape"
+
+
+@pytest.mark.parametrize("name, change, text", list(changes()))
+def test_refused_by_the_python_face(name, change, text):
+    with pytest.raises(tvm_amd.KVError, match=text):
+        call(name, dict(tensors(), **change))
+
+
+def test_kernels_keep_their_values_in_registers(tmp_path):
+    """Nothing that the kernels of eviction hold is spilled, nor by the decode kernels that keep their scores."""
+    import os
+    import re
+
+    from tests.test_host_support import READELF, ROOT, _kernel_metadata
+    library = os.path.join(ROOT, "tvm_amd", "lib", "libtvmkv.so")
+    if not (os.path.exists(READELF) and os.path.exists(library)):
+        pytest.skip("needs the built library and llvm-readelf")
+    kernels = [k for k in _kernel_metadata(library, tmp_path)
+               if re.search(r"key_weights_kernel|kept_scores_kernel|select_|move_kept_kernel", k[0])
+               or ("decode_mfma_kernel" in k[0] and k[0].split("EEEv")[0].endswith("Lb1"))]
+    assert len(kernels) == 11 + 1 + 6 + 3 + 4
+    assert [k for k in kernels if k[1] or k[2]] == []
