@@ -483,7 +483,12 @@ int tvmkv_mxfp4_batch_prefill_paged_kv(const void* q, const int32_t* q_indptr, c
  * different (passing page_values for both is fine where no page is shared).  Sums of slots that hold no token stay as they are.
  *
  * Built for fp16 rows, pages of 16, 32, 64 or 128 tokens, head dims 64, 80, 96, 112, 128 and 256, any GQA group; keys are stored
- * rotated, caches without sliding windows.  q, pages and output are aligned to 16 bytes. */
+ * rotated, caches without sliding windows.  q, pages and output are aligned to 16 bytes.  A call reads what the device arrays hold, not
+ * their copies on the host, so it may be captured; scratch memory (decode's scores, prefill's shares, long lists of the choice) is that
+ * of the other launchers, one buffer per (device, stream): two graphs captured on one stream share it and are replayed one after the
+ * other.  A query without keys: output 0, lse -5e4, no weights.  Rows of output and lse behind the last query of q_indptr stay as they
+ * are.  What unused slots hold does not matter, NaN included; a stored row of V that is not finite reaches, as in
+ * tvmkv_batch_prefill_paged_kv, also those queries of its tile that do not see it. */
 
 /* tvmkv_batch_decode_paged_kv with the sums: one query token a sequence, q and output (batch, h_q, d), lse (batch, h_q),
  * length_info (batch). */
@@ -506,7 +511,8 @@ int tvmkv_batch_prefill_paged_kv_weights(const void* q, const int32_t* q_indptr,
  * first; NaN is below everything).  kept (batch, h_kv, max_keep) names the token that each of the first n places takes, -1 behind
  * them: the recent tokens have the last places, in order; in front of them a token that stays and has a place already keeps it, and
  * the other places, from the front, take the others in order.  keep (batch) is in device memory.  A sequence that already has n
- * tokens keeps all as they are.  More than 262144 tokens in all need scratch memory, kept as that of the decode entry point. */
+ * tokens keeps all as they are.  Calls with more than 65536 tokens in all may need scratch memory.  Fewer than 65536 sequences, tables
+ * of at most 2^30 tokens, max_keep at most 2^30. */
 int tvmkv_select_kept_tokens(const float* key_weights, const int32_t* page_indptr, const int32_t* weight_page_values,
                              const int32_t* length_info, const int32_t* keep, int32_t* kept, int64_t num_sinks, int64_t num_recent,
                              int32_t batch_size, int64_t nnz_pages, int32_t h_kv, int32_t page_size, int32_t max_keep, void* stream);
@@ -515,7 +521,8 @@ int tvmkv_select_kept_tokens(const float* key_weights, const int32_t* page_indpt
  * place.  Lists of the caller's own may name any token that is not in front of its place (an ascending list does); entries that
  * name none behind it, or none of the sequence's pages, move nothing.  The sequence then has as many tokens as the list names, on
  * the first of its pages.  Pages that other sequences share are copied first (tvmkv_copy_single_page).  Rows of d elements of
- * dtype_bits (16 or 32), a multiple of 16 bytes; pages of 16, 32, 64 or 128 tokens. */
+ * dtype_bits (16 or 32), a multiple of 16 bytes, d at most 256; pages of 16, 32, 64 or 128 tokens, pools of fewer than 2^32 rows, fewer
+ * than 65536 sequences and heads.  No scratch memory. */
 int tvmkv_move_kept_tokens(void* pages, float* key_weights, const int32_t* page_indptr, const int32_t* page_values,
                            const int32_t* weight_page_values, const int32_t* kept, int32_t batch_size, int64_t nnz_pages,
                            int64_t num_pages, int32_t h_kv, int32_t page_size, int32_t d, int32_t dtype_bits, int32_t max_keep,

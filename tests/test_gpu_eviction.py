@@ -173,6 +173,28 @@ def test_rows_and_sums_behind_the_last_sequence_stay_as_they_are(q_lens, stored)
     check_attention(q[:n], q_lens, pool, True, 0, (out[:n], lse[:n], sums))
 
 
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("causal, observed", [(1, 0), (0, 2), (1, 3)])
+@pytest.mark.parametrize("q_lens, stored", [([5], [700]), ([2, 1, 0, 3], [3000, 900, 40, 0]), ([4], [9000]), ([30] + [0] * 7, [1000] + [200] * 7),
+                                            ([9, 1], [4, 600])])
+def test_few_rows_on_long_sequences(q_lens, stored, d, causal, observed):
+    """Launches in shares: of few and of many, a sequence with most of the rows, queries without keys."""
+    rng = np.random.default_rng(sum(q_lens) + d)
+    pool = Pool(rng, stored, 2, 64, d)
+    q = queries(rng, sum(q_lens) + 2, 8, d)  # two rows are no sequence's
+    out, lse, sums = prefill(q, q_lens, pool, causal, observed)
+    n = sum(q_lens)
+    assert (out[n:] == 7.0).all() and (lse[n:] == 7.0).all()
+    check_attention(q[:n], q_lens, pool, causal, observed, (out[:n], lse[:n], sums))
+
+
+def test_more_queries_observed_than_there_are():
+    rng = np.random.default_rng(8)
+    pool = Pool(rng, [300, 20], 2, 16, 64)
+    q = queries(rng, 12, 8, 64)
+    check_attention(q, [10, 2], pool, True, 0, prefill(q, [10, 2], pool, 1, (1 << 63) - 1))
+
+
 def test_pools_of_more_than_4_gib():
     """Offsets of rows and of sums that 32 bits do not hold."""
     rng = np.random.default_rng(12)

@@ -7,11 +7,13 @@
 // which workgroups run.
 #include <algorithm>
 #include <cstdint>
+#include <functional>
 #include <initializer_list>
 #include <type_traits>
 
 #include "kept_scores.cuh"
 #include "kernels_common.cuh"
+#include "prefill_merge.cuh"
 #include "runtime_support.h"
 #include "typed_kernels.h"
 #include "exact_division.h"
@@ -105,6 +107,30 @@ __device__ __forceinline__ void copy4_to_lds(const void* src_base, uint32_t byte
   asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(byte_off), "s"(src_base), "s"(lds_addr) : "memory");
 }
 
+// A lane's part of token t's K as the A operand of 32 tokens' products: 8 of every 16 elements.
+template <int D>
+__device__ __forceinline__ void load_key(half8_t (&k)[D / 16], const KeyWeightsParams& p, const SequenceOf& s, int kvh, int t, int half) {
+  const int page = p.page_values[s.page_begin + (t >> p.page_shift)];
+  const half_t* row = p.pages + ((((static_cast<int64_t>(page) * 2 * p.h_kv + kvh) << p.page_shift) + (t & ((1 << p.page_shift) - 1))) * D) + half * 8;
+#pragma unroll
+  for (int ks = 0; ks < D / 16; ++ks) k[ks] = ld16(row + ks * 16).h8;
+}
+// Adds up a block's sums over the rows and to the pool's: lane i of 32 takes the sum of its half's i-th token.
+__device__ __forceinline__ void add_block_sums(const float (&sum)[16], const KeyWeightsParams& p, const SequenceOf& s, int kvh, int t0, int stored,
+                                               int col, int half) {
+  float mine = 0.f;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const float total = sum_xor16(group_sum<16>(sum[i]));
+    mine = col == i ? total : mine;
+  }
+  const int t = t0 + (col & 3) + 8 * (col >> 2) + 4 * half;
+  if (col < 16 && t < stored) {
+    const int page = p.weight_page_values[s.page_begin + (t >> p.page_shift)];
+    p.key_weights[((static_cast<int64_t>(page) * p.h_kv + kvh) << p.page_shift) + (t & ((1 << p.page_shift) - 1))] += mine;
+  }
+}
+
 template <int D, int TB>
 struct WeightTiles {
   static constexpr int kRow = D == 64 ? 64 : D <= 128 ? 128 : 256;  // halfs of a row in shared memory
@@ -147,13 +173,7 @@ __global__ __launch_bounds__(256, 2) void key_weights_kernel(KeyWeightsParams p)
 
   half8_t k[TB][KS];
 #pragma unroll
-  for (int b = 0; b < TB; ++b) {
-    const int t = min(t0 + b * 32 + col, stored - 1);
-    const int page = p.page_values[s.page_begin + (t >> p.page_shift)];
-    const half_t* row = p.pages + ((((static_cast<int64_t>(page) * 2 * p.h_kv + kvh) << p.page_shift) + (t & ((1 << p.page_shift) - 1))) * D) + half * 8;
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) k[b][ks] = ld16(row + ks * 16).h8;
-  }
+  for (int b = 0; b < TB; ++b) load_key<D>(k[b], p, s, kvh, min(t0 + b * 32 + col, stored - 1), half);
   float sum[TB][16];
 #pragma unroll
   for (int b = 0; b < TB; ++b) {
@@ -268,21 +288,48 @@ __global__ __launch_bounds__(256, 2) void key_weights_kernel(KeyWeightsParams p)
     }
   }
   wait_vmcnt<0>();  // no copy is on its way into memory that is another workgroup's then
-  // lane i of 32 takes the sum of its half's i-th token of a block
 #pragma unroll
-  for (int b = 0; b < TB; ++b) {
-    float mine = 0.f;
+  for (int b = 0; b < TB; ++b) add_block_sums(sum[b], p, s, kvh, t0 + b * 32, stored, col, half);
+}
+
+// Few rows in shares: the merge and the weights in one launch.  The first workgroups merge, the others weigh 128 tokens each, a wave 32;
+// rows come straight from memory, and each workgroup finds its rows' lse from the shares'.
+template <int D>
+__global__ __launch_bounds__(256) void merge_and_weigh_kernel(KeyWeightsParams p, PrefillShares shares, half_t* output, float* lse, int merging) {
+  if (static_cast<int>(blockIdx.x) < merging) {
+    merge_prefill_shares<float, D>(shares.output, shares.lse, output, lse, shares.rows, shares.splits, 0, p.q_indptr + p.batch, p.h_q, blockIdx.x);
+    return;
+  }
+  constexpr int KS = D / 16;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
+  const int item = blockIdx.x - merging, kvh = item % p.h_kv, slot = item / p.h_kv;
+  const SequenceOf s = sequence_of_slot(p.page_indptr, p.last_page_len, p.batch, p.page_shift, 7, slot, lane);
+  const int stored = s.stored(p.page_shift), t0 = (slot - s.slot_begin) * 128 + wave * 32;
+  if (t0 >= stored) return;
+  const int q_begin = p.q_indptr[s.index], q_len = p.q_indptr[s.index + 1] - q_begin;
+  const int in_front = stored - q_len;
+  const int row_begin = (p.observed > 0 ? max(q_len - p.observed, 0) : 0) * p.group, row_end = q_len * p.group;
+  half8_t k[KS];
+  load_key<D>(k, p, s, kvh, min(t0 + col, stored - 1), half);
+  float sum[16] = {};
+  for (int r0 = row_begin; r0 < row_end; r0 += 32) {
+    const int row = min(r0 + col, row_end - 1), token = p.by_group(row);
+    const int64_t at = static_cast<int64_t>(q_begin + token) * p.h_q + kvh * p.group + (row - token * p.group);
+    half8_t q[KS];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) q[ks] = ld16(p.q + at * D + half * 8 + ks * 16).h8;
+    const float row_lse = merged_lse(shares.lse, shares.rows, shares.splits, at);
+    float16_t x = {};
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) x = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[ks], q[ks], x, 0, 0, 0);
+    const int end = r0 + col >= row_end ? 0 : p.causal ? min(in_front + token + 1, stored) : stored;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      const float total = sum_xor16(group_sum<16>(sum[b][i]));
-      mine = col == i ? total : mine;
-    }
-    const int t = t0 + b * 32 + (col & 3) + 8 * (col >> 2) + 4 * half;
-    if (col < 16 && t < stored) {
-      const int page = p.weight_page_values[s.page_begin + (t >> p.page_shift)];
-      p.key_weights[((static_cast<int64_t>(page) * p.h_kv + kvh) << p.page_shift) + (t & ((1 << p.page_shift) - 1))] += mine;
+      const float w = fast_exp2(fmaf(x[i], p.scale_log2, -row_lse));
+      sum[i] += t0 + (i & 3) + 8 * (i >> 2) + 4 * half < end ? w : 0.f;
     }
   }
+  add_block_sums(sum, p, s, kvh, t0, stored, col, half);
 }
 
 // ------------------------------------------------------------------------------------------
@@ -1105,11 +1152,10 @@ static void check_aligned16(const char* what, std::initializer_list<const void*>
 
 constexpr size_t kMostKept = size_t{1} << 29;  // bytes of a decode call's kept scores; more than that is computed again
 
-static void add_key_weights(const char* what, const void* q, const int32_t* q_indptr, const void* pages, const int32_t* page_indptr,
-                            const int32_t* page_values, const int32_t* length_info, const float* lse, float* key_weights,
-                            const int32_t* weight_page_values, bool causal, int64_t observed, double sm_scale, int32_t batch_size,
-                            int64_t total_q, int64_t nnz_pages, int32_t h_q, int32_t h_kv, int32_t d, int page_shift, hipStream_t stream) {
-  if (batch_size == 0 || nnz_pages == 0) return;
+static KeyWeightsParams weights_of_call(const void* q, const int32_t* q_indptr, const void* pages, const int32_t* page_indptr,
+                                        const int32_t* page_values, const int32_t* length_info, const float* lse, float* key_weights,
+                                        const int32_t* weight_page_values, bool causal, int64_t observed, double sm_scale, int32_t batch_size,
+                                        int32_t h_q, int32_t h_kv, int page_shift) {
   KeyWeightsParams p;
   p.q = static_cast<const half_t*>(q);
   p.pages = static_cast<const half_t*>(pages);
@@ -1130,7 +1176,14 @@ static void add_key_weights(const char* what, const void* q, const int32_t* q_in
   p.observed = static_cast<int>(std::min<int64_t>(observed, INT32_MAX));
   p.page_shift = page_shift;
   p.scale_log2 = static_cast<float>(sm_scale) * kLog2e;
-  const int64_t rows = std::min<int64_t>(total_q, observed > 0 ? observed * batch_size : total_q) * p.group;  // that count, at most
+  return p;
+}
+// The sums from q, K and the lse that attention has written.
+static void add_key_weights(const char* what, const KeyWeightsParams& p, int64_t total_q, int64_t nnz_pages, int32_t d, hipStream_t stream) {
+  const int64_t batch_size = p.batch, h_kv = p.h_kv;
+  const int page_shift = p.page_shift;
+  if (batch_size == 0 || nnz_pages == 0) return;
+  const int64_t rows = (p.observed > 0 ? std::min<int64_t>(total_q, p.observed * batch_size) : total_q) * p.group;  // that count, at most
   const auto launch = [&](auto dim, auto blocks) {
     constexpr int D = decltype(dim)::value, TB = decltype(blocks)::value;
     const int64_t items = (((nnz_pages << page_shift) / (128 * TB)) + batch_size) * h_kv;
@@ -1216,8 +1269,9 @@ int tvmkv_batch_decode_paged_kv_weights(const void* q, const void* pages, const 
   }
   run(tvmkv_batch_decode_paged_kv(q, pages, page_indptr, page_values, length_info, nullptr, nullptr, output, lse, 0, 1.0, 1e4, sm_scale,
                                   batch_size, nnz_pages, num_pages, h_q, h_kv, d, page_size, 0, stream));
-  add_key_weights(what, q, nullptr, pages, page_indptr, page_values, length_info, lse, key_weights, weight_page_values, false, 0, sm_scale,
-                  batch_size, batch_size, nnz_pages, h_q, h_kv, d, shift_of_page(what, page_size), as_stream(stream));
+  add_key_weights(what, weights_of_call(q, nullptr, pages, page_indptr, page_values, length_info, lse, key_weights, weight_page_values, false, 0,
+                                        sm_scale, batch_size, h_q, h_kv, shift_of_page(what, page_size)),
+                  batch_size, nnz_pages, d, as_stream(stream));
   KV_API_END();
 }
 
@@ -1235,11 +1289,35 @@ int tvmkv_batch_prefill_paged_kv_weights(const void* q, const int32_t* q_indptr,
                   h_q, h_kv, d, page_size);
   if (batch_size == 0) return TVMKV_OK;
   KV_CHECK(q_indptr) << what << ": NULL tensor";
+  const hipStream_t s = as_stream(stream);
+  const KeyWeightsParams p = weights_of_call(q, q_indptr, pages, page_indptr, page_values, length_info, lse, key_weights, weight_page_values,
+                                             causal != 0, observed, sm_scale, batch_size, h_q, h_kv, shift_of_page(what, page_size));
+  // Up to 16 rows of a kv head on average, or 32 in 8 shares at most, merge and weights are one launch; with more of them its workgroups, which
+  // all go over the shares' lse, take longer than two launches.  Apart / in one, us (32 / 8 heads of dim 128): 1 x 700 tokens 8 rows 16.2 /
+  // 13.8, 20 rows 16.0 / 13.1, 32 rows 15.5 / 13.5; 1 x 8000 8 rows 30.5 / 26.3, 32 rows 30.4 / 32.4, 64 rows 33 / 46; 8 x 2000 8 rows
+  // 33.7 / 33.9, 20 rows 35.4 / 36.6, 64 rows 43 / 53; 32 x 1000 8 rows 53.5 / 50.4, 32 rows 58.4 / 59.6, 64 rows 67 / 75.
+  bool added = false;
+  const int64_t rows = total_q * p.group;
+  const std::function<bool(const PrefillShares&)> merge_and_weigh = [&](const PrefillShares& shares) {
+    if (rows > int64_t{shares.splits <= 8 ? 32 : 16} * batch_size) return false;
+    const auto launch = [&](auto dim) {
+      constexpr int D = decltype(dim)::value, rows_of_block = 256 / (D / 8);
+      const int64_t merging = (shares.rows + rows_of_block - 1) / rows_of_block;
+      const int64_t items = merging + (((nnz_pages << p.page_shift) >> 7) + batch_size) * h_kv;
+      KV_CHECK(items < (int64_t{1} << 31)) << what << ": too many work items";
+      hipLaunchKernelGGL(merge_and_weigh_kernel<D>, dim3(static_cast<unsigned>(items)), dim3(256), 0, s, p, shares, static_cast<half_t*>(output), lse,
+                         static_cast<int>(merging));
+    };
+    if (d == 64) launch(std::integral_constant<int, 64>{});
+    if (d == 128) launch(std::integral_constant<int, 128>{});
+    if (d == 256) launch(std::integral_constant<int, 256>{});
+    added = true;
+    return true;
+  };
   // Shares of 128 keys: what launches of few rows on few keys take is the walk along them (five tokens on 700 keys 17.6 -> 11.3 us).
   run(prefill_paged_in_float(q, q_indptr, pages, page_indptr, page_values, length_info, output, lse, causal, sm_scale, batch_size, total_q,
-                             nnz_pages, num_pages, h_q, h_kv, d, page_size, 128, stream));
-  add_key_weights(what, q, q_indptr, pages, page_indptr, page_values, length_info, lse, key_weights, weight_page_values, causal != 0, observed,
-                  sm_scale, batch_size, total_q, nnz_pages, h_q, h_kv, d, shift_of_page(what, page_size), as_stream(stream));
+                             nnz_pages, num_pages, h_q, h_kv, d, page_size, 128, &merge_and_weigh, stream));
+  if (!added) add_key_weights(what, p, total_q, nnz_pages, d, s);
   KV_API_END();
 }
 

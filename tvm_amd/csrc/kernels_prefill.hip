@@ -30,6 +30,7 @@
 #include <type_traits>
 
 #include "prefill_kernel.cuh"
+#include "prefill_merge.cuh"
 #include "runtime_support.h"
 #include "typed_kernels.h"
 
@@ -74,48 +75,7 @@ __global__ __launch_bounds__(256) void prefill_split_merge_kernel(const T* __res
                                                                   const float* __restrict__ part_lse, half_t* __restrict__ output,
                                                                   float* __restrict__ lse, int64_t rows, int splits,
                                                                   int merge_into, const int32_t* __restrict__ q_end, int h_q) {
-  constexpr int TPR = DV / 8;  // threads per row, 8 features each
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * (256 / TPR) + threadIdx.x / TPR;
-  const int piece = threadIdx.x % TPR;
-  // (rows behind the last sequence have no shares and stay as they are)
-  if (row >= min(rows, static_cast<int64_t>(*q_end) * h_q)) return;
-  // the shares' loads do not depend on each other: unrolled, eight are in flight at once (64 shares of a
-  // 64-token chunk: 35 us as a loop of dependent round trips)
-  float s_max = kNegInit;
-#pragma unroll 8
-  for (int i = 0; i < splits; ++i) s_max = fmaxf(s_max, part_lse[i * rows + row]);
-  float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  float w_sum = 0.f;
-  const bool any_share = s_max > kNegInit;
-  if (merge_into) {
-    // output / lse already hold a state of the same rows (the launch was asked to merge into it): it is one more
-    // state of the sum; shares that are all empty count as the one empty state (out 0, lse -5e4) an unsplit
-    // launch would have merged
-    const float s_prev = lse[row];
-    s_max = fmaxf(s_max, s_prev);
-    const float w = fast_exp2(s_prev - s_max);
-    const Vec16 v = ld16(output + row * DV + piece * 8);
-    w_sum = w + (any_share ? 0.f : fast_exp2(kNegInit - s_max));
-#pragma unroll
-    for (int e = 0; e < 8; ++e) acc[e] = w * static_cast<float>(v.h8[e]);
-  }
-  if (any_share) {
-#pragma unroll 8
-    for (int i = 0; i < splits; ++i) {
-      const float w = fast_exp2(part_lse[i * rows + row] - s_max);
-      typedef T share_t __attribute__((ext_vector_type(8)));
-      const share_t v = *reinterpret_cast<const share_t*>(part_o + (i * rows + row) * DV + piece * 8);
-      w_sum += w;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) acc[e] += w * static_cast<float>(v[e]);
-    }
-  }
-  const float inv = w_sum > 0.f ? 1.0f / w_sum : 0.f;
-  Vec16 out;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) out.h8[e] = static_cast<half_t>(acc[e] * inv);
-  *reinterpret_cast<Vec16*>(output + row * DV + piece * 8) = out;
-  if (piece == 0) lse[row] = w_sum > 0.f ? s_max + fast_log2(w_sum) : kNegInit;
+  merge_prefill_shares<T, DV>(part_o, part_lse, output, lse, rows, splits, merge_into, q_end, h_q, blockIdx.x);
 }
 
 // Redirects the launch described by p to scratch memory when it is to be split (prefill_kv_splits); finish() merges.
@@ -489,7 +449,7 @@ static int paged_prefill(const void* q, const int32_t* q_indptr, const void* pag
                          int32_t sliding_window_size, bool merge_into, void* stream,
                          const tvmkv_rope_scaling* scaling = nullptr, int64_t longest = 0,
                          const std::function<int(const PromptLaunch*)>* beside = nullptr, bool float_shares = false,
-                         int64_t least_keys = kMinShareKeys) {
+                         int64_t least_keys = kMinShareKeys, const std::function<bool(const PrefillShares&)>* merge = nullptr) {
   // pages other than 16 / 32 / 64 / 128 tokens, other head dims (80 / 96 / 112 with a sliding-window cache or RoPE
   // inside the kernel among them): the generic matrix-core kernel (its caller merges states with merge_state_inplace)
   const bool plain = rotary_mode == 0 && sliding_window == 0;
@@ -593,7 +553,10 @@ static int paged_prefill(const void* q, const int32_t* q_indptr, const void* pag
   } else {
     KV_UNSUPPORTED(true) << "batch_prefill_paged_kv: head_dim " << d << " is not built (64, 80, 96, 112, 128, 256)";
   }
-  split.finish(p, d, s);
+  if (split.splits > 1) KV_LAUNCH_CHECK();
+  const bool merged = merge != nullptr && split.splits > 1 &&  // (while split holds the shares' memory)
+                      (*merge)({reinterpret_cast<const float*>(p.output), p.lse, split.rows, split.splits});
+  if (!merged) split.finish(p, d, s);
   KV_LAUNCH_CHECK();
   KV_API_END();
 }
@@ -658,10 +621,11 @@ int tvmkv::prefill_paged_with_lengths(const void* q, const int32_t* q_indptr, co
 int tvmkv::prefill_paged_in_float(const void* q, const int32_t* q_indptr, const void* pages, const int32_t* page_indptr,
                                   const int32_t* page_values, const int32_t* length_info, void* output, float* lse, int64_t causal,
                                   double sm_scale, int32_t batch_size, int64_t total_q, int64_t nnz_pages, int64_t num_pages, int32_t h_q,
-                                  int32_t h_kv, int32_t d, int32_t page_size, int64_t least_keys, void* stream) {
+                                  int32_t h_kv, int32_t d, int32_t page_size, int64_t least_keys,
+                                  const std::function<bool(const PrefillShares&)>* merge, void* stream) {
   return paged_prefill(q, q_indptr, pages, page_indptr, page_values, length_info, nullptr, nullptr, output, lse, causal, 0, 1.0, 1e4, sm_scale,
                        batch_size, total_q, nnz_pages, num_pages, h_q, h_kv, d, page_size, 0, 0, false, stream, nullptr, 0, nullptr, true,
-                       least_keys);
+                       least_keys, merge);
 }
 
 int tvmkv::prefill_shared_prefix(const SharedPrefixDecode& a, const std::function<int(const PromptLaunch*)>& own, void* stream) {
