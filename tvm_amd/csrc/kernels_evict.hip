@@ -1292,14 +1292,17 @@ int tvmkv_batch_prefill_paged_kv_weights(const void* q, const int32_t* q_indptr,
   const hipStream_t s = as_stream(stream);
   const KeyWeightsParams p = weights_of_call(q, q_indptr, pages, page_indptr, page_values, length_info, lse, key_weights, weight_page_values,
                                              causal != 0, observed, sm_scale, batch_size, h_q, h_kv, shift_of_page(what, page_size));
-  // Up to 16 rows of a kv head on average, or 32 in 8 shares at most, merge and weights are one launch; with more of them its workgroups, which
-  // all go over the shares' lse, take longer than two launches.  Apart / in one, us (32 / 8 heads of dim 128): 1 x 700 tokens 8 rows 16.2 /
-  // 13.8, 20 rows 16.0 / 13.1, 32 rows 15.5 / 13.5; 1 x 8000 8 rows 30.5 / 26.3, 32 rows 30.4 / 32.4, 64 rows 33 / 46; 8 x 2000 8 rows
-  // 33.7 / 33.9, 20 rows 35.4 / 36.6, 64 rows 43 / 53; 32 x 1000 8 rows 53.5 / 50.4, 32 rows 58.4 / 59.6, 64 rows 67 / 75.
+  // Where a launch is split: up to 16 rows of a kv head on average, or 64 on 16384 (token, kv head)s at most, merge and weights are one launch;
+  // with more of them its workgroups, which all go over the lse of all shares of their rows, take longer than a launch.  Apart / in one, us:
+  //   32 / 8 heads of dim 128    1 x 700 tokens   8 rows 17.1 / 14.1, 32 rows 16.6 / 13.7, 64 rows 17.0 / 15.8, 128 rows 20.1 / 19.8
+  //                              1 x 2000         16 rows 17.7 / 13.9, 64 rows 19.8 / 18.4, 128 rows 24.5 / 26.1
+  //                              1 x 8000         16 rows 26.0 / 22.1, 32 rows 25.8 / 25.6, 64 rows 28 / 34
+  //                              8 x 2000         8 rows 29.3 / 28.5, 16 rows 30.0 / 29.9, 32 rows 30.8 / 32.9, 64 rows 36 / 42
+  //   16 / 2 heads of dim 256    1 x 8000         16 rows 33.5 / 28.6, 64 rows 36.6 / 36.6, 128 rows 44 / 51
+  //   32 / 1 heads of dim 64     4 x 4000         32 rows 18.6 / 14.1, 64 rows 19.8 / 17.4, 128 rows 23 / 26
   bool added = false;
-  const int64_t rows = total_q * p.group;
-  const std::function<bool(const PrefillShares&)> merge_and_weigh = [&](const PrefillShares& shares) {
-    if (rows > int64_t{shares.splits <= 8 ? 32 : 16} * batch_size) return false;
+  const bool in_one = total_q * p.group <= int64_t{(nnz_pages << p.page_shift) * h_kv <= 16384 ? 64 : 16} * batch_size;
+  const std::function<void(const PrefillShares&)> merge_and_weigh = [&](const PrefillShares& shares) {
     const auto launch = [&](auto dim) {
       constexpr int D = decltype(dim)::value, rows_of_block = 256 / (D / 8);
       const int64_t merging = (shares.rows + rows_of_block - 1) / rows_of_block;
@@ -1312,11 +1315,9 @@ int tvmkv_batch_prefill_paged_kv_weights(const void* q, const int32_t* q_indptr,
     if (d == 128) launch(std::integral_constant<int, 128>{});
     if (d == 256) launch(std::integral_constant<int, 256>{});
     added = true;
-    return true;
   };
-  // Shares of 128 keys: what launches of few rows on few keys take is the walk along them (five tokens on 700 keys 17.6 -> 11.3 us).
   run(prefill_paged_in_float(q, q_indptr, pages, page_indptr, page_values, length_info, output, lse, causal, sm_scale, batch_size, total_q,
-                             nnz_pages, num_pages, h_q, h_kv, d, page_size, 128, &merge_and_weigh, stream));
+                             nnz_pages, num_pages, h_q, h_kv, d, page_size, in_one ? &merge_and_weigh : nullptr, stream));
   if (!added) add_key_weights(what, p, total_q, nnz_pages, d, s);
   KV_API_END();
 }

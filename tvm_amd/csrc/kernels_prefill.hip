@@ -81,7 +81,7 @@ __global__ __launch_bounds__(256) void prefill_split_merge_kernel(const T* __res
 // Redirects the launch described by p to scratch memory when it is to be split (prefill_kv_splits); finish() merges.
 // The shares' outputs are fp16 where the launch has always been split, and float32 where it would otherwise run whole:
 //  * float_shares: the prompts of a step whose decoding sequences run elsewhere (prefill_prompts); attention that also adds up weights
-//    (prefill_paged_in_float), whose shares may be shorter too;
+//    (prefill_paged_in_float), with a rule of its own for their number;
 //  * longest, the keys of the longest sequence where the caller knows them, else 0: one round of full row tiles lasts as
 //    long as its longest walk, so two shares each where that is well above the mean.  How much it has to be above is what
 //    the shares' traffic costs, and how many workgroups share a compute unit (one that ends early leaves its unit to the
@@ -99,12 +99,13 @@ struct KvSplit {
   ScratchLease lease{};
   // work_q, work_seqs: the query tokens and sequences that the launch works on, where they are not all (skip_single)
   KvSplit(PrefillParams& p, int64_t total_q, int64_t avg_keys, int dv, hipStream_t stream, int64_t longest = 0, int64_t work_q = 0,
-          int64_t work_seqs = 0, bool float_shares = false, int64_t least_keys = kMinShareKeys)
+          int64_t work_seqs = 0, bool float_shares = false, bool one_round = false)
       : output(p.output), lse(p.lse), rows(total_q * p.h_q), splits(1) {
     if (work_seqs == 0) work_q = total_q, work_seqs = p.batch_size;
     // at most one row tile per (sequence, kv head) on average: the paged kernels stream the K/V rows
     p.stream_kv = work_q * p.group <= work_seqs * BM;
-    splits = prefill_kv_splits(work_q, p.group, work_seqs, p.h_kv, avg_keys, compute_units(), least_keys);
+    splits = one_round ? prefill_float_kv_splits(work_q, p.group, work_seqs, p.h_kv, avg_keys, compute_units(), dv)
+                       : prefill_kv_splits(work_q, p.group, work_seqs, p.h_kv, avg_keys, compute_units());
     const bool unlike = dv == 64 ? longest * 10 >= avg_keys * 14 && longest - avg_keys >= 1024
                                  : dv == 128 && longest * 4 >= avg_keys * 7 && longest - avg_keys >= 2048;
     if (splits == 1 && unlike && avg_keys >= 2 * kMinShareKeys && option(kOptPrefillKvSplits) == 0 &&
@@ -449,7 +450,7 @@ static int paged_prefill(const void* q, const int32_t* q_indptr, const void* pag
                          int32_t sliding_window_size, bool merge_into, void* stream,
                          const tvmkv_rope_scaling* scaling = nullptr, int64_t longest = 0,
                          const std::function<int(const PromptLaunch*)>* beside = nullptr, bool float_shares = false,
-                         int64_t least_keys = kMinShareKeys, const std::function<bool(const PrefillShares&)>* merge = nullptr) {
+                         const std::function<void(const PrefillShares&)>* merge = nullptr) {
   // pages other than 16 / 32 / 64 / 128 tokens, other head dims (80 / 96 / 112 with a sliding-window cache or RoPE
   // inside the kernel among them): the generic matrix-core kernel (its caller merges states with merge_state_inplace)
   const bool plain = rotary_mode == 0 && sliding_window == 0;
@@ -525,7 +526,7 @@ static int paged_prefill(const void* q, const int32_t* q_indptr, const void* pag
   const bool ext = p.rotary != 0 || sliding_window != 0;
   hipStream_t s = as_stream(stream);
   // (a launch under capture keeps the scratch memory that it has always needed)
-  const KvSplit split(p, total_q, nnz_pages * page_size / batch_size, d, s, stream_is_capturing(s) ? 0 : longest, 0, 0, float_shares, least_keys);
+  const KvSplit split(p, total_q, nnz_pages * page_size / batch_size, d, s, stream_is_capturing(s) ? 0 : longest, 0, 0, float_shares, float_shares);
   if (beside != nullptr) {  // the work that writes the state which this launch merges into
     const bool together = split.splits > 1 && !p.stream_kv && !ext && (d == 64 || d == 128);
     PromptLaunch shares;
@@ -553,10 +554,12 @@ static int paged_prefill(const void* q, const int32_t* q_indptr, const void* pag
   } else {
     KV_UNSUPPORTED(true) << "batch_prefill_paged_kv: head_dim " << d << " is not built (64, 80, 96, 112, 128, 256)";
   }
-  if (split.splits > 1) KV_LAUNCH_CHECK();
-  const bool merged = merge != nullptr && split.splits > 1 &&  // (while split holds the shares' memory)
-                      (*merge)({reinterpret_cast<const float*>(p.output), p.lse, split.rows, split.splits});
-  if (!merged) split.finish(p, d, s);
+  if (merge != nullptr && split.splits > 1) {
+    KV_LAUNCH_CHECK();
+    (*merge)({reinterpret_cast<const float*>(p.output), p.lse, split.rows, split.splits});  // while split holds their memory
+  } else {
+    split.finish(p, d, s);
+  }
   KV_LAUNCH_CHECK();
   KV_API_END();
 }
@@ -621,11 +624,11 @@ int tvmkv::prefill_paged_with_lengths(const void* q, const int32_t* q_indptr, co
 int tvmkv::prefill_paged_in_float(const void* q, const int32_t* q_indptr, const void* pages, const int32_t* page_indptr,
                                   const int32_t* page_values, const int32_t* length_info, void* output, float* lse, int64_t causal,
                                   double sm_scale, int32_t batch_size, int64_t total_q, int64_t nnz_pages, int64_t num_pages, int32_t h_q,
-                                  int32_t h_kv, int32_t d, int32_t page_size, int64_t least_keys,
-                                  const std::function<bool(const PrefillShares&)>* merge, void* stream) {
+                                  int32_t h_kv, int32_t d, int32_t page_size,
+                                  const std::function<void(const PrefillShares&)>* merge, void* stream) {
   return paged_prefill(q, q_indptr, pages, page_indptr, page_values, length_info, nullptr, nullptr, output, lse, causal, 0, 1.0, 1e4, sm_scale,
                        batch_size, total_q, nnz_pages, num_pages, h_q, h_kv, d, page_size, 0, 0, false, stream, nullptr, 0, nullptr, true,
-                       least_keys, merge);
+                       merge);
 }
 
 int tvmkv::prefill_shared_prefix(const SharedPrefixDecode& a, const std::function<int(const PromptLaunch*)>& own, void* stream) {

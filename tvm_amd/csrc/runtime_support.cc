@@ -308,18 +308,35 @@ int64_t prefill_workgroups(int64_t work_q, int group, int64_t work_seqs, int h_k
 //    2000-6000 keys, 512 workgroups: 0.171 ms unsplit, 0.183 with 2 shares; a 63-node tree per sequence,
 //    1008 workgroups, matrix-bound: 0.409 against 0.442).
 // No share shorter than 8 tiles on average, at most 64 shares.
-int prefill_kv_splits(int64_t work_q, int group, int64_t work_seqs, int h_kv, int64_t avg_keys, int cus, int64_t least_keys) {
+static int64_t wanted_kv_splits(int64_t workgroups, int64_t rows, int64_t resident) {
+  if (workgroups * 2 <= resident) return (2 * resident + workgroups - 1) / workgroups;
+  return workgroups <= resident && rows * 2 <= workgroups * 128 ? 2 : 1;
+}
+int prefill_kv_splits(int64_t work_q, int group, int64_t work_seqs, int h_kv, int64_t avg_keys, int cus) {
   const int64_t forced = option(kOptPrefillKvSplits);
   if (forced > 0) return static_cast<int>(std::min<int64_t>(forced, 64));
-  const int64_t resident = static_cast<int64_t>(cus) * 2;
-  const int64_t workgroups = prefill_workgroups(work_q, group, work_seqs, h_kv);
-  int64_t want = 1;
-  if (workgroups * 2 <= resident) {
-    want = (2 * resident + workgroups - 1) / workgroups;
-  } else if (workgroups <= resident && work_q * group * h_kv * 2 <= workgroups * 128) {
-    want = 2;
-  }
-  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(std::min(want, avg_keys / least_keys), 64)));
+  const int64_t want = wanted_kv_splits(prefill_workgroups(work_q, group, work_seqs, h_kv), work_q * group * h_kv, static_cast<int64_t>(cus) * 2);
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(std::min(want, avg_keys / kMinShareKeys), 64)));
+}
+
+// The same for shares in float32, which cost the merge twice as much: as many as make one round (at head dim 256 a workgroup fills a compute
+// unit), where that makes three or, of two, fills seven eighths of it; at least 128 keys a share, at most 32 shares.  In two rounds / one
+// round, with the sums of weights, us (query heads / kv heads x dim):
+//   16/2x128  1 x 40 on 8000 41 / 33, 2 x 100 on 4000 64 / 54, 4 x 64 on 8000-16 000 90 / 78, 8 x 5 on 8000 48 / 40, 2 x 190 on 20 000-32 768 195 / 179
+//   32/8x128  1 x 40 on 8000 48 / 39, 1 x 300 on 20 000 234 / 202, 2 x 100 on 4000 73 / 58, 1 x 500 on 2000 98 / 86, 2 x 190 as above 360 / 368
+//   32/8x64   2 x 100 on 4000 51 / 42, 4 x 64 93 / 86, 2 x 190 232 / 228       64/8x128  1 x 300 400 / 368, 4 x 64 225 / 213
+//   16/2x256  1 x 300 on 20 000 296 / 258, 4 x 64 226 / 171, 2 x 190 498 / 438      32/8x256  1 x 300 556 / 515, 8 x 5 on 8000 237 / 216
+//   two shares that fill three quarters of the round: 64/8x128 2 x 190 612 / 658, 32/8x256 2 x 190 950 / 1090; that need more than one:
+//   28/4x256 8 x 10-135 on 3600 238 / 256
+int prefill_float_kv_splits(int64_t work_q, int group, int64_t work_seqs, int h_kv, int64_t avg_keys, int cus, int d) {
+  const int64_t forced = option(kOptPrefillKvSplits);
+  if (forced > 0) return static_cast<int>(std::min<int64_t>(forced, 64));
+  const int64_t workgroups = prefill_workgroups(work_q, group, work_seqs, h_kv), resident = static_cast<int64_t>(cus) * (d == 256 ? 1 : 2);
+  int64_t want = resident / workgroups;
+  // (with each sequence's last row tile, which may be a part of one, two shares must still be one round)
+  const bool two = workgroups * 16 >= resident * 7 && (work_q * group / 128 + work_seqs) * h_kv * 2 <= resident;
+  if (want < 2 || (want == 2 && !two)) want = wanted_kv_splits(workgroups, work_q * group * h_kv, static_cast<int64_t>(cus) * 2);
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(std::min(want, avg_keys / 128), 32)));
 }
 
 // Few row tiles against long page lists: split the keys over workgroups until the chip has ~16 workgroups per compute

@@ -127,7 +127,8 @@ int decode_pick_chunk_pages_wide(int64_t nnz_pages, int h_kv, int batch, int hea
 // group query heads per kv head) on a device of `cus` compute units, and the workgroups that it has unsplit.
 constexpr int64_t kMinShareKeys = 512;  // eight tiles of 64 keys
 int64_t prefill_workgroups(int64_t work_q, int group, int64_t work_seqs, int h_kv);
-int prefill_kv_splits(int64_t work_q, int group, int64_t work_seqs, int h_kv, int64_t avg_keys, int cus, int64_t least_keys = kMinShareKeys);
+int prefill_kv_splits(int64_t work_q, int group, int64_t work_seqs, int h_kv, int64_t avg_keys, int cus);
+int prefill_float_kv_splits(int64_t work_q, int group, int64_t work_seqs, int h_kv, int64_t avg_keys, int cus, int d);
 // The same of a launch of the generic kernel, whose workgroups own generic_row_tile() query rows.
 inline int generic_row_tile(int d, int64_t rows_per_sequence) { return d > 128 || rows_per_sequence <= 16 ? 16 : 32; }
 int generic_kv_splits(int elem_bits, int d, int64_t work_q, int group, int64_t work_seqs, int h_kv, int64_t avg_keys, int cus);

@@ -208,8 +208,8 @@ int prefill_paged_with_lengths(const void* q, const int32_t* q_indptr, const voi
                                int32_t sliding_window, int32_t sliding_window_size, int32_t merge_into,
                                const tvmkv_rope_scaling* rope_scaling, int64_t longest, void* stream);
 
-// tvmkv_batch_prefill_paged_kv over a plain cache, the states of a split launch's shares in float32, least_keys keys a share at least.
-// merge, where it isn't NULL, is asked behind a split launch whether it merges the shares itself.
+// tvmkv_batch_prefill_paged_kv over a plain cache, the states of a split launch's shares in float32, in one round.
+// merge, where it isn't NULL: called in place of the launch that merges a split launch's shares.
 struct PrefillShares {
   const float* output;  // (share, row, d), a row a (query, head)
   const float* lse;     // (share, row)
@@ -219,7 +219,7 @@ struct PrefillShares {
 int prefill_paged_in_float(const void* q, const int32_t* q_indptr, const void* pages, const int32_t* page_indptr, const int32_t* page_values,
                            const int32_t* length_info, void* output, float* lse, int64_t causal, double sm_scale, int32_t batch_size,
                            int64_t total_q, int64_t nnz_pages, int64_t num_pages, int32_t h_q, int32_t h_kv, int32_t d, int32_t page_size,
-                           int64_t least_keys, const std::function<bool(const PrefillShares&)>* merge, void* stream);
+                           const std::function<void(const PrefillShares&)>* merge, void* stream);
 
 // A decode step behind a shared prefix (fp16, plain cache): decode attention over the sequences' own pages, which writes
 // out and lse, and paged prefill attention of all queries over the prefix, merged into them.  One launch and the merge of
