@@ -173,9 +173,9 @@ def test_rows_and_sums_behind_the_last_sequence_stay_as_they_are(q_lens, stored)
     check_attention(q[:n], q_lens, pool, True, 0, (out[:n], lse[:n], sums))
 
 
-@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("d", [64, 80, 96, 112, 128, 256])
 @pytest.mark.parametrize("causal, observed", [(1, 0), (0, 2), (1, 3)])
-@pytest.mark.parametrize("q_lens, stored", [([5], [700]), ([2, 1, 0, 3], [3000, 900, 40, 0]), ([4], [9000]), ([30] + [0] * 7, [1000] + [200] * 7),
+@pytest.mark.parametrize("q_lens, stored", [([5], [700]), ([70, 9], [2500, 700]), ([2, 1, 0, 3], [3000, 900, 40, 0]), ([4], [9000]), ([30] + [0] * 7, [1000] + [200] * 7),
                                             ([9, 1], [4, 600])])
 def test_few_rows_on_long_sequences(q_lens, stored, d, causal, observed):
     """Launches in shares: of few and of many, a sequence with most of the rows, queries without keys."""

@@ -1312,6 +1312,9 @@ int tvmkv_batch_prefill_paged_kv_weights(const void* q, const int32_t* q_indptr,
                          static_cast<int>(merging));
     };
     if (d == 64) launch(std::integral_constant<int, 64>{});
+    if (d == 80) launch(std::integral_constant<int, 80>{});
+    if (d == 96) launch(std::integral_constant<int, 96>{});
+    if (d == 112) launch(std::integral_constant<int, 112>{});
     if (d == 128) launch(std::integral_constant<int, 128>{});
     if (d == 256) launch(std::integral_constant<int, 256>{});
     added = true;

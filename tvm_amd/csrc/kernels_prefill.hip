@@ -113,7 +113,7 @@ struct KvSplit {
       splits = 2;
       float_shares = true;
     }
-    if (dv % 64 != 0) splits = 1;  // padded head dims (80, 96, 112): the merge kernel is not built for their rows
+    if (dv % 64 != 0 && !one_round) splits = 1;  // padded head dims (80, 96, 112): the merge kernel is built for shares in float32 only
     if (splits <= 1) return;
     const size_t o_bytes = static_cast<size_t>(splits) * rows * dv * (float_shares ? sizeof(float) : sizeof(half_t));
     const size_t lse_bytes = static_cast<size_t>(splits) * rows * sizeof(float);
@@ -143,7 +143,14 @@ struct KvSplit {
         merge(prefill_split_merge_kernel<half_t, kD>, static_cast<const half_t*>(p.output));
       }
     };
-    if (dv == 128) {
+    auto merge_padded = [&](auto dim) { merge(prefill_split_merge_kernel<float, decltype(dim)::value>, reinterpret_cast<const float*>(p.output)); };
+    if (dv == 80) {
+      merge_padded(std::integral_constant<int, 80>{});
+    } else if (dv == 96) {
+      merge_padded(std::integral_constant<int, 96>{});
+    } else if (dv == 112) {
+      merge_padded(std::integral_constant<int, 112>{});
+    } else if (dv == 128) {
       merge_dim(std::integral_constant<int, 128>{});
     } else if (dv == 64) {
       merge_dim(std::integral_constant<int, 64>{});

@@ -741,12 +741,13 @@ __device__ __forceinline__ void prefill_row_tile(const PrefillParams& p, const P
         }
       }
       if (half == 0) *lse_ptr = fast_log2(w_prev + w_mine) + s_max;
-    } else if (SRC != kRagged && DQK == DV && !PAD && p.split_f32) {
-      float* share = reinterpret_cast<float*>(p.output) + out_row * DV + half * 4;
+    } else if (SRC != kRagged && DQK == DV && p.split_f32) {
+      float* share = reinterpret_cast<float*>(p.output) + out_row * dvm + half * 4;
 #pragma unroll
       for (int db = 0; db < DB; ++db) {
 #pragma unroll
         for (int j4 = 0; j4 < 4; ++j4) {
+          if (PAD && db * 32 + j4 * 8 >= dvm) continue;
           *reinterpret_cast<float4*>(share + db * 32 + j4 * 8) =
               make_float4(o[db][j4 * 4] * inv, o[db][j4 * 4 + 1] * inv, o[db][j4 * 4 + 2] * inv, o[db][j4 * 4 + 3] * inv);
         }

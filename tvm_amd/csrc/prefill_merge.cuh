@@ -26,7 +26,7 @@ __device__ __forceinline__ float largest_shares_lse(const float (&l)[kSharesAtOn
   return s_max;
 }
 
-// Rows of the block-th 256 threads.
+// Rows of the block-th 256 threads, 256 / (DV / 8) of them.
 template <typename T, int DV>
 __device__ __forceinline__ void merge_prefill_shares(const T* __restrict__ part_o, const float* __restrict__ part_lse,
                                                      half_t* __restrict__ output, float* __restrict__ lse, int64_t rows, int splits,
@@ -35,7 +35,7 @@ __device__ __forceinline__ void merge_prefill_shares(const T* __restrict__ part_
   constexpr int TPR = DV / 8;  // threads per row, 8 features each
   const int64_t row = static_cast<int64_t>(block) * (256 / TPR) + threadIdx.x / TPR;
   const int piece = threadIdx.x % TPR;
-  if (row >= rows) return;
+  if (threadIdx.x >= 256 / TPR * TPR || row >= rows) return;
   const int64_t end = static_cast<int64_t>(*q_end) * h_q;
   const auto load = [&](share_t(&v)[kSharesAtOnce], int i0) {
 #pragma unroll
