@@ -237,7 +237,7 @@ def test_kernels_keep_their_values_in_registers(tmp_path):
     if not (os.path.exists(READELF) and os.path.exists(library)):
         pytest.skip("needs the built library and llvm-readelf")
     kernels = [k for k in _kernel_metadata(library, tmp_path)
-               if re.search(r"key_weights_kernel|merge_and_weigh_kernel|kept_scores_kernel|select_|move_kept_kernel", k[0])
+               if re.search(r"key_weights_kernel|shared_rows_kernel|merge_and_weigh_kernel|kept_scores_kernel|select_|move_kept_kernel", k[0])
                or ("decode_mfma_kernel" in k[0] and k[0].split("EEEv")[0].endswith("Lb1"))]
-    assert len(kernels) == 11 + 6 + 1 + 6 + 3 + 4
+    assert len(kernels) == 11 + 6 + 1 + 1 + 6 + 3 + 4
     assert [k for k in kernels if k[1] or k[2]] == []

@@ -188,6 +188,21 @@ def test_few_rows_on_long_sequences(q_lens, stored, d, causal, observed):
     check_attention(q[:n], q_lens, pool, causal, observed, (out[:n], lse[:n], sums))
 
 
+@pytest.mark.parametrize("d", [64, 96, 128, 256])
+@pytest.mark.parametrize("causal, observed", [(1, 0), (0, 0), (1, 300)])
+@pytest.mark.parametrize("h_q, h_kv, q_lens, stored", [(40, 1, [150, 0, 43], [261, 100, 229]), (12, 2, [700], [901]), (16, 1, [3, 190, 0, 90, 1], [500, 190, 33, 60, 0]),
+                                                       (8, 1, [40] * 70, [40, 90] * 35)])
+def test_many_rows_on_few_keys(h_q, h_kv, q_lens, stored, d, causal, observed):
+    """Rows that workgroups share: unlike sequences, some without queries, queries without keys, batches of more than 64."""
+    rng = np.random.default_rng(sum(q_lens) + d)
+    pool = Pool(rng, stored, h_kv, 16, d)
+    q = queries(rng, sum(q_lens) + 2, h_q, d)
+    out, lse, sums = prefill(q, q_lens, pool, causal, observed)
+    n = sum(q_lens)
+    assert (out[n:] == 7.0).all() and (lse[n:] == 7.0).all()
+    check_attention(q[:n], q_lens, pool, causal, observed, (out[:n], lse[:n], sums))
+
+
 def test_more_queries_observed_than_there_are():
     rng = np.random.default_rng(8)
     pool = Pool(rng, [300, 20], 2, 16, 64)

@@ -70,6 +70,8 @@ struct KeyWeightsParams {
   const int32_t* last_page_len;
   const float* lse;
   float* key_weights;
+  float* shares;  // where the rows are shared, the sums of each share: (share, kv head, entry of the page table, token of the page)
+  int nnz_pages;
   int batch;
   int h_q;
   int h_kv;
@@ -115,9 +117,9 @@ __device__ __forceinline__ void load_key(half8_t (&k)[D / 16], const KeyWeightsP
 #pragma unroll
   for (int ks = 0; ks < D / 16; ++ks) k[ks] = ld16(row + ks * 16).h8;
 }
-// Adds up a block's sums over the rows and to the pool's: lane i of 32 takes the sum of its half's i-th token.
-__device__ __forceinline__ void add_block_sums(const float (&sum)[16], const KeyWeightsParams& p, const SequenceOf& s, int kvh, int t0, int stored,
-                                               int col, int half) {
+// Adds up a block's sums over the rows and to the pool's, or writes those of a share: lane i of 32 takes the sum of its half's i-th token.
+__device__ __forceinline__ void add_block_sums(const float (&sum)[16], const KeyWeightsParams& p, const SequenceOf& s, int kvh, int share, int t0,
+                                               int stored, int col, int half) {
   float mine = 0.f;
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
@@ -126,6 +128,10 @@ __device__ __forceinline__ void add_block_sums(const float (&sum)[16], const Key
   }
   const int t = t0 + (col & 3) + 8 * (col >> 2) + 4 * half;
   if (col < 16 && t < stored) {
+    if (p.shares != nullptr) {
+      p.shares[((static_cast<int64_t>(share * p.h_kv + kvh) * p.nnz_pages + s.page_begin) << p.page_shift) + t] = mine;
+      return;
+    }
     const int page = p.weight_page_values[s.page_begin + (t >> p.page_shift)];
     p.key_weights[((static_cast<int64_t>(page) * p.h_kv + kvh) << p.page_shift) + (t & ((1 << p.page_shift) - 1))] += mine;
   }
@@ -168,8 +174,14 @@ __global__ __launch_bounds__(256, 2) void key_weights_kernel(KeyWeightsParams p)
   const int row_begin = first_counted * p.group, row_end = q_len * p.group;
   const auto end_of = [&](int token) { return p.causal ? min(in_front + token + 1, stored) : stored; };
   // no row in front of the first tile's sees a token of the workgroup's
-  const int first_tile = max(first_counted, p.causal ? tile_t0 - in_front : 0) * p.group / R, num_tiles = (row_end + R - 1) / R;
-  if (first_tile >= num_tiles) return;
+  int first_tile = max(first_counted, p.causal ? tile_t0 - in_front : 0) * p.group / R, num_tiles = (row_end + R - 1) / R;
+  if (p.shares != nullptr) {
+    const int each = (max(num_tiles - first_tile, 0) + static_cast<int>(gridDim.y) - 1) / static_cast<int>(gridDim.y);
+    first_tile += blockIdx.y * each;
+    num_tiles = min(first_tile + each, num_tiles);
+  } else if (first_tile >= num_tiles) {
+    return;
+  }
 
   half8_t k[TB][KS];
 #pragma unroll
@@ -215,8 +227,10 @@ __global__ __launch_bounds__(256, 2) void key_weights_kernel(KeyWeightsParams p)
     }
   };
   wait_vmcnt<0>();  // K is there: from here on only the copies count
+  if (first_tile < num_tiles) {
 #pragma unroll
-  for (int i = 0; i < STAGES - 1; ++i) issue(first_tile + i, i);
+    for (int i = 0; i < STAGES - 1; ++i) issue(first_tile + i, i);
+  }
   int stage = 0, next_stage = STAGES - 1;
   for (int tile = first_tile; tile < num_tiles; ++tile, stage = stage + 1 < STAGES ? stage + 1 : 0) {
     // The wave's part of the tile has landed where no more than the later tiles' copies are outstanding; behind the barrier everyone's
@@ -289,7 +303,33 @@ __global__ __launch_bounds__(256, 2) void key_weights_kernel(KeyWeightsParams p)
   }
   wait_vmcnt<0>();  // no copy is on its way into memory that is another workgroup's then
 #pragma unroll
-  for (int b = 0; b < TB; ++b) add_block_sums(sum[b], p, s, kvh, t0 + b * 32, stored, col, half);
+  for (int b = 0; b < TB; ++b) add_block_sums(sum[b], p, s, kvh, blockIdx.y, t0 + b * 32, stored, col, half);
+}
+
+// The shares' sums, in their order, to the pool's.  A wave has 256 tokens of a kv head, a lane four.
+constexpr int kSharedTokensShift = 10;  // of a workgroup
+__global__ __launch_bounds__(256) void shared_rows_kernel(KeyWeightsParams p, int shares) {
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int kvh = blockIdx.x % p.h_kv, slot = blockIdx.x / p.h_kv;
+  const SequenceOf s = sequence_of_slot(p.page_indptr, p.last_page_len, p.batch, p.page_shift, kSharedTokensShift, slot, lane);
+  const int stored = s.stored(p.page_shift), t = ((slot - s.slot_begin) << kSharedTokensShift) + (wave * 64 + lane) * 4;
+  // (a sequence without queries may have had no workgroups)
+  if (t >= stored || (p.q_indptr != nullptr && p.q_indptr[s.index + 1] <= p.q_indptr[s.index])) return;
+  const int page = p.weight_page_values[s.page_begin + (t >> p.page_shift)];
+  float* const at = p.key_weights + ((static_cast<int64_t>(page) * p.h_kv + kvh) << p.page_shift) + (t & ((1 << p.page_shift) - 1));
+  const float* from = p.shares + ((static_cast<int64_t>(kvh) * p.nnz_pages + s.page_begin) << p.page_shift) + t;
+  float4_t sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+  for (int i = 0; i < shares; ++i, from += (static_cast<int64_t>(p.h_kv) * p.nnz_pages) << p.page_shift) sum += *reinterpret_cast<const float4_t*>(from);
+  if (t + 4 <= stored) {
+    float4_any_t* const sums = reinterpret_cast<float4_any_t*>(at);
+    *sums = *sums + float4_any_t{sum[0], sum[1], sum[2], sum[3]};
+  } else {
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+      if (t + k < stored) at[k] += sum[k];
+    }
+  }
 }
 
 // Few rows in shares: the merge and the weights in one launch.  The first workgroups merge, the others weigh 128 tokens each, a wave 32;
@@ -329,7 +369,7 @@ __global__ __launch_bounds__(256) void merge_and_weigh_kernel(KeyWeightsParams p
       sum[i] += t0 + (i & 3) + 8 * (i >> 2) + 4 * half < end ? w : 0.f;
     }
   }
-  add_block_sums(sum, p, s, kvh, t0, stored, col, half);
+  add_block_sums(sum, p, s, kvh, 0, t0, stored, col, half);
 }
 
 // ------------------------------------------------------------------------------------------
@@ -1166,6 +1206,7 @@ static KeyWeightsParams weights_of_call(const void* q, const int32_t* q_indptr, 
   p.last_page_len = length_info;
   p.lse = lse;
   p.key_weights = key_weights;
+  p.shares = nullptr;
   p.batch = batch_size;
   p.h_q = h_q;
   p.h_kv = h_kv;
@@ -1179,16 +1220,34 @@ static KeyWeightsParams weights_of_call(const void* q, const int32_t* q_indptr, 
   return p;
 }
 // The sums from q, K and the lse that attention has written.
-static void add_key_weights(const char* what, const KeyWeightsParams& p, int64_t total_q, int64_t nnz_pages, int32_t d, hipStream_t stream) {
+static void add_key_weights(const char* what, KeyWeightsParams p, int64_t total_q, int64_t nnz_pages, int32_t d, hipStream_t stream) {
   const int64_t batch_size = p.batch, h_kv = p.h_kv;
   const int page_shift = p.page_shift;
   if (batch_size == 0 || nnz_pages == 0) return;
   const int64_t rows = (p.observed > 0 ? std::min<int64_t>(total_q, p.observed * batch_size) : total_q) * p.group;  // that count, at most
+  p.nnz_pages = static_cast<int>(nnz_pages);
   const auto launch = [&](auto dim, auto blocks) {
     constexpr int D = decltype(dim)::value, TB = decltype(blocks)::value;
-    const int64_t items = (((nnz_pages << page_shift) / (128 * TB)) + batch_size) * h_kv;
+    const int64_t tokens = nnz_pages << page_shift, items = (tokens / (128 * TB) + batch_size) * h_kv;
     KV_CHECK(items < (int64_t{1} << 31)) << what << ": too many work items";
-    hipLaunchKernelGGL((key_weights_kernel<D, TB>), dim3(static_cast<unsigned>(items)), dim3(256), 0, stream, p);
+    // Few workgroups of many rows share these: two workgroups a compute unit, or four where each has a long way to go, of two row tiles at
+    // least; two shares only where they save more than the second launch costs.  Whole calls alone / shared, us (query heads / kv heads x dim):
+    //   1 x 2048 tokens 32/8x128 216 / 96, on 8000 cached 567 / 522; 1 x 500 on 2000 88 / 65; 2 x 1000 64/8x128 305 / 235; 8 x 512 16/2x64 95 / 35;
+    //   2 x 25-241 on 79-315 40/1x96 173 / 28; 27 x 14-973 40/1x96 913 / 264; not shared: 37 x 9/3x96, 18 tiles on 243 workgroups, 68 / 80,
+    //   1 x 114 32/8x128, 7 tiles on 8, 16 / 18
+    const int64_t tiles = rows / (batch_size * WeightTiles<D, TB>::kRows), per_unit = tiles >= 96 ? 4 : 2;
+    int64_t shares = std::min<int64_t>({per_unit * compute_units() / items, tiles / 2, 32});
+    if (tiles < 9 || shares < 2 || (shares == 2 && tiles < 28)) shares = 1;
+    ScratchLease ws{};
+    if (shares > 1) {
+      ws = lease_scratch(kScratchKept, stream, static_cast<size_t>(shares) * tokens * h_kv * sizeof(float), 0);
+      p.shares = reinterpret_cast<float*>(ws.ptr);
+    }
+    hipLaunchKernelGGL((key_weights_kernel<D, TB>), dim3(static_cast<unsigned>(items), static_cast<unsigned>(shares)), dim3(256), 0, stream, p);
+    if (shares > 1) {
+      const int64_t sums = ((tokens >> kSharedTokensShift) + batch_size) * h_kv;
+      hipLaunchKernelGGL(shared_rows_kernel, dim3(static_cast<unsigned>(sums)), dim3(256), 0, stream, p, static_cast<int>(shares));
+    }
   };
   const bool many_rows = rows >= int64_t{256} * batch_size;
   const auto launch_blocks = [&](auto dim) {
