@@ -380,7 +380,8 @@ def test_select_of_a_long_sequence_among_short_ones(stored, keep, kind):
 
 @pytest.mark.parametrize("kind", ["ties", "equal", "close", "any"])
 @pytest.mark.parametrize("stored, keep, sinks, recent", [([20000, 33000], [4096, 8192], 0, 0), ([50000], [49999], 4097, 4095), ([17000], [1], 0, 0),
-                                                         ([17000], [0], 0, 0), ([40000], [30000], 0, 0), ([4096 * 9 + 1], [4097], 3, 1)])
+                                                         ([17000], [0], 0, 0), ([40000], [30000], 0, 0), ([4096 * 9 + 1], [4097], 3, 1),
+                                                         ([66000, 40000], [4096, 8192], 0, 0), ([40000], [1], 0, 0), ([40000], [0], 0, 0)])
 def test_select_in_chunks(stored, keep, sinks, recent, kind):
     rng = np.random.default_rng(sinks + recent)
     total, table = table_of(rng, stored, 64)
@@ -554,9 +555,10 @@ def test_a_captured_step_replays():
         assert torch.equal(state["sums"], eager["sums"]) and torch.equal(state["pages"].view(torch.int16), eager["pages"].view(torch.int16))
 
 
-def test_a_captured_choice_in_chunks_replays():
+@pytest.mark.parametrize("stored", [[30000, 20000, 9], [60000, 50000, 9]])
+def test_a_captured_choice_of_long_lists_replays(stored):
     rng = np.random.default_rng(35)
-    stored, keep = [30000, 20000, 9], [5000, 300, 50]
+    keep = [5000, 300, 50]
     total, (indptr, info, weight_ids) = table_of(rng, stored, 64)
     sums, kept = torch.zeros((total, 2, 64), device=DEV), torch.zeros((3, 2, 5000), dtype=torch.int32, device=DEV)
     args = (i32(indptr), i32(weight_ids), i32(info), i32(keep))
@@ -577,6 +579,62 @@ def test_a_captured_choice_in_chunks_replays():
         eager = torch.empty_like(kept)
         kernels.select_kept_tokens(sums, *args, eager, 4, 30)
         assert torch.equal(kept, eager)
+
+
+@pytest.mark.parametrize("h_q, h_kv, q_lens, stored", [(8, 2, [5], [700]), (8, 2, [5, 2, 0], [2000, 9000, 30]), (40, 1, [150, 43], [261, 229]),
+                                                       (8, 2, [300], [900])])
+def test_captured_prefill_replays(h_q, h_kv, q_lens, stored):
+    """Shares of keys and of rows, their joins: each replay as the eager call, bit for bit."""
+    rng = np.random.default_rng(sum(q_lens))
+    pool = Pool(rng, stored, h_kv, 16, 128)
+    indptr, ids, info, weight_ids = pool.table()
+    pages, q_indptr = dev(pool.pages), i32(np.concatenate(([0], np.cumsum(q_lens))))
+    q = torch.zeros((sum(q_lens), h_q, 128), dtype=torch.float16, device=DEV)
+
+    def outputs():
+        return torch.zeros_like(q), torch.zeros(q.shape[:2], device=DEV), dev(pool.sums)
+
+    def call(out, lse, sums):
+        kernels.batch_prefill_paged_kv_weights(q, q_indptr, pages, indptr, ids, info, out, lse, sums, weight_ids, 1, 0, 128 ** -0.5)
+
+    got, stream = outputs(), torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        call(*got)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            call(*got)
+    for _ in range(4):
+        fresh, eager = queries(rng, len(q), h_q, 128), outputs()
+        torch.cuda.synchronize()
+        q.copy_(dev(fresh))
+        got[2].copy_(dev(pool.sums))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        call(*eager)
+        for x, y in zip(got, eager):
+            assert torch.equal(x.nan_to_num(9.0), y.nan_to_num(9.0))
+        check_attention(fresh, q_lens, pool, True, 0, tuple(host(x) for x in eager))
+
+
+def test_prefill_on_two_streams_at_once():
+    rng = np.random.default_rng(41)
+    shapes = [([150, 43], [261, 229], 40, 1), ([5], [3000], 8, 2)]
+    pools = [Pool(rng, stored, h_kv, 16, 128) for _, stored, _, h_kv in shapes]
+    qs = [queries(rng, sum(q_lens), h_q, 128) for q_lens, _, h_q, _ in shapes]
+    streams, calls = [torch.cuda.Stream() for _ in shapes], []
+    for (q_lens, *_), pool, q, stream in list(zip(shapes, pools, qs, streams)) * 3:
+        indptr, ids, info, weight_ids = pool.table()
+        inputs = dev(q), i32(np.concatenate(([0], np.cumsum(q_lens)))), dev(pool.pages), indptr, ids, info
+        outs = torch.zeros_like(inputs[0]), torch.zeros(q.shape[:2], device=DEV), dev(pool.sums)
+        calls.append((inputs, outs, weight_ids, stream, q, q_lens, pool))
+    torch.cuda.synchronize()
+    for inputs, outs, weight_ids, stream, *_ in calls:
+        with torch.cuda.stream(stream):
+            kernels.batch_prefill_paged_kv_weights(*inputs, *outs, weight_ids, 1, 0, 128 ** -0.5)
+    torch.cuda.synchronize()
+    for _, outs, _, _, q, q_lens, pool in calls:
+        check_attention(q, q_lens, pool, True, 0, tuple(host(x) for x in outs))
 
 
 def test_scratch_counters_of_an_older_launch_do_not_count():

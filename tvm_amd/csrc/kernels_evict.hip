@@ -1249,7 +1249,11 @@ static void add_key_weights(const char* what, KeyWeightsParams p, int64_t total_
       hipLaunchKernelGGL(shared_rows_kernel, dim3(static_cast<unsigned>(sums)), dim3(256), 0, stream, p, static_cast<int>(shares));
     }
   };
-  const bool many_rows = rows >= int64_t{256} * batch_size;
+  // 64 tokens a wave instead of 32 where rows are many: half as much of q is read, by fewer waves.  32 / 64 tokens, whole calls in us:
+  //   dim 128   1 x 64 queries on 2000 31.2 / 33.7 (256 rows), 64 x 64 on 1000 196.9 / 194.2, 8 x 1500 on 2000 944 / 925 (6000 rows)
+  //   dim 96    28.5 / 29.7, 178.5 / 172.8, 875 / 853
+  //   dim 64    24.5 / 26.1, 129.7 / 140.8, 621 / 601; 8 x 256 on 2000 103 / 108 (1024 rows), 1 x 2048 77.8 / 73.8 (8192)
+  const bool many_rows = rows >= int64_t{d == 64 ? 4096 : 256} * batch_size;
   const auto launch_blocks = [&](auto dim) {
     if (many_rows) launch(dim, std::integral_constant<int, 2>{}); else launch(dim, std::integral_constant<int, 1>{});
   };
@@ -1412,9 +1416,12 @@ int tvmkv_select_kept_tokens(const float* key_weights, const int32_t* page_indpt
   // Scratch memory: arrival counters, then what the launches leave for each other.  Of one workgroup a list it is the bits of lists that
   // are longer than its shared memory has room for: none where all tokens together are few enough.
   const int64_t tokens = nnz_pages << p.page_shift, lists = static_cast<int64_t>(batch_size) * h_kv;
-  const bool small = tokens <= static_cast<int64_t>(batch_size) * 4096;
-  // Long lists that are too few to fill the chip, a workgroup each.
-  const bool chunked = tokens > static_cast<int64_t>(batch_size) * 16384 && lists <= 4 * compute_units() && tokens <= kMostChunkedBlocks * 256 &&
+  // Workgroups of 256 threads where several lists share a compute unit or are short, else of 1024.  256 / 1024 threads, us (lists of tokens):
+  //   8 of 700 7.7 / 8.8, 128 of 2112 9.5 / 9.1, 128 of 4096 14.6 / 11.0, 512 of 4096 16.5 / 20.2, 512 of 6000 27 / 23, 1024 of 1100 10.9 / 30
+  const bool small = tokens <= static_cast<int64_t>(batch_size) * (lists > compute_units() ? 4096 : 2048);
+  // Long lists that are too few to fill the chip, a workgroup each / in chunks, us:
+  //   8 of 24 000 tokens 23.4 / 30.1, 512 of 24 000 76 / 94, 4 of 40 000 31.7 / 30.9, 2 of 131 072 92 / 35
+  const bool chunked = tokens > static_cast<int64_t>(batch_size) * 32768 && lists <= 4 * compute_units() && tokens <= kMostChunkedBlocks * 256 &&
                        lists * kSelectPasses * sizeof(unsigned long long) <= kSelectCounterBytes;
   const int64_t blocks_in_lds = small ? 256 : 1024;
   ScratchLease ws{};
@@ -1475,7 +1482,10 @@ int tvmkv_move_kept_tokens(void* pages, float* key_weights, const int32_t* page_
   p.max_keep = max_keep;
   p.pieces = 2 * (d * dtype_bits / 128);
   const int64_t lists = static_cast<int64_t>(batch_size) * h_kv;
-  // In one launch and in order, in parts of 128 bytes at least, where that makes four workgroups a compute unit, or lists are short.
+  // In one launch and in order, in parts of 128 bytes at least, where that makes two workgroups a compute unit, or lists are short; else by
+  // ranges of places.  In order / by ranges, us (lists, tokens, places; 8 kv heads of dim 128 but for the last):
+  //   8 x 700 to 512 7.9 / 15.3, 16 x 2112 to 2048 9.0 / 18.4, 128 x 2112 to 2048 14.9 / 30, 512 x 4096 to 2048 120 / 126, 128 x 12 000 to 4000
+  //   81 / 88; 32 x 24 000 to 4000 43 / 38, 8 x 12 000 to 4000 28.7 / 20.0, 4 x 40 000 to 8000 61 / 20.5
   const auto cut_rows = [&](int64_t most, int least_pieces) {
     p.slices = 1;
     while (p.slices * 2 <= most && p.pieces % (p.slices * 2) == 0 && p.pieces / (p.slices * 2) >= least_pieces) p.slices *= 2;
@@ -1484,7 +1494,7 @@ int tvmkv_move_kept_tokens(void* pages, float* key_weights, const int32_t* page_
   };
   const int wanted = 4 * compute_units();
   cut_rows(std::max<int64_t>(wanted / lists, 1), 8);
-  if (lists * p.slices >= wanted || max_keep <= 1024) {
+  if (lists * p.slices * 2 >= wanted || max_keep <= 2048) {
     hipLaunchKernelGGL(move_kept_kernel<kMoveInOrder>, dim3(p.slices, h_kv, batch_size), dim3(kMoveThreads), 0, as_stream(stream), p);
   } else {
     const int parts = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>((max_keep + 63) / 64, wanted / lists)));
