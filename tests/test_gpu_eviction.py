@@ -449,6 +449,30 @@ def test_move_of_ascending_and_of_odd_lists(heads):
     check_move(pool, kept)
 
 
+@pytest.mark.parametrize("d, dtype", [(64, np.float16), (80, np.float16), (256, np.float16), (128, np.float32)])
+@pytest.mark.parametrize("keep, recent", [([2600, 500, 9], 100), ([4800, 590, 30], 2500), ([2500, 600, 40], 2499), ([4999, 599, 39], 0)])
+def test_move_of_long_lists(keep, recent, d, dtype):
+    """By ranges of places; recent tokens that move by fewer places than they are."""
+    rng = np.random.default_rng(d + recent)
+    pool = Pool(rng, [5000, 600, 40], 1, 32, d, dtype)
+    kept = eviction.select(pool.sums, pool.indptr, pool.weight_ids, pool.info, keep, keep[0], 4, recent)
+    check_move(pool, kept)
+    check_move(pool, kept, with_sums=False)
+
+
+@pytest.mark.parametrize("heads", [1, 2])
+def test_move_of_long_ascending_and_odd_lists(heads):
+    rng = np.random.default_rng(heads)
+    pool = Pool(rng, [5000, 2600, 40], heads, 16, 64)
+    kept = np.full((3, heads, 2700), -1, np.int32)
+    for h in range(heads):
+        kept[0, h] = np.sort(rng.permutation(5000)[:2700])
+        kept[1, h, :2600 - 1 - h] = np.arange(1 + h, 2600)
+        kept[2, h, :8] = [0, 1, 1 << 30, 2, -5, 39, 6, 48]
+        kept[2, h, 2650] = 2699  # behind the last page
+    check_move(pool, kept)
+
+
 # ---- together, streams, graphs -----------------------------------------------------------------------------------
 
 
