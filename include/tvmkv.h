@@ -511,7 +511,7 @@ int tvmkv_batch_prefill_paged_kv_weights(const void* q, const int32_t* q_indptr,
  * first; NaN is below everything).  kept (batch, h_kv, max_keep) names the token that each of the first n places takes, -1 behind
  * them: the recent tokens have the last places, in order; in front of them a token that stays and has a place already keeps it, and
  * the other places, from the front, take the others in order.  keep (batch) is in device memory.  A sequence that already has n
- * tokens keeps all as they are.  Calls with more than 65536 tokens in all may need scratch memory.  Fewer than 65536 sequences, tables
+ * tokens keeps all as they are.  Calls with more than 32768 tokens in all may need scratch memory.  Fewer than 65536 sequences, tables
  * of at most 2^30 tokens, max_keep at most 2^30. */
 int tvmkv_select_kept_tokens(const float* key_weights, const int32_t* page_indptr, const int32_t* weight_page_values,
                              const int32_t* length_info, const int32_t* keep, int32_t* kept, int64_t num_sinks, int64_t num_recent,

@@ -59,6 +59,12 @@ __device__ __forceinline__ SequenceOf sequence_of_slot(const int32_t* page_indpt
 // row a lane, so that a lane subtracts one lse, and its 16 sums a block are tokens'.  The lanes' sums are added at the end.
 // The four waves share the rows, which asynchronous copies bring to shared memory kStages - 1 tiles ahead, with the rows' lse.
 // A block's products run under the exponentials of the block before it.
+//
+// The product q K^T is done again, as attention writes no scores and a key's weight needs the row's lse first: 2 D operations, an exponential
+// and two more vector instructions for each (row, key), K read once and q once for 128 or 256 tokens.  Bound by the issue of vector and
+// matrix instructions: 8 chunks of 128-2048 queries on up to 4096 tokens, 32 / 8 heads of dim 128, 342 us (795 TFLOP/s of products;
+// 0.63 of the issue slots and 0.34 of the matrix unit in use); two chunks of 100-300 on 20 000-32 768, 16 / 2 heads of dim 256, 108 us
+// (520 TFLOP/s: 32 tokens a wave, as 64 tokens' K do not fit its registers, and so q read from shared memory twice as often).
 // ------------------------------------------------------------------------------------------
 struct KeyWeightsParams {
   const half_t* q;
@@ -333,7 +339,8 @@ __global__ __launch_bounds__(256) void shared_rows_kernel(KeyWeightsParams p, in
 }
 
 // Few rows in shares: the merge and the weights in one launch.  The first workgroups merge, the others weigh 128 tokens each, a wave 32;
-// rows come straight from memory, and each workgroup finds its rows' lse from the shares'.
+// rows come straight from memory, and each workgroup finds its rows' lse from the shares'.  A chain of round trips: five queries on 700
+// tokens (32 / 8 heads of dim 128) 5.5 us, apart 5.0 + 5.6.
 template <int D>
 __global__ __launch_bounds__(256) void merge_and_weigh_kernel(KeyWeightsParams p, PrefillShares shares, half_t* output, float* lse, int merging) {
   if (static_cast<int>(blockIdx.x) < merging) {
@@ -374,7 +381,9 @@ __global__ __launch_bounds__(256) void merge_and_weigh_kernel(KeyWeightsParams p
 
 // ------------------------------------------------------------------------------------------
 // Weights from kept scores: decode's, which are few (4 bytes for each of the group's heads, where K has 2 D).  A wave has 256 tokens
-// of a kv head, a lane the four of a run of 16 that a lane of the decode kernel had.
+// of a kv head, a lane the four of a run of 16 that a lane of the decode kernel had.  Each score is read once, in whole lines: 21 MB of 64
+// sequences of 1024-4096 tokens in 10 us, 102 MB of 8 of 32 768-65 536 with 64 query heads in 22 (4.6 TB/s).  Whole calls with K read
+// again, for all heads of a group at once, took 208 and 458 us, with kept scores 144 and 341.
 // ------------------------------------------------------------------------------------------
 struct KeptScoresParams {
   const float* scores;  // (kv head, 16-token run of the page table, head of the group, 16 tokens in the order of kept_score_token)
@@ -418,6 +427,9 @@ __global__ __launch_bounds__(256) void kept_scores_kernel(KeptScoresParams p) {
 // chunks of 4096 tokens, in six launches: the histograms of 11, 11 and 10 bits are added up in memory and the last of a list's
 // workgroups goes on to find the digit; then the bits; then the places.  (One list of 131072 tokens by a single workgroup, which
 // reads it with 25 GB/s, took 92 us, with T narrowed down by a sample first 60.)
+//
+// What bounds them is the chain of their steps, not the bytes (4 a token): 512 lists of 2112 tokens 11.7 us, 128 of 2000-16 384 14.9, 8 of 700 6.7;
+// 2 of 131 072 in chunks 35 us, of which clearing 1-4, three passes 7.2 each, bits 4.7, places 9.1.
 // ------------------------------------------------------------------------------------------
 struct SelectState {
   uint32_t least;  // of T, the bits that are known
@@ -972,12 +984,16 @@ __global__ __launch_bounds__(256) void select_places_kernel(SelectParams p) {
 
 // ------------------------------------------------------------------------------------------
 // The move: row kept[i] to place i, in place; kept[i] is never in front of i, so that rows taken in order are still there when they
-// are needed.  Where there are many lists (sequence, kv head), a workgroup fills all places of one, with a part of each row's bytes:
-// it reads the rows of a few places, waits until all its waves have theirs, and writes.  Where there are few, a range of places is a
+// are needed.  Where lists (sequence, kv head) are many or short, a workgroup fills all places of one, with a part of each row's bytes:
+// it reads the rows of a few places, waits until all its waves have theirs, and writes.  Where they are few and long, a range of places is a
 // workgroup's, in two launches: with n entries in the list and s the first place that is also a source (n if none is), the places in
 // front of s can be filled in any order, none of the rows that they need is written meanwhile, and the first launch does it.  The
 // second fills the others: in any order again if none of them is the source of one of them, else (recent tokens that move by fewer
 // places than they are) in order as above.  Entries that name no token behind their place are passed over.
+//
+// Bytes alone, each moved row read and written once: 512 lists of 2112 tokens to 2048 (8 kv heads of dim 128) 40 us, 128 of 2000-16 384 to
+// 2048 46, both 4.4 TB/s where a large copy makes 5.2; rows of 256 bytes from all over the pool, a row's two parts in different pages.
+// 2 lists of 131 072 to 16 384 (dim 256) by ranges 20 + 11 us, 3 TB/s in the first launch.
 // ------------------------------------------------------------------------------------------
 struct MoveParams {
   uint8_t* pages;
