@@ -449,8 +449,7 @@ struct SelectParams {
   int32_t* counts;  // one a block
   SelectState* states;  // one a list
   uint32_t* histograms;  // (list, pass, kBins)
-  unsigned long long* arrivals;  // (list, pass): epoch << 32 | workgroups that have added their histogram
-  uint32_t epoch;
+  uint32_t* arrivals;  // (list, pass): workgroups that have added their histogram
   int batch;
   int h_kv;
   int max_keep;
@@ -813,8 +812,8 @@ __global__ __launch_bounds__(THREADS) void select_kept_kernel(SelectParams p) {
 // Long lists, in chunks of 16 blocks.
 constexpr int kChunkShift = 12, kBins = 2048, kSelectPasses = 3;
 constexpr int64_t kMostChunkedBlocks = 8192;  // whose counts a workgroup of the last launch keeps
-__global__ __launch_bounds__(256) void select_clear_kernel(uint32_t* histograms, int64_t count) {
-  for (int64_t i = blockIdx.x * int64_t{256} + threadIdx.x; i < count; i += gridDim.x * int64_t{256}) histograms[i] = 0;
+__global__ __launch_bounds__(256) void select_clear_kernel(uint32_t* words, int64_t count) {
+  for (int64_t i = blockIdx.x * int64_t{256} + threadIdx.x; i < count; i += gridDim.x * int64_t{256}) words[i] = 0;
 }
 // The list and the chunk of a workgroup of the other launches; a list without a choice has no chunks.
 struct Chunk {
@@ -864,14 +863,8 @@ __global__ __launch_bounds__(256) void select_pass_kernel(SelectParams p, int nt
   wait_vmcnt<0>();
   __syncthreads();
   if (tid == 0) {
-    // A word that an older launch left, also one that was abandoned half way, becomes (epoch, 0); back to that behind the last.
-    unsigned long long* const counter = p.arrivals + list * kSelectPasses + nth;
-    const unsigned long long none = static_cast<unsigned long long>(p.epoch) << 32;
-    __hip_atomic_fetch_max(counter, none, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    const unsigned long long before = __hip_atomic_fetch_add(counter, 1ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    const int chunks = (l.num_blocks() + 15) >> 4;
-    is_last = static_cast<uint32_t>(before) == static_cast<uint32_t>(chunks - 1);
-    if (is_last) __hip_atomic_store(counter, none, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const uint32_t chunks = (l.num_blocks() + 15) >> 4;
+    is_last = __hip_atomic_fetch_add(p.arrivals + list * kSelectPasses + nth, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == chunks - 1;
   }
   __syncthreads();
   if (!is_last) return;
@@ -1188,8 +1181,6 @@ __global__ __launch_bounds__(kMoveThreads) void move_kept_kernel(MoveParams p) {
 // ------------------------------------------------------------------------------------------
 // Launches
 // ------------------------------------------------------------------------------------------
-constexpr size_t kSelectCounterBytes = 64 * 1024;  // of the scratch memory: arrival counters
-
 static int shift_of_page(const char* what, int32_t page_size) {
   KV_UNSUPPORTED(page_size < 16 || page_size > 128 || (page_size & (page_size - 1)) != 0)
       << what << ": page_size " << page_size << " is not built (16, 32, 64, 128)";
@@ -1429,35 +1420,32 @@ int tvmkv_select_kept_tokens(const float* key_weights, const int32_t* page_indpt
   p.sinks = static_cast<int>(std::min<int64_t>(num_sinks, INT32_MAX));
   p.recent = static_cast<int>(std::min<int64_t>(num_recent, INT32_MAX));
   p.batch = batch_size;
-  // Scratch memory: arrival counters, then what the launches leave for each other.  Of one workgroup a list it is the bits of lists that
-  // are longer than its shared memory has room for: none where all tokens together are few enough.
+  // Scratch memory: what the launches leave for each other.  Of one workgroup a list it is the bits of lists that are longer than its shared
+  // memory has room for: none where all tokens together are few enough.
   const int64_t tokens = nnz_pages << p.page_shift, lists = static_cast<int64_t>(batch_size) * h_kv;
   // Workgroups of 256 threads where several lists share a compute unit or are short, else of 1024.  256 / 1024 threads, us (lists of tokens):
   //   8 of 700 7.7 / 8.8, 128 of 2112 9.5 / 9.1, 128 of 4096 14.6 / 11.0, 512 of 4096 16.5 / 20.2, 512 of 6000 27 / 23, 1024 of 1100 10.9 / 30
   const bool small = tokens <= static_cast<int64_t>(batch_size) * (lists > compute_units() ? 4096 : 2048);
   // Long lists that are too few to fill the chip, a workgroup each / in chunks, us:
   //   8 of 24 000 tokens 23.4 / 30.1, 512 of 24 000 76 / 94, 4 of 40 000 31.7 / 30.9, 2 of 131 072 92 / 35
-  const bool chunked = tokens > static_cast<int64_t>(batch_size) * 32768 && lists <= 4 * compute_units() && tokens <= kMostChunkedBlocks * 256 &&
-                       lists * kSelectPasses * sizeof(unsigned long long) <= kSelectCounterBytes;
+  const bool chunked = tokens > static_cast<int64_t>(batch_size) * 32768 && lists <= 4 * compute_units() && tokens <= kMostChunkedBlocks * 256;
   const int64_t blocks_in_lds = small ? 256 : 1024;
   ScratchLease ws{};
   if (chunked || tokens > blocks_in_lds * 256) {
-    const size_t blocks = static_cast<size_t>((tokens >> 8) + batch_size) * h_kv, bins = chunked ? static_cast<size_t>(lists) * kSelectPasses * kBins : 0;
-    const size_t states = chunked ? static_cast<size_t>(lists) : 0;
+    const size_t blocks = static_cast<size_t>((tokens >> 8) + batch_size) * h_kv, states = chunked ? static_cast<size_t>(lists) : 0;
     ws = lease_scratch(kScratchSelect, s,
-                       kSelectCounterBytes + blocks * 4 * sizeof(uint64_t) + states * sizeof(SelectState) + (blocks + bins) * sizeof(uint32_t),
-                       kSelectCounterBytes);
-    p.arrivals = reinterpret_cast<unsigned long long*>(ws.ptr);
-    p.epoch = ws.epoch;
-    p.words = reinterpret_cast<uint64_t*>(ws.ptr + kSelectCounterBytes);
+                       blocks * (4 * sizeof(uint64_t) + sizeof(int32_t)) + states * (sizeof(SelectState) + kSelectPasses * (kBins + 1) * sizeof(uint32_t)), 0);
+    p.words = reinterpret_cast<uint64_t*>(ws.ptr);
     p.states = reinterpret_cast<SelectState*>(p.words + blocks * 4);
-    p.counts = reinterpret_cast<int32_t*>(p.states + states);
-    p.histograms = reinterpret_cast<uint32_t*>(p.counts + blocks);
+    p.histograms = reinterpret_cast<uint32_t*>(p.states + states);
+    p.arrivals = p.histograms + states * kSelectPasses * kBins;
+    p.counts = reinterpret_cast<int32_t*>(p.arrivals + states * kSelectPasses);
   }
   if (chunked) {
-    const int64_t bins = lists * kSelectPasses * kBins, items = ((tokens >> kChunkShift) + batch_size) * h_kv;
+    const int64_t to_clear = lists * kSelectPasses * (kBins + 1), items = ((tokens >> kChunkShift) + batch_size) * h_kv;
     const dim3 grid(static_cast<unsigned>(items));
-    hipLaunchKernelGGL(select_clear_kernel, dim3(static_cast<unsigned>(std::min<int64_t>((bins + 255) / 256, 1024))), dim3(256), 0, s, p.histograms, bins);
+    hipLaunchKernelGGL(select_clear_kernel, dim3(static_cast<unsigned>(std::min<int64_t>((to_clear + 255) / 256, 1024))), dim3(256), 0, s, p.histograms,
+                       to_clear);
     for (int nth = 0; nth < kSelectPasses; ++nth) hipLaunchKernelGGL(select_pass_kernel, grid, dim3(256), 0, s, p, nth);
     hipLaunchKernelGGL(select_bits_kernel, grid, dim3(256), 0, s, p);
     hipLaunchKernelGGL(select_places_kernel, dim3((max_keep + 1023) / 1024, h_kv, batch_size), dim3(256), 0, s, p);
