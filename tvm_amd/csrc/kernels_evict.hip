@@ -429,7 +429,7 @@ __global__ __launch_bounds__(256) void kept_scores_kernel(KeptScoresParams p) {
 // reads it with 25 GB/s, took 92 us, with T narrowed down by a sample first 60.)
 //
 // What bounds them is the chain of their steps, not the bytes (4 a token): 512 lists of 2112 tokens 11.7 us, 128 of 2000-16 384 14.9, 8 of 700 6.7;
-// 2 of 131 072 in chunks 35 us, of which clearing 1-4, three passes 7.2 each, bits 4.7, places 9.1.
+// 2 of 131 072 in chunks 33 us, of which clearing 1-4, three passes 6.6 each, bits 4.7, places 9.1.
 // ------------------------------------------------------------------------------------------
 struct SelectState {
   uint32_t least;  // of T, the bits that are known
@@ -1427,7 +1427,7 @@ int tvmkv_select_kept_tokens(const float* key_weights, const int32_t* page_indpt
   //   8 of 700 7.7 / 8.8, 128 of 2112 9.5 / 9.1, 128 of 4096 14.6 / 11.0, 512 of 4096 16.5 / 20.2, 512 of 6000 27 / 23, 1024 of 1100 10.9 / 30
   const bool small = tokens <= static_cast<int64_t>(batch_size) * (lists > compute_units() ? 4096 : 2048);
   // Long lists that are too few to fill the chip, a workgroup each / in chunks, us:
-  //   8 of 24 000 tokens 23.4 / 30.1, 512 of 24 000 76 / 94, 4 of 40 000 31.7 / 30.9, 2 of 131 072 92 / 35
+  //   8 of 24 000 tokens 23.4 / 30.1, 512 of 24 000 76 / 94, 4 of 40 000 31.7 / 30.9, 2 of 131 072 92 / 33
   const bool chunked = tokens > static_cast<int64_t>(batch_size) * 32768 && lists <= 4 * compute_units() && tokens <= kMostChunkedBlocks * 256;
   const int64_t blocks_in_lds = small ? 256 : 1024;
   ScratchLease ws{};
