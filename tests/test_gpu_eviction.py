@@ -203,6 +203,17 @@ def test_many_rows_on_few_keys(h_q, h_kv, q_lens, stored, d, causal, observed):
     check_attention(q[:n], q_lens, pool, causal, observed, (out[:n], lse[:n], sums))
 
 
+@pytest.mark.parametrize("h_q, h_kv", [(64, 1), (100, 1), (128, 1), (71, 1), (130, 2)])
+def test_many_query_heads_on_one(h_q, h_kv):
+    rng = np.random.default_rng(h_q)
+    pool = Pool(rng, [300, 40, 1], h_kv, 16, 64)
+    q = queries(rng, 3, h_q, 64)
+    check_attention(q, [1] * 3, pool, False, 0, decode(q, pool))
+    for q_lens in ([2, 1, 0], [50, 40, 1]):
+        q = queries(rng, sum(q_lens), h_q, 64)
+        check_attention(q, q_lens, pool, True, 0, prefill(q, q_lens, pool, 1))
+
+
 def test_more_queries_observed_than_there_are():
     rng = np.random.default_rng(8)
     pool = Pool(rng, [300, 20], 2, 16, 64)
