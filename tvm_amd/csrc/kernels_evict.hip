@@ -1006,17 +1006,18 @@ struct MoveParams {
 constexpr int kMoveThreads = 256;
 constexpr int kMoveWaves = kMoveThreads / 64;
 
+// shared: words that no thread reads any more; they are free again afterwards.
 __device__ __forceinline__ int smallest_of_workgroup(int x, int* shared, int wave, int lane) {
   x = min(x, __builtin_amdgcn_update_dpp(x, x, kDppXor1, 0xf, 0xf, false));
   x = min(x, __builtin_amdgcn_update_dpp(x, x, kDppXor2, 0xf, 0xf, false));
   x = min(x, __builtin_amdgcn_update_dpp(x, x, kDppRowHalfMirror, 0xf, 0xf, false));
   x = min(x, __builtin_amdgcn_update_dpp(x, x, kDppRowMirror, 0xf, 0xf, false));
   x = min(min(__builtin_amdgcn_readlane(x, 0), __builtin_amdgcn_readlane(x, 16)), min(__builtin_amdgcn_readlane(x, 32), __builtin_amdgcn_readlane(x, 48)));
-  __syncthreads();
   if (lane == 0) shared[wave] = x;
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < kMoveWaves; ++w) x = min(x, shared[w]);
+  __syncthreads();  // every wave has read them: the words are free again
   return x;
 }
 
