@@ -481,6 +481,9 @@ int tvmkv_mxfp4_batch_prefill_paged_kv(const void* q, const int32_t* q_indptr, c
  * of its group.  The sums are key_weights, float32 (num_weight_pages, h_kv, page_size), on pages of their own: entry i of
  * weight_page_values has the sums of the tokens on page page_values[i].  Sequences may share K/V pages; their weight pages are all
  * different (passing page_values for both is fine where no page is shared).  Sums of slots that hold no token stay as they are.
+ * The calls only add, and the move leaves the sums of the places that it empties: a slot has the sum of the token that was last in it,
+ * an evicted one or one of another sequence, until the caller clears it.  Whoever stores a token sets the sums of its slot to 0, for
+ * all kv heads, before the first attention call that sees the token.
  *
  * Built for fp16 rows, pages of 16, 32, 64 or 128 tokens, head dims 64, 80, 96, 112, 128 and 256, any GQA group; keys are stored
  * rotated, caches without sliding windows.  q, pages and output are aligned to 16 bytes.  A call reads what the device arrays hold, not
@@ -520,7 +523,8 @@ int tvmkv_select_kept_tokens(const float* key_weights, const int32_t* page_indpt
 /* Moves the rows of the tokens kept (batch, h_kv, max_keep) to their places, K, V and, where key_weights is not NULL, the sums, in
  * place.  Lists of the caller's own may name any token that is not in front of its place (an ascending list does); entries that
  * name none behind it, or none of the sequence's pages, move nothing.  The sequence then has as many tokens as the list names, on
- * the first of its pages.  Pages that other sequences share are copied first (tvmkv_copy_single_page).  Rows of d elements of
+ * the first of its pages; the rows and sums behind them stay as they are (sums are set to 0 where a token is stored, as above).
+ * Pages that other sequences share are copied first (tvmkv_copy_single_page).  Rows of d elements of
  * dtype_bits (16 or 32), a multiple of 16 bytes, d at most 256; pages of 16, 32, 64 or 128 tokens, pools of fewer than 2^32 rows, fewer
  * than 65536 sequences and heads.  No scratch memory. */
 int tvmkv_move_kept_tokens(void* pages, float* key_weights, const int32_t* page_indptr, const int32_t* page_values,

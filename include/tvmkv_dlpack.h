@@ -207,7 +207,8 @@ int tvmkv_dl_mxfp4_batch_prefill_paged_kv(const DLTensor* q, const DLTensor* qo_
 /* Eviction by attention weight (tvmkv.h says what the calls compute): q, pages and out float16, key_weights float32
  * (num_weight_pages, h_kv, page_size), kept int32 (batch, h_kv, max_keep).  No counterparts among the reference's kernels; the
  * arguments of the attention calls are those of slots 17 and 16 without the ones of in-kernel RoPE, and the sums with their pages.
- * tvmkv_dl_move_kept_tokens takes float16 or float32 pages; key_weights and weight_page_indices may be NULL there. */
+ * The caller sets key_weights to 0 in the slot of every token that it stores: no call here does, and the slot has the sum of the token
+ * that was there before.  tvmkv_dl_move_kept_tokens takes float16 or float32 pages; key_weights and weight_page_indices may be NULL there. */
 int tvmkv_dl_batch_decode_paged_kv_weights(const DLTensor* q, const DLTensor* pages, const DLTensor* page_indptr,
                                            const DLTensor* page_indices, const DLTensor* length_info, const DLTensor* out,
                                            const DLTensor* lse, const DLTensor* key_weights, const DLTensor* weight_page_indices,

@@ -380,7 +380,10 @@ def mxfp4_batch_prefill_paged_kv(q, q_indptr, pages, page_indptr, page_values, l
 
 
 def key_weight_pages(num_pages, h_kv, page_size, device="cuda"):
-    """Sums of the attention weights that stored tokens have received, for the *_weights calls: none yet."""
+    """Sums of the attention weights that stored tokens have received, for the *_weights calls: none yet.
+
+    The calls only add to them, and move_kept_tokens leaves those of the places that it empties.  Whoever stores a token sets the sums of
+    its slot to 0 (sums[slots // page_size, :, slots % page_size] = 0), or it begins with those of the token that was there."""
     return torch.zeros((num_pages, h_kv, page_size), dtype=torch.float32, device=device)
 
 
@@ -475,7 +478,7 @@ def select_kept_tokens(key_weights, page_indptr, weight_page_values, length_info
 
 def move_kept_tokens(pages, key_weights, page_indptr, page_values, weight_page_values, kept):
     """Moves the rows of the tokens `kept`, K, V and (key_weights not None) their sums, to their places at the front of each sequence's
-    pages; float16 or float32 pages."""
+    pages; float16 or float32 pages.  The sums of the places behind them stay as they are (key_weight_pages)."""
     _i32(page_indptr, page_values, weight_page_values, kept)
     if pages.dtype not in (torch.float16, torch.float32):
         raise KVError(-2, f"only float16 and float32 rows are built, got {pages.dtype}")
