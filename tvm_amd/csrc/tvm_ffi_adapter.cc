@@ -19,6 +19,7 @@
 #include <tvm/ffi/container/tensor.h>
 #include <tvm/ffi/extra/c_env_api.h>
 #include <tvm/ffi/function.h>
+#include <tvm/ffi/optional.h>
 #include <tvm/ffi/reflection/registry.h>
 
 #include "../../include/tvmkv_dlpack.h"
@@ -26,9 +27,11 @@
 namespace {
 
 using tvm::ffi::Function;
+using tvm::ffi::Optional;
 using tvm::ffi::Tensor;
 
 inline const DLTensor* T(const Tensor& t) { return t.operator->(); }
+inline const DLTensor* T(const Optional<Tensor>& t) { return t.has_value() ? T(t.value()) : nullptr; }
 inline void* StreamOf(const Tensor& t) { return TVMFFIEnvGetStream(t->device.device_type, t->device.device_id); }
 inline void Check(int rc) { TVM_FFI_ICHECK_EQ(rc, 0) << "tvmkv: " << tvmkv_last_error(); }
 
@@ -285,7 +288,8 @@ TVM_FFI_STATIC_INIT_BLOCK() {
                                                num_sinks, num_recent, StreamOf(key_weights)));
            })
       .def("tvmkv.move_kept_tokens",
-           [](Tensor pages, Tensor key_weights, Tensor page_indptr, Tensor page_indices, Tensor weight_page_indices, Tensor kept) {
+           [](Tensor pages, Optional<Tensor> key_weights, Tensor page_indptr, Tensor page_indices, Optional<Tensor> weight_page_indices,
+              Tensor kept) {  // None, None: a pool without sums
              Check(tvmkv_dl_move_kept_tokens(T(pages), T(key_weights), T(page_indptr), T(page_indices), T(weight_page_indices), T(kept),
                                              StreamOf(pages)));
            });
