@@ -70,12 +70,12 @@ static void launch_prefill_ext(const PrefillParams& p, int64_t total_q, const Pr
 // (python/tvm/relax/frontend/nn/llm/_decode_kernels.py:441-450) over kv_splits states at once.  A row
 // whose states are all empty (lse = -5e4) stays the empty state: out 0, lse -5e4.
 // T: the type of the shares' outputs, half_t or float (KvSplit).
-template <typename T, int DV>
+template <typename T, int DV, bool AT_ONCE>
 __global__ __launch_bounds__(256) void prefill_split_merge_kernel(const T* __restrict__ part_o,
                                                                   const float* __restrict__ part_lse, half_t* __restrict__ output,
                                                                   float* __restrict__ lse, int64_t rows, int splits,
                                                                   int merge_into, const int32_t* __restrict__ q_end, int h_q) {
-  merge_prefill_shares<T, DV>(part_o, part_lse, output, lse, rows, splits, merge_into, q_end, h_q, blockIdx.x);
+  merge_prefill_shares<T, DV, AT_ONCE>(part_o, part_lse, output, lse, rows, splits, merge_into, q_end, h_q, blockIdx.x);
 }
 
 // Redirects the launch described by p to scratch memory when it is to be split (prefill_kv_splits); finish() merges.
@@ -132,18 +132,27 @@ struct KvSplit {
     KV_LAUNCH_CHECK();
     const unsigned rows_per_block = 256 / (dv / 8);
     const dim3 grid(static_cast<unsigned>((rows + rows_per_block - 1) / rows_per_block));
-    auto merge = [&](auto kernel, const auto* shares) {
+    const bool at_once = merge_shares_at_once(grid.x, splits, p.split_f32, merge_into != 0, compute_units());
+    auto launch = [&](auto kernel, const auto* shares) {
       hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, shares, p.lse, output, lse, rows, splits, merge_into, p.q_indptr + p.batch_size, p.h_q);
     };
-    auto merge_dim = [&](auto dim) {
+    auto merge = [&](auto dim, const auto* shares) {
+      using T = std::remove_cv_t<std::remove_pointer_t<decltype(shares)>>;
       constexpr int kD = decltype(dim)::value;
-      if (p.split_f32) {
-        merge(prefill_split_merge_kernel<float, kD>, reinterpret_cast<const float*>(p.output));
+      if (at_once) {
+        launch(prefill_split_merge_kernel<T, kD, true>, shares);
       } else {
-        merge(prefill_split_merge_kernel<half_t, kD>, static_cast<const half_t*>(p.output));
+        launch(prefill_split_merge_kernel<T, kD, false>, shares);
       }
     };
-    auto merge_padded = [&](auto dim) { merge(prefill_split_merge_kernel<float, decltype(dim)::value>, reinterpret_cast<const float*>(p.output)); };
+    auto merge_dim = [&](auto dim) {
+      if (p.split_f32) {
+        merge(dim, reinterpret_cast<const float*>(p.output));
+      } else {
+        merge(dim, static_cast<const half_t*>(p.output));
+      }
+    };
+    auto merge_padded = [&](auto dim) { merge(dim, reinterpret_cast<const float*>(p.output)); };
     if (dv == 80) {
       merge_padded(std::integral_constant<int, 80>{});
     } else if (dv == 96) {

@@ -6,8 +6,8 @@
 
 namespace tvmkv {
 
-// Shares are taken eight at a time, the last one again in place of those that are not there: their loads do not depend on each other and
-// are all in flight at once (five of 160 rows as a loop of round trips 5.0 us, 64 of a 64-token chunk 35).
+// Shares in loops of as many as there are, unrolled by eight, or eight at once, the last one again in place of those that are not there:
+// all that is needed is in flight together, and what is not needed costs loads and registers (merge_shares_at_once says when which).
 constexpr int kSharesAtOnce = 8;
 __device__ __forceinline__ void load_shares_lse(float (&l)[kSharesAtOnce], const float* part_lse, int64_t rows, int splits, int64_t row, int i0) {
 #pragma unroll
@@ -27,7 +27,7 @@ __device__ __forceinline__ float largest_shares_lse(const float (&l)[kSharesAtOn
 }
 
 // Rows of the block-th 256 threads, 256 / (DV / 8) of them.
-template <typename T, int DV>
+template <typename T, int DV, bool AT_ONCE>
 __device__ __forceinline__ void merge_prefill_shares(const T* __restrict__ part_o, const float* __restrict__ part_lse,
                                                      half_t* __restrict__ output, float* __restrict__ lse, int64_t rows, int splits,
                                                      int merge_into, const int32_t* __restrict__ q_end, int h_q, int block) {
@@ -43,11 +43,17 @@ __device__ __forceinline__ void merge_prefill_shares(const T* __restrict__ part_
   };
   float l[kSharesAtOnce];
   share_t v[kSharesAtOnce];
-  load_shares_lse(l, part_lse, rows, splits, row, 0);
-  load(v, 0);
+  float s_max = kNegInit;
+  if constexpr (AT_ONCE) {
+    load_shares_lse(l, part_lse, rows, splits, row, 0);
+    load(v, 0);
+  } else {
+#pragma unroll 8
+    for (int i = 0; i < splits; ++i) s_max = fmaxf(s_max, part_lse[i * rows + row]);
+  }
   // (rows behind the last sequence have no shares and stay as they are)
   if (row >= end) return;
-  float s_max = largest_shares_lse(l, part_lse, rows, splits, row);
+  if constexpr (AT_ONCE) s_max = largest_shares_lse(l, part_lse, rows, splits, row);
   float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   float w_sum = 0.f;
   const bool any_share = s_max > kNegInit;
@@ -63,7 +69,16 @@ __device__ __forceinline__ void merge_prefill_shares(const T* __restrict__ part_
 #pragma unroll
     for (int e = 0; e < 8; ++e) acc[e] = w * static_cast<float>(x.h8[e]);
   }
-  if (any_share) {
+  if (any_share && !AT_ONCE) {
+#pragma unroll 8
+    for (int i = 0; i < splits; ++i) {
+      const float w = fast_exp2(part_lse[i * rows + row] - s_max);
+      const share_t x = *reinterpret_cast<const share_t*>(part_o + (i * rows + row) * DV + piece * 8);
+      w_sum += w;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[e] += w * static_cast<float>(x[e]);
+    }
+  } else if (any_share) {
     for (int i0 = 0;;) {
 #pragma unroll
       for (int u = 0; u < kSharesAtOnce; ++u) {
