@@ -8,7 +8,7 @@ import torch
 import tvm_amd
 from oracle import eviction
 from tests.gpu_util import DEV, dev, host, i32
-from tests.test_gpu_eviction import Pool, check_attention, prefill, queries
+from tests.test_gpu_eviction import Pool, check_attention, decode, prefill, queries, table_of, values
 from tvm_amd import kernels
 
 pytestmark = pytest.mark.gpu
@@ -63,3 +63,79 @@ def test_shares_in_fp16(shares, d):
         assert (np.abs(out[:n] - want) <= bound).all()
         reach = np.abs(q[:n].astype(np.float64)).sum(-1) * np.nanmax(np.abs(pool.pages[:, 0].astype(np.float64))) * d ** -0.5 * 1.4427
         assert (np.abs(lse[:n] - want_lse) <= ((d + 2) * reach + np.abs(want_lse) + 8) * 2.0 ** -23).all()
+
+
+@pytest.mark.parametrize("stored", [[500], [1, 300, 17, 0], [900, 100, 100]])
+@pytest.mark.parametrize("d", [64, 96, 128, 256])
+def test_decode_with_chunks_and_separate_merges(d, stored):
+    """Launches that add their own sums: several chunks a sequence; a merge of its own, which leaves the sums to another launch."""
+    rng = np.random.default_rng(d + len(stored))
+    pool = Pool(rng, stored, 2, 16, d)
+    q = queries(rng, len(stored), 8, d)
+    for chosen in (dict(decode_chunk_pages=8), dict(decode_separate_merge=1), dict(decode_separate_merge=1, decode_chunk_pages=8)):
+        with options(**chosen):
+            check_attention(q, [1] * len(stored), pool, False, 0, decode(q, pool), f"{chosen}")
+
+
+def test_decode_whose_scores_are_not_kept():
+    """More than 512 MiB of scores: K is read again.  A sequence of 2.1 million tokens on pages that repeat, with sums of their own."""
+    rng = np.random.default_rng(70)
+    h_q, h_kv, d, page, distinct, table = 64, 4, 64, 128, 40, 16700
+    stored = [(table - 4) * page + 77, 300]
+    assert table * page * h_q * 4 > 1 << 29
+    pages = rng.standard_normal((distinct, 2, h_kv, page, d)).astype(np.float16)
+    ids = rng.integers(0, distinct, table).astype(np.int32)
+    weight_ids = rng.permutation(table).astype(np.int32)
+    indptr, info = np.array([0, table - 3, table], np.int32), np.array([77, 300 - 2 * page], np.int32)
+    before = rng.random((table, h_kv, page)).astype(np.float32)
+    q = queries(rng, 2, h_q, d)
+    sums, out = dev(before), torch.empty(q.shape, dtype=torch.float16, device=DEV)
+    lse = torch.empty(q.shape[:2], device=DEV)
+    kernels.batch_decode_paged_kv_weights(dev(q), dev(pages), i32(indptr), i32(ids), i32(info), out, lse, sums, i32(weight_ids), d ** -0.5)
+    out, lse, sums = host(out), host(lse), host(sums)
+    want_sums, slack = before.astype(np.float64), np.zeros(before.shape)
+    for b, n in enumerate(stored):
+        mine, weights = ids[indptr[b]:indptr[b + 1]], weight_ids[indptr[b]:indptr[b + 1]]
+        times = np.zeros((distinct, page))  # how often a row is a token
+        np.add.at(times, mine[:-1], 1.0)
+        times[mine[-1], :info[b]] += 1.0
+        for h in range(h_q):
+            k, v = pages[:, 0, h // 16].astype(np.float64), pages[:, 1, h // 16].astype(np.float64)
+            x = q[b, h].astype(np.float64)
+            s, reach = k @ x * d ** -0.5 / np.log(2.0), np.abs(k) @ np.abs(x) * d ** -0.5 / np.log(2.0)
+            top = s[times > 0].max()
+            total = (times * np.exp2(s - top)).sum()
+            want_lse = top + np.log2(total)
+            w = np.exp2(s - want_lse)
+            worst = reach[times > 0].max()
+            want = np.einsum("pt,ptd->d", times * w, v)
+            size = np.einsum("pt,ptd->d", times * w, np.abs(v))
+            assert (np.abs(out[b, h] - want) <= 1.25 * (2.0 ** -10 * size + n * 2.0 ** -24 * np.abs(v).max()) + 2.0 ** -25).all()
+            assert abs(lse[b, h] - want_lse) <= ((d + 2) * worst + abs(want_lse) + 8) * 2.0 ** -23
+            rel = np.log(2.0) * ((d + 2) * (reach + worst) + 2 * abs(want_lse) + 8) * 2.0 ** -23 + (1 + 16 + 4) * 2.0 ** -23
+            want_sums[weights[:-1], h // 16] += w[mine[:-1]]
+            slack[weights[:-1], h // 16] += (rel * w)[mine[:-1]]
+            want_sums[weights[-1], h // 16, :info[b]] += w[mine[-1], :info[b]]
+            slack[weights[-1], h // 16, :info[b]] += (rel * w)[mine[-1], :info[b]]
+    assert (np.abs(sums - want_sums) <= slack + want_sums * 2.0 ** -23).all()
+
+
+def test_what_an_earlier_choice_left_in_scratch_memory_does_not_count():
+    """Choices of other shapes on the same stream, in an order in which the words of one lie where the next has its histograms and counts of
+    arrivals; the first needs the most memory, so that the buffer stays."""
+    rng = np.random.default_rng(71)
+    shapes = [([300000, 310000], [60000, 70000], 2, "sums"), ([33000, 34000], [4000, 7000], 1, "ties"), ([300000, 310000], [300, 290000], 2, "any"),
+              ([40000], [30000], 1, "equal"), ([70000] + [1] * 20, [20000] * 21, 1, "ties"), ([33000, 36000], [4000, 35000], 2, "close"),
+              ([36000, 33000, 40000], [4000, 7000, 100], 1, "sums")]
+    stream = torch.cuda.Stream()
+    for _ in range(2):
+        for stored, keep, heads, kind in shapes:
+            total, (indptr, info, weight_ids) = table_of(rng, stored, 64)
+            sums = values(rng, kind, (total, heads, 64))
+            kept = torch.full((len(stored), heads, max(keep)), 77, dtype=torch.int32, device=DEV)
+            args = dev(sums), i32(indptr), i32(weight_ids), i32(info), i32(keep)
+            torch.cuda.synchronize()
+            with torch.cuda.stream(stream):
+                kernels.select_kept_tokens(*args, kept, 4, 30)
+            torch.cuda.synchronize()
+            assert np.array_equal(host(kept), eviction.select(sums, indptr, weight_ids, info, keep, max(keep), 4, 30)), (stored, kind)
