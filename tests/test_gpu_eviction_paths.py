@@ -139,3 +139,49 @@ def test_what_an_earlier_choice_left_in_scratch_memory_does_not_count():
                 kernels.select_kept_tokens(*args, kept, 4, 30)
             torch.cuda.synchronize()
             assert np.array_equal(host(kept), eviction.select(sums, indptr, weight_ids, info, keep, max(keep), 4, 30)), (stored, kind)
+
+
+@pytest.mark.parametrize("begin, batch", [(30, 40), (30, 400), (210, 70), (1, 1)])
+def test_some_sequences_of_a_larger_table(begin, batch):
+    """page_indptr and q_indptr that do not begin at 0: rows, sums and pages of the other sequences stay as they are."""
+    rng = np.random.default_rng(begin + batch)
+    total = begin + batch + 25
+    pool = Pool(rng, [int(n) for n in rng.integers(1, 60, total - 1)] + [500], 2, 16, 64)
+    q_lens = [int(min(n, x)) for n, x in zip(rng.integers(0, 4, total), pool.stored)]
+    some, pages, ids, weight_ids = slice(begin, begin + batch), dev(pool.pages), i32(pool.ids), i32(pool.weight_ids)
+    whole = Pool.__new__(Pool)
+    whole.__dict__.update(pool.__dict__, indptr=pool.indptr[begin:begin + batch + 1], info=pool.info[some], stored=pool.stored[some])
+    indptr, info = i32(pool.indptr)[begin:begin + batch + 1], i32(pool.info)[some]
+    q_indptr = np.concatenate(([0], np.cumsum(q_lens)))
+    rows = slice(q_indptr[begin], q_indptr[begin + batch])
+    others = np.ones(q_indptr[-1], bool)
+    others[rows] = False
+
+    def outputs(n):
+        return (torch.full((n, 8, 64), 7.0, dtype=torch.float16, device=DEV), torch.full((n, 8), 7.0, device=DEV), dev(pool.sums))
+
+    for chosen in (dict(), dict(decode_chunk_pages=8, prefill_kv_splits=3), dict(decode_separate_merge=1, prefill_kv_splits=7)):
+        with options(**chosen):
+            q = queries(rng, batch, 8, 64)
+            out, lse, sums = outputs(batch)
+            kernels.batch_decode_paged_kv_weights(dev(q), pages, indptr, ids, info, out, lse, sums, weight_ids, 0.125)
+            check_attention(q, [1] * batch, whole, False, 0, (host(out), host(lse), host(sums)), f"decode {chosen}")
+            plain = outputs(batch)
+            zero = i32([0] * batch)
+            kernels.batch_decode_paged_kv(dev(q), pages, indptr, ids, info, zero, zero, plain[0], plain[1], 0, 1.0, 1e4, 0.125)
+            check_attention(q, [1] * batch, whole, False, 0, (host(plain[0]), host(plain[1]), host(sums)), f"plain decode {chosen}")
+            q = queries(rng, q_indptr[-1], 8, 64)
+            out, lse, sums = outputs(len(q))
+            kernels.batch_prefill_paged_kv_weights(dev(q), i32(q_indptr)[begin:begin + batch + 1], pages, indptr, ids, info, out, lse, sums,
+                                                   weight_ids, 1, 2, 0.125)
+            out, lse = host(out), host(lse)
+            check_attention(q[rows], q_lens[some], whole, True, 2, (out[rows], lse[rows], host(sums)), f"prefill {chosen}")
+            assert (out[others] == 7.0).all() and (lse[others] == 7.0).all()
+    kept = torch.full((batch, 2, 20), 77, dtype=torch.int32, device=DEV)
+    kernels.select_kept_tokens(dev(pool.sums), indptr, weight_ids, info, i32([20] * batch), kept, 2, 5)
+    want = eviction.select(pool.sums, whole.indptr, pool.weight_ids, whole.info, [20] * batch, 20, 2, 5)
+    assert np.array_equal(host(kept), want)
+    sums = dev(pool.sums)
+    kernels.move_kept_tokens(pages, sums, indptr, ids, weight_ids, kept)
+    want_pages, want_sums = eviction.move(pool.pages, pool.sums, whole.indptr, pool.ids, pool.weight_ids, want)
+    assert np.array_equal(host(pages).view(np.uint16), want_pages.view(np.uint16)) and np.array_equal(host(sums), want_sums)

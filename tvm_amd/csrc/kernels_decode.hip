@@ -101,15 +101,15 @@ struct DecodeParams {
 // increasing the number of lanes that qualify tells which sixty-fourth holds the answer.  One round
 // trip to memory per factor of 64 in the batch size (a linear scan in blocks of 64 sequences cost a
 // launch of 2048 sequences up to 32 dependent round trips per work item).  Returns the first of the (at most 64)
-// sequences that are left.
+// sequences that are left: the first of all for slots in front of theirs (page_indptr may begin behind 0).
 __device__ __forceinline__ int narrow_sequences(const int32_t* page_indptr, int batch, int cp, int slot, int lane, int& n) {
-  int lo = 0;  // the answer lies in [lo, lo + n), and slot_begin(lo) <= slot
+  int lo = 0;  // the answer lies in [lo, lo + n)
   n = batch;
   while (n > 64) {
     const int stride = (n + 63) >> 6;
     const int idx = lo + lane * stride;
     const bool le = idx < lo + n && slot_begin(page_indptr, idx, cp) <= slot;
-    const int first = lo + (__popcll(__ballot(le)) - 1) * stride;  // lane 0 always qualifies
+    const int first = lo + (max(static_cast<int>(__popcll(__ballot(le))), 1) - 1) * stride;
     n = min(stride, lo + n - first);
     lo = first;
   }
@@ -443,7 +443,7 @@ __device__ __forceinline__ void decode_items(const DecodeParams& p, const int gr
   const int token = __builtin_amdgcn_readlane(row_at, hit);  // of q and the output
   const int chunk = slot - __builtin_amdgcn_readlane(slot_at, hit);
   const int nchunks = SELF ? max(1, (npages + cp - 1) / cp) : (npages + cp - 1) / cp;
-  if (chunk >= nchunks) {  // spare slot (uniform over the workgroup)
+  if (static_cast<uint32_t>(chunk) >= static_cast<uint32_t>(nchunks)) {  // spare slot (uniform over the workgroup)
     if (p.arrivals != nullptr && npages == 0 && chunk == 0) {  // a sequence without pages: nobody else answers for it
       for (int g = wave; g < heads; g += 4) empty_row<D>(p, b, hq0 + g, lane);
     }

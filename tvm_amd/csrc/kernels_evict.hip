@@ -344,7 +344,7 @@ __global__ __launch_bounds__(256) void shared_rows_kernel(KeyWeightsParams p, in
 template <int D>
 __global__ __launch_bounds__(256) void merge_and_weigh_kernel(KeyWeightsParams p, PrefillShares shares, half_t* output, float* lse, int merging) {
   if (static_cast<int>(blockIdx.x) < merging) {
-    merge_prefill_shares<float, D, true>(shares.output, shares.lse, output, lse, shares.rows, shares.splits, 0, p.q_indptr + p.batch, p.h_q, blockIdx.x);
+    merge_prefill_shares<float, D, true>(shares.output, shares.lse, output, lse, shares.rows, shares.splits, 0, p.q_indptr, p.batch, p.h_q, blockIdx.x);
     return;
   }
   constexpr int KS = D / 16;

@@ -74,8 +74,8 @@ template <typename T, int DV, bool AT_ONCE>
 __global__ __launch_bounds__(256) void prefill_split_merge_kernel(const T* __restrict__ part_o,
                                                                   const float* __restrict__ part_lse, half_t* __restrict__ output,
                                                                   float* __restrict__ lse, int64_t rows, int splits,
-                                                                  int merge_into, const int32_t* __restrict__ q_end, int h_q) {
-  merge_prefill_shares<T, DV, AT_ONCE>(part_o, part_lse, output, lse, rows, splits, merge_into, q_end, h_q, blockIdx.x);
+                                                                  int merge_into, const int32_t* __restrict__ q_indptr, int batch, int h_q) {
+  merge_prefill_shares<T, DV, AT_ONCE>(part_o, part_lse, output, lse, rows, splits, merge_into, q_indptr, batch, h_q, blockIdx.x);
 }
 
 // Redirects the launch described by p to scratch memory when it is to be split (prefill_kv_splits); finish() merges.
@@ -134,7 +134,7 @@ struct KvSplit {
     const dim3 grid(static_cast<unsigned>((rows + rows_per_block - 1) / rows_per_block));
     const bool at_once = merge_shares_at_once(grid.x, splits, p.split_f32, merge_into != 0, compute_units());
     auto launch = [&](auto kernel, const auto* shares) {
-      hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, shares, p.lse, output, lse, rows, splits, merge_into, p.q_indptr + p.batch_size, p.h_q);
+      hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, shares, p.lse, output, lse, rows, splits, merge_into, p.q_indptr, p.batch_size, p.h_q);
     };
     auto merge = [&](auto dim, const auto* shares) {
       using T = std::remove_cv_t<std::remove_pointer_t<decltype(shares)>>;

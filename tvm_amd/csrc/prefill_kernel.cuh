@@ -148,13 +148,13 @@ __device__ __forceinline__ void prefill_row_tile(const PrefillParams& p, const P
   } else {
     // the last sequence whose first slot is at or before this one, by a 64-ary search of the wave: the
     // lanes probe 64 evenly spaced sequences of the range that is left, one round trip to memory per
-    // factor of 64 in the batch size (tile_slot_begin is increasing and 0 for sequence 0)
+    // factor of 64 in the batch size (tile_slot_begin is increasing; slots in front of sequence 0's, where q_indptr begins behind 0, are spare)
     int lo = 0, n = p.batch_size;
     while (n > 64) {
       const int stride = (n + 63) >> 6;
       const int idx = lo + lane * stride;
       const bool le = idx < lo + n && tile_slot_begin(p.q_indptr, idx, group) <= slot;
-      const int first = lo + (__popcll(__ballot(le)) - 1) * stride;
+      const int first = lo + (max(static_cast<int>(__popcll(__ballot(le))), 1) - 1) * stride;
       n = min(stride, lo + n - first);
       lo = first;
     }
@@ -177,7 +177,7 @@ __device__ __forceinline__ void prefill_row_tile(const PrefillParams& p, const P
   const int qo_len = seq_q1 - q_start;
   const int rows = qo_len * group;
   const int n_row_tiles = (rows + BM - 1) / BM;
-  if (local_slot >= n_row_tiles || (SKIPS && p.skip_single && qo_len == 1)) return;
+  if (static_cast<uint32_t>(local_slot) >= static_cast<uint32_t>(n_row_tiles) || (SKIPS && p.skip_single && qo_len == 1)) return;
   const int r0 = (n_row_tiles - 1 - local_slot) * BM;
 
   // phys_len: tokens the K/V storage of the sequence covers; kv_len: keys attended to (logical)

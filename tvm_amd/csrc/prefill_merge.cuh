@@ -30,13 +30,13 @@ __device__ __forceinline__ float largest_shares_lse(const float (&l)[kSharesAtOn
 template <typename T, int DV, bool AT_ONCE>
 __device__ __forceinline__ void merge_prefill_shares(const T* __restrict__ part_o, const float* __restrict__ part_lse,
                                                      half_t* __restrict__ output, float* __restrict__ lse, int64_t rows, int splits,
-                                                     int merge_into, const int32_t* __restrict__ q_end, int h_q, int block) {
+                                                     int merge_into, const int32_t* __restrict__ q_indptr, int batch, int h_q, int block) {
   typedef T share_t __attribute__((ext_vector_type(8)));
   constexpr int TPR = DV / 8;  // threads per row, 8 features each
   const int64_t row = static_cast<int64_t>(block) * (256 / TPR) + threadIdx.x / TPR;
   const int piece = threadIdx.x % TPR;
   if (threadIdx.x >= 256 / TPR * TPR || row >= rows) return;
-  const int64_t end = static_cast<int64_t>(*q_end) * h_q;
+  const int64_t begin = static_cast<int64_t>(q_indptr[0]) * h_q, end = static_cast<int64_t>(q_indptr[batch]) * h_q;
   const auto load = [&](share_t(&v)[kSharesAtOnce], int i0) {
 #pragma unroll
     for (int u = 0; u < kSharesAtOnce; ++u) v[u] = *reinterpret_cast<const share_t*>(part_o + (min(i0 + u, splits - 1) * rows + row) * DV + piece * 8);
@@ -51,8 +51,8 @@ __device__ __forceinline__ void merge_prefill_shares(const T* __restrict__ part_
 #pragma unroll 8
     for (int i = 0; i < splits; ++i) s_max = fmaxf(s_max, part_lse[i * rows + row]);
   }
-  // (rows behind the last sequence have no shares and stay as they are)
-  if (row >= end) return;
+  // (rows in front of the first sequence and behind the last one have no shares and stay as they are)
+  if (row < begin || row >= end) return;
   if constexpr (AT_ONCE) s_max = largest_shares_lse(l, part_lse, rows, splits, row);
   float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   float w_sum = 0.f;
