@@ -132,7 +132,7 @@ struct KvSplit {
     KV_LAUNCH_CHECK();
     const unsigned rows_per_block = 256 / (dv / 8);
     const dim3 grid(static_cast<unsigned>((rows + rows_per_block - 1) / rows_per_block));
-    const bool at_once = merge_shares_at_once(grid.x, splits, p.split_f32, merge_into != 0, compute_units());
+    const bool at_once = merge_shares_at_once(grid.x, splits, p.split_f32, compute_units());
     auto launch = [&](auto kernel, const auto* shares) {
       hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, shares, p.lse, output, lse, rows, splits, merge_into, p.q_indptr, p.batch_size, p.h_q);
     };

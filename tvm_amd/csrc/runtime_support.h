@@ -129,16 +129,18 @@ constexpr int64_t kMinShareKeys = 512;  // eight tiles of 64 keys
 int64_t prefill_workgroups(int64_t work_q, int group, int64_t work_seqs, int h_kv);
 int prefill_kv_splits(int64_t work_q, int group, int64_t work_seqs, int h_kv, int64_t avg_keys, int cus);
 int prefill_float_kv_splits(int64_t work_q, int group, int64_t work_seqs, int h_kv, int64_t avg_keys, int cus, int d);
-// Whether the merge of a split launch takes its shares eight at once or in loops (prefill_merge.cuh).  The merge alone, in loops / at once,
-// us, 32 heads of dim 128, by query tokens:
-//   5      fp16, two shares 2.6 / 2.6, five 2.95 / 2.7, 16 2.9 / 3.4, 32 4.0 / 5.1      float32, five 2.95 / 2.65, eight 3.3 / 2.7, 32 7.9 / 5.8
-//   64     fp16, three 2.7 / 2.6, five 3.1 / 2.6, eight 2.5 / 2.6                         float32, five 3.1 / 2.8, 32 14.6 / 6.9
-//   300    fp16, two 3.0 / 3.4, three 3.2 / 3.4, five 3.6 / 3.5, seven 4.1 / 3.6          float32, two 3.0 / 4.0, five 3.8 / 4.1, six 4.6 / 4.3
-//   1000   fp16, two 4.3 / 5.5, four 6.4 / 6.9, seven 12.1 / 11.8, eight 12.7 / 13.4      float32, two 5.9 / 8.1, four 12.4 / 12.4
-// into a state that is there, 5 query tokens: two in float32 2.7 / 3.1, eight 3.6 / 3.1.
-inline bool merge_shares_at_once(int64_t workgroups, int splits, bool float_shares, bool merge_into, int cus) {
-  if (float_shares ? splits > 5 : splits > 4 && splits < 8) return true;
-  return workgroups <= cus && splits > 2 && splits < 8 && !merge_into;
+// Whether the merge of a split launch takes its shares eight at once or in loops (prefill_merge.cuh).  Eight at once is more loads in flight;
+// loops load no more shares than there are and need fewer registers, which two shares of many rows, whole groups of eight in fp16 and many
+// float32 shares of many rows are better with.  The merge alone, its shares just written, in loops / at once, us, 32 heads of dim 128, by
+// query tokens:
+//   5      fp16, two shares 3.2 / 2.7, five 4.8 / 2.8, 12 4.9 / 3.9, 16 3.9 / 4.0, 32 5.8 / 6.4     float32, two 3.4 / 2.8, eight 5.3 / 3.0, 32 15.2 / 7.2
+//   300    fp16, two 3.8 / 3.8, three 4.6 / 4.1, seven 6.7 / 5.0, eight 5.1 / 5.1                    float32, two 4.0 / 4.7, five 6.2 / 5.8, eight 8.0 / 7.6
+//   500    fp16, two 4.2 / 4.5, five 6.5 / 5.9, 16 12.9 / 13.1                                        float32, two 5.0 / 5.6, eight 11.6 / 12.0, 16 20.4 / 21.4
+//   1000   fp16, two 5.7 / 6.2, four 8.2 / 7.8                                                        float32, two 7.4 / 8.4, four 12.3 / 12.2
+inline bool merge_shares_at_once(int64_t workgroups, int splits, bool float_shares, int cus) {
+  if (splits == 2) return workgroups <= cus;
+  if (float_shares) return splits < 8 || workgroups <= 3 * static_cast<int64_t>(cus);
+  return splits < 16 || splits % 8 != 0;
 }
 // The same of a launch of the generic kernel, whose workgroups own generic_row_tile() query rows.
 inline int generic_row_tile(int d, int64_t rows_per_sequence) { return d > 128 || rows_per_sequence <= 16 ? 16 : 32; }
