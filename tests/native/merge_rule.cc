@@ -11,7 +11,7 @@ int main() {
       const bool single = tvmkv::merge_shares_at_once(workgroups, shares, true, 256);
       // two shares of many rows are not read eight times
       if (shares == 2 && workgroups > 256 && (half || single)) return std::printf("two shares at once\n"), 1;
-      if (half != (shares == 2 ? workgroups <= 256 : !(shares >= 16 && shares % 8 == 0))) return std::printf("fp16 %d\n", shares), 1;
+      if (half != (shares == 2 ? workgroups <= 256 : shares <= 8 || shares % 8 > 1 + shares / 16)) return std::printf("fp16 %d\n", shares), 1;
       if (single != (shares == 2 ? workgroups <= 256 : shares < 8 || workgroups <= 768)) return std::printf("float32 %d\n", shares), 1;
     }
   }

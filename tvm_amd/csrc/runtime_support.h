@@ -130,17 +130,18 @@ int64_t prefill_workgroups(int64_t work_q, int group, int64_t work_seqs, int h_k
 int prefill_kv_splits(int64_t work_q, int group, int64_t work_seqs, int h_kv, int64_t avg_keys, int cus);
 int prefill_float_kv_splits(int64_t work_q, int group, int64_t work_seqs, int h_kv, int64_t avg_keys, int cus, int d);
 // Whether the merge of a split launch takes its shares eight at once or in loops (prefill_merge.cuh).  Eight at once is more loads in flight;
-// loops load no more shares than there are and need fewer registers, which two shares of many rows, whole groups of eight in fp16 and many
-// float32 shares of many rows are better with.  The merge alone, its shares just written, in loops / at once, us, 32 heads of dim 128, by
+// loops load no more shares than there are and need fewer registers, which two shares of many rows, groups of eight in fp16, with few left
+// over, and many float32 shares of many rows are better with.  The merge alone, its shares just written, in loops / at once, us, 32 heads of dim 128, by
 // query tokens:
 //   5      fp16, two shares 3.2 / 2.7, five 4.8 / 2.8, 12 4.9 / 3.9, 16 3.9 / 4.0, 32 5.8 / 6.4     float32, two 3.4 / 2.8, eight 5.3 / 3.0, 32 15.2 / 7.2
 //   300    fp16, two 3.8 / 3.8, three 4.6 / 4.1, seven 6.7 / 5.0, eight 5.1 / 5.1                    float32, two 4.0 / 4.7, five 6.2 / 5.8, eight 8.0 / 7.6
 //   500    fp16, two 4.2 / 4.5, five 6.5 / 5.9, 16 12.9 / 13.1                                        float32, two 5.0 / 5.6, eight 11.6 / 12.0, 16 20.4 / 21.4
 //   1000   fp16, two 5.7 / 6.2, four 8.2 / 7.8                                                        float32, two 7.4 / 8.4, four 12.3 / 12.2
+// Whole calls, 64 tokens on 30 000, 16 / 2 heads, 58 fp16 shares 39.4 / 40.5, 16 on 60 000, 8 / 1 heads, 64 shares 34.5 / 35.8.
 inline bool merge_shares_at_once(int64_t workgroups, int splits, bool float_shares, int cus) {
   if (splits == 2) return workgroups <= cus;
   if (float_shares) return splits < 8 || workgroups <= 3 * static_cast<int64_t>(cus);
-  return splits < 16 || splits % 8 != 0;
+  return splits <= 8 || splits % 8 > 1 + splits / 16;
 }
 // The same of a launch of the generic kernel, whose workgroups own generic_row_tile() query rows.
 inline int generic_row_tile(int d, int64_t rows_per_sequence) { return d > 128 || rows_per_sequence <= 16 ? 16 : 32; }
