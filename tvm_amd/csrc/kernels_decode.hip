@@ -109,7 +109,7 @@ __device__ __forceinline__ int narrow_sequences(const int32_t* page_indptr, int 
     const int stride = (n + 63) >> 6;
     const int idx = lo + lane * stride;
     const bool le = idx < lo + n && slot_begin(page_indptr, idx, cp) <= slot;
-    const int first = lo + (max(static_cast<int>(__popcll(__ballot(le))), 1) - 1) * stride;
+    const int first = lo + (__popcll(__ballot(le) | 1) - 1) * stride;  // (a maximum cost the kernels scalar registers: 394 -> 397 us)
     n = min(stride, lo + n - first);
     lo = first;
   }

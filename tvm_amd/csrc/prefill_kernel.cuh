@@ -154,7 +154,7 @@ __device__ __forceinline__ void prefill_row_tile(const PrefillParams& p, const P
       const int stride = (n + 63) >> 6;
       const int idx = lo + lane * stride;
       const bool le = idx < lo + n && tile_slot_begin(p.q_indptr, idx, group) <= slot;
-      const int first = lo + (max(static_cast<int>(__popcll(__ballot(le))), 1) - 1) * stride;
+      const int first = lo + (__popcll(__ballot(le) | 1) - 1) * stride;
       n = min(stride, lo + n - first);
       lo = first;
     }
