@@ -54,6 +54,7 @@ LISTS = {
     "choice": lambda n: [np.concatenate((np.arange(n // 3), np.arange(n - n // 4, n)))],
     "recent": lambda n: [np.arange(7, n)],                # every token by fewer places than they are: in order
     "few": lambda n: [np.concatenate(([n - 3], np.arange(1, 200), [n - 2, n - 1]))],
+    "same": lambda n: [np.maximum(np.sort(np.random.default_rng(n).integers(0, n, n - n // 4)), np.arange(n - n // 4))],  # tokens several times
     "odd": lambda n: [np.array([n - 1, 1, 1 << 30, 9, -5] + [-1] * 300)],
 }
 

@@ -185,3 +185,20 @@ def test_some_sequences_of_a_larger_table(begin, batch):
     kernels.move_kept_tokens(pages, sums, indptr, ids, weight_ids, kept)
     want_pages, want_sums = eviction.move(pool.pages, pool.sums, whole.indptr, pool.ids, pool.weight_ids, want)
     assert np.array_equal(host(pages).view(np.uint16), want_pages.view(np.uint16)) and np.array_equal(host(sums), want_sums)
+
+
+@pytest.mark.parametrize("stored, entries", [([600, 90], 400), ([5000, 2600], 4100), ([5000, 40], 2600)])
+def test_move_of_lists_that_name_a_token_several_times(stored, entries):
+    rng = np.random.default_rng(entries)
+    pool = Pool(rng, stored, 2, 16, 64)
+    kept = np.full((2, 2, entries), -1, np.int32)
+    for b, n in enumerate(stored):
+        for h in range(2):
+            m = min(entries, n - n // 5)
+            kept[b, h, :m] = np.maximum(np.sort(rng.integers(0, n, m)), np.arange(m))
+    assert len(set(kept[0, 0].tolist())) < entries - 10
+    indptr, ids, _, weight_ids = pool.table()
+    pages, sums = dev(pool.pages), dev(pool.sums)
+    kernels.move_kept_tokens(pages, sums, indptr, ids, weight_ids, i32(kept))
+    want, want_sums = eviction.move(pool.pages, pool.sums, pool.indptr, pool.ids, pool.weight_ids, kept)
+    assert np.array_equal(host(pages).view(np.uint16), want.view(np.uint16)) and np.array_equal(host(sums), want_sums)
