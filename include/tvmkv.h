@@ -485,14 +485,15 @@ int tvmkv_mxfp4_batch_prefill_paged_kv(const void* q, const int32_t* q_indptr, c
  * an evicted one or one of another sequence, until the caller clears it.  Whoever stores a token sets the sums of its slot to 0, for
  * all kv heads, before the first attention call that sees the token.
  *
- * Built for fp16 rows, pages of 16, 32, 64 or 128 tokens, head dims 64, 80, 96, 112, 128 and 256, any GQA group; keys are stored
- * rotated, caches without sliding windows.  q, pages and output are aligned to 16 bytes.  A call reads what the device arrays hold, not
- * their copies on the host, so it may be captured; scratch memory (decode's scores, prefill's shares, long lists of the choice) is that
- * of the other launchers, one buffer per (device, stream): two graphs captured on one stream share it and are replayed one after the
- * other.  A query without keys: output 0, lse -5e4, no weights.  page_indptr and q_indptr need not begin at 0: they may be some of a
- * larger batch's, with the whole page_values and, in prefill, the whole q.  Rows of output and lse in front of the first query of
- * q_indptr and behind the last one stay as they are.  What unused slots hold does not matter, NaN included; a stored row of V that is not finite reaches, as in
- * tvmkv_batch_prefill_paged_kv, also those queries of its tile that do not see it. */
+ * Built for fp16 rows, pages of 16, 32, 64 or 128 tokens, head dims 64, 80, 96, 112, 128 and 256, any GQA group; keys are
+ * stored rotated, caches without sliding windows.  q, pages and output are aligned to 16 bytes.  A call reads what the device
+ * arrays hold, not their copies on the host, so it may be captured; scratch memory (decode's scores, 4 bytes a (token, query
+ * head) and 512 MiB at most and half of it in reserve, prefill's shares, long lists of the choice) is that of the other
+ * launchers, one buffer per (device, stream): two graphs captured on one stream share it and are replayed one after the other.
+ * A query without keys: output 0, lse -5e4, no weights.  page_indptr and q_indptr need not begin at 0: they may be some of a
+ * larger batch's, with the whole page_values and, in prefill, the whole q.  Rows of output and lse in front of the first query
+ * of q_indptr and behind the last one stay as they are.  What unused slots hold does not matter, NaN included; a stored row of
+ * V that is not finite reaches, as in tvmkv_batch_prefill_paged_kv, also those queries of its tile that do not see it. */
 
 /* tvmkv_batch_decode_paged_kv with the sums: one query token a sequence, q and output (batch, h_q, d), lse (batch, h_q),
  * length_info (batch). */

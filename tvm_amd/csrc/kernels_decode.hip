@@ -327,7 +327,7 @@ struct DecodeRopeRunning : DecodeRopeDivisors {
 // KEEP (plain cache, groups of one block): the scores also go to memory, for the sums of attention weights (kernels_evict.hip).  In
 // small launches the workgroup that has the last state of a (sequence, kv head) also adds the weights of its keys to the sums.  Bound by
 // memory as without them: 64 sequences of 1024-4096 tokens (32 / 8 heads of dim 128) 134 us, 119 without the 21 MB of scores; 8 of 32 768-
-// 65 536 with 64 query heads 319 and 260 (102 MB).
+// 65 536 with 64 query heads 316 and 260 (102 MB).
 //
 // decode_items works on items first_item, first_item + stride, ... below num_items.
 template <int D, bool FUSED, bool RUNNING>

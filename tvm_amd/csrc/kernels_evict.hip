@@ -62,9 +62,9 @@ __device__ __forceinline__ SequenceOf sequence_of_slot(const int32_t* page_indpt
 //
 // The product q K^T is done again, as attention writes no scores and a key's weight needs the row's lse first: 2 D operations, an exponential
 // and two more vector instructions for each (row, key), K read once and q once for 128 or 256 tokens.  Bound by the issue of vector and
-// matrix instructions: 8 chunks of 128-2048 queries on up to 4096 tokens, 32 / 8 heads of dim 128, 342 us (795 TFLOP/s of products;
-// 0.63 of the issue slots and 0.34 of the matrix unit in use); two chunks of 100-300 on 20 000-32 768, 16 / 2 heads of dim 256, 108 us
-// (520 TFLOP/s: 32 tokens a wave, as 64 tokens' K do not fit its registers, and so q read from shared memory twice as often).
+// matrix instructions: 8 chunks of 128-2048 queries on up to 4096 tokens, 32 / 8 heads of dim 128, 337 us (807 TFLOP/s of products;
+// 0.64 of the issue slots and 0.35 of the matrix unit in use); two chunks of 100-300 on 20 000-32 768, 16 / 2 heads of dim 256, 108 us
+// (521 TFLOP/s: 32 tokens a wave, as 64 tokens' K do not fit its registers, and so q read from shared memory twice as often).
 // ------------------------------------------------------------------------------------------
 struct KeyWeightsParams {
   const half_t* q;
@@ -382,8 +382,8 @@ __global__ __launch_bounds__(256) void merge_and_weigh_kernel(KeyWeightsParams p
 // ------------------------------------------------------------------------------------------
 // Weights from kept scores: decode's, which are few (4 bytes for each of the group's heads, where K has 2 D).  A wave has 256 tokens
 // of a kv head, a lane the four of a run of 16 that a lane of the decode kernel had.  Each score is read once, in whole lines: 21 MB of 64
-// sequences of 1024-4096 tokens in 10 us, 102 MB of 8 of 32 768-65 536 with 64 query heads in 22 (4.6 TB/s).  Whole calls with K read
-// again, for all heads of a group at once, took 208 and 458 us, with kept scores 144 and 341.
+// sequences of 1024-4096 tokens in 10.6 us, 102 MB of 8 of 32 768-65 536 with 64 query heads in 23 (4.4 TB/s).  Whole calls with K read
+// again, for all heads of a group at once, took 208 and 458 us, with kept scores 144 and 340.
 // ------------------------------------------------------------------------------------------
 struct KeptScoresParams {
   const float* scores;  // (kv head, 16-token run of the page table, head of the group, 16 tokens in the order of kept_score_token)
@@ -428,8 +428,10 @@ __global__ __launch_bounds__(256) void kept_scores_kernel(KeptScoresParams p) {
 // workgroups goes on to find the digit; then the bits; then the places.  (One list of 131072 tokens by a single workgroup, which
 // reads it with 25 GB/s, took 92 us, with T narrowed down by a sample first 60.)
 //
-// What bounds them is the chain of their steps, not the bytes (4 a token): 512 lists of 2112 tokens 11.7 us, 128 of 2000-16 384 14.9, 8 of 700 6.7;
-// 2 of 131 072 in chunks 33 us, of which clearing 1-4, three passes 6.6 each, bits 4.7, places 9.1.
+// What bounds them is the chain of their steps, not the bytes (4 a token): 512 lists of 2112 tokens 11.7 us, 128 of 2000-16 384 14.9, 8 of 700 7.8;
+// 2 of 131 072 in chunks 33 us, of which clearing 1-5, three passes 6.6 each, bits 4.8, places 9.0.  Where the choice is among equal
+// weights, as of sums that are all 0, a chunk's workgroup reads those in front of its own, and the last one is the longest: 2 of 131 072
+// equal ones 77 us, 2 of 2 000 000 1119 (unlike ones 106); 512 of 2112, in registers, 14.1.
 // ------------------------------------------------------------------------------------------
 struct SelectState {
   uint32_t least;  // of T, the bits that are known
@@ -902,7 +904,7 @@ __global__ __launch_bounds__(256) void select_bits_kernel(SelectParams p) {
 #pragma unroll
   for (int u = 0; u < 4; ++u) w[u] = l.weights_of(p, c.kvh, page[u], (block0 + u) * 64 + lane);
   int equal_before = 0;
-  if (t.cut) {  // weights equal to T in front of the wave's: its workgroup counts them in the chunks in front of its own
+  if (t.cut) {  // weights equal to T in front of the wave's: its workgroup counts them in the chunks in front of its own, a load a step
     int equal = 0;
     for (int k = wave; k < c.first_block; k += 4) {
       const int group = k * 64 + lane;
@@ -985,7 +987,7 @@ __global__ __launch_bounds__(256) void select_places_kernel(SelectParams p) {
 // places than they are) in order as above.  Entries that name no token behind their place are passed over.
 //
 // Bytes alone, each moved row read and written once: 512 lists of 2112 tokens to 2048 (8 kv heads of dim 128) 40 us, 128 of 2000-16 384 to
-// 2048 46, both 4.4 TB/s where a large copy makes 5.2; rows of 256 bytes from all over the pool, a row's two parts in different pages.
+// 2048 45, 4.4 and 4.5 TB/s where a large copy makes 5.2; rows of 256 bytes from all over the pool, a row's two parts in different pages.
 // 2 lists of 131 072 to 16 384 (dim 256) by ranges 20 + 11 us, 3 TB/s in the first launch.
 // ------------------------------------------------------------------------------------------
 struct MoveParams {
@@ -1239,7 +1241,8 @@ static void add_key_weights(const char* what, KeyWeightsParams p, int64_t total_
     const int64_t tokens = nnz_pages << page_shift, items = (tokens / (128 * TB) + batch_size) * h_kv;
     KV_CHECK(items < (int64_t{1} << 31)) << what << ": too many work items";
     // Few workgroups of many rows share these: two workgroups a compute unit, or four where each has a long way to go, of two row tiles at
-    // least; two shares only where they save more than the second launch costs.  Whole calls alone / shared, us (query heads / kv heads x dim):
+    // least, by the average sequence; two shares only where they save more than the second launch costs.  Whole calls alone / shared, us (query
+    // heads / kv heads x dim):
     //   1 x 2048 tokens 32/8x128 216 / 96, on 8000 cached 567 / 522; 1 x 500 on 2000 88 / 65; 2 x 1000 64/8x128 305 / 235; 8 x 512 16/2x64 95 / 35;
     //   2 x 25-241 on 79-315 40/1x96 173 / 28; 27 x 14-973 40/1x96 913 / 264; not shared: 37 x 9/3x96, 18 tiles on 243 workgroups, 68 / 80,
     //   1 x 114 32/8x128, 7 tiles on 8, 16 / 18
@@ -1326,7 +1329,9 @@ int tvmkv_batch_decode_paged_kv_weights(const void* q, const void* pages, const 
     const int64_t items = (((nnz_pages << p.page_shift) >> kKeptTokensShift) + batch_size) * h_kv;
     KV_CHECK(items < (int64_t{1} << 31)) << what << ": too many work items";
     // A launch of a few short sequences adds the weights itself (one of 500 tokens 12.9 -> 10.3 us); a sequence's are added by one
-    // workgroup, and longer ones take it longer than a second launch (41 of up to 2500 tokens 23.5 -> 26.4).
+    // workgroup, and longer ones take it longer than a second launch (41 of up to 2500 tokens 23.5 -> 26.4).  Lengths are on the device: the
+    // rule goes by their average, and one long sequence among short ones is added by a workgroup a kv head, too (itself / a second launch: 2500 among
+    // 15 of 20 tokens 18.4 / 17.3, 8000 35 / 28, 15 000 47 / 30).
     const int64_t tokens = nnz_pages * page_size;
     const bool itself = tokens <= 16384 && tokens <= int64_t{1024} * batch_size;
     bool added = false;
@@ -1371,6 +1376,8 @@ int tvmkv_batch_prefill_paged_kv_weights(const void* q, const int32_t* q_indptr,
   //                              8 x 2000         8 rows 29.3 / 28.5, 16 rows 30.0 / 29.9, 32 rows 30.8 / 32.9, 64 rows 36 / 42
   //   16 / 2 heads of dim 256    1 x 8000         16 rows 33.5 / 28.6, 64 rows 36.6 / 36.6, 128 rows 44 / 51
   //   32 / 1 heads of dim 64     4 x 4000         32 rows 18.6 / 14.1, 64 rows 19.8 / 17.4, 128 rows 23 / 26
+  // Rows are counted on average, as they are on the device: of 16 sequences of 2000 tokens one with 64 queries and none in the others 31 / 32.5,
+  // of 8000 and 15 of 200 63 / 71, of 64 of 2000 one with 256 81 / 75.
   bool added = false;
   const bool in_one = total_q * p.group <= int64_t{(nnz_pages << p.page_shift) * h_kv <= 16384 ? 64 : 16} * batch_size;
   const std::function<void(const PrefillShares&)> merge_and_weigh = [&](const PrefillShares& shares) {
@@ -1491,6 +1498,9 @@ int tvmkv_move_kept_tokens(void* pages, float* key_weights, const int32_t* page_
   // ranges of places.  In order / by ranges, us (lists, tokens, places; 8 kv heads of dim 128 but for the last):
   //   8 x 700 to 512 7.9 / 15.3, 16 x 2112 to 2048 9.0 / 18.4, 128 x 2112 to 2048 14.9 / 30, 512 x 4096 to 2048 120 / 126, 128 x 12 000 to 4000
   //   81 / 88; 32 x 24 000 to 4000 43 / 38, 8 x 12 000 to 4000 28.7 / 20.0, 4 x 40 000 to 8000 61 / 20.5
+  // Few lists around the 2048 places, captured: to 2048 from 16 000 one 14.5 / 15.9, 8 17.0 / 16.8, 32 22 / 26, from 65 536 one 15.3 / 16.0, 8 18.4 / 17.0,
+  // 32 26 / 27; to 1536 from 16 000 8 13.3 / 16.5; to 2500 from 16 000 one 17.8 / 15.8, 8 21.7 / 18.3, 32 27 / 29, from 65 536 8 23 / 19, 32 32 / 31.
+  // Lists that lose few tokens are better in order up to 4000 places (8 x 5000 to 4000 13.8 / 16.6), which max_keep alone does not say.
   const auto cut_rows = [&](int64_t most, int least_pieces) {
     p.slices = 1;
     while (p.slices * 2 <= most && p.pieces % (p.slices * 2) == 0 && p.pieces / (p.slices * 2) >= least_pieces) p.slices *= 2;
